@@ -279,6 +279,45 @@ int pdk_decode_attn_rope_rms(const float* qkv_partials, int splits,
                              float scale, void* workspace, size_t workspace_bytes,
                              uint16_t* out, int plan_batch, uintptr_t stream);
 
+/* ---- a sliding window with sinks ----------------------------------------------
+ * The query at position p = ctx[b]-1 sees the tokens t <= p with t > p - window
+ * or t < sinks: the last `window` tokens, itself among them, and the first
+ * `sinks`. Only blocks that hold such tokens are read, so those between the two
+ * may be freed and their table entries set to -1, and contexts may be as long as
+ * the table (max_blocks <= 65535); window, sinks and max_ctx together may leave
+ * up to 16384 tokens to read (pdk_decode_attn_window_span; else PDK_ENOTSUP).
+ * Other arguments as pdk_decode_attn (masked and invalid blocks included), any
+ * Hq/Hkv from 1 to 16; the workspace is pdk_decode_attn_workspace_bytes() of
+ * max_ctx, or of pdk_decode_attn_window_span(max_ctx, window, sinks), which is
+ * smaller. No counterpart in the reference, whose lanes are attended to whole
+ * (kernels/decode_batch.py:81-85).
+ *
+ * pdk_decode_attn_window: with k_new and v_new (both or neither) the new token's
+ * rows go to their cache slot and take part, as in pdk_decode_attn_append.
+ * pdk_decode_attn_rope_window: pdk_decode_attn_rope (splits 1 or 2), or with
+ * out_tiled != 0 pdk_decode_attn_rope_xt. */
+int pdk_decode_attn_window_span(int max_ctx, int window, int sinks);
+
+int pdk_decode_attn_window(const uint16_t* q, const uint16_t* k_new,
+                           const uint16_t* v_new, uint16_t* cache_k,
+                           uint16_t* cache_v, int num_blocks,
+                           const int32_t* block_tables, int max_blocks,
+                           const int32_t* ctx_lens, int max_ctx, int window,
+                           int sinks, int B, int n_q_heads, int n_kv_heads,
+                           int head_dim, float scale, void* workspace,
+                           size_t workspace_bytes, uint16_t* out,
+                           uintptr_t stream);
+
+int pdk_decode_attn_rope_window(const float* qkv_partials, int splits,
+                                const float* inv_freq, uint16_t* cache_k,
+                                uint16_t* cache_v, int num_blocks,
+                                const int32_t* block_tables, int max_blocks,
+                                const int32_t* ctx_lens, int max_ctx, int window,
+                                int sinks, int B, int n_q_heads, int n_kv_heads,
+                                int head_dim, float scale, void* workspace,
+                                size_t workspace_bytes, uint16_t* out,
+                                int out_tiled, int plan_batch, uintptr_t stream);
+
 /* Write one new token's k and v per stream at slot ctx[b]-1 of the paged
  * cache: the one-hot cache injection Kf = Kp + k*oh, Vf = Vp + v*oh
  * (kernels/decode_batch.py:81-82), done as a store.
@@ -295,6 +334,57 @@ int pdk_cache_append(const uint16_t* k_new, const uint16_t* v_new,
  * NaN counts as the maximum). out: device int32 [B]. */
 int pdk_greedy_argmax(const uint16_t* logits, int B, int V, int64_t ld,
                       int32_t* out, uintptr_t stream);
+
+/* ---- blocks copied inside the paged cache ------------------------------------
+ * Block src[i] to block dst[i], i < n, K and V of all layers (a layer's K and V
+ * blocks start cache_layer_stride elements after the previous layer's). src and
+ * dst are host arrays, read before the call returns. Ids outside [0, num_blocks),
+ * a block that two pairs write and one that is both a source and a destination
+ * are refused with PDK_EINVAL before anything is copied; one block may be the
+ * source of many pairs. No reference counterpart: its lanes are never shared or
+ * moved (engines/decode_batch.py:305-377). */
+int pdk_copy_blocks(uint16_t* cache_k, uint16_t* cache_v,
+                    int64_t cache_layer_stride, int n_layers, int num_blocks,
+                    int n_kv_heads, int head_dim, const int32_t* src,
+                    const int32_t* dst, int n, uintptr_t stream);
+
+/* ---- beam search ---------------------------------------------------------------
+ * The n best continuations of each of R requests' K beams: over beams k and
+ * tokens v
+ *   total(k, v) = scores[r][k] + x[v] - log(sum_u exp(x[u])),
+ * x row r*K + k of logits [R*K] rows of V values, ld elements apart, bf16
+ * (elem_bytes 2) or fp32 (4). Results in order of total, the lower beam first
+ * among equals, a beam's tokens in order of their logits, the lower token first
+ * among equals: tokens, parents (the beam) and out_scores (the total) [R][n].
+ * Sums and totals are 64-bit; out_scores is rounded once. last_tokens [R][K] (may
+ * be NULL): a beam whose last token is eos has ended; its one candidate is (eos,
+ * its score), its logits are not read. No candidates come from -inf logits, from
+ * a beam whose score is not finite, nor from one whose row holds NaN or +inf, or
+ * only -inf. Where there are fewer than n, the rest is token -1, parent -1,
+ * score -inf. 1 <= K <= 16, 1 <= n <= 32, V <= 2^20. The workspace (16-byte
+ * aligned, one call at a time) needs no clearing. The reference samples greedily
+ * only (greedy_tokens, engines/decode_batch.py:162-171). */
+int64_t pdk_beam_select_workspace_bytes(int R, int K, int V, int n);
+int pdk_beam_select(const void* logits, int elem_bytes, int64_t ld, int R, int K,
+                    int V, const float* scores, const int32_t* last_tokens,
+                    int eos, int n, void* workspace, int64_t workspace_bytes,
+                    int32_t* tokens, int32_t* parents, float* out_scores,
+                    uintptr_t stream);
+
+/* The cache follows a selection: beam k of request r goes on as parents[r][k]
+ * (one outside [0, K): as itself). tables [R*K][max_blocks], row r*K + k beam
+ * k's; ctx_lens [R*K] the tokens in the cache, the same for a request's beams
+ * (the first one's is read). With f = ctx/16, table entries 0 .. f-1 become the
+ * parent's (blocks that are full: shared from now on), and where ctx % 16 > 0 the
+ * block at entry f, which must be the beam's own, receives the contents of the
+ * parent's there, K and V of all layers, as if every beam were read before any is
+ * written. Entries f and up stay. An id outside [0, num_blocks) is not copied
+ * from or to. A request with ctx <= 0 is left alone. K <= 16. */
+int pdk_beam_reorder(const int32_t* parents, const int32_t* ctx_lens, int R,
+                     int K, int32_t* tables, int max_blocks, uint16_t* cache_k,
+                     uint16_t* cache_v, int64_t cache_layer_stride, int n_layers,
+                     int num_blocks, int n_kv_heads, int head_dim,
+                     uintptr_t stream);
 
 /* ---- decode step: the non-GEMM operations of one Llama layer ----------------
  * The rest of the reference's DecodeLayer.forward (kernels/decode_batch.py:73-91)
@@ -741,6 +831,22 @@ int pdk_prefill_argmax(const float* partials, int splits, int N, uint64_t* keys,
 int pdk_prefill_attn(const uint16_t* q, int64_t q_tok_stride, const uint16_t* kt,
                      const uint16_t* vt, int T, int n_q_heads, int n_kv_heads,
                      int head_dim, float scale, uint16_t* out, uintptr_t stream);
+
+/* pdk_prefill_attn under a sliding window with sinks: the query at position p
+ * sees the tokens t <= p with t > p - window or t < sinks (window >= 1, sinks >=
+ * 0). */
+int pdk_prefill_attn_window(const uint16_t* q, int64_t q_tok_stride,
+                            const uint16_t* kt, const uint16_t* vt, int T,
+                            int n_q_heads, int n_kv_heads, int head_dim,
+                            float scale, int window, int sinks, uint16_t* out,
+                            uintptr_t stream);
+
+/* kt and vt from k and v as rows ([T] rows of [Hkv][128], token strides in
+ * elements, multiples of 8), for keys that pdk_prefill_rope_kv did not rotate. */
+int pdk_prefill_kv_tiles(const uint16_t* k, int64_t k_tok_stride,
+                         const uint16_t* v, int64_t v_tok_stride, int T,
+                         int n_kv_heads, int head_dim, uint16_t* kt, uint16_t* vt,
+                         uintptr_t stream);
 
 /* ---- streams and events ------------------------------------------------------
  * Fences for the side-stream staging and for wait_for_save()

@@ -90,6 +90,15 @@ SIGNATURES = {
     "pdk_decode_attn_rope_rms": (_I, [_P, _I, _P, _I, ctypes.c_float, _P, _P, _P, _I, _P, _I,
                                       _P, _I, _I, _I, _I, _I, ctypes.c_float, _P, _SZ, _P, _I,
                                       _U]),
+    "pdk_decode_attn_window_span": (_I, [_I, _I, _I]),
+    "pdk_decode_attn_window": (_I, [_P, _P, _P, _P, _P, _I, _P, _I, _P, _I, _I, _I, _I, _I, _I, _I,
+                                    ctypes.c_float, _P, _SZ, _P, _U]),
+    "pdk_decode_attn_rope_window": (_I, [_P, _I, _P, _P, _P, _I, _P, _I, _P, _I, _I, _I, _I, _I,
+                                         _I, _I, ctypes.c_float, _P, _SZ, _P, _I, _I, _U]),
+    "pdk_copy_blocks": (_I, [_P, _P, _I64, _I, _I, _I, _I, _P, _P, _I, _U]),
+    "pdk_beam_select_workspace_bytes": (_I64, [_I, _I, _I, _I]),
+    "pdk_beam_select": (_I, [_P, _I, _I64, _I, _I, _I, _P, _P, _I, _I, _P, _I64, _P, _P, _P, _U]),
+    "pdk_beam_reorder": (_I, [_P, _P, _I, _I, _P, _I, _P, _P, _I64, _I, _I, _I, _I, _U]),
     "pdk_cache_append": (_I, [_P, _P, _P, _P, _I, _P, _I, _P, _I, _I, _I, _U]),
     "pdk_greedy_argmax": (_I, [_P, _I, _I, _I64, _P, _U]),
     "pdk_rmsnorm": (_I, [_P, _P, _P, _I, _I, ctypes.c_float, _P, _U]),
@@ -145,6 +154,8 @@ SIGNATURES = {
     "pdk_prefill_rmsnorm_partials": (_I, [_P, _P, _I64, _I, _P, _I, _I, _F, _P, _U]),
     "pdk_prefill_argmax": (_I, [_P, _I, _I, _P, _U]),
     "pdk_prefill_attn": (_I, [_P, _I64, _P, _P, _I, _I, _I, _I, _F, _P, _U]),
+    "pdk_prefill_attn_window": (_I, [_P, _I64, _P, _P, _I, _I, _I, _I, _F, _I, _I, _P, _U]),
+    "pdk_prefill_kv_tiles": (_I, [_P, _I64, _P, _I64, _I, _I, _I, _P, _P, _U]),
     "pdk_scatter_koni": (_I, [_P, _I64, _P, _I, _I, _P, _I, _P, _P, _I64, _I, _I, _I, _U]),
     "pdk_host_alloc": (_I, [_SZ, ctypes.POINTER(_P)]),
     "pdk_host_free": (_I, [_P]),

@@ -89,6 +89,25 @@ struct AttnArgs {
   float scale_log2;              // scale * log2(e)
 };
 
+// A sliding window with sinks (kWin): the query at position p sees the tokens t
+// <= p with t > p - window or t < sinks. The spans that hold such tokens, laid
+// end to end, are what the wavefronts walk: positions v of that sequence below
+// sink_end (the sinks rounded up to whole spans) are tokens v, the others tokens
+// v + shift, shift (a multiple of the span) leading to the span that holds the
+// window's first token `lo`. Where the two parts meet or overlap shift is 0.
+struct Window {
+  int lo, sinks, sink_end, shift;
+};
+
+__device__ __forceinline__ Window window_of(int ctx, int window, int sinks) {
+  Window w;
+  w.lo = max(ctx, 0) - window;
+  w.sinks = sinks;
+  w.sink_end = (sinks + kSpan - 1) & ~(kSpan - 1);
+  w.shift = max((max(w.lo, 0) & ~(kSpan - 1)) - w.sink_end, 0);
+  return w;
+}
+
 // Registers of one span between its loads and its use.
 struct Span {
   v8 ka[4], kb[4], vf[8];
@@ -281,14 +300,17 @@ __device__ __forceinline__ void fold_span(const Span& r, f32x4 o[8]) {
 // wavefront.
 // With kPatch (the fused RoPE path) the span's K and V take the new token nt
 // in place of the cache's contents, after those that others(f) hands to f.
-template <bool kPatch, int kNV, class F>
+// With kWin the tokens outside the window w (and not sinks) take no part either.
+template <bool kPatch, bool kWin, int kNV, class F>
 __device__ __forceinline__ void attend_span(const AttnArgs& a, Span& r, const v8 qv[4], int span,
                                             int lo, int hi, int lim, int g, int j, bool first,
                                             float& m, float& lsum, f32x4 o[8],
-                                            const NewToken& nt, F others) {
+                                            const NewToken& nt, const Window& win, F others) {
   const int tv = span + 8 * g;
   const bool full = span + kSpan <= lim && valid_block(lo, a.num_blocks) &&
-                    valid_block(hi, a.num_blocks);
+                    valid_block(hi, a.num_blocks) &&
+                    (!kWin || span >= win.lo || span + kSpan <= win.sinks);
+  auto live = [&](int t) { return t < lim && (!kWin || t >= win.lo || t < win.sinks); };
   others([&](const NewToken& t) { patch_k(r, span, t, g, j); });
   int blk = -1;
   if constexpr (kPatch) {
@@ -313,7 +335,7 @@ __device__ __forceinline__ void attend_span(const AttnArgs& a, Span& r, const v8
     // Tokens past the context and tokens of an invalid block id take no part.
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      if (!blk_ok || tv + e >= lim) sc[e] = -INFINITY;
+      if (!blk_ok || !live(tv + e)) sc[e] = -INFINITY;
   }
   float mx = vmax(vmax(vmax(sc[0], sc[1]), vmax(sc[2], sc[3])),
                   vmax(vmax(sc[4], sc[5]), vmax(sc[6], sc[7])));
@@ -356,8 +378,8 @@ __device__ __forceinline__ void attend_span(const AttnArgs& a, Span& r, const v8
     uint32_t mk[4];
 #pragma unroll
     for (int w = 0; w < 4; ++w)
-      mk[w] = (blk_ok && tv + 2 * w < lim ? 0x0000ffffu : 0u) |
-              (blk_ok && tv + 2 * w + 1 < lim ? 0xffff0000u : 0u);
+      mk[w] = (blk_ok && live(tv + 2 * w) ? 0x0000ffffu : 0u) |
+              (blk_ok && live(tv + 2 * w + 1) ? 0xffff0000u : 0u);
 #pragma unroll
     for (int n = 0; n < kNV; ++n)
 #pragma unroll
@@ -427,13 +449,14 @@ __device__ __forceinline__ void attend_span(const AttnArgs& a, Span& r, const v8
 // wavefront became a wait for nearly all of its loads.
 constexpr int kAppend = 8;
 
-template <int kRope, int kNV, bool kAct = false, bool kKnt = false>
+// kWin: a sliding window with sinks (struct Window; window, sinks arguments).
+template <int kRope, int kNV, bool kAct = false, bool kKnt = false, bool kWin = false>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void decode_attn_kernel(
     const void* src, const uint16_t* ck, const uint16_t* cv, const int32_t* tables,
     const int32_t* ctx_lens, uint32_t hgw, uint32_t mb_b, int num_blocks, uint32_t st_ns,
     float scale_log2, uint16_t* out, float* ws_ml, float* ws_o, const float* inv_freq,
     uint16_t* ck_w, uint16_t* cv_w, const float* ssq, int n_ssq, float eps,
-    const uint16_t* k_new, const uint16_t* v_new) {
+    const uint16_t* k_new, const uint16_t* v_new, int window, int sinks) {
   constexpr bool kRot = kRope > 0 && kRope != kAppend;   // the fused RoPE
   constexpr bool kOthers = kRope == kAppend;
   const uint16_t* q = static_cast<const uint16_t*>(src);
@@ -553,8 +576,11 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   // that waiting for them never waits for the wavefront's K/V loads.
   typedef const __attribute__((address_space(4))) int32_t* ctable_t;
   const ctable_t ctab = (ctable_t)table;
-  auto ids = [&](int sa, int* id) {
-    const int sb = sa + stride;
+  Window win{};
+  if constexpr (kWin) win = window_of(ctx_raw, window, sinks);
+  auto token_of = [&](int v) { return kWin && v >= win.sink_end ? v + win.shift : v; };
+  auto ids = [&](int va, int* id) {
+    const int sa = token_of(va), sb = token_of(va + stride);
     id[0] = ctab[min(sa >> 4, mb)];
     id[1] = ctab[min((sa >> 4) + 1, mb)];
     id[2] = ctab[min(sb >> 4, mb)];
@@ -568,7 +594,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   }
   int id0[4];
   ids(sa0, id0);
-  asm volatile("" : "+s"(ctx_raw) : "s"(id0[0]), "s"(id0[1]), "s"(id0[2]), "s"(id0[3]));
+  if constexpr (!kWin)
+    asm volatile("" : "+s"(ctx_raw) : "s"(id0[0]), "s"(id0[1]), "s"(id0[2]), "s"(id0[3]));
   // The arguments past the preloaded ones (inv_freq, ssq) arrive with the
   // block ids; the row scale's loads and the frequencies go out after the
   // partial sums' and before any K/V load (a wavefront's loads complete in
@@ -578,8 +605,13 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     ifreq = inv_freq[lane];
   }
   const int ctx = min(ctx_raw, a.max_blocks * 16);
-  const int s_end = (split == a.nsplit - 1) ? ctx : min(ctx, s_begin + a.split_tokens);
+  // With a window, s_begin and s_end count in its sequence of spans (of a context
+  // past the table only the sinks may be left there).
+  const int n_seen = kWin ? max(ctx - win.shift, min(ctx, win.sink_end)) : ctx;
+  const int s_end = (split == a.nsplit - 1) ? n_seen : min(n_seen, s_begin + a.split_tokens);
+  const int lim = kWin ? ctx : s_end;            // tokens from here on take no part
   const int pos = ctx_raw - 1;                   // the new token (fused RoPE path)
+  const int vpos = kWin ? (pos < ctx ? pos - win.shift : INT_MAX) : pos;
   // Loads and waits. A wavefront's loads complete in order, and the compiler
   // waits for a register with a count of the loads issued after it, taken
   // over every path that reaches the wait. So no load of the span loop sits
@@ -679,7 +711,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     // unit's first workgroup (part 0), in the split that holds the position: issued now, behind every K/V load of the wavefront, the
     // stores complete while the loads' data arrives (the spans that hold the
     // token take its k and v from LDS, not from the cache).
-    if (part_id == 0 && wv == 0 && pos >= s_begin && pos < s_end) {
+    if (part_id == 0 && wv == 0 && vpos >= s_begin && vpos < s_end) {
       const int blk = ctab[min(pos >> 4, mb)];
       if (valid_block(blk, a.num_blocks)) {
         const int slot = pos & 15;
@@ -711,8 +743,9 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   // been used. The block ids of the next pair are read one pair ahead.
   auto use = [&](auto first_c, Span& r, int s, int lo, int hi) __attribute__((always_inline)) {
     if constexpr (kRope < 0) fold_span<kNV>(r, o);
-    else attend_span<(kRope > 0), kNV>(a, r, qv, s, lo, hi, s_end, g, j,
-                                       decltype(first_c)::value, m, lsum, o, nt, [](auto) {});
+    else attend_span<(kRope > 0), kWin, kNV>(a, r, qv, token_of(s), lo, hi, lim, g, j,
+                                             decltype(first_c)::value, m, lsum, o, nt, win,
+                                             [](auto) {});
   };
   // Spans sa and sa + stride with the span sa + 2 stride still to come: use
   // both and refill both (the second refill dead when sa + 3 stride has no
@@ -781,22 +814,23 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       }
     }
     if constexpr (kOthers) {
-      const bool own = lane == b && pos >= s_begin && pos < s_end &&
-                       ((pos - s_begin) / kSpan) % W == wv;
+      const bool own = lane == b && vpos >= s_begin && vpos < s_end &&
+                       ((vpos - s_begin) / kSpan) % W == wv;
       if (__builtin_expect(__any(met > (own ? 1 : 0)), 0)) {   // once more, with others' tokens
         m = -INFINITY;
         lsum = 0.f;
 #pragma unroll
         for (int n = 0; n < kNV; ++n) o[n] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
-        for (int sa = sa0; sa < s_end; sa += stride) {
+        for (int va = sa0; va < s_end; va += stride) {
+          const int sa = token_of(va);
           const int lo = ctab[min(sa >> 4, mb)], hi = ctab[min((sa >> 4) + 1, mb)];
           load_span<kNV, false, false>(a, h, sa, g, j, lo, hi, ra0);
           auto others = [&](auto f) __attribute__((always_inline)) {
 #pragma unroll 1
             for (int half = 0; half < 2; ++half) {
               uint64_t in = others_in_block(written, b, pos, sa + 16 * half, half ? hi : lo,
-                                            s_end, a.num_blocks);
+                                            lim, a.num_blocks);
 #pragma unroll 1
               for (; in; in &= in - 1) {
                 const int s = __builtin_ctzll(in);
@@ -806,7 +840,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
               }
             }
           };
-          attend_span<true, kNV>(a, ra0, qv, sa, lo, hi, s_end, g, j, false, m, lsum, o, nt, others);
+          attend_span<true, kWin, kNV>(a, ra0, qv, sa, lo, hi, lim, g, j, false, m, lsum, o, nt,
+                                       win, others);
         }
       }
     }
@@ -842,7 +877,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       }
     }
     __syncthreads();
-    for (int idx = threadIdx.x; idx < R * kDV; idx += 64 * kMaxWaves) {
+    const int rows = kWin ? min(R, G - r0) : R;  // any group with a window, else powers of two
+    for (int idx = threadIdx.x; idx < rows * kDV; idx += 64 * kMaxWaves) {
       const int row = idx / kDV, d = idx % kDV;
       const f32x4 ma = *reinterpret_cast<const f32x4*>(&sm_m[r0 + row][0]);
       const f32x4 mb = *reinterpret_cast<const f32x4*>(&sm_m[r0 + row][4]);
@@ -1019,7 +1055,7 @@ Plan plan_for(int B, int plan_B, int Hkv, int G, int max_ctx) {
   const int64_t units = (int64_t)B * Hkv * ns;
   const int vs = units * 2 <= kTargetWorkgroups ? 1 : 0;
   int qs = 0;
-  while ((2 << qs) <= G && (units << (vs + qs + 1)) <= kTargetWorkgroups) ++qs;
+  while (G % (2 << qs) == 0 && (units << (vs + qs + 1)) <= kTargetWorkgroups) ++qs;
   return {ns, split_tokens, qs, vs};
 }
 
@@ -1053,16 +1089,26 @@ struct RopeIn {
   const uint16_t* k_new = nullptr;   // pdk_decode_attn_append: the new token's rows
   const uint16_t* v_new = nullptr;
   bool act = false;              // out in the tiled activation layout (pdk::act_at)
+  int window = 0;                // > 0: a sliding window, with sinks
+  int sinks = 0;
 };
 
 // The kernel for a plan: V in halves or whole, and on the plain path and the
 // probe non-temporal K when the two V halves are K's only readers.
-template <int kRope, bool kAct>
+template <int kRope, bool kAct, bool kWin>
 auto attn_kernel_for(const Plan& p) {
   if constexpr (kRope <= 0 || kRope == kAppend) {
-    if (p.vsplit && p.qsplit == 0) return decode_attn_kernel<kRope, 4, kAct, true>;
+    if (p.vsplit && p.qsplit == 0) return decode_attn_kernel<kRope, 4, kAct, true, kWin>;
   }
-  return p.vsplit ? decode_attn_kernel<kRope, 4, kAct, false> : decode_attn_kernel<kRope, 8, kAct, false>;
+  return p.vsplit ? decode_attn_kernel<kRope, 4, kAct, false, kWin>
+                  : decode_attn_kernel<kRope, 8, kAct, false, kWin>;
+}
+
+// The longest sequence of spans that a window and its sinks leave of max_ctx
+// tokens (struct Window), which is what a launch is planned for.
+int window_span(int max_ctx, int window, int sinks) {
+  const int64_t n = round_up(sinks, kSpan) + (int64_t)window + kSpan - 1;
+  return (int)std::min<int64_t>(max_ctx, n);
 }
 
 int launch_attn(const uint16_t* q, const uint16_t* cache_k, const uint16_t* cache_v,
@@ -1079,7 +1125,12 @@ int launch_attn(const uint16_t* q, const uint16_t* cache_k, const uint16_t* cach
   PDK_REQUIRE(n_q_heads >= n_kv_heads && n_q_heads % n_kv_heads == 0,
               "n_q_heads=%d must be a multiple of n_kv_heads=%d", n_q_heads, n_kv_heads);
   const int G = n_q_heads / n_kv_heads;
-  if (G > kMaxG || (G & (G - 1)) != 0) {
+  const bool win = rope.window > 0;
+  if (win && G > kMaxG) {
+    pdk::set_error("GQA group %d above the supported %d", G, kMaxG);
+    return PDK_ENOTSUP;
+  }
+  if (!win && (G > kMaxG || (G & (G - 1)) != 0)) {
     pdk::set_error("GQA group %d not in {1,2,4,8,16}", G);
     return PDK_ENOTSUP;
   }
@@ -1091,6 +1142,16 @@ int launch_attn(const uint16_t* q, const uint16_t* cache_k, const uint16_t* cach
               "num_blocks must be >= 1 and max_blocks in [1, 65535]");
   PDK_REQUIRE(max_ctx >= 1 && max_ctx <= max_blocks * 16,
               "max_ctx=%d outside [1, max_blocks*16=%d]", max_ctx, max_blocks * 16);
+  PDK_REQUIRE(rope.sinks >= 0 && rope.sinks <= kMaxCtx, "sinks=%d outside [0, %d]", rope.sinks,
+              kMaxCtx);
+  if (win) {
+    max_ctx = window_span(max_ctx, rope.window, rope.sinks);
+    if (max_ctx > kMaxCtx) {
+      pdk::set_error("window=%d with sinks=%d reads %d tokens, above the supported %d",
+                     rope.window, rope.sinks, max_ctx, kMaxCtx);
+      return PDK_ENOTSUP;
+    }
+  }
   // The largest context the tests cover (and the header promises).
   if (max_ctx > kMaxCtx) {
     pdk::set_error("max_ctx=%d above the supported %d", max_ctx, kMaxCtx);
@@ -1134,32 +1195,44 @@ int launch_attn(const uint16_t* q, const uint16_t* cache_k, const uint16_t* cach
   const uint32_t st_ns = (uint32_t)p.split_tokens | ((uint32_t)p.nsplit << 16);
   const dim3 grid((uint32_t)n_wg), block(64 * kMaxWaves);
   const void* src = rope.part ? static_cast<const void*>(rope.part) : static_cast<const void*>(a.q);
-#define PDK_ATTN_LAUNCH(R, A)                                                                   \
+#define PDK_ATTN_LAUNCH(R, A, W)                                                                \
   do {                                                                                         \
-    const auto kern = attn_kernel_for<R, A>(p);                                                \
+    const auto kern = attn_kernel_for<R, A, W>(p);                                             \
     hipLaunchKernelGGL(kern, grid, block, lds, st, src, a.ck, a.cv, a.tables, a.ctx, hgw, mb_b, \
                        a.num_blocks, st_ns, a.scale_log2, a.out, a.ws_ml, a.ws_o,              \
                        rope.inv_freq, rope.ck_w, rope.cv_w, rope.ssq, rope.n_ssq, rope.eps,    \
-                       rope.k_new, rope.v_new);                                                \
+                       rope.k_new, rope.v_new, rope.window, rope.sinks);                       \
   } while (0)
   const int mode = rope.probe ? -1 : rope.part ? rope.splits : rope.k_new ? kAppend : 0;
-  if (rope.act) {
+  if (win) {
+    // The decoder's projection comes in one or two splits.
+    const bool act = rope.act;
     switch (mode) {
-      case 1: PDK_ATTN_LAUNCH(1, true); break;
-      case 2: PDK_ATTN_LAUNCH(2, true); break;
-      case 4: PDK_ATTN_LAUNCH(4, true); break;
+      case 0: PDK_ATTN_LAUNCH(0, false, true); break;
+      case kAppend: PDK_ATTN_LAUNCH(kAppend, false, true); break;
+      case 1: if (act) PDK_ATTN_LAUNCH(1, true, true); else PDK_ATTN_LAUNCH(1, false, true); break;
+      case 2: if (act) PDK_ATTN_LAUNCH(2, true, true); else PDK_ATTN_LAUNCH(2, false, true); break;
+      default:
+        pdk::set_error("splits must be 1 or 2 with a window (got %d)", rope.splits);
+        return PDK_EINVAL;
+    }
+  } else if (rope.act) {
+    switch (mode) {
+      case 1: PDK_ATTN_LAUNCH(1, true, false); break;
+      case 2: PDK_ATTN_LAUNCH(2, true, false); break;
+      case 4: PDK_ATTN_LAUNCH(4, true, false); break;
       default:
         pdk::set_error("splits must be 1, 2 or 4 (got %d)", rope.splits);
         return PDK_EINVAL;
     }
   } else {
     switch (mode) {
-      case -1: PDK_ATTN_LAUNCH(-1, false); break;
-      case 0: PDK_ATTN_LAUNCH(0, false); break;
-      case 1: PDK_ATTN_LAUNCH(1, false); break;
-      case 2: PDK_ATTN_LAUNCH(2, false); break;
-      case 4: PDK_ATTN_LAUNCH(4, false); break;
-      case kAppend: PDK_ATTN_LAUNCH(kAppend, false); break;
+      case -1: PDK_ATTN_LAUNCH(-1, false, false); break;
+      case 0: PDK_ATTN_LAUNCH(0, false, false); break;
+      case 1: PDK_ATTN_LAUNCH(1, false, false); break;
+      case 2: PDK_ATTN_LAUNCH(2, false, false); break;
+      case 4: PDK_ATTN_LAUNCH(4, false, false); break;
+      case kAppend: PDK_ATTN_LAUNCH(kAppend, false, false); break;
       default:
         pdk::set_error("splits must be 1, 2 or 4 (got %d)", rope.splits);
         return PDK_EINVAL;
@@ -1175,6 +1248,49 @@ int launch_attn(const uint16_t* q, const uint16_t* cache_k, const uint16_t* cach
     hipLaunchKernelGGL(merge_kernel<false>, dim3(B * n_q_heads), dim3(kD), 0, st, a.ws_ml,
                        a.ws_o, p.nsplit, out, n_q_heads);
   return pdk::check_launch("merge_kernel");
+}
+
+// pdk_cache_append and the attention, in one launch where that is no slower.
+int attn_append(const uint16_t* q, const uint16_t* k_new, const uint16_t* v_new, uint16_t* cache_k,
+                uint16_t* cache_v, int num_blocks, const int32_t* block_tables, int max_blocks,
+                const int32_t* ctx_lens, int max_ctx, int B, int n_q_heads, int n_kv_heads,
+                int head_dim, float scale, void* workspace, size_t workspace_bytes, uint16_t* out,
+                uintptr_t stream, int window, int sinks) {
+  // With several rounds of workgroups, each round's wait for the new rows costs
+  // more than the append's launch where it reads next to nothing, and again
+  // where the launch is a small part of the whole (us per layer in two launches
+  // and in one, 8 KV heads: B=64 ctx 64 11.6 and 12.6, 192 17.3 and 16.7, 512 31.0
+  // and 29.8, 900 46.4 and 47.3, 2048 92.7 and 90.5; B=56 ctx 700 34.7 and 35.2,
+  // 1500 60.8 and 62.1; B=40 ctx 700 30.2 and 29.1, 1500 52.6 and 52.3). More
+  // streams than a wavefront has lanes, and rows that the output overwrites (the
+  // append has read them before the attention writes), take two launches as well.
+  const int64_t row = (int64_t)n_kv_heads * head_dim, pairs = (int64_t)B * n_kv_heads;
+  const int span = window > 0 ? window_span(max_ctx, window, sinks) : max_ctx;
+  auto overwritten = [&](const uint16_t* rows) {
+    return std::less<const uint16_t*>()(rows, out + (int64_t)B * n_q_heads * head_dim) &&
+           std::less<const uint16_t*>()(out, rows + B * row);
+  };
+  const bool rounds = pairs > kTargetWorkgroups &&
+                      (span <= 128 || (pairs > 352 && span > 640 && span <= 1536));
+  if (B > kMaxShared || rounds || overwritten(k_new) || overwritten(v_new)) {
+    if (int rc = pdk_cache_append(k_new, v_new, cache_k, cache_v, num_blocks, block_tables,
+                                  max_blocks, ctx_lens, B, n_kv_heads, head_dim, stream))
+      return rc;
+    RopeIn in{nullptr, 0, nullptr, nullptr, nullptr};
+    in.window = window;
+    in.sinks = sinks;
+    return launch_attn(q, cache_k, cache_v, num_blocks, block_tables, max_blocks, ctx_lens,
+                       max_ctx, B, n_q_heads, n_kv_heads, head_dim, scale, workspace,
+                       workspace_bytes, out, stream, in, B);
+  }
+  RopeIn in{nullptr, 0, nullptr, cache_k, cache_v};
+  in.k_new = k_new;
+  in.v_new = v_new;
+  in.window = window;
+  in.sinks = sinks;
+  return launch_attn(q, cache_k, cache_v, num_blocks, block_tables, max_blocks, ctx_lens, max_ctx,
+                     B, n_q_heads, n_kv_heads, head_dim, scale, workspace, workspace_bytes, out,
+                     stream, in, B);
 }
 
 }  // namespace
@@ -1200,35 +1316,66 @@ extern "C" int pdk_decode_attn_append(const uint16_t* q, const uint16_t* k_new,
   pdk::clear_error();
   PDK_REQUIRE(q && k_new && v_new, "null pointer argument");
   PDK_REQUIRE(pdk::aligned16(k_new) && pdk::aligned16(v_new), "k_new/v_new must be 16-byte aligned");
-  // With several rounds of workgroups, each round's wait for the new rows costs
-  // more than the append's launch where it reads next to nothing, and again
-  // where the launch is a small part of the whole (us per layer in two launches
-  // and in one, 8 KV heads: B=64 ctx 64 11.6 and 12.6, 192 17.3 and 16.7, 512 31.0
-  // and 29.8, 900 46.4 and 47.3, 2048 92.7 and 90.5; B=56 ctx 700 34.7 and 35.2,
-  // 1500 60.8 and 62.1; B=40 ctx 700 30.2 and 29.1, 1500 52.6 and 52.3). More
-  // streams than a wavefront has lanes, and rows that the output overwrites (the
-  // append has read them before the attention writes), take two launches as well.
-  const int64_t row = (int64_t)n_kv_heads * head_dim, pairs = (int64_t)B * n_kv_heads;
-  auto overwritten = [&](const uint16_t* rows) {
-    return std::less<const uint16_t*>()(rows, out + (int64_t)B * n_q_heads * head_dim) &&
-           std::less<const uint16_t*>()(out, rows + B * row);
-  };
-  const bool rounds = pairs > kTargetWorkgroups &&
-                      (max_ctx <= 128 || (pairs > 352 && max_ctx > 640 && max_ctx <= 1536));
-  if (B > kMaxShared || rounds || overwritten(k_new) || overwritten(v_new)) {
-    if (int rc = pdk_cache_append(k_new, v_new, cache_k, cache_v, num_blocks, block_tables,
-                                  max_blocks, ctx_lens, B, n_kv_heads, head_dim, stream))
-      return rc;
-    return pdk_decode_attn(q, cache_k, cache_v, num_blocks, block_tables, max_blocks, ctx_lens,
-                           max_ctx, B, n_q_heads, n_kv_heads, head_dim, scale, workspace,
-                           workspace_bytes, out, stream);
+  return attn_append(q, k_new, v_new, cache_k, cache_v, num_blocks, block_tables, max_blocks,
+                     ctx_lens, max_ctx, B, n_q_heads, n_kv_heads, head_dim, scale, workspace,
+                     workspace_bytes, out, stream, 0, 0);
+}
+
+extern "C" int pdk_decode_attn_window(const uint16_t* q, const uint16_t* k_new,
+                                      const uint16_t* v_new, uint16_t* cache_k, uint16_t* cache_v,
+                                      int num_blocks, const int32_t* block_tables, int max_blocks,
+                                      const int32_t* ctx_lens, int max_ctx, int window, int sinks,
+                                      int B, int n_q_heads, int n_kv_heads, int head_dim,
+                                      float scale, void* workspace, size_t workspace_bytes,
+                                      uint16_t* out, uintptr_t stream) {
+  pdk::clear_error();
+  PDK_REQUIRE(q, "null pointer argument");
+  PDK_REQUIRE(!k_new == !v_new, "k_new and v_new come together or not at all");
+  PDK_REQUIRE(window >= 1 && sinks >= 0, "window must be >= 1 and sinks >= 0 (got %d, %d)", window,
+              sinks);
+  if (k_new) {
+    PDK_REQUIRE(pdk::aligned16(k_new) && pdk::aligned16(v_new),
+                "k_new/v_new must be 16-byte aligned");
+    return attn_append(q, k_new, v_new, cache_k, cache_v, num_blocks, block_tables, max_blocks,
+                       ctx_lens, max_ctx, B, n_q_heads, n_kv_heads, head_dim, scale, workspace,
+                       workspace_bytes, out, stream, window, sinks);
   }
-  RopeIn in{nullptr, 0, nullptr, cache_k, cache_v};
-  in.k_new = k_new;
-  in.v_new = v_new;
+  RopeIn in{nullptr, 0, nullptr, nullptr, nullptr};
+  in.window = window;
+  in.sinks = sinks;
   return launch_attn(q, cache_k, cache_v, num_blocks, block_tables, max_blocks, ctx_lens, max_ctx,
                      B, n_q_heads, n_kv_heads, head_dim, scale, workspace, workspace_bytes, out,
                      stream, in, B);
+}
+
+extern "C" int pdk_decode_attn_rope_window(const float* qkv_partials, int splits,
+                                           const float* inv_freq, uint16_t* cache_k,
+                                           uint16_t* cache_v, int num_blocks,
+                                           const int32_t* block_tables, int max_blocks,
+                                           const int32_t* ctx_lens, int max_ctx, int window,
+                                           int sinks, int B, int n_q_heads, int n_kv_heads,
+                                           int head_dim, float scale, void* workspace,
+                                           size_t workspace_bytes, uint16_t* out, int out_tiled,
+                                           int plan_batch, uintptr_t stream) {
+  pdk::clear_error();
+  PDK_REQUIRE(qkv_partials && inv_freq, "null pointer argument");
+  PDK_REQUIRE(window >= 1 && sinks >= 0, "window must be >= 1 and sinks >= 0 (got %d, %d)", window,
+              sinks);
+  PDK_REQUIRE(splits == 1 || splits == 2, "splits must be 1 or 2 with a window (got %d)", splits);
+  PDK_REQUIRE(!out_tiled || (int64_t)n_q_heads * head_dim % 128 == 0,
+              "tiled activations need n_q_heads * head_dim %% 128 == 0");
+  RopeIn rope{qkv_partials, splits, inv_freq, cache_k, cache_v};
+  rope.act = out_tiled != 0;
+  rope.window = window;
+  rope.sinks = sinks;
+  return launch_attn(nullptr, cache_k, cache_v, num_blocks, block_tables, max_blocks, ctx_lens,
+                     max_ctx, B, n_q_heads, n_kv_heads, head_dim, scale, workspace,
+                     workspace_bytes, out, stream, rope, plan_batch > 0 ? plan_batch : B);
+}
+
+extern "C" int pdk_decode_attn_window_span(int max_ctx, int window, int sinks) {
+  if (max_ctx < 1 || window < 1 || sinks < 0 || sinks > kMaxCtx) return 0;
+  return window_span(max_ctx, window, sinks);
 }
 
 extern "C" int pdk_decode_attn_noalloc(const uint16_t* q, const uint16_t* cache_k,

@@ -1,0 +1,99 @@
+// Whole blocks of the paged KV cache copied inside it, gfx950: what sharing a
+// prompt between requests (its last, partly filled block), compacting the cache
+// and beam search's reordering move.
+//
+// One launch copies every pair's K and V block in all layers. The pairs lie in
+// host memory (block tables are the host's) and travel as kernel arguments, so a
+// call needs no device array, no copy to the device and no synchronisation, and
+// a captured graph holds them.
+//
+// Bound by HBM: each byte is read and written once.
+#include <algorithm>
+#include <new>
+#include <vector>
+
+#include "pdk_common.h"
+
+namespace {
+
+constexpr int kPairs = 448;               // per launch: 3.5 KiB of the 4 KiB of arguments
+constexpr int kUnits = 4;                 // 16-byte loads in flight per lane
+constexpr int kChunk = 256 * kUnits;      // 16-byte units of one workgroup
+
+struct Pairs {
+  int32_t src[kPairs], dst[kPairs];
+};
+
+// grid: x = chunk of a block, y = 2 * layer + (0 for K, 1 for V), z = pair.
+__global__ __launch_bounds__(256) void copy_blocks_kernel(uint16_t* ck, uint16_t* cv,
+                                                          int64_t layer_stride, int block_units,
+                                                          Pairs p) {
+  uint16_t* base = (blockIdx.y & 1 ? cv : ck) + (int64_t)(blockIdx.y >> 1) * layer_stride;
+  const int64_t block = (int64_t)block_units * 8;
+  const uint16_t* from = base + p.src[blockIdx.z] * block;
+  uint16_t* to = base + p.dst[blockIdx.z] * block;
+  const int u0 = blockIdx.x * kChunk + threadIdx.x;
+  pdk::v8 r[kUnits];
+#pragma unroll
+  for (int i = 0; i < kUnits; ++i)
+    if (u0 + 256 * i < block_units) r[i] = pdk::ld16(from + (int64_t)(u0 + 256 * i) * 8);
+#pragma unroll
+  for (int i = 0; i < kUnits; ++i)
+    if (u0 + 256 * i < block_units) pdk::st16(to + (int64_t)(u0 + 256 * i) * 8, r[i]);
+}
+
+// PDK_OK if the pairs' ids are blocks of the cache, no block is written twice
+// and none is both read and written, so that the copies' order does not matter.
+int check_pairs(const int32_t* src, const int32_t* dst, int n, int num_blocks) {
+  std::vector<uint64_t> written((num_blocks + 63) / 64, 0);
+  auto bit = [](int32_t id) { return 1ull << (id & 63); };
+  for (int i = 0; i < n; ++i) {
+    PDK_REQUIRE(src[i] >= 0 && src[i] < num_blocks && dst[i] >= 0 && dst[i] < num_blocks,
+                "pair %d: block %d -> %d outside [0, %d)", i, src[i], dst[i], num_blocks);
+    PDK_REQUIRE(!(written[dst[i] >> 6] & bit(dst[i])), "block %d is the destination of two pairs",
+                dst[i]);
+    written[dst[i] >> 6] |= bit(dst[i]);
+  }
+  for (int i = 0; i < n; ++i)
+    PDK_REQUIRE(!(written[src[i] >> 6] & bit(src[i])), "block %d is both a source and a destination",
+                src[i]);
+  return PDK_OK;
+}
+
+}  // namespace
+
+extern "C" int pdk_copy_blocks(uint16_t* cache_k, uint16_t* cache_v, int64_t cache_layer_stride,
+                               int n_layers, int num_blocks, int n_kv_heads, int head_dim,
+                               const int32_t* src, const int32_t* dst, int n, uintptr_t stream) {
+  pdk::clear_error();
+  PDK_REQUIRE(n >= 0, "n must be >= 0 (got %d)", n);
+  PDK_REQUIRE(cache_k && cache_v && (n == 0 || (src && dst)), "null pointer argument");
+  PDK_REQUIRE(pdk::aligned16(cache_k) && pdk::aligned16(cache_v), "caches must be 16-byte aligned");
+  PDK_REQUIRE(n_layers >= 1 && n_layers <= 32767 && num_blocks >= 1, "n_layers or num_blocks out of range");
+  PDK_REQUIRE(n_kv_heads >= 1 && n_kv_heads <= 65535 && head_dim >= 1 && head_dim <= 4096,
+              "n_kv_heads or head_dim out of range");
+  const int64_t block = (int64_t)n_kv_heads * PDK_BLOCK_SIZE * head_dim;
+  PDK_REQUIRE(cache_layer_stride % 8 == 0 &&
+                  (n_layers == 1 || cache_layer_stride >= (int64_t)num_blocks * block),
+              "the layer stride must be a multiple of 8 and hold num_blocks blocks");
+  try {
+    if (int rc = check_pairs(src, dst, n, num_blocks)) return rc;
+  } catch (const std::bad_alloc&) {
+    pdk::set_error("no host memory to check %d blocks", num_blocks);
+    return PDK_ENOMEM;
+  }
+  const int units = (int)(block / 8);
+  for (int at = 0; at < n; at += kPairs) {
+    Pairs p;
+    const int m = std::min(n - at, kPairs);
+    std::copy(src + at, src + at + m, p.src);
+    std::copy(dst + at, dst + at + m, p.dst);
+    std::fill(p.src + m, p.src + kPairs, 0);
+    std::fill(p.dst + m, p.dst + kPairs, 0);
+    hipLaunchKernelGGL(copy_blocks_kernel, dim3((units + kChunk - 1) / kChunk, 2 * n_layers, m),
+                       dim3(256), 0, pdk::as_stream(stream), cache_k, cache_v, cache_layer_stride,
+                       units, p);
+    if (int rc = pdk::check_launch("copy_blocks_kernel")) return rc;
+  }
+  return PDK_OK;
+}

@@ -7,7 +7,8 @@ softmax_dsl (kernels/dsl_batch.py:73-86) and greedy_tokens
 import torch
 
 from .. import _lib
-from .handoff import _need, stream_handle
+from .handoff import _need, launch_scope, need_device, stream_handle
+from .prefill import check_window
 
 BF16 = torch.bfloat16
 
@@ -47,9 +48,11 @@ def _check_layer_cache(cache_k, cache_v):
     return nb, H, D
 
 
-def _attention_call(q, cache_k, cache_v, block_tables, ctx_lens, max_ctx, out, workspace):
+def _attention_call(q, cache_k, cache_v, block_tables, ctx_lens, max_ctx, out, workspace,
+                    span=None):
     """Checked operands of one attention call: (geometry, workspace pointer and
-    bytes, out)."""
+    bytes, out). ``span``: the tokens read at most, under a window; such a call's
+    workspace is its own where none is given."""
     _need(q, "q")
     nb, H, D = _check_layer_cache(cache_k, cache_v)
     if q.dim() != 3 or q.shape[2] != D or not q.is_contiguous():
@@ -63,13 +66,15 @@ def _attention_call(q, cache_k, cache_v, block_tables, ctx_lens, max_ctx, out, w
         raise ValueError("ctx_lens must hold B entries")
     if out is None:
         out = torch.empty_like(q)
-    need = workspace_bytes(B, Hq, max_ctx, D)
+    need = workspace_bytes(B, Hq, span or max_ctx, D)
     ws = None
     if need:
         if workspace is not None:
             if workspace.numel() * workspace.element_size() < need:
                 raise ValueError(f"workspace holds fewer than the {need} bytes needed")
             ws = workspace
+        elif span is not None:
+            ws = torch.empty(need, dtype=torch.uint8, device=q.device)
         else:
             ws = get_workspace(need, q.device)
     ws_ptr = ws.data_ptr() if ws is not None else None
@@ -77,13 +82,80 @@ def _attention_call(q, cache_k, cache_v, block_tables, ctx_lens, max_ctx, out, w
     return (nb, B, Hq, H, D), ws_ptr, ws_bytes, out
 
 
+def window_span(max_ctx, window=None, sinks=0):
+    """The most tokens that a stream of up to ``max_ctx`` reads under a window with
+    sinks, in whole 32-token spans: workspace_bytes of it is what such a call
+    needs. max_ctx itself without a window."""
+    window, sinks = check_window(window, sinks)
+    if not window:
+        return max_ctx
+    n = int(_lib.lib().pdk_decode_attn_window_span(int(max_ctx), window, sinks))
+    if not n:
+        raise ValueError(f"max_ctx={max_ctx}, window={window}, sinks={sinks} out of range")
+    return n
+
+
+def _window_attention(q, new, cache_k, cache_v, block_tables, ctx_lens, max_ctx, scale, out,
+                      workspace, stream, window, sinks):
+    """decode_attention (new None) or decode_attention_append (new (k, v)) under a
+    window."""
+    if not isinstance(q, torch.Tensor) or not q.is_cuda:
+        raise TypeError("q must be a CUDA tensor")
+    with launch_scope(q.device, stream):
+        max_ctx = int(max_ctx)
+        if not 1 <= max_ctx <= block_tables.shape[-1] * 16:
+            raise ValueError(f"max_ctx={max_ctx} outside [1, {block_tables.shape[-1] * 16}]")
+        for t, name in ((cache_k, "cache_k"), (cache_v, "cache_v"),
+                        (block_tables, "block_tables"), (ctx_lens, "ctx_lens")):
+            need_device(q.device, t, name)
+        if not ctx_lens.is_contiguous():
+            raise ValueError("ctx_lens must be contiguous")
+        if out is not None:
+            _need(out, "out")
+            need_device(q.device, out, "out")
+            if out.shape != q.shape or not out.is_contiguous():
+                raise ValueError(f"out must be contiguous {tuple(q.shape)}")
+        if workspace is not None:
+            need_device(q.device, workspace, "workspace")
+        (nb, B, Hq, H, D), ws_ptr, ws_bytes, out = _attention_call(
+            q, cache_k, cache_v, block_tables, ctx_lens, max_ctx, out, workspace,
+            span=window_span(max_ctx, window, sinks))
+        window, sinks = check_window(window, sinks)
+        kp = vp = None
+        if new is not None:
+            k_new, v_new = new
+            _need(k_new, "k_new")
+            _need(v_new, "v_new")
+            need_device(q.device, k_new, "k_new")
+            need_device(q.device, v_new, "v_new")
+            if tuple(k_new.shape) != (B, H, D) or tuple(v_new.shape) != (B, H, D):
+                raise ValueError("k_new/v_new must be [B, Hkv, D]")
+            # Rows of other strides, or off 16 bytes, are copied.
+            k_new, v_new = (t if t.is_contiguous() and t.data_ptr() % 16 == 0 else
+                            t.clone(memory_format=torch.contiguous_format) for t in new)
+            kp, vp = k_new.data_ptr(), v_new.data_ptr()
+        _lib.call("pdk_decode_attn_window", q.data_ptr(), kp, vp, cache_k.data_ptr(),
+                  cache_v.data_ptr(), nb, block_tables.data_ptr(), block_tables.shape[1],
+                  ctx_lens.data_ptr(), max_ctx, window, sinks, B, Hq, H, D, float(scale), ws_ptr,
+                  ws_bytes, out.data_ptr(), stream_handle(stream))
+        return out
+
+
 def decode_attention(q, cache_k, cache_v, block_tables, ctx_lens, max_ctx, scale=1.0,
-                     out=None, workspace=None, stream=None):
+                     out=None, workspace=None, stream=None, window=None, sinks=0):
     """GQA decode attention for one layer.
 
     q [B, Hq, D] bf16 (query head h reads KV head h // (Hq/Hkv)); cache_k
     [nb, Hkv, 16, D] (tiled K blocks), cache_v [nb, Hkv, D, 16]; block_tables int32 [B, max_blocks]
-    and ctx_lens int32 [B] on the device; ``max_ctx`` >= every ctx_lens[b]."""
+    and ctx_lens int32 [B] on the device; ``max_ctx`` >= every ctx_lens[b].
+
+    With ``window`` stream b sees only its last ``window`` tokens and the first
+    ``sinks``: no block between them is read (its table entry may be -1), contexts
+    may be as long as the table, and any Hq/Hkv up to 16 is taken. Without
+    ``workspace`` such a call allocates its own."""
+    if window is not None or sinks:
+        return _window_attention(q, None, cache_k, cache_v, block_tables, ctx_lens, max_ctx, scale,
+                                 out, workspace, stream, window, sinks)
     (nb, B, Hq, H, D), ws_ptr, ws_bytes, out = _attention_call(
         q, cache_k, cache_v, block_tables, ctx_lens, max_ctx, out, workspace)
     _lib.call("pdk_decode_attn", q.data_ptr(), cache_k.data_ptr(), cache_v.data_ptr(), nb,
@@ -93,11 +165,15 @@ def decode_attention(q, cache_k, cache_v, block_tables, ctx_lens, max_ctx, scale
 
 
 def decode_attention_append(q, k_new, v_new, cache_k, cache_v, block_tables, ctx_lens, max_ctx,
-                            scale=1.0, out=None, workspace=None, stream=None):
+                            scale=1.0, out=None, workspace=None, stream=None, window=None, sinks=0):
     """cache_append(k_new, v_new) then decode_attention, in one launch where the
     kernel takes it (head_dim 128, 16-byte aligned rows, up to 64 streams), with
     the same results bit for bit, also where streams' tables share the blocks
-    that the new tokens go to. k_new, v_new bf16 [B, Hkv, D]."""
+    that the new tokens go to. k_new, v_new bf16 [B, Hkv, D]. ``window`` and
+    ``sinks`` as decode_attention's."""
+    if window is not None or sinks:
+        return _window_attention(q, (k_new, v_new), cache_k, cache_v, block_tables, ctx_lens,
+                                 max_ctx, scale, out, workspace, stream, window, sinks)
     _need(k_new, "k_new")
     _need(v_new, "v_new")
     nb, H, D = _check_layer_cache(cache_k, cache_v)

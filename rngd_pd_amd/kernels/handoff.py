@@ -12,6 +12,7 @@ Shapes (bf16 CUDA tensors):
                units of 8 dims of one token, ordered for the attention's QK reads);
                engines.paged_cache.k_block_rows converts a block to token rows.
 """
+import contextlib
 import ctypes
 
 import torch
@@ -37,6 +38,45 @@ def stream_handle(stream=None):
     if isinstance(stream, int):
         return stream
     return stream.cuda_stream
+
+
+_AS_IT_IS = contextlib.nullcontext()
+
+
+class _Scope:
+    """A device made current and, with one, a stream."""
+
+    def __init__(self, device, stream):
+        self.device, self.stream = torch.cuda.device(device), stream
+
+    def __enter__(self):
+        self.device.__enter__()
+        self.on = None
+        if self.stream is not None:
+            st = self.stream
+            if isinstance(st, int):
+                st = torch.cuda.ExternalStream(st)
+            self.on = torch.cuda.stream(st)
+            self.on.__enter__()
+
+    def __exit__(self, *exc):
+        if self.on is not None:
+            self.on.__exit__(*exc)
+        self.device.__exit__(*exc)
+
+
+def launch_scope(device, stream=None):
+    """The context of a call that works on tensors of ``device``: what it launches
+    and allocates belongs to that device and to ``stream`` (a torch stream or a
+    handle; None: that device's current stream), whatever is current outside."""
+    if stream is None and device.index == _current_device():
+        return _AS_IT_IS
+    return _Scope(device, stream)
+
+
+def need_device(device, t, name):
+    if t.device != device:
+        raise ValueError(f"{name} must be on {device}, is on {t.device}")
 
 
 def _need(t, name, dtype=BF16):

@@ -1,0 +1,77 @@
+"""torch-facing wrapper of the prompt's attention."""
+import torch
+
+from .. import _lib
+from .handoff import BF16, _need, launch_scope, need_device, stream_handle
+
+HEAD_DIM = 128
+
+
+def check_window(window, sinks):
+    """(window, sinks) as the C entry points take them; window None or a positive
+    int (as long as any context beyond 2^30), sinks only with a window."""
+    if window is None:
+        if sinks:
+            raise ValueError("sinks need a window")
+        return 0, 0
+    window, sinks = int(window), int(sinks)
+    if window < 1 or not 0 <= sinks < 1 << 31:
+        raise ValueError(f"window must be >= 1 and sinks in [0, 2^31), got {window}, {sinks}")
+    return min(window, 1 << 30), sinks
+
+
+def _rows(t, T):
+    """t [T, heads, 128] with contiguous [heads, 128], 16-byte aligned rows, and
+    its token stride; a copy where it is laid out otherwise."""
+    heads, D = t.shape[1:]
+    ld = t.stride(0) if T > 1 else heads * D
+    if t.stride(2) != 1 or (heads > 1 and t.stride(1) != D) or ld < heads * D or ld % 8 \
+            or t.data_ptr() % 16:
+        t, ld = t.clone(memory_format=torch.contiguous_format), heads * D
+    return t, ld
+
+
+def prefill_attention(q, k, v, scale=1.0, window=None, sinks=0, out=None, stream=None):
+    """Causal GQA attention over one prompt of T tokens -> out [T, Hq, 128] bf16.
+
+    q [T, Hq, 128], k and v [T, Hkv, 128] bf16, after RoPE (query head h reads KV
+    head h // (Hq/Hkv)); columns of one projection's tensor are taken as they lie,
+    other layouts than contiguous [heads, 128] rows are copied first. With
+    ``window`` the query at position p sees the tokens t <= p with t > p - window
+    or t < ``sinks``."""
+    if not isinstance(q, torch.Tensor) or not q.is_cuda:
+        raise TypeError("q must be a CUDA tensor")
+    with launch_scope(q.device, stream):
+        window, sinks = check_window(window, sinks)
+        for t, name in ((q, "q"), (k, "k"), (v, "v")):
+            _need(t, name)
+            need_device(q.device, t, name)
+            if t.dim() != 3 or t.shape[0] != q.shape[0]:
+                raise ValueError(f"{name} must be [T, heads, {HEAD_DIM}], got {tuple(t.shape)}")
+        T, Hq, D = q.shape
+        Hkv = k.shape[1]
+        if k.shape != v.shape or k.shape[2] != D:
+            raise ValueError("k and v must be [T, Hkv, D] with q's head_dim")
+        if out is None:
+            out = torch.empty((T, Hq, D), dtype=BF16, device=q.device)
+        else:
+            _need(out, "out")
+            need_device(q.device, out, "out")
+            if out.shape != q.shape or not out.is_contiguous() or out.data_ptr() % 16:
+                raise ValueError(f"out must be contiguous and 16-byte aligned {tuple(q.shape)}")
+        if T == 0:
+            return out
+        st = stream_handle(stream)
+        (q, q_ld), (k, k_ld), (v, v_ld) = _rows(q, T), _rows(k, T), _rows(v, T)
+        n = int(_lib.lib().pdk_prefill_kv_tile_elems(T, Hkv))
+        tiles = torch.empty(2 * n, dtype=BF16, device=q.device)
+        kt, vt = tiles.data_ptr(), tiles.data_ptr() + 2 * n
+        _lib.call("pdk_prefill_kv_tiles", k.data_ptr(), k_ld, v.data_ptr(), v_ld, T, Hkv, D, kt, vt,
+                  st)
+        if window:
+            _lib.call("pdk_prefill_attn_window", q.data_ptr(), q_ld, kt, vt, T, Hq, Hkv, D,
+                      float(scale), window, sinks, out.data_ptr(), st)
+        else:
+            _lib.call("pdk_prefill_attn", q.data_ptr(), q_ld, kt, vt, T, Hq, Hkv, D, float(scale),
+                      out.data_ptr(), st)
+        return out
