@@ -832,21 +832,17 @@ int pdk_prefill_attn(const uint16_t* q, int64_t q_tok_stride, const uint16_t* kt
                      const uint16_t* vt, int T, int n_q_heads, int n_kv_heads,
                      int head_dim, float scale, uint16_t* out, uintptr_t stream);
 
-/* pdk_prefill_attn under a sliding window with sinks: the query at position p
- * sees the tokens t <= p with t > p - window or t < sinks (window >= 1, sinks >=
- * 0). */
+/* Causal GQA attention of the prompt under a sliding window with sinks, from rows:
+ * q [T] rows of [Hq][128], k and v [T] rows of [Hkv][128] after RoPE (token
+ * strides in elements, multiples of 8), out [T][Hq][128]. The query at position p
+ * sees the tokens t <= p with t > p - window or t < sinks; a window of T or more
+ * is plain causal attention. A weight is rounded to bf16 once. */
 int pdk_prefill_attn_window(const uint16_t* q, int64_t q_tok_stride,
-                            const uint16_t* kt, const uint16_t* vt, int T,
+                            const uint16_t* k, int64_t k_tok_stride,
+                            const uint16_t* v, int64_t v_tok_stride, int T,
                             int n_q_heads, int n_kv_heads, int head_dim,
                             float scale, int window, int sinks, uint16_t* out,
                             uintptr_t stream);
-
-/* kt and vt from k and v as rows ([T] rows of [Hkv][128], token strides in
- * elements, multiples of 8), for keys that pdk_prefill_rope_kv did not rotate. */
-int pdk_prefill_kv_tiles(const uint16_t* k, int64_t k_tok_stride,
-                         const uint16_t* v, int64_t v_tok_stride, int T,
-                         int n_kv_heads, int head_dim, uint16_t* kt, uint16_t* vt,
-                         uintptr_t stream);
 
 /* ---- streams and events ------------------------------------------------------
  * Fences for the side-stream staging and for wait_for_save()

@@ -7,7 +7,7 @@ import sys
 _HERE = os.path.dirname(os.path.abspath(__file__))
 _ROOT = os.path.dirname(_HERE)
 SOURCES = ["handoff.hip", "attention.hip", "decode_step.hip", "wgemm.hip",
-           "wgemm_wide.hip", "prefill.hip", "prefill_gemm.hip", "pages.hip", "beam.hip", "koni.hip",
+           "wgemm_wide.hip", "prefill.hip", "prefill_gemm.hip", "prefill_window.hip", "pages.hip", "beam.hip", "koni.hip",
            "staging.hip", "runtime.hip"]
 OUT = os.path.join(_HERE, "librngdpd.so")
 NET_SOURCES = ["net/tcpkv.cpp"]
@@ -35,7 +35,7 @@ def hipcc_command(out=OUT):
 NO_SCRATCH = ("decode_attn_kernel", "merge_kernel", "pack_kernel", "scatter_kernel",
               "gather_kernel", "koni_scatter_kernel", "koni_gather_kernel",
               "rope_kv_kernel", "prefill_attn_kernel", "prefill_gemm_kernel",
-              "wgemm_wide_kernel", "wgemm_kernelILi3ELi2ELi8E", "kv_tiles_kernel",
+              "wgemm_wide_kernel", "wgemm_kernelILi3ELi2ELi8E", "prefill_window_kernel",
               "copy_blocks_kernel", "beam_part_kernel", "beam_join_kernel", "beam_reorder_kernel")
 
 

@@ -65,40 +65,6 @@ __global__ __launch_bounds__(256) void rope_table_kernel(const float* inv_freq, 
   table[idx] = make_float2(c, s);
 }
 
-// The tiles kt and vt of rope_kv_kernel from k and v as rows ([T] rows of
-// [NKV][128], token strides k_ld and v_ld): one workgroup per tile and KV head.
-// Bound by its bytes, each read and written once.
-__global__ __launch_bounds__(256) void kv_tiles_kernel(const uint16_t* k, int64_t k_ld,
-                                                       const uint16_t* v, int64_t v_ld, int T,
-                                                       uint16_t* kt, uint16_t* vt) {
-  __shared__ uint16_t vs[kTile][kD + 2];
-  const int tile = blockIdx.x, n_tiles = gridDim.x, h = blockIdx.y;
-  const int64_t at = ((int64_t)h * n_tiles + tile) * kTileElems;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int r = (threadIdx.x >> 4) + 16 * i, o = threadIdx.x & 15;   // token, dims 8o .. + 7
-    const int t = tile * kTile + r;
-    const int64_t d = h * kD + 8 * o;
-    const v8 x = t < T ? pdk::ld16(k + (int64_t)t * k_ld + d) : pdk::zero8();
-    const v8 y = t < T ? pdk::ld16(v + (int64_t)t * v_ld + d) : pdk::zero8();
-    pdk::st16(kt + at + ((o >> 1) * 64 + (o & 1) * 32 + pi(r)) * 8, x);
-#pragma unroll
-    for (int w = 0; w < 4; ++w) *reinterpret_cast<uint32_t*>(&vs[r][8 * o + 2 * w]) = y.w[w];
-  }
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int u = threadIdx.x + 256 * i;           // unit (n, ks, lane)
-    const int lane = u & 63, ks = (u >> 6) & 1, n = u >> 7;
-    const int d = 32 * n + (lane & 31), t0 = 16 * ks + 8 * (lane >> 5);
-    v8 g;
-#pragma unroll
-    for (int w = 0; w < 4; ++w)
-      g.w[w] = (uint32_t)vs[t0 + 2 * w][d] | ((uint32_t)vs[t0 + 2 * w + 1][d] << 16);
-    pdk::st16(vt + at + u * 8, g);
-  }
-}
-
 // Eight elements of `splits` partial rows, added in order and rounded to bf16.
 __device__ __forceinline__ v8 partial_sum(const float* p, int splits, int64_t stride) {
   float s[8];
@@ -260,13 +226,9 @@ __global__ __launch_bounds__(256) void rope_kv_kernel(uint16_t* qkv, const float
 // 1024 cycles of matrix work against 16 KiB of LDS reads and the softmax of 16
 // scores per lane; two workgroups per CU overlap one's softmax with the
 // other's products.
-//
-// kWin: a sliding window with sinks. The workgroup walks the sinks' tiles, then
-// those from its first query's window on.
-template <bool kWin>
 __global__ __launch_bounds__(64 * kAttnWaves, 2) void prefill_attn_kernel(
     const uint16_t* q, int64_t q_ld, const uint16_t* kt, const uint16_t* vt, int T, int NH,
-    int NKV, float c, uint16_t* out, int window, int sinks) {
+    int NKV, float c, uint16_t* out) {
   __shared__ __align__(16) uint16_t smem[2][2 * kTileElems];   // [buffer][K tile, V tile]
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int j = lane & 31, hh = lane >> 5;
@@ -278,17 +240,6 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void prefill_attn_kernel(
   const int qt = unit / G, head = kvh * G + (unit - qt * G);
   // K/V tiles the workgroup walks: up to its last unit's query tile.
   const int n_kv = min(wg * kAttnWaves + kAttnWaves - 1, units - 1) / G + 1;
-  // With a window: tile number i of those the workgroup walks is i below `lead`,
-  // i + skip from there on.
-  int lead = 0, skip = 0;
-  if constexpr (kWin) {
-    const int q_first = min(wg * kAttnWaves, units - 1) / G * kTile;
-    const int w_tile = max(q_first - window + 1, 0) / kTile;
-    lead = min((sinks + kTile - 1) / kTile, w_tile);
-    skip = w_tile - lead;
-  }
-  const int n_walk = n_kv - skip;
-  auto tile_at = [&](int i) { return kWin && i >= lead ? i + skip : i; };
 
   v8 qv[8];
   {
@@ -322,14 +273,13 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void prefill_attn_kernel(
     for (int i = 0; i < 16; ++i) o[n][i] = 0.f;
   float m = -INFINITY, l = 0.f;           // m: raw-score maximum in use; l: this lane's tokens
 
-  fetch(tile_at(0));
+  fetch(0);
   stash(0);
   __syncthreads();
-  for (int i_tile = 0; i_tile < n_walk; ++i_tile) {
-    const int buf = i_tile & 1, tile = tile_at(i_tile);
-    if (i_tile + 1 < n_walk) fetch(tile_at(i_tile + 1));
-    const bool in_window = tile * kTile + kTile - 1 > qt * kTile - window || tile * kTile < sinks;
-    if (tile <= qt && (!kWin || in_window)) {   // uniform across the wavefront
+  for (int tile = 0; tile < n_kv; ++tile) {
+    const int buf = tile & 1;
+    if (tile + 1 < n_kv) fetch(tile + 1);
+    if (tile <= qt) {                     // uniform across the wavefront
       const uint16_t* ks_ = &smem[buf][lane * 8];
       const uint16_t* vs_ = &smem[buf][kTileElems + lane * 8];
       f32x16 s;
@@ -341,16 +291,6 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void prefill_attn_kernel(
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           if (16 * (i >> 3) + 8 * hh + (i & 7) > j) s[i] = -INFINITY;
-      }
-      if constexpr (kWin) {               // tokens that have left some query's window
-        if (tile * kTile <= qt * kTile + kTile - 1 - window && tile * kTile + kTile > sinks) {
-          const int p = qt * kTile + j;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int t = tile * kTile + 16 * (i >> 3) + 8 * hh + (i & 7);
-            if (t <= p - window && t >= sinks) s[i] = -INFINITY;
-          }
-        }
       }
       float mx = s[0];
 #pragma unroll
@@ -403,7 +343,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void prefill_attn_kernel(
           o[n] = mfma32(va, p0[k], o[n]);
         }
     }
-    if (i_tile + 1 < n_walk) stash(buf ^ 1);  // last read before the previous barrier
+    if (tile + 1 < n_kv) stash(buf ^ 1);  // last read before the previous barrier
     __syncthreads();
   }
   {
@@ -507,11 +447,10 @@ extern "C" int pdk_prefill_rope_kv_partials(const float* partials, int splits, c
                        k_tok_stride, v_out, v_tok_stride, kt, vt, stream);
 }
 
-namespace {
-
-int prefill_attn(const uint16_t* q, int64_t q_tok_stride, const uint16_t* kt, const uint16_t* vt,
-                 int T, int n_q_heads, int n_kv_heads, int head_dim, float scale, uint16_t* out,
-                 uintptr_t stream, int window, int sinks) {
+extern "C" int pdk_prefill_attn(const uint16_t* q, int64_t q_tok_stride, const uint16_t* kt,
+                                const uint16_t* vt, int T, int n_q_heads, int n_kv_heads,
+                                int head_dim, float scale, uint16_t* out, uintptr_t stream) {
+  pdk::clear_error();
   if (head_dim != kD) {
     pdk::set_error("the prefill kernels implement head_dim %d only (got %d)", kD, head_dim);
     return PDK_ENOTSUP;
@@ -527,51 +466,8 @@ int prefill_attn(const uint16_t* q, int64_t q_tok_stride, const uint16_t* kt, co
   const int64_t units = (int64_t)((T + kTile - 1) / kTile) * (n_q_heads / n_kv_heads);
   const int64_t blocks = (units + kAttnWaves - 1) / kAttnWaves * n_kv_heads;
   PDK_REQUIRE(units < (1ll << 30) && blocks < (1ll << 31), "launch too large");
-  const auto kern = window > 0 ? prefill_attn_kernel<true> : prefill_attn_kernel<false>;
-  hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(64 * kAttnWaves), 0,
+  hipLaunchKernelGGL(prefill_attn_kernel, dim3((unsigned)blocks), dim3(64 * kAttnWaves), 0,
                      pdk::as_stream(stream), q, q_tok_stride, kt, vt, T, n_q_heads, n_kv_heads,
-                     scale * 1.4426950408889634f, out, window, sinks);
+                     scale * 1.4426950408889634f, out);
   return pdk::check_launch("prefill_attn_kernel");
-}
-
-}  // namespace
-
-extern "C" int pdk_prefill_attn(const uint16_t* q, int64_t q_tok_stride, const uint16_t* kt,
-                                const uint16_t* vt, int T, int n_q_heads, int n_kv_heads,
-                                int head_dim, float scale, uint16_t* out, uintptr_t stream) {
-  pdk::clear_error();
-  return prefill_attn(q, q_tok_stride, kt, vt, T, n_q_heads, n_kv_heads, head_dim, scale, out,
-                      stream, 0, 0);
-}
-
-extern "C" int pdk_prefill_attn_window(const uint16_t* q, int64_t q_tok_stride, const uint16_t* kt,
-                                       const uint16_t* vt, int T, int n_q_heads, int n_kv_heads,
-                                       int head_dim, float scale, int window, int sinks,
-                                       uint16_t* out, uintptr_t stream) {
-  pdk::clear_error();
-  PDK_REQUIRE(window >= 1 && sinks >= 0, "window must be >= 1 and sinks >= 0 (got %d, %d)", window,
-              sinks);
-  // Beyond T neither hides anything.
-  return prefill_attn(q, q_tok_stride, kt, vt, T, n_q_heads, n_kv_heads, head_dim, scale, out,
-                      stream, std::min(window, std::max(T, 1)), std::min(sinks, std::max(T, 1)));
-}
-
-extern "C" int pdk_prefill_kv_tiles(const uint16_t* k, int64_t k_tok_stride, const uint16_t* v,
-                                    int64_t v_tok_stride, int T, int n_kv_heads, int head_dim,
-                                    uint16_t* kt, uint16_t* vt, uintptr_t stream) {
-  pdk::clear_error();
-  if (head_dim != kD) {
-    pdk::set_error("the prefill kernels implement head_dim %d only (got %d)", kD, head_dim);
-    return PDK_ENOTSUP;
-  }
-  if (int rc = check_prefill(T, n_kv_heads, n_kv_heads)) return rc;
-  PDK_REQUIRE(k && v && kt && vt, "null pointer argument");
-  PDK_REQUIRE(pdk::aligned16(k) && pdk::aligned16(v) && pdk::aligned16(kt) && pdk::aligned16(vt),
-              "tensors must be 16-byte aligned");
-  PDK_REQUIRE(k_tok_stride >= (int64_t)n_kv_heads * kD && k_tok_stride % 8 == 0 &&
-                  v_tok_stride >= (int64_t)n_kv_heads * kD && v_tok_stride % 8 == 0,
-              "token strides must be multiples of 8 and hold Hkv * D elements");
-  hipLaunchKernelGGL(kv_tiles_kernel, dim3((T + kTile - 1) / kTile, n_kv_heads), dim3(256), 0,
-                     pdk::as_stream(stream), k, k_tok_stride, v, v_tok_stride, T, kt, vt);
-  return pdk::check_launch("kv_tiles_kernel");
 }

@@ -26,7 +26,7 @@ def _rows(t, T):
     heads, D = t.shape[1:]
     ld = t.stride(0) if T > 1 else heads * D
     if t.stride(2) != 1 or (heads > 1 and t.stride(1) != D) or ld < heads * D or ld % 8 \
-            or t.data_ptr() % 16:
+            or ld >= 1 << 24 or t.data_ptr() % 16:
         t, ld = t.clone(memory_format=torch.contiguous_format), heads * D
     return t, ld
 
@@ -63,15 +63,6 @@ def prefill_attention(q, k, v, scale=1.0, window=None, sinks=0, out=None, stream
             return out
         st = stream_handle(stream)
         (q, q_ld), (k, k_ld), (v, v_ld) = _rows(q, T), _rows(k, T), _rows(v, T)
-        n = int(_lib.lib().pdk_prefill_kv_tile_elems(T, Hkv))
-        tiles = torch.empty(2 * n, dtype=BF16, device=q.device)
-        kt, vt = tiles.data_ptr(), tiles.data_ptr() + 2 * n
-        _lib.call("pdk_prefill_kv_tiles", k.data_ptr(), k_ld, v.data_ptr(), v_ld, T, Hkv, D, kt, vt,
-                  st)
-        if window:
-            _lib.call("pdk_prefill_attn_window", q.data_ptr(), q_ld, kt, vt, T, Hq, Hkv, D,
-                      float(scale), window, sinks, out.data_ptr(), st)
-        else:
-            _lib.call("pdk_prefill_attn", q.data_ptr(), q_ld, kt, vt, T, Hq, Hkv, D, float(scale),
-                      out.data_ptr(), st)
+        _lib.call("pdk_prefill_attn_window", q.data_ptr(), q_ld, k.data_ptr(), k_ld, v.data_ptr(),
+                  v_ld, T, Hq, Hkv, D, float(scale), window or T, sinks, out.data_ptr(), st)
         return out

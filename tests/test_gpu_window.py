@@ -324,6 +324,28 @@ def test_prompt_large_scores(cuda):
     assert_within(K.prefill_attention(q, k, v, scale=SCALE, window=100, sinks=4), want, bound)
 
 
+@pytest.mark.parametrize("window,sinks", [(40, 4), (300, 0)])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+def test_prompt_hidden_values_reach_no_query(cuda, window, sinks, value):
+    """NaN or infinity in k and v of token t spoils the queries that see it and no
+    other, those of its own tile among them."""
+    from rngd_pd_amd import kernels as K
+    rng = np.random.default_rng(17)
+    T, Hq, Hkv, at = 230, 8, 2, [101, 117]
+    q = to_dev(rand_bf16(rng, (T, Hq, D)))
+    k, v = (to_dev(rand_bf16(rng, (T, Hkv, D))) for _ in range(2))
+    want, bound = _prompt_reference(q, k, v, window, sinks, SCALE)
+    k[at[0]], v[at[1]] = value, value
+    got = K.prefill_attention(q, k, v, scale=SCALE, window=window, sinks=sinks)
+    t = torch.arange(T, device=cuda)
+    clean = torch.ones(T, dtype=torch.bool, device=cuda)
+    for a in at:
+        clean &= (t < a) | (t - a >= window)
+    assert 0 < int(clean.sum()) < T
+    assert_within(got[clean], want[clean], bound[clean])
+    assert not torch.isfinite(got[at[1]]).any()
+
+
 def test_refusals(cuda):
     from rngd_pd_amd import kernels as K
     from rngd_pd_amd._lib import PdkError

@@ -68,8 +68,9 @@ def test_window_span():
 def test_prefill_window_refusals():
     lib = _lib.lib()
 
-    def call(T=64, hq=32, hkv=8, d=128, window=8, sinks=0, scale=1.0, ld=4096, q=P):
-        return lib.pdk_prefill_attn_window(q, ld, P, P, T, hq, hkv, d, scale, window, sinks, P, 0)
+    def call(T=64, hq=32, hkv=8, d=128, window=8, sinks=0, scale=1.0, ld=4096, q=P, k_ld=1024):
+        return lib.pdk_prefill_attn_window(q, ld, P, k_ld, P, 1024, T, hq, hkv, d, scale, window, sinks,
+                                           P, 0)
     assert call(window=0) == _lib.PDK_EINVAL and "window" in _lib.last_error()
     assert call(sinks=-1) == _lib.PDK_EINVAL
     assert call(T=0) == _lib.PDK_EINVAL
@@ -78,12 +79,8 @@ def test_prefill_window_refusals():
     assert call(ld=4097) == _lib.PDK_EINVAL and call(ld=4088) == _lib.PDK_EINVAL
     assert call(scale=-1.0) == _lib.PDK_EINVAL
     assert call(q=P + 8) == _lib.PDK_EINVAL
-
-    def tiles(T=64, hkv=8, d=128, k=P, k_ld=1024):
-        return lib.pdk_prefill_kv_tiles(k, k_ld, P, 1024, T, hkv, d, P, P, 0)
-    assert tiles(T=0) == _lib.PDK_EINVAL and tiles(d=32) == _lib.PDK_ENOTSUP
-    assert tiles(k=None) == _lib.PDK_EINVAL and tiles(k_ld=1020) == _lib.PDK_EINVAL
-    assert tiles(hkv=0) == _lib.PDK_EINVAL
+    assert call(k_ld=1020) == _lib.PDK_EINVAL and call(k_ld=1016) == _lib.PDK_EINVAL
+    assert call(hkv=0) == _lib.PDK_EINVAL and call(q=None) == _lib.PDK_EINVAL
 
 
 def test_copy_blocks_refusals():
