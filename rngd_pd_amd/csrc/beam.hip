@@ -5,20 +5,22 @@
 // Selection. total(k, v) = score_k + logit_kv - log sum_v exp(logit_kv) over the
 // K beams of a request and the vocabulary; the n largest, the lower beam and then
 // the lower token first among equals. Inside a beam the order of the totals is
-// that of the logits, so the vocabulary is read once: a workgroup takes a part of
-// a row, and leaves its maximum, its sum of exponentials and its n best tokens;
-// one workgroup per request joins the parts.
+// that of the logits, so the vocabulary is read once: a wavefront takes a part of
+// a row into registers and leaves its maximum, its sum of exponentials and its n
+// best tokens; one workgroup per request joins the parts.
 //
 // The sums and totals are 64-bit: which of two beams' tokens comes first hangs on
 // their difference, and 32 bits of a sum over a vocabulary of 1e5 leave 1e-6 of a
 // total undecided, which a search over a thousand candidates a step does meet.
-// exp is a degree-9 polynomial (below 1e-11), a dozen full-rate operations.
 //
-// n best of 64 lanes' values: values are made unique integer keys (the value in
-// an order-preserving code above the complement of the token). The n-th largest
-// of the lanes' own maxima bounds the n-th largest key from below, and only n
-// lanes hold keys above that bound, so at most n times a lane's values are
-// compacted into LDS and ranked there by counting, whatever the logits are.
+// n best of a wavefront's values: the n-th largest of the 64 lanes' own maxima
+// bounds the n-th largest value from below, bit by bit with one ballot each until
+// exactly n lanes reach it (some 10 to 15 bits). Mostly a few more than n values
+// then reach the bound; they are compacted into LDS and ranked by counting. Where
+// equal values let more than 64 reach it, the bound is taken again over unique
+// 64-bit keys (the value in an order-preserving code above the complement of the
+// token): only n lanes reach that one, so at most n times a lane's values do,
+// whatever the logits are.
 #include <math.h>
 
 #include <algorithm>
@@ -31,11 +33,9 @@ using pdk::v8;
 
 constexpr int kMaxBeams = 16;
 constexpr int kMaxOut = 32;
-constexpr int kWaves = 4;                 // of a part's workgroup
-constexpr int kLaneVals = 16;             // values a lane holds
-constexpr int kPartVals = 64 * kWaves * kLaneVals;   // 4096 values of a row per workgroup
-constexpr int kMaxLists = 4;              // parts' lists a lane of the join looks at
-constexpr int kMaxParts = 64 * kMaxLists;
+constexpr int kWaves = 4;                 // of a part workgroup, each a part of its own
+constexpr int kMaxLists = 8;              // parts of a row per lane of the join
+constexpr int kMaxVocab = 1 << 20;
 
 typedef unsigned long long Key;
 
@@ -55,24 +55,25 @@ __device__ __forceinline__ Key key_of(float x, uint32_t token) {
   return c ? ((Key)c << 32) | (0xffffffffu - token) : 0ull;
 }
 
-// e^x for x <= 0 (0 below -700): 2^k p(f), x = (k + f) ln 2, |f| <= 1/2, p the
-// Taylor polynomial of 2^f to degree 9, off by (ln 2 / 2)^10 / 10! = 7e-12.
-__device__ __forceinline__ double exp_neg(double x) {
-  const double y = fmax(x, -700.0) * 1.4426950408889634074;
-  const double k = rint(y);
-  const double f = (y - k) * 0.69314718055994530942;
-  double p = 1.0 / 362880.0;
-  p = fma(p, f, 1.0 / 40320.0);
-  p = fma(p, f, 1.0 / 5040.0);
-  p = fma(p, f, 1.0 / 720.0);
-  p = fma(p, f, 1.0 / 120.0);
-  p = fma(p, f, 1.0 / 24.0);
-  p = fma(p, f, 1.0 / 6.0);
-  p = fma(p, f, 0.5);
-  p = fma(p, f, 1.0);
-  p = fma(p, f, 1.0);
-  return x < -700.0 ? 0.0 : ldexp(p, (int)k);
+// 2^y for y <= 0: 2^k p(f), y = k + f, |f| <= 1/2, p the polynomial of degree 7
+// that meets 2^f at the 8 Chebyshev nodes (off by less than 6e-11 of it). Down to
+// y = -1000; the callers clamp.
+__device__ __forceinline__ double exp2_neg(double y) {
+  const double k = rint(y), f = y - k;
+  double p = 1.5303701161442145e-05;
+  p = fma(p, f, 0.00015469729221575116);
+  p = fma(p, f, 0.0013333478471058548);
+  p = fma(p, f, 0.009618025613268967);
+  p = fma(p, f, 0.055504109063307244);
+  p = fma(p, f, 0.24022651213498578);
+  p = fma(p, f, 0.6931471805568296);
+  p = fma(p, f, 0.9999999999595621);
+  return __builtin_amdgcn_ldexp(p, (int)k);
 }
+
+constexpr double kLog2e = 1.4426950408889634074;
+
+__device__ __forceinline__ double exp_neg(double x) { return exp2_neg(fmax(x, -690.0) * kLog2e); }
 
 __device__ __forceinline__ double wave_sum(double x) {
 #pragma unroll
@@ -80,32 +81,21 @@ __device__ __forceinline__ double wave_sum(double x) {
   return x;
 }
 
-// The n-th largest of the wavefront's 64 keys (0 if fewer than n are not 0):
-// bit by bit from the top, the largest bound that n lanes reach.
-__device__ __forceinline__ Key nth_largest(Key mine, int n) {
-  Key bound = 0;
+// The n-th largest of the wavefront's 64 values (0 if no more than n are not 0),
+// or a lower bound that no more of them reach: bit by bit from the top, the
+// largest bound that n lanes reach.
+template <typename U>
+__device__ __forceinline__ U nth_largest(U mine, int n) {
+  if (__popcll(__ballot(mine != 0)) <= n) return 0;
+  U bound = 0;
 #pragma unroll 1
-  for (int bit = 63; bit >= 0; --bit) {
-    const Key t = bound | (1ull << bit);
+  for (int bit = 8 * sizeof(U) - 1; bit >= 0; --bit) {
+    const U t = bound | ((U)1 << bit);
     const int c = __popcll(__ballot(mine >= t));
     if (c >= n) bound = t;
     if (c == n) break;
   }
   return bound;
-}
-
-// The keys >= bound of the wavefront's lanes, compacted into list; how many.
-template <int kN>
-__device__ __forceinline__ int compact(const Key (&keys)[kN], Key bound, Key* list) {
-  int at = 0;
-#pragma unroll
-  for (int i = 0; i < kN; ++i) {
-    const bool in = keys[i] >= bound;
-    const uint64_t who = __ballot(in);
-    if (in) list[at + __popcll(who & ((1ull << (threadIdx.x & 63)) - 1))] = keys[i];
-    at += __popcll(who);
-  }
-  return at;
 }
 
 // What the wavefront's lanes wrote to LDS is there for all of them.
@@ -115,18 +105,28 @@ __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
+__device__ __forceinline__ Key lane_key(Key k, int lane) {
+  return ((Key)__builtin_amdgcn_readlane((uint32_t)(k >> 32), lane) << 32) |
+         (uint32_t)__builtin_amdgcn_readlane((uint32_t)k, lane);
+}
+
 // The largest n of list[0..c) in order to best[0..n), zeros behind them.
 __device__ __forceinline__ void rank(const Key* list, int c, Key* best, int n) {
   const int lane = threadIdx.x & 63;
-  if (lane < n) best[lane] = 0;
-  wave_sync();
+  if (c <= 64) {
+    const Key mine = lane < c ? list[lane] : 0;
+    int r = 0;
+    for (int j = 0; j < c; ++j) r += lane_key(mine, j) > mine;
+    if (lane < c && r < n) best[r] = mine;
+    if (lane >= c && lane < n) best[lane] = 0;
+    return;
+  }
   for (int i = lane; i < c; i += 64) {
     const Key mine = list[i];
     int r = 0;
     for (int j = 0; j < c; ++j) r += list[j] > mine;
     if (r < n) best[r] = mine;
   }
-  wave_sync();
 }
 
 // What a part leaves: its maximum and its sum of e^(x - maximum) (NaN where the
@@ -139,7 +139,7 @@ struct Part {
 // start anywhere: the 16-byte loads take any address, and a row's parts and sums
 // do not depend on where it lies (equal rows have equal totals).
 template <typename T>
-__device__ __forceinline__ void load_vals(const T* row, int64_t e, int64_t V, float* x) {
+__device__ __forceinline__ void load_vals(const T* row, int e, int V, float* x) {
   constexpr int kEl = 16 / sizeof(T);
   if (e + kEl <= V) {
     uint32_t w[4];
@@ -165,74 +165,79 @@ __device__ __forceinline__ void load_vals(const T* row, int64_t e, int64_t V, fl
   }
 }
 
-// grid: x = part, y = row. T is uint16_t (bf16) or float.
-template <typename T>
+// grid: x = kWaves parts, y = row. T is uint16_t (bf16) or float; a lane holds
+// kVals values.
+template <typename T, int kVals>
 __global__ __launch_bounds__(64 * kWaves) void beam_part_kernel(const T* logits, int64_t ld, int V,
-                                                                int n, const int32_t* last_tokens,
+                                                                int n, int n_parts,
+                                                                const int32_t* last_tokens,
                                                                 int eos, Part* parts, Key* keys) {
-  constexpr int kEl = 16 / sizeof(T), kGroups = kLaneVals / kEl;
-  __shared__ Key list[kWaves][64 * kLaneVals / 2];   // n * kLaneVals <= 512 per wavefront
-  __shared__ Key best[kWaves][kMaxOut];
-  __shared__ float tops[kWaves];
-  __shared__ double sums[kWaves];
-  const int row = blockIdx.y, part = blockIdx.x, n_parts = gridDim.x;
+  constexpr int kEl = 16 / sizeof(T), kGroups = kVals / kEl;
+  __shared__ Key lists[kWaves][kMaxOut * kVals];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int row = blockIdx.y, part = blockIdx.x * kWaves + wave;
+  if (part >= n_parts) return;
   if (last_tokens && last_tokens[row] == eos) return;   // an ended beam's logits count for nothing
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const T* p = logits + (int64_t)row * ld;
-  float x[kLaneVals];
-  int64_t e[kGroups];
+  float x[kVals];
+  const int e0 = part * (64 * kVals) + lane * kEl;
 #pragma unroll
-  for (int i = 0; i < kGroups; ++i) {
-    e[i] = (int64_t)part * kPartVals + ((wave * kGroups + i) * 64 + lane) * kEl;
-    load_vals(p, e[i], V, x + i * kEl);
-  }
-  float top = x[0];
+  for (int i = 0; i < kGroups; ++i) load_vals(p, e0 + i * 64 * kEl, V, x + i * kEl);
+  float mine = x[0];
 #pragma unroll
-  for (int i = 1; i < kLaneVals; ++i) top = __builtin_elementwise_maximum(top, x[i]);
+  for (int i = 1; i < kVals; ++i) mine = __builtin_elementwise_maximum(mine, x[i]);
+  float top = mine;
 #pragma unroll
   for (int o = 32; o; o >>= 1) top = __builtin_elementwise_maximum(top, __shfl_xor(top, o));
-  if (lane == 0) tops[wave] = top;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) top = __builtin_elementwise_maximum(top, tops[w]);
   double sum = 0.0;
   if (top < INFINITY && top > -INFINITY) {
 #pragma unroll
-    for (int i = 0; i < kLaneVals; ++i) sum += exp_neg((double)x[i] - (double)top);
+    for (int i = 0; i < kVals; ++i) sum += exp_neg((double)x[i] - (double)top);
     sum = wave_sum(sum);
   } else if (!(top == -INFINITY)) {
     sum = NAN;
   }
-  if (lane == 0) sums[wave] = sum;
-
-  Key k[kLaneVals], mine = 0;
-#pragma unroll
-  for (int i = 0; i < kLaneVals; ++i) {
-    k[i] = key_of(x[i], (uint32_t)(e[i / kEl] + i % kEl));
-    mine = k[i] > mine ? k[i] : mine;
-  }
-  const Key bound = nth_largest(mine, n);
-  const int c = compact(k, bound ? bound : 1, list[wave]);
-  __syncthreads();
-  rank(list[wave], c, best[wave], n);
-  __syncthreads();
-  // The wavefronts' ordered lists become one.
   const int64_t at = (int64_t)row * n_parts + part;
-  if ((int)threadIdx.x < kWaves * n) {
-    const int w = threadIdx.x / n, i = threadIdx.x - w * n;
-    const Key m = best[w][i];
-    int r = i;
-    for (int o = 0; o < kWaves; ++o)
-      if (o != w)
-        for (int j = 0; j < n; ++j) r += best[o][j] > m || (m == 0 && best[o][j] == 0 && o < w);
-    if (r < n) keys[at * n + r] = m;
-  }
-  if (threadIdx.x == 0) {
-    double s = 0.0;
+  if (lane == 0) parts[at] = Part{(double)top, sum};
+
+  // The values that reach the bound; all but -inf where there are few enough.
+  Key* list = lists[wave];
+  const uint32_t bound = nth_largest(code_of(mine), n);
+  const float least = bound ? value_of(bound) : -3.402823466e38f;
+  auto token = [&](int i) { return (uint32_t)(e0 + (i / kEl) * 64 * kEl + i % kEl); };
+  int c = 0;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) s += sums[w];
-    parts[at] = Part{(double)top, s};
+  for (int i = 0; i < kVals; ++i) {
+    const bool in = x[i] >= least;
+    const uint64_t who = __ballot(in);
+    if (who == 0) continue;
+    const int to = c + __popcll(who & ((1ull << lane) - 1));
+    if (in && to < 64) list[to] = key_of(x[i], token(i));
+    c += __popcll(who);
   }
+  if (c > 64) {                                          // equal values
+    Key best = 0;
+#pragma unroll 1
+    for (int i = 0; i < kVals; ++i) {
+      Key k = 0;
+#pragma unroll
+      for (int j = 0; j < kVals; ++j)
+        if (j == i) k = key_of(x[j], token(j));
+      best = k > best ? k : best;
+    }
+    const Key b = nth_largest(best, n);
+    c = 0;
+#pragma unroll
+    for (int i = 0; i < kVals; ++i) {
+      const Key k = key_of(x[i], token(i));
+      const bool in = k >= (b ? b : 1);
+      const uint64_t who = __ballot(in);
+      if (in) list[c + __popcll(who & ((1ull << lane) - 1))] = k;
+      c += __popcll(who);
+    }
+  }
+  wave_sync();
+  rank(list, c, keys + at * n, n);
 }
 
 // One workgroup per request, one wavefront per beam: the beam's log sum, its n
@@ -241,71 +246,85 @@ __global__ __launch_bounds__(64 * kWaves) void beam_part_kernel(const T* logits,
 __global__ __launch_bounds__(64 * kMaxBeams) void beam_join_kernel(
     const Part* parts, const Key* keys, int n_parts, int n, const float* scores, int K,
     const int32_t* last_tokens, int eos, int32_t* tokens, int32_t* parents, float* out_scores) {
-  __shared__ Key list[kMaxBeams][kMaxOut * 8];
+  constexpr int kList = 256;                             // keys of a beam held at a time
+  __shared__ Key list[kMaxBeams][kList];
   __shared__ Key best[kMaxBeams][kMaxOut];
+  __shared__ uint16_t lists[kMaxBeams][kMaxOut * kMaxLists];
   __shared__ double totals[kMaxBeams][kMaxOut];
   __shared__ int32_t token[kMaxBeams][kMaxOut];
   __shared__ int found;
-  const int r = blockIdx.x, k = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int r = blockIdx.x, lane = threadIdx.x & 63;
+  const int k = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int row = r * K + k;
   const bool ended = last_tokens && last_tokens[row] == eos;
   const float score = scores[row];
   const bool alive = score > -INFINITY && score < INFINITY;
   if (threadIdx.x == 0) found = 0;
   if (!ended) {
-    // Heads of the parts' lists; only lists whose head reaches the n-th largest
-    // head hold any of the n best.
-    Key head[kMaxLists], mine = 0;
+    // Heads of the parts' lists; only lists whose head reaches the n-th largest of
+    // the lanes' own best heads hold any of the n best: those of at most n lanes.
+    const Key* kp = keys + (int64_t)row * n_parts * n;
+    const Part* pp = parts + (int64_t)row * n_parts;
+    Key mine = 0;
     double top = -INFINITY, sum = 0.0;
-#pragma unroll
-    for (int i = 0; i < kMaxLists; ++i) {
-      const int s = lane + 64 * i;
-      head[i] = 0;
-      if (s < n_parts) {
-        head[i] = keys[((int64_t)row * n_parts + s) * n];
-        const Part q = parts[(int64_t)row * n_parts + s];
-        // NaN in q.sum stays; a part without a finite value adds nothing.
-        if (q.sum != 0.0) {
-          const double m = fmax(top, q.top);
-          sum = sum * exp_neg(top - m) + q.sum * exp_neg(q.top - m);
-          top = m;
-        }
+    for (int s = lane; s < n_parts; s += 64) {
+      const Key head = kp[s * n];
+      const Part q = pp[s];
+      mine = head > mine ? head : mine;
+      // NaN in q.sum stays; a part without a finite value adds nothing.
+      if (q.sum != 0.0) {
+        const double m = fmax(top, q.top);
+        sum = sum * exp_neg(top - m) + q.sum * exp_neg(q.top - m);
+        top = m;
       }
-      mine = head[i] > mine ? head[i] : mine;
     }
     double all = top;
 #pragma unroll
     for (int o = 32; o; o >>= 1) all = fmax(all, __shfl_xor(all, o));
     sum = wave_sum(top > -INFINITY || sum != sum ? sum * exp_neg(top - all) : 0.0);
-    const double lse = all + log(sum);
-    const Key bound = nth_largest(mine, n);
+    const double log_sum = log(sum);                     // beside the maximum: it may be any size
+    const Key bound = nth_largest(mine, n), least = bound ? bound : 1;
+    int m = 0;                                           // lists that reach it
+    for (int s = lane; s - lane < n_parts; s += 64) {
+      const bool in = s < n_parts && kp[s * n] >= least;
+      const uint64_t who = __ballot(in);
+      if (in) lists[k][m + __popcll(who & ((1ull << lane) - 1))] = (uint16_t)s;
+      m += __popcll(who);
+    }
+    wave_sync();
     int c = 0;
+    for (int i0 = 0; i0 < m * n; i0 += 256) {            // four loads of a lane in flight
+      Key q[4];
 #pragma unroll
-    for (int i = 0; i < kMaxLists; ++i) {
-      // Lists that reach the bound, one after the other: their keys from the bound on.
-      const Key least = bound ? bound : 1;
-      for (uint64_t who = __ballot(head[i] >= least); who; who &= who - 1) {
-        const int s = __ffsll((long long)who) - 1 + 64 * i;
-        const Key q = lane < n ? keys[((int64_t)row * n_parts + s) * n + lane] : 0;
-        const uint64_t in = __ballot(q >= least);
-        const int m = __popcll(in);
-        if (c + m > kMaxOut * 8) {
-          // More than the list holds: keep the n best so far.
-          rank(list[k], c, best[k], n);
-          if (lane < n) list[k][lane] = best[k][lane];
+      for (int x = 0; x < 4; ++x) {
+        const int i = i0 + 64 * x + lane, which = i / n;
+        q[x] = i < m * n ? kp[(int)lists[k][which] * n + (i - which * n)] : 0;
+      }
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const bool in = q[x] >= least;
+        const uint64_t who = __ballot(in);
+        const int more = __popcll(who);
+        if (c + more > kList) {                          // keep the n best so far
           wave_sync();
-          c = min(c, n);
+          rank(list[k], c, best[k], n);
+          wave_sync();
+          if (lane < n) list[k][lane] = best[k][lane];
+          c = n;
         }
-        if (q >= least) list[k][c + lane] = q;          // the list is ordered: a prefix of lanes
-        c += m;
+        if (in) list[k][c + __popcll(who & ((1ull << lane) - 1))] = q[x];
+        c += more;
       }
     }
+    wave_sync();
     rank(list[k], c, best[k], n);
+    wave_sync();
     if (lane < n) {
       const Key b = best[k][lane];
-      const bool ok = b && alive && lse > -INFINITY && lse < INFINITY;
+      const bool ok = b && alive && log_sum > -INFINITY && log_sum < INFINITY;
       token[k][lane] = (int32_t)(0xffffffffu - (uint32_t)b);
-      totals[k][lane] = ok ? (double)score + ((double)value_of((uint32_t)(b >> 32)) - lse) : -INFINITY;
+      totals[k][lane] = ok ? (double)score + (((double)value_of((uint32_t)(b >> 32)) - all) - log_sum)
+                            : -INFINITY;
     }
   } else if (lane < n) {
     token[k][lane] = eos;
@@ -406,7 +425,17 @@ __global__ __launch_bounds__(256) void beam_reorder_kernel(const int32_t* parent
   }
 }
 
-int parts_of(int V) { return (V + kPartVals - 1) / kPartVals; }
+// Values of a lane: 32, or 16 where rows are too few for 32 to give every SIMD two
+// wavefronts.
+int lane_vals(int rows, int V) {
+  const bool many = (int64_t)rows * ((V + 2047) / 2048) >= 2048;
+  return many || V > kMaxVocab / 2 ? 32 : 16;
+}
+
+int parts_of(int rows, int V) {
+  const int part = 64 * lane_vals(rows, V);
+  return (V + part - 1) / part;
+}
 
 int check_select(int R, int K, int V, int n) {
   PDK_REQUIRE(R >= 1 && R <= 65535 / kMaxBeams, "R must be in [1, %d] (got %d)", 65535 / kMaxBeams, R);
@@ -416,8 +445,8 @@ int check_select(int R, int K, int V, int n) {
     return PDK_ENOTSUP;
   }
   PDK_REQUIRE(V >= 1, "V must be >= 1 (got %d)", V);
-  if (V > kMaxParts * kPartVals) {
-    pdk::set_error("a vocabulary of %d is above the supported %d", V, kMaxParts * kPartVals);
+  if (V > kMaxVocab) {
+    pdk::set_error("a vocabulary of %d is above the supported %d", V, kMaxVocab);
     return PDK_ENOTSUP;
   }
   return PDK_OK;
@@ -428,7 +457,7 @@ int check_select(int R, int K, int V, int n) {
 extern "C" int64_t pdk_beam_select_workspace_bytes(int R, int K, int V, int n) {
   pdk::clear_error();
   if (check_select(R, K, V, n)) return 0;
-  return (int64_t)R * K * parts_of(V) * (sizeof(Part) + n * sizeof(Key));
+  return (int64_t)R * K * parts_of(R * K, V) * (sizeof(Part) + n * sizeof(Key));
 }
 
 extern "C" int pdk_beam_select(const void* logits, int elem_bytes, int64_t ld, int R, int K, int V,
@@ -446,17 +475,23 @@ extern "C" int pdk_beam_select(const void* logits, int elem_bytes, int64_t ld, i
   PDK_REQUIRE(workspace && workspace_bytes >= need && pdk::aligned16(workspace),
               "workspace of %lld bytes needed (got %lld)", (long long)need,
               (long long)workspace_bytes);
-  const int rows = R * K, n_parts = parts_of(V);
+  const int rows = R * K, n_parts = parts_of(rows, V), vals = lane_vals(rows, V);
   Part* parts = static_cast<Part*>(workspace);
   Key* keys = reinterpret_cast<Key*>(parts + (int64_t)rows * n_parts);
-  const dim3 grid(n_parts, rows), block(64 * kWaves);
+  const dim3 grid((n_parts + kWaves - 1) / kWaves, rows), block(64 * kWaves);
   hipStream_t st = pdk::as_stream(stream);
-  if (elem_bytes == 2)
-    hipLaunchKernelGGL(beam_part_kernel<uint16_t>, grid, block, 0, st,
-                       static_cast<const uint16_t*>(logits), ld, V, n, last_tokens, eos, parts, keys);
-  else
-    hipLaunchKernelGGL(beam_part_kernel<float>, grid, block, 0, st,
-                       static_cast<const float*>(logits), ld, V, n, last_tokens, eos, parts, keys);
+  auto launch = [&](auto kern, auto x) {
+    hipLaunchKernelGGL(kern, grid, block, 0, st, x, ld, V, n, n_parts, last_tokens, eos, parts, keys);
+  };
+  const uint16_t* x16 = static_cast<const uint16_t*>(logits);
+  const float* x32 = static_cast<const float*>(logits);
+  if (elem_bytes == 2) {
+    if (vals == 32) launch(beam_part_kernel<uint16_t, 32>, x16);
+    else launch(beam_part_kernel<uint16_t, 16>, x16);
+  } else {
+    if (vals == 32) launch(beam_part_kernel<float, 32>, x32);
+    else launch(beam_part_kernel<float, 16>, x32);
+  }
   if (int rc = pdk::check_launch("beam_part_kernel")) return rc;
   hipLaunchKernelGGL(beam_join_kernel, dim3(R), dim3(64 * K), 0, st, parts, keys, n_parts, n,
                      scores, K, last_tokens, eos, tokens, parents, out_scores);

@@ -28,9 +28,11 @@ def select_reference(logits, scores, n, eos=None, last=None):
             row = x[r, k]
             if np.isnan(row).any() or not row.max() > -np.inf or row.max() == np.inf:
                 continue
-            lse = row.max() + math.log(math.fsum(np.exp(row - row.max())))
+            # The maximum apart from the sum's logarithm, which it would swallow
+            # where it is the type's lowest value.
+            log_sum = math.log(math.fsum(np.exp(row - row.max())))
             order = np.lexsort((np.arange(V), -row))[:n]
-            found += [(-(s[r, k] + (row[t] - lse)), k, -row[t], int(t)) for t in order
+            found += [(-(s[r, k] + ((row[t] - row.max()) - log_sum)), k, -row[t], int(t)) for t in order
                       if row[t] > -np.inf]
         found.sort()
         for i, (t, k, _, tok) in enumerate(found[:n]):
