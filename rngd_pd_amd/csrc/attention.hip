@@ -1044,9 +1044,18 @@ constexpr int kTargetWorkgroups = 256;
 // (1, 1) 6.99; B=4 (2, 0) 7.13, (1, 1) 6.17, (2, 1) 6.07.
 // The context split is chosen for plan_B streams (it orders the fp32 sums, so
 // a decoder keeps it fixed across steps), the sharing for the B launched.
-Plan plan_for(int B, int plan_B, int Hkv, int G, int max_ctx) {
+//
+// With a window (win; max_ctx the tokens it leaves to read) a launch is not split
+// up to 640 of them, or 1152 from 32 pairs on, and in splits of 512 above: us per
+// layer with the new token's write, 8 KV heads, one launch / splits of 512 / of
+// 128: B=1 window 512 8.4 / 9.6 / 8.9, 1024 10.9 / 10.1 / 9.9, 2048 14.8 / 10.4 /
+// 11.2, 4096 24.8 / 11.4 / 13.6; B=4 512 9.3 / 10.2 / 10.5, 1024 11.4 / 11.2 / 11.8;
+// B=8 512 10.1 / 11.3 / 11.8, 1024 12.4 / 13.8 / 13.3, 2048 17.4 / 17.6 / 17.5. (The
+// second launch also costs an eager caller's host some 3 us.)
+Plan plan_for(int B, int plan_B, int Hkv, int G, int max_ctx, bool win = false) {
   const int64_t pairs = (int64_t)plan_B * Hkv;
-  const int min_split = pairs >= 128 ? 2048 : pairs >= 32 ? 512 : 128;
+  int min_split = pairs >= 128 ? 2048 : pairs >= 32 ? 512 : 128;
+  if (win && pairs < 128) min_split = max_ctx <= (pairs >= 32 ? 1152 : 640) ? max_ctx : 512;
   int64_t nsplit = (kTargetWorkgroups + pairs - 1) / pairs;
   nsplit = std::min<int64_t>(nsplit, (max_ctx + min_split - 1) / min_split);
   nsplit = std::max<int64_t>(1, std::min<int64_t>(nsplit, kMaxSplits));
@@ -1160,7 +1169,7 @@ int launch_attn(const uint16_t* q, const uint16_t* cache_k, const uint16_t* cach
   PDK_REQUIRE(scale > 0.f && scale < INFINITY, "scale must be positive and finite (got %g)",
               (double)scale);
   PDK_REQUIRE(plan_B >= B && plan_B <= 65535, "plan_batch=%d must be in [B=%d, 65535]", plan_B, B);
-  const Plan p = plan_for(B, plan_B, n_kv_heads, G, max_ctx);
+  const Plan p = plan_for(B, plan_B, n_kv_heads, G, max_ctx, win);
   AttnArgs a{};
   a.q = q;
   a.ck = cache_k;

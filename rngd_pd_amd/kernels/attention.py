@@ -4,10 +4,12 @@ Replaces the attention slice of DecodeLayer.forward (kernels/decode_batch.py:81-
 softmax_dsl (kernels/dsl_batch.py:73-86) and greedy_tokens
 (engines/decode_batch.py:162-171) with HIP kernels over the paged cache.
 """
+import functools
+
 import torch
 
 from .. import _lib
-from .handoff import _need, launch_scope, need_device, stream_handle
+from .handoff import _current_device, _need, launch_scope, need_device, stream_handle
 from .prefill import check_window
 
 BF16 = torch.bfloat16
@@ -95,50 +97,103 @@ def window_span(max_ctx, window=None, sinks=0):
     return n
 
 
+@functools.lru_cache(maxsize=4096)
+def _window_plan(B, Hq, D, max_ctx, capacity, window, sinks):
+    """(window, sinks) as the C call takes them and the workspace's bytes."""
+    if not 1 <= max_ctx <= capacity:
+        raise ValueError(f"max_ctx={max_ctx} outside [1, {capacity}]")
+    span = window_span(max_ctx, window, sinks)
+    return (*check_window(window, sinks), workspace_bytes(B, Hq, span, D))
+
+
+def _check_window_operands(q, new, cache_k, cache_v, block_tables, ctx_lens, out, workspace):
+    """Raises for operands that _window_attention's own test did not pass."""
+    for t, name in ((cache_k, "cache_k"), (cache_v, "cache_v"), (block_tables, "block_tables"),
+                    (ctx_lens, "ctx_lens")):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a CUDA tensor")
+        need_device(q.device, t, name)
+    if not ctx_lens.is_contiguous():
+        raise ValueError("ctx_lens must be contiguous")
+    # Shapes and types; the workspace is another matter.
+    _attention_call(q, cache_k, cache_v, block_tables, ctx_lens, 1, q, None, span=1)
+    B, H, D = q.shape[0], cache_k.shape[1], q.shape[2]
+    for t, name in zip(new or (), ("k_new", "v_new")):
+        _need(t, name)
+        need_device(q.device, t, name)
+        if tuple(t.shape) != (B, H, D):
+            raise ValueError("k_new/v_new must be [B, Hkv, D]")
+    if out is not None:
+        _need(out, "out")
+        need_device(q.device, out, "out")
+        if out.shape != q.shape or not out.is_contiguous():
+            raise ValueError(f"out must be contiguous {tuple(q.shape)}")
+    if workspace is not None:
+        need_device(q.device, workspace, "workspace")
+        if not workspace.is_contiguous():
+            raise ValueError("workspace must be contiguous")
+
+
+def _rows16(t):
+    """t itself, or a copy where its rows are strided or off 16 bytes."""
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
 def _window_attention(q, new, cache_k, cache_v, block_tables, ctx_lens, max_ctx, scale, out,
                       workspace, stream, window, sinks):
     """decode_attention (new None) or decode_attention_append (new (k, v)) under a
     window."""
     if not isinstance(q, torch.Tensor) or not q.is_cuda:
         raise TypeError("q must be a CUDA tensor")
-    with launch_scope(q.device, stream):
-        max_ctx = int(max_ctx)
-        if not 1 <= max_ctx <= block_tables.shape[-1] * 16:
-            raise ValueError(f"max_ctx={max_ctx} outside [1, {block_tables.shape[-1] * 16}]")
-        for t, name in ((cache_k, "cache_k"), (cache_v, "cache_v"),
-                        (block_tables, "block_tables"), (ctx_lens, "ctx_lens")):
-            need_device(q.device, t, name)
-        if not ctx_lens.is_contiguous():
-            raise ValueError("ctx_lens must be contiguous")
-        if out is not None:
-            _need(out, "out")
-            need_device(q.device, out, "out")
-            if out.shape != q.shape or not out.is_contiguous():
-                raise ValueError(f"out must be contiguous {tuple(q.shape)}")
-        if workspace is not None:
-            need_device(q.device, workspace, "workspace")
-        (nb, B, Hq, H, D), ws_ptr, ws_bytes, out = _attention_call(
-            q, cache_k, cache_v, block_tables, ctx_lens, max_ctx, out, workspace,
-            span=window_span(max_ctx, window, sinks))
-        window, sinks = check_window(window, sinks)
-        kp = vp = None
-        if new is not None:
+    dev = q.device
+    if stream is not None or dev.index != _current_device():
+        with launch_scope(dev, stream):
+            return _window_attention(q, new, cache_k, cache_v, block_tables, ctx_lens, max_ctx,
+                                     scale, out, workspace, None, window, sinks)
+    # The usual operands pass one test; what does not is told apart.
+    try:
+        B, Hq, D = q.shape
+        nb, H, block, _ = cache_k.shape
+        fine = (q.dtype is BF16 and cache_k.dtype is BF16 and cache_v.dtype is BF16
+                and block_tables.dtype is torch.int32 and ctx_lens.dtype is torch.int32
+                and cache_k.device == dev and cache_v.device == dev
+                and block_tables.device == dev and ctx_lens.device == dev
+                and cache_k.shape == (nb, H, 16, D) and cache_v.shape == (nb, H, D, 16)
+                and block_tables.shape[0] == B and block_tables.dim() == 2
+                and ctx_lens.numel() == B and q.is_contiguous() and cache_k.is_contiguous()
+                and cache_v.is_contiguous() and block_tables.is_contiguous()
+                and ctx_lens.is_contiguous() and out is None and workspace is None)
+        if fine and new is not None:
             k_new, v_new = new
-            _need(k_new, "k_new")
-            _need(v_new, "v_new")
-            need_device(q.device, k_new, "k_new")
-            need_device(q.device, v_new, "v_new")
-            if tuple(k_new.shape) != (B, H, D) or tuple(v_new.shape) != (B, H, D):
-                raise ValueError("k_new/v_new must be [B, Hkv, D]")
-            # Rows of other strides, or off 16 bytes, are copied.
-            k_new, v_new = (t if t.is_contiguous() and t.data_ptr() % 16 == 0 else
-                            t.clone(memory_format=torch.contiguous_format) for t in new)
-            kp, vp = k_new.data_ptr(), v_new.data_ptr()
-        _lib.call("pdk_decode_attn_window", q.data_ptr(), kp, vp, cache_k.data_ptr(),
-                  cache_v.data_ptr(), nb, block_tables.data_ptr(), block_tables.shape[1],
-                  ctx_lens.data_ptr(), max_ctx, window, sinks, B, Hq, H, D, float(scale), ws_ptr,
-                  ws_bytes, out.data_ptr(), stream_handle(stream))
-        return out
+            fine = (k_new.dtype is BF16 and v_new.dtype is BF16 and k_new.device == dev
+                    and v_new.device == dev and k_new.shape == (B, H, D)
+                    and v_new.shape == (B, H, D))
+    except (AttributeError, TypeError, ValueError):
+        fine = False
+    if not fine:
+        _check_window_operands(q, new, cache_k, cache_v, block_tables, ctx_lens, out, workspace)
+    width = block_tables.shape[1]
+    window, sinks, need = _window_plan(B, Hq, D, int(max_ctx), width * 16, window, sinks)
+    if out is None:
+        out = torch.empty_like(q)
+    ws_ptr, ws_bytes = None, 0
+    if need:
+        if workspace is None:
+            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        ws_ptr, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        if ws_bytes < need:
+            raise ValueError(f"workspace holds fewer than the {need} bytes needed")
+    kp = vp = None
+    if new is not None:
+        k_new, v_new = _rows16(new[0]), _rows16(new[1])
+        kp, vp = k_new.data_ptr(), v_new.data_ptr()
+    _lib.call("pdk_decode_attn_window", q.data_ptr(), kp, vp, cache_k.data_ptr(),
+              cache_v.data_ptr(), nb, block_tables.data_ptr(), width, ctx_lens.data_ptr(),
+              int(max_ctx), window, sinks, B, Hq, H, D, scale, ws_ptr, ws_bytes, out.data_ptr(),
+              stream_handle())
+    return out
 
 
 def decode_attention(q, cache_k, cache_v, block_tables, ctx_lens, max_ctx, scale=1.0,

@@ -4,10 +4,12 @@ beams and vocabulary, and the cache's reordering after it.
 The reference decodes greedily (greedy_tokens, engines/decode_batch.py:162-171);
 these stand beside greedy_argmax.
 """
+import functools
+
 import torch
 
 from .. import _lib
-from .handoff import _need, launch_scope, need_device, stream_handle
+from .handoff import _current_device, _need, launch_scope, need_device, stream_handle
 from .pages import check_caches
 
 MAX_BEAMS = 16
@@ -37,60 +39,63 @@ def beam_select(logits, scores, n_out=None, eos=None, last_tokens=None, out=None
     allocated by the call on its stream)."""
     if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
         raise TypeError("logits must be a CUDA tensor")
-    with launch_scope(logits.device, stream):
-        if logits.dtype not in (torch.bfloat16, torch.float32):
-            raise TypeError(f"logits must be bfloat16 or float32, got {logits.dtype}")
-        _need(scores, "scores", torch.float32)
-        if scores.dim() != 2 or not scores.is_contiguous():
-            raise ValueError("scores must be contiguous [R, K]")
-        R, K = scores.shape
-        if logits.dim() != 2 or logits.shape[0] != R * K or R * K == 0 or logits.shape[1] == 0:
-            raise ValueError(f"logits must be [R*K = {R * K}, V], got {tuple(logits.shape)}")
-        V = logits.shape[1]
-        ld = logits.stride(0) if R * K > 1 else V
-        if (V > 1 and logits.stride(1) != 1) or ld < V:
-            raise ValueError("logits must have unit column stride and rows that do not overlap")
-        n = K if n_out is None else int(n_out)
-        need_device(logits.device, scores, "scores")
-        if (eos is None) != (last_tokens is None):
-            raise ValueError("eos and last_tokens come together")
-        last = None
-        if eos is not None:
-            eos = int(eos)
-            if not -(1 << 31) <= eos < 1 << 31:
-                raise ValueError(f"eos={eos} is no int32")
-            _need(last_tokens, "last_tokens", torch.int32)
-            need_device(logits.device, last_tokens, "last_tokens")
-            if last_tokens.numel() != R * K or not last_tokens.is_contiguous():
-                raise ValueError(f"last_tokens must be contiguous int32, {R * K} of them")
-            last = last_tokens.data_ptr()
-        need = beam_select_workspace_bytes(R, K, V, n)
-        if out is None:
-            out = (torch.empty((R, n), dtype=torch.int32, device=logits.device),
-                   torch.empty((R, n), dtype=torch.int32, device=logits.device),
-                   torch.empty((R, n), dtype=torch.float32, device=logits.device))
-        else:
-            for t, name, dt in zip(out, ("tokens", "parents", "scores"),
-                                   (torch.int32, torch.int32, torch.float32)):
-                _need(t, f"out {name}", dt)
-                need_device(logits.device, t, f"out {name}")
-                if t.numel() != R * n or not t.is_contiguous():
-                    raise ValueError(f"out {name} must be contiguous, {R * n} values")
-        if workspace is None:
-            workspace = torch.empty(need, dtype=torch.uint8, device=logits.device)
-        else:
-            need_device(logits.device, workspace, "workspace")
-            if not workspace.is_contiguous() \
-                    or workspace.numel() * workspace.element_size() < need:
-                raise ValueError(f"workspace holds fewer than the {need} bytes needed")
-        tokens, parents, totals = out
-        _lib.call("pdk_beam_select", logits.data_ptr(), logits.element_size(), ld, R, K, V,
-                  scores.data_ptr(), last, eos or 0, n, workspace.data_ptr(),
-                  workspace.numel() * workspace.element_size(), tokens.data_ptr(),
-                  parents.data_ptr(), totals.data_ptr(), stream_handle(stream))
-        return tokens, parents, totals
+    dev = logits.device
+    if stream is not None or dev.index != _current_device():
+        with launch_scope(dev, stream):
+            return beam_select(logits, scores, n_out, eos, last_tokens, out, workspace)
+    if logits.dtype is not torch.bfloat16 and logits.dtype is not torch.float32:
+        raise TypeError(f"logits must be bfloat16 or float32, got {logits.dtype}")
+    _need(scores, "scores", torch.float32)
+    need_device(dev, scores, "scores")
+    if scores.dim() != 2 or not scores.is_contiguous():
+        raise ValueError("scores must be contiguous [R, K]")
+    R, K = scores.shape
+    rows = R * K
+    if logits.dim() != 2 or logits.shape[0] != rows or rows == 0 or logits.shape[1] == 0:
+        raise ValueError(f"logits must be [R*K = {rows}, V], got {tuple(logits.shape)}")
+    V = logits.shape[1]
+    ld = logits.stride(0) if rows > 1 else V
+    if (V > 1 and logits.stride(1) != 1) or ld < V:
+        raise ValueError("logits must have unit column stride and rows that do not overlap")
+    n = K if n_out is None else int(n_out)
+    if (eos is None) != (last_tokens is None):
+        raise ValueError("eos and last_tokens come together")
+    last = None
+    if eos is not None:
+        eos = int(eos)
+        if not -(1 << 31) <= eos < 1 << 31:
+            raise ValueError(f"eos={eos} is no int32")
+        _need(last_tokens, "last_tokens", torch.int32)
+        need_device(dev, last_tokens, "last_tokens")
+        if last_tokens.numel() != rows or not last_tokens.is_contiguous():
+            raise ValueError(f"last_tokens must be contiguous int32, {rows} of them")
+        last = last_tokens.data_ptr()
+    need = beam_select_workspace_bytes(R, K, V, n)
+    if out is None:
+        out = (scores.new_empty((R, n), dtype=torch.int32),
+               scores.new_empty((R, n), dtype=torch.int32), scores.new_empty((R, n)))
+    else:
+        for t, name, dt in zip(out, ("tokens", "parents", "scores"),
+                               (torch.int32, torch.int32, torch.float32)):
+            _need(t, f"out {name}", dt)
+            need_device(dev, t, f"out {name}")
+            if t.numel() != R * n or not t.is_contiguous():
+                raise ValueError(f"out {name} must be contiguous, {R * n} values")
+    if workspace is None:
+        workspace, ws_bytes = scores.new_empty(need // 4), need   # a multiple of 8
+    else:
+        need_device(dev, workspace, "workspace")
+        ws_bytes = workspace.numel() * workspace.element_size()
+        if not workspace.is_contiguous() or ws_bytes < need:
+            raise ValueError(f"workspace holds fewer than the {need} bytes needed")
+    tokens, parents, totals = out
+    _lib.call("pdk_beam_select", logits.data_ptr(), logits.element_size(), ld, R, K, V,
+              scores.data_ptr(), last, eos or 0, n, workspace.data_ptr(), ws_bytes,
+              tokens.data_ptr(), parents.data_ptr(), totals.data_ptr(), stream_handle())
+    return tokens, parents, totals
 
 
+@functools.lru_cache(maxsize=1024)
 def beam_select_workspace_bytes(R, K, V, n):
     """Bytes of beam_select's workspace; raises for sizes it does not take."""
     for name, v in (("R", R), ("K", K), ("V", V), ("n_out", n)):
@@ -116,18 +121,21 @@ def beam_reorder(parents, ctx_lens, tables, cache_k, cache_v, stream=None):
     read before any is written."""
     if not isinstance(cache_k, torch.Tensor) or not cache_k.is_cuda:
         raise TypeError("cache_k must be a CUDA tensor")
-    with launch_scope(cache_k.device, stream):
-        L, nb, H, D, stride = check_caches(cache_k, cache_v)
-        for t, name in ((parents, "parents"), (ctx_lens, "ctx_lens"), (tables, "tables")):
-            _need(t, name, torch.int32)
-            need_device(cache_k.device, t, name)
-            if not t.is_contiguous():
-                raise ValueError(f"{name} must be contiguous")
-        if parents.dim() != 2:
-            raise ValueError("parents must be [R, K]")
-        R, K = parents.shape
-        if tables.dim() != 2 or tables.shape[0] != R * K or ctx_lens.numel() != R * K:
-            raise ValueError(f"tables [R*K, max_blocks] and ctx_lens [R*K] need R*K = {R * K} rows")
-        _lib.call("pdk_beam_reorder", parents.data_ptr(), ctx_lens.data_ptr(), R, K,
-                  tables.data_ptr(), tables.shape[1], cache_k.data_ptr(), cache_v.data_ptr(),
-                  stride, L, nb, H, D, stream_handle(stream))
+    dev = cache_k.device
+    if stream is not None or dev.index != _current_device():
+        with launch_scope(dev, stream):
+            return beam_reorder(parents, ctx_lens, tables, cache_k, cache_v)
+    L, nb, H, D, stride = check_caches(cache_k, cache_v)
+    for t, name in ((parents, "parents"), (ctx_lens, "ctx_lens"), (tables, "tables")):
+        _need(t, name, torch.int32)
+        need_device(dev, t, name)
+        if not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
+    if parents.dim() != 2:
+        raise ValueError("parents must be [R, K]")
+    R, K = parents.shape
+    if tables.dim() != 2 or tables.shape[0] != R * K or ctx_lens.numel() != R * K:
+        raise ValueError(f"tables [R*K, max_blocks] and ctx_lens [R*K] need R*K = {R * K} rows")
+    _lib.call("pdk_beam_reorder", parents.data_ptr(), ctx_lens.data_ptr(), R, K, tables.data_ptr(),
+              tables.shape[1], cache_k.data_ptr(), cache_v.data_ptr(), stride, L, nb, H, D,
+              stream_handle())

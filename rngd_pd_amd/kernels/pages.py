@@ -3,12 +3,18 @@ import numpy as np
 import torch
 
 from .. import _lib
-from .handoff import _need, launch_scope, need_device, stream_handle
+from .handoff import BF16, _current_device, _need, launch_scope, need_device, stream_handle
 
 
 def check_caches(cache_k, cache_v):
     """(layers, num_blocks, Hkv, D, layer stride) of cache_k [L, nb, Hkv, 16, D]
     and cache_v [L, nb, Hkv, D, 16], or of one layer's."""
+    if cache_k.dtype is BF16 and cache_k.dim() == 5 and isinstance(cache_v, torch.Tensor):
+        L, nb, H, block, D = cache_k.shape                # the usual whole cache, in one test
+        if (block == 16 and cache_v.shape == (L, nb, H, D, 16) and cache_v.dtype is BF16
+                and cache_v.device == cache_k.device and cache_k.is_contiguous()
+                and cache_v.is_contiguous()):
+            return L, nb, H, D, nb * H * 16 * D
     _need(cache_k, "cache_k")
     _need(cache_v, "cache_v")
     need_device(cache_k.device, cache_v, "cache_v")
@@ -30,10 +36,16 @@ def check_caches(cache_k, cache_v):
     return L, nb, H, D, stride
 
 
+def _address(a):
+    return a.__array_interface__["data"][0]
+
+
 def _ids(ids, name, num_blocks):
     """Host block ids as int32."""
     if isinstance(ids, torch.Tensor) and ids.is_cuda:
         raise TypeError(f"{name} must be on the host (a list, a numpy array or a CPU tensor)")
+    if type(ids) is np.ndarray and ids.dtype == np.int32 and ids.ndim == 1:
+        return ids if ids.flags.c_contiguous else np.ascontiguousarray(ids)
     a = np.asarray(ids)
     if a.ndim != 1 or (a.size and a.dtype.kind not in "iu"):
         raise TypeError(f"{name} must be a list of block ids")
@@ -55,11 +67,13 @@ def copy_blocks(cache_k, cache_v, src, dst, stream=None):
     result does not hang on an order."""
     if not isinstance(cache_k, torch.Tensor) or not cache_k.is_cuda:
         raise TypeError("cache_k must be a CUDA tensor")
-    with launch_scope(cache_k.device, stream):
-        L, nb, H, D, stride = check_caches(cache_k, cache_v)
-        s, d = _ids(src, "src", nb), _ids(dst, "dst", nb)
-        if s.size != d.size:
-            raise ValueError(f"{s.size} sources for {d.size} destinations")
-        if s.size:
-            _lib.call("pdk_copy_blocks", cache_k.data_ptr(), cache_v.data_ptr(), stride, L, nb, H,
-                      D, s.ctypes.data, d.ctypes.data, s.size, stream_handle(stream))
+    if stream is not None or cache_k.device.index != _current_device():
+        with launch_scope(cache_k.device, stream):
+            return copy_blocks(cache_k, cache_v, src, dst)
+    L, nb, H, D, stride = check_caches(cache_k, cache_v)
+    s, d = _ids(src, "src", nb), _ids(dst, "dst", nb)
+    if s.size != d.size:
+        raise ValueError(f"{s.size} sources for {d.size} destinations")
+    if s.size:
+        _lib.call("pdk_copy_blocks", cache_k.data_ptr(), cache_v.data_ptr(), stride, L, nb, H, D,
+                  _address(s), _address(d), s.size, stream_handle())

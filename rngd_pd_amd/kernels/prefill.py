@@ -2,7 +2,7 @@
 import torch
 
 from .. import _lib
-from .handoff import BF16, _need, launch_scope, need_device, stream_handle
+from .handoff import BF16, _current_device, _need, launch_scope, need_device, stream_handle
 
 HEAD_DIM = 128
 
@@ -41,28 +41,30 @@ def prefill_attention(q, k, v, scale=1.0, window=None, sinks=0, out=None, stream
     or t < ``sinks``."""
     if not isinstance(q, torch.Tensor) or not q.is_cuda:
         raise TypeError("q must be a CUDA tensor")
-    with launch_scope(q.device, stream):
-        window, sinks = check_window(window, sinks)
-        for t, name in ((q, "q"), (k, "k"), (v, "v")):
-            _need(t, name)
-            need_device(q.device, t, name)
-            if t.dim() != 3 or t.shape[0] != q.shape[0]:
-                raise ValueError(f"{name} must be [T, heads, {HEAD_DIM}], got {tuple(t.shape)}")
-        T, Hq, D = q.shape
-        Hkv = k.shape[1]
-        if k.shape != v.shape or k.shape[2] != D:
-            raise ValueError("k and v must be [T, Hkv, D] with q's head_dim")
-        if out is None:
-            out = torch.empty((T, Hq, D), dtype=BF16, device=q.device)
-        else:
-            _need(out, "out")
-            need_device(q.device, out, "out")
-            if out.shape != q.shape or not out.is_contiguous() or out.data_ptr() % 16:
-                raise ValueError(f"out must be contiguous and 16-byte aligned {tuple(q.shape)}")
-        if T == 0:
-            return out
-        st = stream_handle(stream)
-        (q, q_ld), (k, k_ld), (v, v_ld) = _rows(q, T), _rows(k, T), _rows(v, T)
-        _lib.call("pdk_prefill_attn_window", q.data_ptr(), q_ld, k.data_ptr(), k_ld, v.data_ptr(),
-                  v_ld, T, Hq, Hkv, D, float(scale), window or T, sinks, out.data_ptr(), st)
+    dev = q.device
+    if stream is not None or dev.index != _current_device():
+        with launch_scope(dev, stream):
+            return prefill_attention(q, k, v, scale, window, sinks, out)
+    window, sinks = check_window(window, sinks)
+    for t, name in ((q, "q"), (k, "k"), (v, "v")):
+        _need(t, name)
+        need_device(dev, t, name)
+        if t.dim() != 3 or t.shape[0] != q.shape[0]:
+            raise ValueError(f"{name} must be [T, heads, {HEAD_DIM}], got {tuple(t.shape)}")
+    T, Hq, D = q.shape
+    Hkv = k.shape[1]
+    if k.shape != v.shape or k.shape[2] != D:
+        raise ValueError("k and v must be [T, Hkv, D] with q's head_dim")
+    if out is None:
+        out = torch.empty((T, Hq, D), dtype=BF16, device=dev)
+    else:
+        _need(out, "out")
+        need_device(dev, out, "out")
+        if out.shape != q.shape or not out.is_contiguous() or out.data_ptr() % 16:
+            raise ValueError(f"out must be contiguous and 16-byte aligned {tuple(q.shape)}")
+    if T == 0:
         return out
+    (q, q_ld), (k, k_ld), (v, v_ld) = _rows(q, T), _rows(k, T), _rows(v, T)
+    _lib.call("pdk_prefill_attn_window", q.data_ptr(), q_ld, k.data_ptr(), k_ld, v.data_ptr(), v_ld,
+              T, Hq, Hkv, D, scale, window or T, sinks, out.data_ptr(), stream_handle())
+    return out
