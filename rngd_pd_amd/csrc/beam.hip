@@ -24,6 +24,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "pdk_common.h"
 
@@ -71,31 +72,93 @@ __device__ __forceinline__ double exp2_neg(double y) {
   return __builtin_amdgcn_ldexp(p, (int)k);
 }
 
+// ln x for x >= 1/2: a 32-bit logarithm and one Newton step in 64 bits, which
+// leaves the square of its error and exp2_neg's.
+__device__ __forceinline__ double log_of(double x) {
+  const double y = (double)__logf((float)x);
+  const double e = x * exp2_neg(-y * 1.4426950408889634074) - 1.0;
+  return y + (e - 0.5 * e * e);
+}
+
 constexpr double kLog2e = 1.4426950408889634074;
 
 __device__ __forceinline__ double exp_neg(double x) { return exp2_neg(fmax(x, -690.0) * kLog2e); }
 
-__device__ __forceinline__ double wave_sum(double x) {
+// x reduced over the wavefront by f, the same in every lane: halves and quarters
+// exchanged by the lane swaps, rows of 16 lanes by rotations (no LDS round trip, a
+// tenth of the time of six __shfl_xor). f is symmetric, so all lanes end with the
+// same bits.
+template <typename T, class F>
+__device__ __forceinline__ T wave_all(T x, F f) {
+  constexpr int W = sizeof(T) / 4;
+  union U {
+    T v;
+    uint32_t w[W];
+  };
+  U a{x}, b;
+  auto swap = [&](auto op) __attribute__((always_inline)) {
+    U c;
 #pragma unroll
-  for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
-  return x;
+    for (int i = 0; i < W; ++i) {
+      const auto r = op(a.w[i]);
+      b.w[i] = r[0];
+      c.w[i] = r[1];
+    }
+    a.v = f(b.v, c.v);
+  };
+  swap([](uint32_t v) { return __builtin_amdgcn_permlane32_swap(v, v, false, false); });
+  swap([](uint32_t v) { return __builtin_amdgcn_permlane16_swap(v, v, false, false); });
+  auto turn = [&](auto ctrl) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < W; ++i)
+      b.w[i] = __builtin_amdgcn_update_dpp(0, a.w[i], decltype(ctrl)::value, 0xf, 0xf, true);
+    a.v = f(a.v, b.v);
+  };
+  turn(std::integral_constant<int, 0x128>{});            // row_ror:8, 4, 2, 1
+  turn(std::integral_constant<int, 0x124>{});
+  turn(std::integral_constant<int, 0x122>{});
+  turn(std::integral_constant<int, 0x121>{});
+  return a.v;
+}
+
+__device__ __forceinline__ double wave_sum(double x) {
+  return wave_all(x, [](double a, double b) { return a + b; });
 }
 
 // The n-th largest of the wavefront's 64 values (0 if no more than n are not 0),
-// or a lower bound that no more of them reach: bit by bit from the top, the
-// largest bound that n lanes reach.
+// or a lower bound that no more of them reach: two bits at a time from the top,
+// the largest bound that n lanes reach.
 template <typename U>
 __device__ __forceinline__ U nth_largest(U mine, int n) {
   if (__popcll(__ballot(mine != 0)) <= n) return 0;
   U bound = 0;
 #pragma unroll 1
-  for (int bit = 8 * sizeof(U) - 1; bit >= 0; --bit) {
-    const U t = bound | ((U)1 << bit);
-    const int c = __popcll(__ballot(mine >= t));
-    if (c >= n) bound = t;
+  for (int bit = 8 * sizeof(U) - 2; bit >= 0; bit -= 2) {
+    const U t1 = bound | ((U)1 << bit), t2 = bound | ((U)2 << bit), t3 = bound | ((U)3 << bit);
+    const int c1 = __popcll(__ballot(mine >= t1)), c2 = __popcll(__ballot(mine >= t2));
+    const int c3 = __popcll(__ballot(mine >= t3));
+    const U next = c3 >= n ? t3 : c2 >= n ? t2 : c1 >= n ? t1 : bound;
+    const int c = c3 >= n ? c3 : c2 >= n ? c2 : c1;
+    bound = next;
     if (c == n) break;
   }
   return bound;
+}
+
+// x[i], i a lane's own: halved bit by bit with masks (a choice between registers
+// would be made through memory).
+template <int kN>
+__device__ __forceinline__ float pick(const float (&x)[kN], int i) {
+  uint32_t y[kN];
+#pragma unroll
+  for (int j = 0; j < kN; ++j) y[j] = __float_as_uint(x[j]);
+#pragma unroll
+  for (int w = kN / 2, bit = 0; w; w >>= 1, ++bit) {
+    const uint32_t odd = 0u - ((i >> bit) & 1u);
+#pragma unroll
+    for (int j = 0; j < w; ++j) y[j] = (y[2 * j + 1] & odd) | (y[2 * j] & ~odd);
+  }
+  return __uint_as_float(y[0]);
 }
 
 // What the wavefront's lanes wrote to LDS is there for all of them.
@@ -186,9 +249,7 @@ __global__ __launch_bounds__(64 * kWaves) void beam_part_kernel(const T* logits,
   float mine = x[0];
 #pragma unroll
   for (int i = 1; i < kVals; ++i) mine = __builtin_elementwise_maximum(mine, x[i]);
-  float top = mine;
-#pragma unroll
-  for (int o = 32; o; o >>= 1) top = __builtin_elementwise_maximum(top, __shfl_xor(top, o));
+  const float top = wave_all(mine, [](float a, float b) { return __builtin_elementwise_maximum(a, b); });
   double sum = 0.0;
   if (top < INFINITY && top > -INFINITY) {
 #pragma unroll
@@ -204,15 +265,17 @@ __global__ __launch_bounds__(64 * kWaves) void beam_part_kernel(const T* logits,
   Key* list = lists[wave];
   const uint32_t bound = nth_largest(code_of(mine), n);
   const float least = bound ? value_of(bound) : -3.402823466e38f;
-  auto token = [&](int i) { return (uint32_t)(e0 + (i / kEl) * 64 * kEl + i % kEl); };
-  int c = 0;
+  auto token = [&](int i) { return (uint32_t)(e0 + i / kEl * (64 * kEl) + i % kEl); };
+  uint32_t mask = 0;                                     // bit i: value i reaches the bound
 #pragma unroll
-  for (int i = 0; i < kVals; ++i) {
-    const bool in = x[i] >= least;
-    const uint64_t who = __ballot(in);
-    if (who == 0) continue;
+  for (int i = 0; i < kVals; ++i) mask |= x[i] >= least ? 1u << i : 0u;
+  int c = 0;
+  for (uint64_t who; (who = __ballot(mask != 0)) && c <= 64;) {   // a value of every such lane
+    const int i = __builtin_ctz(mask | 0x80000000u);
+    const float v = pick(x, i);
     const int to = c + __popcll(who & ((1ull << lane) - 1));
-    if (in && to < 64) list[to] = key_of(x[i], token(i));
+    if (mask && to < 64) list[to] = key_of(v, token(i));
+    mask &= mask - 1;
     c += __popcll(who);
   }
   if (c > 64) {                                          // equal values
@@ -241,25 +304,25 @@ __global__ __launch_bounds__(64 * kWaves) void beam_part_kernel(const T* logits,
 }
 
 // One workgroup per request, one wavefront per beam: the beam's log sum, its n
-// best tokens of all parts and their totals; then every candidate counts those of
-// the other beams that come before it.
+// best tokens of all parts and their totals; then every candidate counts those
+// that come before it. Each workgroup runs this code once, so what it takes is
+// mostly the instructions' first fetch: one call of each helper, no unrolling.
 __global__ __launch_bounds__(64 * kMaxBeams) void beam_join_kernel(
     const Part* parts, const Key* keys, int n_parts, int n, const float* scores, int K,
     const int32_t* last_tokens, int eos, int32_t* tokens, int32_t* parents, float* out_scores) {
-  constexpr int kList = 256;                             // keys of a beam held at a time
+  constexpr int kList = 512;                             // keys of a beam held at a time
   __shared__ Key list[kMaxBeams][kList];
   __shared__ Key best[kMaxBeams][kMaxOut];
   __shared__ uint16_t lists[kMaxBeams][kMaxOut * kMaxLists];
-  __shared__ double totals[kMaxBeams][kMaxOut];
-  __shared__ int32_t token[kMaxBeams][kMaxOut];
-  __shared__ int found;
+  __shared__ double totals[kMaxBeams * kMaxOut];         // [beam][n]
   const int r = blockIdx.x, lane = threadIdx.x & 63;
   const int k = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int row = r * K + k;
   const bool ended = last_tokens && last_tokens[row] == eos;
   const float score = scores[row];
   const bool alive = score > -INFINITY && score < INFINITY;
-  if (threadIdx.x == 0) found = 0;
+  double total = lane == 0 && alive ? (double)score : -INFINITY;   // of an ended beam
+  int32_t token = eos;
   if (!ended) {
     // Heads of the parts' lists; only lists whose head reaches the n-th largest of
     // the lanes' own best heads hold any of the n best: those of at most n lanes.
@@ -267,24 +330,30 @@ __global__ __launch_bounds__(64 * kMaxBeams) void beam_join_kernel(
     const Part* pp = parts + (int64_t)row * n_parts;
     Key mine = 0;
     double top = -INFINITY, sum = 0.0;
+#pragma unroll 1
     for (int s = lane; s < n_parts; s += 64) {
       const Key head = kp[s * n];
-      const Part q = pp[s];
       mine = head > mine ? head : mine;
-      // NaN in q.sum stays; a part without a finite value adds nothing.
-      if (q.sum != 0.0) {
-        const double m = fmax(top, q.top);
-        sum = sum * exp_neg(top - m) + q.sum * exp_neg(q.top - m);
-        top = m;
-      }
+      top = fmax(top, pp[s].top);
     }
-    double all = top;
-#pragma unroll
-    for (int o = 32; o; o >>= 1) all = fmax(all, __shfl_xor(all, o));
-    sum = wave_sum(top > -INFINITY || sum != sum ? sum * exp_neg(top - all) : 0.0);
-    const double log_sum = log(sum);                     // beside the maximum: it may be any size
-    const Key bound = nth_largest(mine, n), least = bound ? bound : 1;
+    top = wave_all(top, [](double a, double b) { return fmax(a, b); });
+#pragma unroll 1
+    for (int s = lane; s < n_parts; s += 64) {
+      const Part q = pp[s];
+      // NaN in q.sum stays; a part without a finite value adds nothing.
+      sum += q.sum != 0.0 ? q.sum * exp_neg(q.top - top) : 0.0;
+    }
+    const double log_sum = log_of(wave_sum(sum));        // beside the maximum: it may be any size
+    // By the codes first; the tokens count only where equal codes leave too many.
+    const uint32_t code = nth_largest((uint32_t)(mine >> 32), n);
+    Key least = code ? (Key)code << 32 : 1;
+    if (__popcll(__ballot(mine >= least)) > n) {         // equal codes: of those, the first tokens
+      const uint32_t c = (uint32_t)(mine >> 32);
+      const int more = n - __popcll(__ballot(c > code));
+      least |= nth_largest(c == code ? (uint32_t)mine : 0u, more);
+    }
     int m = 0;                                           // lists that reach it
+#pragma unroll 1
     for (int s = lane; s - lane < n_parts; s += 64) {
       const bool in = s < n_parts && kp[s * n] >= least;
       const uint64_t who = __ballot(in);
@@ -293,6 +362,7 @@ __global__ __launch_bounds__(64 * kMaxBeams) void beam_join_kernel(
     }
     wave_sync();
     int c = 0;
+#pragma unroll 1
     for (int i0 = 0; i0 < m * n; i0 += 256) {            // four loads of a lane in flight
       Key q[4];
 #pragma unroll
@@ -304,61 +374,47 @@ __global__ __launch_bounds__(64 * kMaxBeams) void beam_join_kernel(
       for (int x = 0; x < 4; ++x) {
         const bool in = q[x] >= least;
         const uint64_t who = __ballot(in);
-        const int more = __popcll(who);
-        if (c + more > kList) {                          // keep the n best so far
-          wave_sync();
-          rank(list[k], c, best[k], n);
-          wave_sync();
-          if (lane < n) list[k][lane] = best[k][lane];
-          c = n;
-        }
         if (in) list[k][c + __popcll(who & ((1ull << lane) - 1))] = q[x];
-        c += more;
+        c += __popcll(who);
       }
+      if (c <= kList - 256 && i0 + 256 < m * n) continue;
+      wave_sync();                                       // the n best so far
+      rank(list[k], c, best[k], n);
+      wave_sync();
+      if (lane < n) list[k][lane] = best[k][lane];
+      c = n;
     }
-    wave_sync();
-    rank(list[k], c, best[k], n);
-    wave_sync();
-    if (lane < n) {
-      const Key b = best[k][lane];
-      const bool ok = b && alive && log_sum > -INFINITY && log_sum < INFINITY;
-      token[k][lane] = (int32_t)(0xffffffffu - (uint32_t)b);
-      totals[k][lane] = ok ? (double)score + (((double)value_of((uint32_t)(b >> 32)) - all) - log_sum)
-                            : -INFINITY;
-    }
-  } else if (lane < n) {
-    token[k][lane] = eos;
-    totals[k][lane] = lane == 0 && alive ? (double)score : -INFINITY;
+    const Key b = m && lane < n ? best[k][lane] : 0;
+    // (log_sum of a row without a finite value, or with NaN or +inf, is NaN.)
+    const bool ok = b && alive && log_sum >= 0.0 - 1e-6;
+    token = (int32_t)(0xffffffffu - (uint32_t)b);
+    total = ok ? (double)score + (((double)value_of((uint32_t)(b >> 32)) - top) - log_sum) : -INFINITY;
   }
+  if (lane < n) totals[k * n + lane] = total;
   __syncthreads();
-  if (lane < n) {
-    const double t = totals[k][lane];
-    if (t > -INFINITY) {
-      int at = lane;
-      for (int o = 0; o < K; ++o) {
-        if (o == k) continue;
-        int lo = 0, hi = n;                              // the first of beam o behind this one
-        while (lo < hi) {
-          const int mid = (lo + hi) >> 1;
-          const double u = totals[o][mid];
-          if (u > t || (u == t && o < k)) lo = mid + 1;
-          else hi = mid;
-        }
-        at += lo;
-      }
-      atomicAdd(&found, 1);
-      if (at < n) {
-        tokens[(int64_t)r * n + at] = token[k][lane];
-        parents[(int64_t)r * n + at] = k;
-        out_scores[(int64_t)r * n + at] = (float)t;
-      }
-    }
+  // Candidate lane % w of the beam counts every 64 / w-th of all that there are.
+  const int w = n <= 4 ? 4 : n <= 8 ? 8 : n <= 16 ? 16 : 32, i = lane & (w - 1);
+  const double mine = i < n ? totals[k * n + i] : -INFINITY;
+  int at = 0, found = 0;
+#pragma unroll 2
+  for (int j = lane / w; j < K * n; j += 64 / w) {
+    const double u = totals[j];
+    at += (u > mine) | ((u == mine) & (j < k * n + i));
+    found += u > -INFINITY;
   }
-  __syncthreads();
-  if ((int)threadIdx.x < n && (int)threadIdx.x >= found) {   // fewer candidates than asked for
-    tokens[(int64_t)r * n + threadIdx.x] = -1;
-    parents[(int64_t)r * n + threadIdx.x] = -1;
-    out_scores[(int64_t)r * n + threadIdx.x] = -INFINITY;
+  for (int o = w; o < 64; o <<= 1) {
+    at += __shfl_xor(at, o);
+    found += __shfl_xor(found, o);
+  }
+  if (lane < n && total > -INFINITY && at < n) {
+    tokens[(int64_t)r * n + at] = token;
+    parents[(int64_t)r * n + at] = k;
+    out_scores[(int64_t)r * n + at] = (float)total;
+  }
+  if (k == 0 && lane < n && lane >= found) {             // fewer candidates than asked for
+    tokens[(int64_t)r * n + lane] = -1;
+    parents[(int64_t)r * n + lane] = -1;
+    out_scores[(int64_t)r * n + lane] = -INFINITY;
   }
 }
 
