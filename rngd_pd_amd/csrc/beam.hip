@@ -396,11 +396,17 @@ __global__ __launch_bounds__(64 * kMaxBeams) void beam_join_kernel(
   const int w = n <= 4 ? 4 : n <= 8 ? 8 : n <= 16 ? 16 : 32, i = lane & (w - 1);
   const double mine = i < n ? totals[k * n + i] : -INFINITY;
   int at = 0, found = 0;
-#pragma unroll 2
-  for (int j = lane / w; j < K * n; j += 64 / w) {
-    const double u = totals[j];
-    at += (u > mine) | ((u == mine) & (j < k * n + i));
-    found += u > -INFINITY;
+  for (int j0 = lane / w; j0 < K * n; j0 += 4 * (64 / w)) {
+    double u[4];                                         // four reads in flight
+#pragma unroll
+    for (int x = 0; x < 4; ++x) u[x] = totals[min(j0 + x * (64 / w), K * n - 1)];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int j = j0 + x * (64 / w);
+      const bool in = j < K * n;
+      at += in & ((u[x] > mine) | ((u[x] == mine) & (j < k * n + i)));
+      found += in & (u[x] > -INFINITY);
+    }
   }
   for (int o = w; o < 64; o <<= 1) {
     at += __shfl_xor(at, o);
@@ -425,64 +431,71 @@ __global__ __launch_bounds__(64 * kMaxBeams) void beam_join_kernel(
 // (or one table column): it has read every beam's before it writes any, so beams
 // may swap, and no two lanes touch one address: no staging, no second launch.
 // Bound by the bytes of the blocks that move.
+// What steers a workgroup (the count of tokens, the parents, the blocks' ids) is
+// read as scalars; the launch writes none of it (of the tables only entries below
+// the one that is read).
 // grid: x = chunk, y = 2 * layer + (0 for K, 1 for V) or, last, the tables, z = r.
+// kK: at least K.
+template <int kK>
 __global__ __launch_bounds__(256) void beam_reorder_kernel(const int32_t* parents,
                                                            const int32_t* ctx_lens, int K,
                                                            int32_t* tables, int max_blocks,
                                                            uint16_t* ck, uint16_t* cv,
                                                            int64_t layer_stride, int num_blocks,
                                                            int block_units) {
+  typedef const __attribute__((address_space(4))) int32_t* scalars;
   const int r = blockIdx.z;
-  const int held = ctx_lens[r * K];                      // the same for a request's beams
+  const int held = ((scalars)ctx_lens)[(int64_t)r * K];  // the same for a request's beams
+  int32_t* rows = tables + (int64_t)r * K * max_blocks;
+  int from[kK];                                          // the beam that beam k goes on from
+#pragma unroll
+  for (int k = 0; k < kK; ++k) {
+    const int p = ((scalars)parents)[(int64_t)r * K + min(k, K - 1)];
+    from[k] = k < K && p >= 0 && p < K ? p : k;          // no parent: the beam stays itself
+  }
   if (held <= 0) return;
   const int full = held / PDK_BLOCK_SIZE;
-  int32_t* rows = tables + (int64_t)r * K * max_blocks;
-  auto parent = [&](int k) {
-    const int p = k < K ? parents[r * K + k] : -1;
-    return p >= 0 && p < K ? p : k;                      // no parent: the beam stays itself
-  };
   if (blockIdx.y == gridDim.y - 1) {
     const int cols = min(full, max_blocks);
     for (int j = blockIdx.x * 256 + threadIdx.x; j < cols; j += gridDim.x * 256) {
-      int32_t id[kMaxBeams];
+      int32_t id[kK];
 #pragma unroll
-      for (int k = 0; k < kMaxBeams; ++k)
-        if (k < K) id[k] = rows[(int64_t)parent(k) * max_blocks + j];
+      for (int k = 0; k < kK; ++k)
+        if (from[k] != k) id[k] = rows[(int64_t)from[k] * max_blocks + j];
 #pragma unroll
-      for (int k = 0; k < kMaxBeams; ++k)
-        if (k < K && parent(k) != k) rows[(int64_t)k * max_blocks + j] = id[k];
+      for (int k = 0; k < kK; ++k)
+        if (from[k] != k) rows[(int64_t)k * max_blocks + j] = id[k];
     }
     return;
   }
   const int u = blockIdx.x * 256 + threadIdx.x;
-  if (held % PDK_BLOCK_SIZE == 0 || full >= max_blocks || u >= block_units) return;
-  uint16_t* base = (blockIdx.y & 1 ? cv : ck) + (int64_t)(blockIdx.y >> 1) * layer_stride;
+  if (held % PDK_BLOCK_SIZE == 0 || full >= max_blocks) return;
+  int place[kK];                                         // beam k's partly filled block
+#pragma unroll
+  for (int k = 0; k < kK; ++k)
+    place[k] = ((scalars)rows)[(int64_t)min(k, K - 1) * max_blocks + full];
+  uint16_t* base = (blockIdx.y & 1 ? cv : ck) + (int64_t)(blockIdx.y >> 1) * layer_stride +
+                   (int64_t)u * 8;
   const int64_t block = (int64_t)block_units * 8;
-  auto place = [&](int k) {                              // beam k's partly filled block, or -1
-    const int id = rows[(int64_t)k * max_blocks + full];
-    return id >= 0 && id < num_blocks ? id : -1;
-  };
-  v8 x[kMaxBeams];
+  v8 x[kK];
+  bool moves[kK];
 #pragma unroll
-  for (int k = 0; k < kMaxBeams; ++k) {
-    const int p = parent(k);
-    if (k < K && p != k) {
-      const int s = place(p);
-      if (s >= 0) x[k] = pdk::ld16(base + s * block + (int64_t)u * 8);
-    }
+  for (int k = 0; k < kK; ++k) {
+    int src = place[0];
+#pragma unroll
+    for (int p = 1; p < kK; ++p) src = from[k] == p ? place[p] : src;
+    moves[k] = from[k] != k && src >= 0 && src < num_blocks && place[k] >= 0 &&
+               place[k] < num_blocks;
+    if (moves[k] && u < block_units) x[k] = pdk::ld16(base + src * block);
   }
 #pragma unroll
-  for (int k = 0; k < kMaxBeams; ++k) {
-    const int p = parent(k);
-    if (k < K && p != k) {
-      const int s = place(p), d = place(k);
-      if (s >= 0 && d >= 0) pdk::st16(base + d * block + (int64_t)u * 8, x[k]);
-    }
-  }
+  for (int k = 0; k < kK; ++k)
+    if (moves[k] && u < block_units) pdk::st16(base + place[k] * block, x[k]);
 }
 
 // Values of a lane: 32, or 16 where rows are too few for 32 to give every SIMD two
-// wavefronts.
+// wavefronts (128256 bf16 or fp32 values a row, in us with 16 and with 32: 4 rows
+// 13.5 and 14.9, 64 rows 16.8 and 15.8, 256 fp32 rows 49.6 and 44.6).
 int lane_vals(int rows, int V) {
   const bool many = (int64_t)rows * ((V + 2047) / 2048) >= 2048;
   return many || V > kMaxVocab / 2 ? 32 : 16;
@@ -575,7 +588,9 @@ extern "C" int pdk_beam_reorder(const int32_t* parents, const int32_t* ctx_lens,
                   (n_layers == 1 || cache_layer_stride >= (int64_t)num_blocks * block),
               "the layer stride must be a multiple of 8 and hold num_blocks blocks");
   const int units = (int)(block / 8);
-  hipLaunchKernelGGL(beam_reorder_kernel, dim3((units + 255) / 256, 2 * n_layers + 1, R), dim3(256),
+  const auto kern = K <= 4 ? beam_reorder_kernel<4> : K <= 8 ? beam_reorder_kernel<8>
+                                                             : beam_reorder_kernel<16>;
+  hipLaunchKernelGGL(kern, dim3((units + 255) / 256, 2 * n_layers + 1, R), dim3(256),
                      0, pdk::as_stream(stream), parents, ctx_lens, K, tables, max_blocks, cache_k,
                      cache_v, cache_layer_stride, num_blocks, units);
   return pdk::check_launch("beam_reorder_kernel");
