@@ -361,7 +361,8 @@ int pdk_copy_blocks(uint16_t* cache_k, uint16_t* cache_v,
  * its score), its logits are not read. No candidates come from -inf logits, from
  * a beam whose score is not finite, nor from one whose row holds NaN or +inf, or
  * only -inf. Where there are fewer than n, the rest is token -1, parent -1,
- * score -inf. 1 <= K <= 16, 1 <= n <= 32, V <= 2^20. The workspace (16-byte
+ * score -inf. With n = K, tokens may be last_tokens and out_scores scores.
+ * 1 <= K <= 16, 1 <= n <= 32, V <= 2^20. The workspace (16-byte
  * aligned, one call at a time) needs no clearing. The reference samples greedily
  * only (greedy_tokens, engines/decode_batch.py:162-171). */
 int64_t pdk_beam_select_workspace_bytes(int R, int K, int V, int n);

@@ -434,7 +434,8 @@ __global__ __launch_bounds__(64 * kMaxBeams) void beam_join_kernel(
 // What steers a workgroup (the count of tokens, the parents, the blocks' ids) is
 // read as scalars; the launch writes none of it (of the tables only entries below
 // the one that is read).
-// grid: x = chunk, y = 2 * layer + (0 for K, 1 for V) or, last, the tables, z = r.
+// Consecutive workgroups move the blocks of one layer.
+// grid: x = chunk, y = r, z = 2 * layer + (0 for K, 1 for V) or, last, the tables.
 // kK: at least K.
 template <int kK>
 __global__ __launch_bounds__(256) void beam_reorder_kernel(const int32_t* parents,
@@ -444,7 +445,7 @@ __global__ __launch_bounds__(256) void beam_reorder_kernel(const int32_t* parent
                                                            int64_t layer_stride, int num_blocks,
                                                            int block_units) {
   typedef const __attribute__((address_space(4))) int32_t* scalars;
-  const int r = blockIdx.z;
+  const int r = blockIdx.y;
   const int held = ((scalars)ctx_lens)[(int64_t)r * K];  // the same for a request's beams
   int32_t* rows = tables + (int64_t)r * K * max_blocks;
   int from[kK];                                          // the beam that beam k goes on from
@@ -455,7 +456,7 @@ __global__ __launch_bounds__(256) void beam_reorder_kernel(const int32_t* parent
   }
   if (held <= 0) return;
   const int full = held / PDK_BLOCK_SIZE;
-  if (blockIdx.y == gridDim.y - 1) {
+  if (blockIdx.z == gridDim.z - 1) {
     const int cols = min(full, max_blocks);
     for (int j = blockIdx.x * 256 + threadIdx.x; j < cols; j += gridDim.x * 256) {
       int32_t id[kK];
@@ -474,7 +475,7 @@ __global__ __launch_bounds__(256) void beam_reorder_kernel(const int32_t* parent
 #pragma unroll
   for (int k = 0; k < kK; ++k)
     place[k] = ((scalars)rows)[(int64_t)min(k, K - 1) * max_blocks + full];
-  uint16_t* base = (blockIdx.y & 1 ? cv : ck) + (int64_t)(blockIdx.y >> 1) * layer_stride +
+  uint16_t* base = (blockIdx.z & 1 ? cv : ck) + (int64_t)(blockIdx.z >> 1) * layer_stride +
                    (int64_t)u * 8;
   const int64_t block = (int64_t)block_units * 8;
   v8 x[kK];
@@ -590,7 +591,7 @@ extern "C" int pdk_beam_reorder(const int32_t* parents, const int32_t* ctx_lens,
   const int units = (int)(block / 8);
   const auto kern = K <= 4 ? beam_reorder_kernel<4> : K <= 8 ? beam_reorder_kernel<8>
                                                              : beam_reorder_kernel<16>;
-  hipLaunchKernelGGL(kern, dim3((units + 255) / 256, 2 * n_layers + 1, R), dim3(256),
+  hipLaunchKernelGGL(kern, dim3((units + 255) / 256, R, 2 * n_layers + 1), dim3(256),
                      0, pdk::as_stream(stream), parents, ctx_lens, K, tables, max_blocks, cache_k,
                      cache_v, cache_layer_stride, num_blocks, units);
   return pdk::check_launch("beam_reorder_kernel");

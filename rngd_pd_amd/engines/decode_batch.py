@@ -23,8 +23,11 @@ from .paged_cache import PagedKVCache
 class BatchDecodeAttention:
     """Decode attention for a batch of streams sharing one PagedKVCache."""
 
-    def __init__(self, cache: PagedKVCache, n_q_heads=32, scale=None):
+    def __init__(self, cache: PagedKVCache, n_q_heads=32, scale=None, window=None, sinks=0):
+        """``window``, ``sinks``: streams see their last ``window`` tokens and the
+        first ``sinks`` (trim returns the blocks between the two)."""
         self.cache = cache
+        self.window, self.sinks = window, sinks
         self.Hq = n_q_heads
         self.G = n_q_heads // cache.n_kv_heads
         self.scale = (1.0 / math.sqrt(cache.head_dim)) if scale is None else scale
@@ -52,6 +55,18 @@ class BatchDecodeAttention:
         self.cache.free(req_id)
         self._batch_key = None
 
+    def trim(self, req_ids):
+        """Return the blocks that the streams' windows have left behind to the
+        pool; how many. Call it when the steps queued so far have finished, or
+        where no other stream fills blocks."""
+        if self.window is None:
+            return 0
+        n = sum(self.cache.drop_before(r, self.positions[r] + 1 - self.window, self.sinks)
+                for r in req_ids)
+        if n:
+            self._batch_key = None
+        return n
+
     def prepare(self, req_ids):
         """Block tables and context lengths for one step of ``req_ids`` (growing
         each stream's blocks to hold its new token)."""
@@ -70,12 +85,15 @@ class BatchDecodeAttention:
         (streams may share blocks: each sees the others' new tokens in them).
         q [B, Hq, D], k_new/v_new [B, Hkv, D] bf16 on the device."""
         ck, cv = self.cache.k[layer], self.cache.v[layer]
-        need = _attn.workspace_bytes(q.shape[0], self.Hq, max_ctx, self.cache.head_dim)
+        need = _attn.workspace_bytes(q.shape[0], self.Hq,
+                                     _attn.window_span(max_ctx, self.window, self.sinks),
+                                     self.cache.head_dim)
         if need and (self._ws is None or self._ws.numel() * 4 < need):
             self._ws = torch.zeros(need // 4 + 64, dtype=torch.float32, device=self.cache.device)
         return _attn.decode_attention_append(q, k_new, v_new, ck, cv, tables, ctx, max_ctx,
                                              scale=self.scale, out=out,
-                                             workspace=self._ws if need else None, stream=stream)
+                                             workspace=self._ws if need else None, stream=stream,
+                                             window=self.window, sinks=self.sinks)
 
     def advance(self, req_ids):
         """After all layers of a step: every stream moves to its next position."""

@@ -13,7 +13,8 @@ layer, one launch per line:
 
   qkv halves = r x . (Wqkv diag g1)^T              pdk_linear_splitk_rms (fp32 halves of K, rows scaled)
   q, k, v = bf16(sum of halves); RoPE(q, k); new
-  k, v into the paged cache; ao = attention        pdk_decode_attn_rope (+ its merge when split)
+  k, v into the paged cache; ao = attention        pdk_decode_attn_rope (+ its merge when split),
+                                                   pdk_decode_attn_rope_window for a config with one
   x = x + ao . Wo^T; ssq                            pdk_linear_ssq, residual fused
   a = silu(r g) * (r u), [g; u] = x . (Wgu diag g2)^T  pdk_linear_swiglu_rms
   x = x + a . Wd^T; ssq                             pdk_linear_ssq, residual fused
@@ -42,6 +43,7 @@ from .. import _lib
 from ..kernels import attention as _attn
 from ..kernels.decode_step import act_rows, act_untile, fold_norm, tile_weight
 from ..kernels.handoff import stream_handle
+from ..kernels.prefill import check_window
 
 BF16 = torch.bfloat16
 
@@ -51,10 +53,13 @@ class LlamaConfig:
 
     def __init__(self, hidden=4096, n_heads=32, n_kv_heads=8, head_dim=128, inter=14336,
                  vocab=128256, n_layers=32, eps=1e-5, theta=500000.0,
-                 rope_scaling=(8.0, 1.0, 4.0, 8192)):
+                 rope_scaling=(8.0, 1.0, 4.0, 8192), window=None, sinks=0):
+        """``window``, ``sinks``: every layer's attention sees the last ``window``
+        tokens and the first ``sinks`` (None: all)."""
         self.hidden, self.n_heads, self.n_kv_heads, self.head_dim = hidden, n_heads, n_kv_heads, head_dim
         self.inter, self.vocab, self.n_layers, self.eps = inter, vocab, n_layers, eps
         self.theta = theta
+        self.window, self.sinks = window, sinks
         self.rope_scaling = rope_scaling   # (factor, low_freq_factor, high_freq_factor, original_max_pos) or None
 
     @property
@@ -223,6 +228,7 @@ class LlamaDecoder:
                                               else "pdk_decode_attn_rope")
         if cfg.hidden % 16 or cfg.head_dim != 128:
             raise ValueError("the fused norms need hidden % 16 == 0 and head_dim 128")
+        self._window = check_window(cfg.window, cfg.sinks)
         self._layers = [tuple(t.data_ptr() for t in (wt[0], wt[1], wt[2], wt[3], cache.k[i],
                                                      cache.v[i]))
                         for i, wt in enumerate(self._wt)]
@@ -246,7 +252,9 @@ class LlamaDecoder:
         graph holds the address it was captured with, so once any graph exists
         a step that would need a larger one raises instead (reserve() the
         largest max_ctx before capturing)."""
-        need = _attn.workspace_bytes(B, self.cfg.n_heads, max_ctx, self.cfg.head_dim)
+        need = _attn.workspace_bytes(B, self.cfg.n_heads,
+                                     _attn.window_span(max_ctx, self.cfg.window, self.cfg.sinks),
+                                     self.cfg.head_dim)
         if need and (self._ws is None or self._ws.numel() * 4 < need):
             if self._captured:
                 raise RuntimeError(f"the attention workspace would have to grow to {need} bytes "
@@ -298,6 +306,7 @@ class LlamaDecoder:
         ssqp, ssqa, n_ssq = self.ssq.data_ptr(), self.ssq_a.data_ptr(), H // 16
         down_ws = None if self.down_ws is None else (self.down_ws.data_ptr(),
                                                      self.down_ws.numel() * 4)
+        window, sinks = self._window
         emb, attn = g["pdk_embed_ssq"], g["pdk_decode_attn_rope"]
         with torch.cuda.stream(stream) if stream is not None else contextlib.nullcontext():
             call(emb, w.embed.data_ptr(), cfg.vocab, tokens.data_ptr(),
@@ -305,8 +314,13 @@ class LlamaDecoder:
             pqp, qs = self.part_qkv.data_ptr(), self.qkv_splits
             for wqkv, wo, wgu, wd, ck, cv in self._layers:
                 call(lin_skr, xp, wqkv, B, H, QKV, qs, ssqa, n_ssq, eps, pqp, st)
-                call(attn, pqp, qs, inv, ck, cv, nb, tp, mb, cp, int(max_ctx),
-                     B, NH, NKV, HD, self.scale, ws_ptr, ws_bytes, aop, self.plan_batch, st)
+                if window:
+                    call("pdk_decode_attn_rope_window", pqp, qs, inv, ck, cv, nb, tp, mb, cp,
+                         int(max_ctx), window, sinks, B, NH, NKV, HD, self.scale, ws_ptr, ws_bytes,
+                         aop, self.act_tiled, self.plan_batch, st)
+                else:
+                    call(attn, pqp, qs, inv, ck, cv, nb, tp, mb, cp, int(max_ctx),
+                         B, NH, NKV, HD, self.scale, ws_ptr, ws_bytes, aop, self.plan_batch, st)
                 call(lin_ssq, aop, wo, B, NH * HD, H, xp, xp, ssqp, st)
                 call(lin_swr, xp, wgu, B, H, M, ssqp, n_ssq, eps, actp, st)
                 if down_ws is None:

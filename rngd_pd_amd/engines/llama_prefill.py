@@ -17,7 +17,8 @@ of a layer, the short prompt's on the right:
   h = rmsnorm(x + down)                pdk_rmsnorm          pdk_prefill_rmsnorm_partials
   qkv = h . Wqkv^T                     library              pdk_prefill_gemm
   RoPE; K/V rows; attention's operands pdk_prefill_rope_kv  pdk_prefill_rope_kv_partials
-  ao = causal GQA attention            pdk_prefill_attn (fp32 weights)
+  ao = causal GQA attention            pdk_prefill_attn (fp32 weights), or
+                                       pdk_prefill_attn_window for a config with one
   o = ao . Wo^T                        library              pdk_prefill_gemm
   h = rmsnorm(x + o)                   pdk_rmsnorm          pdk_prefill_rmsnorm_partials
   gu = h . Wgu^T                       library              pdk_prefill_gemm_swiglu, with
@@ -35,6 +36,7 @@ import torch
 
 from .. import _lib
 from ..kernels.handoff import stream_handle
+from ..kernels.prefill import check_window
 
 BF16 = torch.bfloat16
 
@@ -143,6 +145,7 @@ class LlamaPrefill:
         kt, vt = (torch.empty(n, dtype=BF16, device=dev) for _ in range(2))
         ao = torch.empty((T, NH * HD), dtype=BF16, device=dev)
         q_rows = None
+        window, sinks = check_window(cfg.window, cfg.sinks)
 
         def attention(qkv, k_l, v_l, before):
             nonlocal q_rows
@@ -168,6 +171,11 @@ class LlamaPrefill:
             if v is not v_l:
                 v_l.copy_(v)
             before()
+            if window:
+                _lib.call("pdk_prefill_attn_window", qkv.data_ptr(), qkv.stride(0), k.data_ptr(),
+                          rows[0][1], v.data_ptr(), rows[1][1], T, NH, NKV, HD, self.scale, window,
+                          sinks, ao.data_ptr(), stream_handle())
+                return ao
             _lib.call("pdk_prefill_attn", qkv.data_ptr(), qkv.stride(0), kt.data_ptr(),
                       vt.data_ptr(), T, NH, NKV, HD, self.scale, ao.data_ptr(), stream_handle())
             return ao
@@ -183,6 +191,10 @@ class LlamaPrefill:
         ang = pos[:, None] * self.inv[None, :]                     # fp32 angles, [T, HD/2]
         cos, sin = torch.cos(ang)[:, None, :], torch.sin(ang)[:, None, :]
         causal = torch.full((T, T), float("-inf"), device=dev).triu(1)
+        window, sinks = check_window(cfg.window, cfg.sinks)
+        if window:
+            t = torch.arange(T, device=dev)
+            causal.masked_fill_((t <= t[:, None] - window) & (t >= sinks), float("-inf"))
 
         def attention(qkv, k_l, v_l, before):
             q = self._rope(qkv[:, :NH * HD].view(T, NH, HD), cos, sin)

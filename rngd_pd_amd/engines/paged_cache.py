@@ -11,6 +11,12 @@ Layout (bf16): K [L, num_blocks, Hkv, 16, D] and V [L, num_blocks, Hkv, D, 16]
 16-byte units of 8 dims of one token, tiled in the order the decode-attention
 QK tiles read them (k_block_index); V is already in the order the PV tiles
 read. k_block_rows / k_block_tiled convert K blocks to and from token rows.
+
+Requests may share blocks: fork gives new requests the full blocks of a prefix
+(counted; the partly filled one is copied), and a block returns to the pool with
+its last holder. drop_before returns the blocks that a sliding window has left
+behind (their table entries become -1, which attention under that window does not
+read), compact moves what is held to the lowest ids.
 """
 import threading
 
@@ -18,6 +24,7 @@ import numpy as np
 import torch
 
 from ..kernels import handoff as _h
+from ..kernels import pages as _pages
 
 BLOCK = 16
 
@@ -77,6 +84,16 @@ class BlockAllocator:
         with self._lock:
             self._free.extend(reversed(list(blocks)))
 
+    def repack(self, plan):
+        """Calls ``plan`` on the free ids in increasing order, for the ids that
+        become free in exchange for as many of them, the lowest; returns what it
+        returned. Low ids are handed out first from then on."""
+        with self._lock:
+            free = sorted(self._free)
+            freed = plan(free)
+            self._free = sorted(free[len(freed):] + list(freed), reverse=True)
+            return freed
+
 
 class PagedKVCache:
     """One paged K/V cache for all layers plus per-request block tables."""
@@ -93,6 +110,7 @@ class PagedKVCache:
         self.alloc = BlockAllocator(num_blocks, seed)
         self._tables = {}          # req_id -> [block ids]
         self._dev_tables = {}      # req_id -> device int32 tensor
+        self._shared = {}          # block -> holders beyond the first
         self._lock = threading.Lock()
 
     # -- block tables ---------------------------------------------------------
@@ -119,7 +137,90 @@ class PagedKVCache:
         with self._lock:
             blocks = self._tables.pop(req_id, [])
             self._dev_tables.pop(req_id, None)
-        self.alloc.release(blocks)
+            self.alloc.release(self._let_go(blocks))
+
+    def _let_go(self, blocks):
+        """Those of a holder's blocks that nobody else holds; the others lose it."""
+        last = []
+        for b in blocks:
+            more = self._shared.get(b, 0)
+            if more > 1:
+                self._shared[b] = more - 1
+            elif more:
+                del self._shared[b]
+            elif b >= 0:
+                last.append(b)
+        return last
+
+    # -- sharing and moving blocks ----------------------------------------------
+    def fork(self, req_id, new_ids, num_tokens, stream=None):
+        """New requests ``new_ids`` that start with the first ``num_tokens`` tokens
+        of ``req_id``: its full blocks are shared, a partly filled one is copied
+        to a block of each (one launch, on ``stream`` or the current one, ordered
+        after what was written there). Shared blocks are not written again: a
+        request's later tokens go to blocks of its own (ensure)."""
+        new_ids = list(new_ids)
+        full, part = divmod(num_tokens, BLOCK)
+        with self._lock:
+            have = self._tables[req_id]
+            if num_tokens < 0 or len(have) < full + (part > 0):
+                raise ValueError(f"{req_id!r} holds {len(have)} blocks, fewer than {num_tokens} tokens")
+            if part and have[full] < 0:
+                raise ValueError(f"{req_id!r} has dropped the block of token {num_tokens - 1}")
+            if len(set(new_ids)) != len(new_ids) or any(r in self._tables for r in new_ids):
+                raise KeyError(f"{new_ids} are not all new, different requests")
+            own = self.alloc.allocate(len(new_ids)) if part else []
+            try:
+                if own:
+                    _pages.copy_blocks(self.k, self.v, [have[full]] * len(own), own, stream=stream)
+            except BaseException:
+                self.alloc.release(own)
+                raise
+            for i, r in enumerate(new_ids):
+                self._tables[r] = have[:full] + own[i:i + 1]
+                self._dev_tables.pop(r, None)
+            for b in have[:full]:
+                if b >= 0 and new_ids:
+                    self._shared[b] = self._shared.get(b, 0) + len(new_ids)
+
+    def drop_before(self, req_id, num_tokens, keep=0):
+        """Return the request's blocks that hold only tokens from ``keep`` on and
+        before ``num_tokens`` (behind a sliding window, beside its sinks) to the
+        pool; their table entries become -1. How many there were. No step that
+        still reads them may be queued where another stream could fill them."""
+        with self._lock:
+            have = self._tables[req_id]
+            gone = [j for j in range(-(-max(keep, 0) // BLOCK), min(num_tokens // BLOCK, len(have)))
+                    if have[j] >= 0]
+            if gone:
+                free = self._let_go([have[j] for j in gone])
+                for j in gone:
+                    have[j] = -1
+                self._dev_tables.pop(req_id, None)
+                self.alloc.release(free)
+            return len(gone)
+
+    def compact(self, stream=None):
+        """Move held blocks onto the lowest free ids until no free id lies below a
+        held one's; returns how many moved. Tables change: device tables and
+        graphs made before are stale, and no other stream may be using the cache."""
+        with self._lock:
+            moved = {}
+
+            def plan(free):
+                held = sorted({b for t in self._tables.values() for b in t if b >= 0})
+                while len(moved) < len(free) and held and held[-1] > free[len(moved)]:
+                    moved[held.pop()] = free[len(moved)]
+                if moved:
+                    _pages.copy_blocks(self.k, self.v, list(moved), list(moved.values()),
+                                       stream=stream)
+                return list(moved)
+            self.alloc.repack(plan)
+            for t in self._tables.values():
+                t[:] = [moved.get(b, b) for b in t]
+            self._shared = {moved.get(b, b): n for b, n in self._shared.items()}
+            self._dev_tables.clear()
+            return len(moved)
 
     def blocks(self, req_id):
         return list(self._tables[req_id])
@@ -145,12 +246,23 @@ class PagedKVCache:
     # -- frames in and out ----------------------------------------------------
     def write_frame(self, req_id, frame, num_tokens, S, stream=None):
         """Scatter tokens 0..num_tokens-1 of a transport frame [L, 2, Hkv*D*S]."""
+        self._whole(req_id, num_tokens, write=True)
         _h.scatter_paged(frame, self.table(req_id), num_tokens, S, self.k, self.v, stream=stream)
 
     def read_frame(self, req_id, num_tokens, S, frame=None, stream=None):
         """The request's S-wide transport frame (zero for t >= num_tokens)."""
+        self._whole(req_id, num_tokens)
         return _h.gather_paged(self.k, self.v, self.table(req_id), num_tokens, S, frame=frame,
                                stream=stream)
+
+    def _whole(self, req_id, num_tokens, write=False):
+        """Refuses a frame of blocks that were dropped, or to be written over
+        blocks that others hold."""
+        blocks = self._tables[req_id][:-(-num_tokens // BLOCK)]
+        if -1 in blocks:
+            raise ValueError(f"{req_id!r} has dropped blocks of its first {num_tokens} tokens")
+        if write and self._shared and any(b in self._shared for b in blocks):
+            raise ValueError(f"{req_id!r} shares blocks of its first {num_tokens} tokens")
 
     def view(self, req_id, num_tokens, S):
         """What the connector's decode side registers for one request."""

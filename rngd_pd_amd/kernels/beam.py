@@ -34,7 +34,9 @@ def beam_select(logits, scores, n_out=None, eos=None, last_tokens=None, out=None
     nothing above -inf; places that no candidate fills hold token -1, parent -1
     and score -inf.
 
-    ``out``: the three tensors to write. ``workspace``: at least
+    ``out``: the three tensors to write; with n_out = K they may be last_tokens and
+    scores themselves (each request's are read before they are written).
+    ``workspace``: at least
     beam_select_workspace_bytes of device memory for one call at a time (default:
     allocated by the call on its stream)."""
     if not isinstance(logits, torch.Tensor) or not logits.is_cuda:

@@ -51,6 +51,10 @@ class ContinuousScheduler:
     def __init__(self, B, decoder, cache, produce, admit_min=1, loaders=None, max_blocks=None,
                  use_graphs=True, on_token=None, device=None):
         self.B, self.dec, self.cache, self.produce = B, decoder, cache, produce
+        # Every step has ended when the next one is set up: nothing queued reads
+        # the blocks that a window leaves behind.
+        cfg = getattr(decoder, "cfg", None)
+        self.window, self.sinks = getattr(cfg, "window", None), getattr(cfg, "sinks", 0)
         self.admit_min = admit_min
         self.on_token = on_token
         self.use_graphs = use_graphs
@@ -244,6 +248,8 @@ class ContinuousScheduler:
             s = self.slots[i]
             req = s["item"]["req_id"]
             self.cache.ensure(req, s["pos"] + 1)                 # a new block every 16 tokens
+            if self.window:                                      # and one behind the window back
+                self.cache.drop_before(req, s["pos"] + 1 - self.window, self.sinks)
             blocks = self.cache.blocks(req)
             host[row] = s["cur"]
             host[B + row] = s["pos"] + 1
