@@ -99,9 +99,11 @@ struct Window {
   int lo, sinks, sink_end, shift;
 };
 
-__device__ __forceinline__ Window window_of(int ctx, int window, int sinks) {
+// `capacity`: the tokens the table holds. A window that starts behind them (ctx is
+// the device's, any value) starts there: nothing of it is left either way.
+__device__ __forceinline__ Window window_of(int ctx, int capacity, int window, int sinks) {
   Window w;
-  w.lo = max(ctx, 0) - window;
+  w.lo = min(max(ctx, 0) - window, capacity);
   w.sinks = sinks;
   w.sink_end = (sinks + kSpan - 1) & ~(kSpan - 1);
   w.shift = max((max(w.lo, 0) & ~(kSpan - 1)) - w.sink_end, 0);
@@ -577,7 +579,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   typedef const __attribute__((address_space(4))) int32_t* ctable_t;
   const ctable_t ctab = (ctable_t)table;
   Window win{};
-  if constexpr (kWin) win = window_of(ctx_raw, window, sinks);
+  if constexpr (kWin) win = window_of(ctx_raw, a.max_blocks * 16, window, sinks);
   auto token_of = [&](int v) { return kWin && v >= win.sink_end ? v + win.shift : v; };
   auto ids = [&](int va, int* id) {
     const int sa = token_of(va), sb = token_of(va + stride);

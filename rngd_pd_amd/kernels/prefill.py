@@ -31,6 +31,15 @@ def _rows(t, T):
     return t, ld
 
 
+def _overlap(a, b):
+    """Whether the memory that a and b span has bytes in common."""
+    def span(t):
+        size = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1 if t.numel() else 0
+        return t.data_ptr(), t.data_ptr() + size * t.element_size()
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
 def prefill_attention(q, k, v, scale=1.0, window=None, sinks=0, out=None, stream=None):
     """Causal GQA attention over one prompt of T tokens -> out [T, Hq, 128] bf16.
 
@@ -62,6 +71,8 @@ def prefill_attention(q, k, v, scale=1.0, window=None, sinks=0, out=None, stream
         need_device(dev, out, "out")
         if out.shape != q.shape or not out.is_contiguous() or out.data_ptr() % 16:
             raise ValueError(f"out must be contiguous and 16-byte aligned {tuple(q.shape)}")
+        if any(_overlap(out, t) for t in (q, k, v)):
+            raise ValueError("out must not overlap q, k or v")
     if T == 0:
         return out
     (q, q_ld), (k, k_ld), (v, v_ld) = _rows(q, T), _rows(k, T), _rows(v, T)

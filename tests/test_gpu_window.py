@@ -136,6 +136,28 @@ def test_rows_without_tokens_and_contexts_past_the_table(cuda):
         assert torch.equal(ck, ck2) and torch.equal(cv, cv2) and torch.equal(got, want)
 
 
+def test_any_length_on_the_device_stays_in_bounds(cuda):
+    """Lengths are device data: whatever they hold, only the table's tokens are
+    read, and a window that starts behind them leaves the sinks."""
+    from rngd_pd_amd import kernels as K
+    rng = np.random.default_rng(18)
+    ctx = [2 ** 31 - 1, -(2 ** 31), -1, 2 ** 31 - 20, 10 ** 9, 64]
+    tables, nb = paged(rng, [64] * 6, 8)
+    q, ck, cv = _inputs(rng, 6, 32, 8, nb)
+    tab, ctx_d = torch.from_numpy(tables).to(cuda), torch.tensor(ctx, dtype=torch.int32, device=cuda)
+    for window, sinks in ((10, 5), (1 << 30, 0), (40, 0)):
+        want, bound = decode_reference(q, ck, cv, tables, ctx[-1:] * 6, window, sinks, SCALE)
+        got = K.decode_attention(q, ck, cv, tab, ctx_d, 64, scale=SCALE, window=window, sinks=sinks)
+        assert_within(got[5:], want[5:], bound[5:])
+        assert (got[1:3] == 0).all() and torch.isfinite(got).all()
+        if sinks:
+            few, few_bound = decode_reference(q, ck, cv, tables, [5] * 6, 5, 0, SCALE)
+            for b in (0, 3, 4):
+                assert_within(got[b], few[b], few_bound[b])
+        elif window == 40:
+            assert (got[[0, 3, 4]] == 0).all()
+
+
 def test_streams_that_share_blocks(cuda):
     """Four rows of one request at consecutive positions (a verification step):
     each sees the others' new tokens, inside its own window."""
@@ -377,3 +399,5 @@ def test_refusals(cuda):
         K.prefill_attention(q, q[:, :5], q[:, :5])       # 32 heads over 5
     with pytest.raises(TypeError):
         K.prefill_attention(q, q[:, :8].float(), q[:, :8])
+    with pytest.raises(ValueError, match="overlap"):
+        K.prefill_attention(q, ck[:1, :, 0], ck[1:2, :, 0], out=q)
