@@ -41,8 +41,14 @@ class BeamSearch:
             raise ValueError(f"{R} requests of {K} beams for a decoder of {self.dec.max_batch} rows")
         if max_new < 1 or any(n < 1 for _, n, _ in requests):
             raise ValueError("max_new and the prompts' lengths must be at least 1")
+        with torch.cuda.device(self.dec.device):
+            return self._search(requests, max_new, length_penalty)
+
+    def _search(self, requests, max_new, length_penalty):
+        R, K = len(requests), self.K
         rows = [[("beam", req, k) for k in range(K)] for req, _, _ in requests]
         ids = [r for row in rows for r in row]
+        captured = self.dec._captured
         forked = []
         try:
             for (req, n, _), row in zip(requests, rows):
@@ -54,6 +60,7 @@ class BeamSearch:
         finally:
             # What was queued may still use the blocks: they go back when it is done.
             torch.cuda.synchronize(self.dec.device)
+            self.dec._captured = captured                # this search's graph is gone
             for r in forked:
                 self.cache.free(r)
         return [self._beams(hist_tokens[:, r], hist_parents[:, r], scores[r], length_penalty)

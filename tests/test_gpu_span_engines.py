@@ -260,3 +260,17 @@ def test_beam_search_refusals(cuda):
         s.search([("r", 20, 1)], 60)
     assert cache.alloc.free_blocks() == free
     assert math.isfinite(s.search([("r", 10, 1)], 2, length_penalty=1.0)[0][0][1])
+
+
+def test_a_longer_search_after_a_captured_one(cuda):
+    """A search's graph dies with it: the decoder's workspace may grow again."""
+    from rngd_pd_amd.engines.beam_search import BeamSearch
+    from rngd_pd_amd.engines.paged_cache import PagedKVCache
+    cache = PagedKVCache(2, 160, 2, D, device=cuda)
+    dec = _decoder(_cfg(), cache, max_batch=2)
+    cache.allocate("r", 200)
+    s = BeamSearch(dec, 2)
+    first = s.search([("r", 10, 1)], 5)
+    s.search([("r", 150, 1)], 400)                      # its contexts are split
+    assert s.search([("r", 10, 1)], 5)[0][0][0] == first[0][0][0]
+    assert cache.alloc.free_blocks() == 160 - 13
