@@ -55,7 +55,7 @@ __global__ __launch_bounds__(256) void copy_blocks_kernel(uint16_t* ck, uint16_t
 // PDK_OK if the pairs' ids are blocks of the cache, no block is written twice
 // and none is both read and written, so that the copies' order does not matter.
 int check_pairs(const int32_t* src, const int32_t* dst, int n, int num_blocks) {
-  std::vector<uint64_t> written((num_blocks + 63) / 64, 0);
+  std::vector<uint64_t> written(((int64_t)num_blocks + 63) / 64, 0);
   auto bit = [](int32_t id) { return 1ull << (id & 63); };
   for (int i = 0; i < n; ++i) {
     PDK_REQUIRE(src[i] >= 0 && src[i] < num_blocks && dst[i] >= 0 && dst[i] < num_blocks,

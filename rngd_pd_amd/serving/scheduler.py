@@ -247,9 +247,9 @@ class ContinuousScheduler:
         for row, i in enumerate(live):
             s = self.slots[i]
             req = s["item"]["req_id"]
-            self.cache.ensure(req, s["pos"] + 1)                 # a new block every 16 tokens
-            if self.window:                                      # and one behind the window back
+            if self.window:                                      # blocks behind the window back,
                 self.cache.drop_before(req, s["pos"] + 1 - self.window, self.sinks)
+            self.cache.ensure(req, s["pos"] + 1)                 # a new block every 16 tokens
             blocks = self.cache.blocks(req)
             host[row] = s["cur"]
             host[B + row] = s["pos"] + 1
