@@ -277,6 +277,8 @@ class PagedRequestView:
         self.num_tokens, self.S = num_tokens, S
         if req_id not in cache._tables:
             cache.allocate(req_id, num_tokens)
+        else:
+            cache._whole(req_id, num_tokens, write=True)
 
     @property
     def table(self):

@@ -175,7 +175,8 @@ def _window_attention(q, new, cache_k, cache_v, block_tables, ctx_lens, max_ctx,
     if not fine:
         _check_window_operands(q, new, cache_k, cache_v, block_tables, ctx_lens, out, workspace)
     width = block_tables.shape[1]
-    window, sinks, need = _window_plan(B, Hq, D, int(max_ctx), width * 16, window, sinks)
+    window, sinks, need = _window_plan(B, Hq, D, int(max_ctx), width * 16,
+                                       None if window is None else int(window), int(sinks))
     if out is None:
         out = torch.empty_like(q)
     ws_ptr, ws_bytes = None, 0

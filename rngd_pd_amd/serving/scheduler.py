@@ -248,7 +248,10 @@ class ContinuousScheduler:
             s = self.slots[i]
             req = s["item"]["req_id"]
             if self.window:                                      # blocks behind the window back,
-                self.cache.drop_before(req, s["pos"] + 1 - self.window, self.sinks)
+                behind = (s["pos"] + 1 - self.window) // 16
+                if behind > s.get("behind", 0):
+                    s["behind"] = behind
+                    self.cache.drop_before(req, behind * 16, self.sinks)
             self.cache.ensure(req, s["pos"] + 1)                 # a new block every 16 tokens
             blocks = self.cache.blocks(req)
             host[row] = s["cur"]

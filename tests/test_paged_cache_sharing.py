@@ -114,6 +114,19 @@ def test_drop_before_keeps_sinks_and_the_window(cache):
         cache.drop_before("a", 10)
 
 
+def test_views_refuse_shared_and_dropped_blocks(cache):
+    """A view's blocks are written by a transport: nobody else may hold them."""
+    cache.allocate("a", 40)
+    cache.view("a", 40, 48)
+    cache.fork("a", ["b"], 32)
+    with pytest.raises(ValueError, match="shares"):
+        cache.view("a", 40, 48)
+    cache.free("b")
+    cache.drop_before("a", 16)
+    with pytest.raises(ValueError, match="dropped"):
+        cache.view("a", 40, 48)
+
+
 def test_fork_of_a_dropped_last_block_is_refused(cache):
     cache.allocate("a", 48)
     cache.drop_before("a", 48)
