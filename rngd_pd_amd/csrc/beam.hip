@@ -16,11 +16,11 @@
 // n best of a wavefront's values: the n-th largest of the 64 lanes' own maxima
 // bounds the n-th largest value from below, bit by bit with one ballot each until
 // exactly n lanes reach it (some 10 to 15 bits). Mostly a few more than n values
-// then reach the bound; they are compacted into LDS and ranked by counting. Where
-// equal values let more than 64 reach it, the bound is taken again over unique
-// 64-bit keys (the value in an order-preserving code above the complement of the
-// token): only n lanes reach that one, so at most n times a lane's values do,
-// whatever the logits are.
+// then reach the bound, all in those lanes; they are compacted into LDS and ranked
+// by counting. Where equal values let more than 64 reach it, the best is taken n
+// times: the largest of the lanes' best keys (the value in an order-preserving code
+// above the complement of the token, so that no two are equal), after which the lane
+// that had it gets its next one, all lanes reading one unit of its values each.
 #include <math.h>
 
 #include <algorithm>
@@ -37,6 +37,9 @@ constexpr int kMaxOut = 32;
 constexpr int kWaves = 4;                 // of a part workgroup, each a part of its own
 constexpr int kMaxLists = 8;              // parts of a row per lane of the join
 constexpr int kMaxVocab = 1 << 20;
+constexpr int kBusyWaves = 4096;          // four for each SIMD
+constexpr int kMaxSteps = 16;             // of a part
+constexpr uint32_t kLeastCode = 0x00800000u;   // of the lowest finite value
 
 typedef unsigned long long Key;
 
@@ -56,11 +59,15 @@ __device__ __forceinline__ Key key_of(float x, uint32_t token) {
   return c ? ((Key)c << 32) | (0xffffffffu - token) : 0ull;
 }
 
-// 2^y for y <= 0: 2^k p(f), y = k + f, |f| <= 1/2, p the polynomial of degree 7
-// that meets 2^f at the 8 Chebyshev nodes (off by less than 6e-11 of it). Down to
-// y = -1000; the callers clamp.
-__device__ __forceinline__ double exp2_neg(double y) {
-  const double k = rint(y), f = y - k;
+constexpr double kLog2e = 1.4426950408889634074;
+
+// e^x for |x| <= 700: 2^k p(f), x log2(e) = k + f, |f| <= 1/2, p the polynomial
+// of degree 7 that meets 2^f at the 8 Chebyshev nodes (off by less than 6e-11 of
+// it). k is left in the low bits of a sum with 3 * 2^51 and added to the exponent.
+__device__ __forceinline__ double exp_of(double x) {
+  constexpr double kRound = 6755399441055744.0;
+  const double t = fma(x, kLog2e, kRound);
+  const double f = fma(x, kLog2e, kRound - t);
   double p = 1.5303701161442145e-05;
   p = fma(p, f, 0.00015469729221575116);
   p = fma(p, f, 0.0013333478471058548);
@@ -69,20 +76,16 @@ __device__ __forceinline__ double exp2_neg(double y) {
   p = fma(p, f, 0.24022651213498578);
   p = fma(p, f, 0.6931471805568296);
   p = fma(p, f, 0.9999999999595621);
-  return __builtin_amdgcn_ldexp(p, (int)k);
+  return __hiloint2double(__double2hiint(p) + (__double2loint(t) << 20), __double2loint(p));
 }
 
-// ln x for x >= 1/2: a 32-bit logarithm and one Newton step in 64 bits, which
-// leaves the square of its error and exp2_neg's.
+// ln x for 1/2 <= x <= 2^64: a 32-bit logarithm and one Newton step in 64 bits,
+// which leaves the square of its error and exp_of's.
 __device__ __forceinline__ double log_of(double x) {
   const double y = (double)__logf((float)x);
-  const double e = x * exp2_neg(-y * 1.4426950408889634074) - 1.0;
+  const double e = x * exp_of(-y) - 1.0;
   return y + (e - 0.5 * e * e);
 }
-
-constexpr double kLog2e = 1.4426950408889634074;
-
-__device__ __forceinline__ double exp_neg(double x) { return exp2_neg(fmax(x, -690.0) * kLog2e); }
 
 // x reduced over the wavefront by f, the same in every lane: halves and quarters
 // exchanged by the lane swaps, rows of 16 lanes by rotations (no LDS round trip, a
@@ -145,20 +148,9 @@ __device__ __forceinline__ U nth_largest(U mine, int n) {
   return bound;
 }
 
-// x[i], i a lane's own: halved bit by bit with masks (a choice between registers
-// would be made through memory).
-template <int kN>
-__device__ __forceinline__ float pick(const float (&x)[kN], int i) {
-  uint32_t y[kN];
-#pragma unroll
-  for (int j = 0; j < kN; ++j) y[j] = __float_as_uint(x[j]);
-#pragma unroll
-  for (int w = kN / 2, bit = 0; w; w >>= 1, ++bit) {
-    const uint32_t odd = 0u - ((i >> bit) & 1u);
-#pragma unroll
-    for (int j = 0; j < w; ++j) y[j] = (y[2 * j + 1] & odd) | (y[2 * j] & ~odd);
-  }
-  return __uint_as_float(y[0]);
+// Bits of `who` below the lane's own.
+__device__ __forceinline__ int below(uint64_t who) {
+  return __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
 }
 
 // What the wavefront's lanes wrote to LDS is there for all of them.
@@ -198,105 +190,228 @@ struct Part {
   double top, sum;
 };
 
-// Values e .. e + kEl - 1 of the row, those from V on as -inf. Rows of odd lengths
-// start anywhere: the 16-byte loads take any address, and a row's parts and sums
-// do not depend on where it lies (equal rows have equal totals).
-template <typename T>
-__device__ __forceinline__ void load_vals(const T* row, int e, int V, float* x) {
-  constexpr int kEl = 16 / sizeof(T);
-  if (e + kEl <= V) {
-    uint32_t w[4];
-    __builtin_memcpy(w, row + e, 16);
+// 16 bytes of a row, the values in their own type.
+struct Unit {
+  uint32_t w[4];
+};
+
+// f(value) of a unit's values in turn.
+template <typename T, class F>
+__device__ __forceinline__ void each_value(const Unit& u, F f) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (sizeof(T) == 2) {
-        x[2 * i] = pdk::bf16_to_f32(w[i] & 0xffffu);
-        x[2 * i + 1] = pdk::bf16_to_f32(w[i] >> 16);
-      } else {
-        x[i] = __uint_as_float(w[i]);
-      }
-    }
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < kEl; ++i) {
-    x[i] = -INFINITY;
-    if (e + i < V) {
-      if constexpr (sizeof(T) == 2) x[i] = pdk::bf16_to_f32(row[e + i]);
-      else x[i] = row[e + i];
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 2) {
+      f(2 * i, __uint_as_float(u.w[i] << 16));
+      f(2 * i + 1, __uint_as_float(u.w[i] & 0xffff0000u));
+    } else {
+      f(i, __uint_as_float(u.w[i]));
     }
   }
 }
 
-// grid: x = kWaves parts, y = row. T is uint16_t (bf16) or float; a lane holds
-// kVals values.
-template <typename T, int kVals>
+// The unit whose first value is the row's value e: it starts at unit_at(e), and the
+// values in front of e, which the unit before it holds, are -inf, all of them where
+// e is V or more. Rows of odd lengths start anywhere: the 16-byte loads take any
+// address, and a row's parts and sums do not depend on where it lies (equal rows
+// have equal totals).
+template <typename T>
+__device__ __forceinline__ int unit_at(int e, int V) {
+  return min(e, max(V - (int)(16 / sizeof(T)), 0));
+}
+
+template <typename T>
+__device__ __forceinline__ void drop_front(Unit& u, int n) {
+  constexpr uint32_t kNone = sizeof(T) == 2 ? 0xff80u : 0xff800000u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 2) {
+      if (2 * i < n) u.w[i] = (u.w[i] & 0xffff0000u) | kNone;
+      if (2 * i + 1 < n) u.w[i] = (u.w[i] & 0xffffu) | (kNone << 16);
+    } else {
+      if (i < n) u.w[i] = kNone;
+    }
+  }
+}
+
+// A row of fewer values than a unit: those in front of value e dropped as above.
+template <typename T>
+__device__ __forceinline__ Unit short_row(const T* p, int V) {
+  T x[16 / sizeof(T)];
+#pragma unroll
+  for (int i = 0; i < (int)(16 / sizeof(T)); ++i) {
+    if constexpr (sizeof(T) == 2) x[i] = i < V ? p[i] : 0xff80;
+    else x[i] = i < V ? p[i] : -INFINITY;
+  }
+  Unit u;
+  __builtin_memcpy(&u, x, 16);
+  return u;
+}
+
+// grid: x = kWaves parts, y = row. T is uint16_t (bf16) or float. A part is `steps`
+// times 64 lanes' kVals values, the next step's on their way while one's are summed;
+// bound by the 64-bit operations of that (14 for a value, of some 20 instructions in
+// all). Of the steps only each lane's maximum is kept: the selection reads the few
+// lanes' values it needs again, from LDS if there is one step only, else from memory.
+// kShort: V is less than a unit.
+template <typename T, int kVals, bool kMany, bool kShort = false>
 __global__ __launch_bounds__(64 * kWaves) void beam_part_kernel(const T* logits, int64_t ld, int V,
-                                                                int n, int n_parts,
+                                                                int n, int n_parts, int steps,
                                                                 const int32_t* last_tokens,
                                                                 int eos, Part* parts, Key* keys) {
-  constexpr int kEl = 16 / sizeof(T), kGroups = kVals / kEl;
-  __shared__ Key lists[kWaves][kMaxOut * kVals];
+  constexpr int kEl = 16 / sizeof(T), kUnits = kVals / kEl, kStep = 64 * kVals;
+  static_assert(!kMany || kMaxSteps * kUnits <= 64, "one unit of a lane's for every lane");
+  __shared__ Unit held[kWaves][kMany ? 1 : kUnits * 64];         // [unit][lane]
+  __shared__ float most[kWaves][kMany ? kMaxSteps * 64 : 1];     // [step][lane]
+  __shared__ Key lists[kWaves][64];
+  __shared__ uint16_t places[kWaves][64];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int row = blockIdx.y, part = blockIdx.x * kWaves + wave;
   if (part >= n_parts) return;
   if (last_tokens && last_tokens[row] == eos) return;   // an ended beam's logits count for nothing
   const T* p = logits + (int64_t)row * ld;
-  float x[kVals];
-  const int e0 = part * (64 * kVals) + lane * kEl;
+  const int first = part * (kMany ? steps : 1) * kStep;  // of the part's values
+  if (kMany) steps = min(steps, (V - first + kStep - 1) / kStep);
+  else steps = 1;
+  auto value_at = [&](int step, int unit, int of) { return first + step * kStep + (unit * 64 + of) * kEl; };
+  auto load = [&](int e) __attribute__((always_inline)) {
+    Unit u;
+    if constexpr (kShort) u = short_row(p, V);
+    else __builtin_memcpy(&u, p + unit_at<T>(e, V), 16);
+    return u;
+  };
+  auto load_step = [&](Unit* u, int step) __attribute__((always_inline)) {
+    if (!kShort && first + (step + 1) * kStep <= V) {
+      const T* q = p + first + step * kStep;
 #pragma unroll
-  for (int i = 0; i < kGroups; ++i) load_vals(p, e0 + i * 64 * kEl, V, x + i * kEl);
-  float mine = x[0];
+      for (int i = 0; i < kUnits; ++i) __builtin_memcpy(&u[i], q + (i * 64 + lane) * kEl, 16);
+      return;
+    }
 #pragma unroll
-  for (int i = 1; i < kVals; ++i) mine = __builtin_elementwise_maximum(mine, x[i]);
-  const float top = wave_all(mine, [](float a, float b) { return __builtin_elementwise_maximum(a, b); });
-  double sum = 0.0;
-  if (top < INFINITY && top > -INFINITY) {
+    for (int i = 0; i < kUnits; ++i) {
+      const int e = value_at(step, i, lane);
+      u[i] = load(e);
+      drop_front<T>(u[i], e - unit_at<T>(e, V));
+    }
+  };
+  // sum is that of e^(x - ref), ref the first step's maximum: 64 bits hold what lies
+  // up to 600 above it, and only beyond that it is taken anew.
+  float ref = -INFINITY, best = -INFINITY;               // of the part; of the lane
+  double sum = 0.0;                                      // the lane's
+  auto use = [&](const Unit* u, int step) __attribute__((always_inline)) {
+    float m = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < kVals; ++i) sum += exp_neg((double)x[i] - (double)top);
-    sum = wave_sum(sum);
-  } else if (!(top == -INFINITY)) {
-    sum = NAN;
+    for (int i = 0; i < kUnits; ++i) {
+      if (!kMany) held[wave][i * 64 + lane] = u[i];
+      each_value<T>(u[i], [&](int, float x) { m = __builtin_elementwise_maximum(m, x); });
+    }
+    if (kMany) most[wave][step * 64 + lane] = m;
+    best = __builtin_elementwise_maximum(best, m);
+    if (__ballot(m > ref + 600.f)) {
+      const float top = wave_all(m, [](float a, float b) { return __builtin_elementwise_maximum(a, b); });
+      if (!(top < INFINITY)) {                           // the part counts for nothing (below)
+        ref = 0.f;
+      } else {
+        if (kMany) sum *= exp_of(fmax((double)ref - (double)top, -690.0));
+        ref = top;
+      }
+    }
+    if (ref == -INFINITY) return;                        // nothing above -inf yet
+    // Clamped in 32 bits, near enough to ref to be exact there.
+    if (fabsf(ref) <= 4096.f) {
+      const double r = ref;
+#pragma unroll
+      for (int i = 0; i < kUnits; ++i)
+        each_value<T>(u[i], [&](int, float x) {
+          sum += exp_of((double)__builtin_amdgcn_fmed3f(x, ref - 690.f, ref + 690.f) - r);
+        });
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < kUnits; ++i) {
+        const int e = value_at(step, i, lane), skip = kMany ? e - unit_at<T>(e, V) : 0;
+        each_value<T>(kMany ? load(e) : held[wave][i * 64 + lane], [&](int j, float x) {
+          sum += j < skip ? 0.0 : exp_of((double)__builtin_amdgcn_fmed3f(x - ref, -690.f, 690.f));
+        });
+      }
+    }
+  };
+  {
+    Unit u[kUnits];
+    load_step(u, 0);
+    if constexpr (kMany) {
+      Unit v[kUnits];
+#pragma unroll 1
+      for (int step = 0; step < steps; step += 2) {
+        if (step + 1 < steps) load_step(v, step + 1);
+        use(u, step);
+        if (step + 1 >= steps) break;
+        if (step + 2 < steps) load_step(u, step + 2);
+        use(v, step + 1);
+      }
+    } else {
+      use(u, 0);
+    }
   }
+  sum = wave_sum(sum);
+  const float top = wave_all(best, [](float a, float b) { return __builtin_elementwise_maximum(a, b); });
+  if (kMany) sum *= exp_of(fmax((double)ref - (double)top, -690.0));
+  if (!(top < INFINITY)) sum = NAN;
   const int64_t at = (int64_t)row * n_parts + part;
   if (lane == 0) parts[at] = Part{(double)top, sum};
 
-  // The values that reach the bound; all but -inf where there are few enough.
+  // The values that reach the bound, of the lanes' steps whose maximum does; all but
+  // -inf where there are few enough.
+  auto unit_of = [&](int step, int unit, int of) {
+    return kMany ? load(value_at(step, unit, of)) : held[wave][unit * 64 + of];
+  };
   Key* list = lists[wave];
-  const uint32_t bound = nth_largest(code_of(mine), n);
-  const float least = bound ? value_of(bound) : -3.402823466e38f;
-  auto token = [&](int i) { return (uint32_t)(e0 + i / kEl * (64 * kEl) + i % kEl); };
-  uint32_t mask = 0;                                     // bit i: value i reaches the bound
-#pragma unroll
-  for (int i = 0; i < kVals; ++i) mask |= x[i] >= least ? 1u << i : 0u;
-  int c = 0;
-  for (uint64_t who; (who = __ballot(mask != 0)) && c <= 64;) {   // a value of every such lane
-    const int i = __builtin_ctz(mask | 0x80000000u);
-    const float v = pick(x, i);
-    const int to = c + __popcll(who & ((1ull << lane) - 1));
-    if (mask && to < 64) list[to] = key_of(v, token(i));
-    mask &= mask - 1;
-    c += __popcll(who);
+  uint16_t* place = places[wave];
+  const uint32_t code = code_of(best), bound = max(nth_largest(code, n), kLeastCode);
+  const float least = value_of(bound);
+  int c = 0, m = 0;
+  for (int s = 0; s < steps; ++s) {
+    const bool in = (kMany ? code_of(most[wave][s * 64 + lane]) : code) >= bound;
+    const uint64_t who = __ballot(in);
+    const int to = m + below(who);
+    if (in && to < 64) place[to] = (uint16_t)(s * 64 + lane);
+    m += __popcll(who);
   }
-  if (c > 64) {                                          // equal values
-    Key best = 0;
+  wave_sync();
+  if (m > 64) c = 65;
 #pragma unroll 1
-    for (int i = 0; i < kVals; ++i) {
-      Key k = 0;
-#pragma unroll
-      for (int j = 0; j < kVals; ++j)
-        if (j == i) k = key_of(x[j], token(j));
-      best = k > best ? k : best;
-    }
-    const Key b = nth_largest(best, n);
-    c = 0;
-#pragma unroll
-    for (int i = 0; i < kVals; ++i) {
-      const Key k = key_of(x[i], token(i));
-      const bool in = k >= (b ? b : 1);
-      const uint64_t who = __ballot(in);
-      if (in) list[c + __popcll(who & ((1ull << lane) - 1))] = k;
-      c += __popcll(who);
+  for (int t0 = 0; t0 < m * kUnits && c <= 64; t0 += 64) {
+    const int t = min(t0 + lane, m * kUnits - 1), unit = t % kUnits, at = place[t / kUnits];
+    const int e = value_at(at >> 6, unit, at & 63), start = unit_at<T>(e, V);
+    each_value<T>(unit_of(at >> 6, unit, at & 63), [&](int i, float x) {
+      const bool in = t0 + lane < m * kUnits && x >= least && (!kMany || start + i >= e);
+      const uint64_t which = __ballot(in);
+      const int to = c + below(which);
+      if (in && to < 64) list[to] = key_of(x, start + i);
+      c += __popcll(which);
+    });
+  }
+  if (c > 64) {                                          // many equal values: one by one
+    auto best_of = [&](Key& k1, int step, int unit, int of, Key last) __attribute__((always_inline)) {
+      const int e = value_at(step, unit, of), start = unit_at<T>(e, V);
+      each_value<T>(unit_of(step, unit, of), [&](int i, float x) {
+        const Key k = key_of(x, start + i);
+        k1 = k > k1 && k < last && (!kMany || start + i >= e) ? k : k1;
+      });
+    };
+    auto larger = [](Key a, Key b) { return a > b ? a : b; };
+    Key mine = 0;                                        // the lane's best that is not taken yet
+#pragma unroll 1
+    for (int i = 0; i < steps * kUnits; ++i) best_of(mine, i / kUnits, i % kUnits, lane, ~0ull);
+#pragma unroll 1
+    for (c = 0; c < n; ++c) {
+      const Key taken = wave_all(mine, larger);
+      if (!taken) break;
+      list[c] = taken;
+      // All lanes look for the next of the lane that had it.
+      const int of = __builtin_ctzll(__ballot(mine == taken));
+      Key next = 0;
+      if (lane < steps * kUnits) best_of(next, lane / kUnits, lane % kUnits, of, taken);
+      next = wave_all(next, larger);
+      if (lane == of) mine = next;
     }
   }
   wave_sync();
@@ -328,6 +443,7 @@ __global__ __launch_bounds__(64 * kMaxBeams) void beam_join_kernel(
     // the lanes' own best heads hold any of the n best: those of at most n lanes.
     const Key* kp = keys + (int64_t)row * n_parts * n;
     const Part* pp = parts + (int64_t)row * n_parts;
+    // Where there are fewer than 64, the lanes' keys are the next of them.
     Key mine = 0;
     double top = -INFINITY, sum = 0.0;
 #pragma unroll 1
@@ -336,12 +452,14 @@ __global__ __launch_bounds__(64 * kMaxBeams) void beam_join_kernel(
       mine = head > mine ? head : mine;
       top = fmax(top, pp[s].top);
     }
+    const int next = lane / n_parts;
+    if (next && next < n) mine = kp[(lane - next * n_parts) * n + next];
     top = wave_all(top, [](double a, double b) { return fmax(a, b); });
 #pragma unroll 1
     for (int s = lane; s < n_parts; s += 64) {
       const Part q = pp[s];
       // NaN in q.sum stays; a part without a finite value adds nothing.
-      sum += q.sum != 0.0 ? q.sum * exp_neg(q.top - top) : 0.0;
+      sum += q.sum != 0.0 ? q.sum * exp_of(fmax(q.top - top, -690.0)) : 0.0;
     }
     const double log_sum = log_of(wave_sum(sum));        // beside the maximum: it may be any size
     // By the codes first; the tokens count only where equal codes leave too many.
@@ -357,7 +475,7 @@ __global__ __launch_bounds__(64 * kMaxBeams) void beam_join_kernel(
     for (int s = lane; s - lane < n_parts; s += 64) {
       const bool in = s < n_parts && kp[s * n] >= least;
       const uint64_t who = __ballot(in);
-      if (in) lists[k][m + __popcll(who & ((1ull << lane) - 1))] = (uint16_t)s;
+      if (in) lists[k][m + below(who)] = (uint16_t)s;
       m += __popcll(who);
     }
     wave_sync();
@@ -374,7 +492,7 @@ __global__ __launch_bounds__(64 * kMaxBeams) void beam_join_kernel(
       for (int x = 0; x < 4; ++x) {
         const bool in = q[x] >= least;
         const uint64_t who = __ballot(in);
-        if (in) list[k][c + __popcll(who & ((1ull << lane) - 1))] = q[x];
+        if (in) list[k][c + below(who)] = q[x];
         c += __popcll(who);
       }
       if (c <= kList - 256 && i0 + 256 < m * n) continue;
@@ -494,17 +612,28 @@ __global__ __launch_bounds__(256) void beam_reorder_kernel(const int32_t* parent
     if (moves[k] && u < block_units) pdk::st16(base + place[k] * block, x[k]);
 }
 
-// Values of a lane: 32, or 16 where rows are too few for 32 to give every SIMD two
-// wavefronts (128256 bf16 or fp32 values a row, in us with 16 and with 32: 4 rows
-// 13.5 and 14.9, 64 rows 16.8 and 15.8, 256 fp32 rows 49.6 and 44.6).
-int lane_vals(int rows, int V) {
-  const bool many = (int64_t)rows * ((V + 2047) / 2048) >= 2048;
-  return many || V > kMaxVocab / 2 ? 32 : 16;
-}
+// How rows are cut into parts (times of both launches, 128256 values a row, in us).
+// Up to four wavefronts for each SIMD a part is one step: 16 values a lane, or 32
+// where that still gives every SIMD two wavefronts (4 rows 13.5 and 14.9, 64 rows
+// 16.8 and 15.2, 16.7 as two steps of 16). Beyond, steps of 16, as many as leave
+// four wavefronts for each SIMD, all of them resident (256 fp32 rows: 38.7, steps of
+// 32 40.8, one step of 32 a part 43.9).
+struct Cut {
+  int vals, steps, n_parts;
+};
 
-int parts_of(int rows, int V) {
-  const int part = 64 * lane_vals(rows, V);
-  return (V + part - 1) / part;
+Cut cut_of(int rows, int V) {
+  Cut c;
+  const int64_t waves = (int64_t)rows * ((V + 2047) / 2048);
+  c.vals = waves <= kBusyWaves && (waves >= 2048 || V > kMaxVocab / 2) ? 32 : 16;
+  c.steps = 1;
+  if (waves > kBusyWaves) {
+    const int64_t w16 = (int64_t)rows * ((V + 1023) / 1024);
+    c.steps = (int)std::min<int64_t>((w16 + kBusyWaves - 1) / kBusyWaves, kMaxSteps);
+  }
+  const int part = 64 * c.vals * c.steps;
+  c.n_parts = (V + part - 1) / part;
+  return c;
 }
 
 int check_select(int R, int K, int V, int n) {
@@ -527,7 +656,7 @@ int check_select(int R, int K, int V, int n) {
 extern "C" int64_t pdk_beam_select_workspace_bytes(int R, int K, int V, int n) {
   pdk::clear_error();
   if (check_select(R, K, V, n)) return 0;
-  return (int64_t)R * K * parts_of(R * K, V) * (sizeof(Part) + n * sizeof(Key));
+  return (int64_t)R * K * cut_of(R * K, V).n_parts * (sizeof(Part) + n * sizeof(Key));
 }
 
 extern "C" int pdk_beam_select(const void* logits, int elem_bytes, int64_t ld, int R, int K, int V,
@@ -545,22 +674,29 @@ extern "C" int pdk_beam_select(const void* logits, int elem_bytes, int64_t ld, i
   PDK_REQUIRE(workspace && workspace_bytes >= need && pdk::aligned16(workspace),
               "workspace of %lld bytes needed (got %lld)", (long long)need,
               (long long)workspace_bytes);
-  const int rows = R * K, n_parts = parts_of(rows, V), vals = lane_vals(rows, V);
+  const int rows = R * K;
+  const Cut cut = cut_of(rows, V);
+  const int n_parts = cut.n_parts;
   Part* parts = static_cast<Part*>(workspace);
   Key* keys = reinterpret_cast<Key*>(parts + (int64_t)rows * n_parts);
   const dim3 grid((n_parts + kWaves - 1) / kWaves, rows), block(64 * kWaves);
   hipStream_t st = pdk::as_stream(stream);
   auto launch = [&](auto kern, auto x) {
-    hipLaunchKernelGGL(kern, grid, block, 0, st, x, ld, V, n, n_parts, last_tokens, eos, parts, keys);
+    hipLaunchKernelGGL(kern, grid, block, 0, st, x, ld, V, n, n_parts, cut.steps, last_tokens,
+                       eos, parts, keys);
   };
   const uint16_t* x16 = static_cast<const uint16_t*>(logits);
   const float* x32 = static_cast<const float*>(logits);
   if (elem_bytes == 2) {
-    if (vals == 32) launch(beam_part_kernel<uint16_t, 32>, x16);
-    else launch(beam_part_kernel<uint16_t, 16>, x16);
+    if (V < 8) launch(beam_part_kernel<uint16_t, 16, false, true>, x16);
+    else if (cut.steps > 1) launch(beam_part_kernel<uint16_t, 16, true>, x16);
+    else if (cut.vals == 32) launch(beam_part_kernel<uint16_t, 32, false>, x16);
+    else launch(beam_part_kernel<uint16_t, 16, false>, x16);
   } else {
-    if (vals == 32) launch(beam_part_kernel<float, 32>, x32);
-    else launch(beam_part_kernel<float, 16>, x32);
+    if (V < 4) launch(beam_part_kernel<float, 16, false, true>, x32);
+    else if (cut.steps > 1) launch(beam_part_kernel<float, 16, true>, x32);
+    else if (cut.vals == 32) launch(beam_part_kernel<float, 32, false>, x32);
+    else launch(beam_part_kernel<float, 16, false>, x32);
   }
   if (int rc = pdk::check_launch("beam_part_kernel")) return rc;
   hipLaunchKernelGGL(beam_join_kernel, dim3(R), dim3(64 * K), 0, st, parts, keys, n_parts, n,

@@ -147,8 +147,8 @@ def _window_attention(q, new, cache_k, cache_v, block_tables, ctx_lens, max_ctx,
     window."""
     if not isinstance(q, torch.Tensor) or not q.is_cuda:
         raise TypeError("q must be a CUDA tensor")
-    dev = q.device
-    if stream is not None or dev.index != _current_device():
+    dev, at = q.device, q.get_device()
+    if stream is not None or at != _current_device():
         with launch_scope(dev, stream):
             return _window_attention(q, new, cache_k, cache_v, block_tables, ctx_lens, max_ctx,
                                      scale, out, workspace, None, window, sinks)
@@ -158,8 +158,8 @@ def _window_attention(q, new, cache_k, cache_v, block_tables, ctx_lens, max_ctx,
         nb, H, block, _ = cache_k.shape
         fine = (q.dtype is BF16 and cache_k.dtype is BF16 and cache_v.dtype is BF16
                 and block_tables.dtype is torch.int32 and ctx_lens.dtype is torch.int32
-                and cache_k.device == dev and cache_v.device == dev
-                and block_tables.device == dev and ctx_lens.device == dev
+                and cache_k.get_device() == at and cache_v.get_device() == at
+                and block_tables.get_device() == at and ctx_lens.get_device() == at
                 and cache_k.shape == (nb, H, 16, D) and cache_v.shape == (nb, H, D, 16)
                 and block_tables.shape[0] == B and block_tables.dim() == 2
                 and ctx_lens.numel() == B and q.is_contiguous() and cache_k.is_contiguous()
@@ -167,8 +167,8 @@ def _window_attention(q, new, cache_k, cache_v, block_tables, ctx_lens, max_ctx,
                 and ctx_lens.is_contiguous() and out is None and workspace is None)
         if fine and new is not None:
             k_new, v_new = new
-            fine = (k_new.dtype is BF16 and v_new.dtype is BF16 and k_new.device == dev
-                    and v_new.device == dev and k_new.shape == (B, H, D)
+            fine = (k_new.dtype is BF16 and v_new.dtype is BF16 and k_new.get_device() == at
+                    and v_new.get_device() == at and k_new.shape == (B, H, D)
                     and v_new.shape == (B, H, D))
     except (AttributeError, TypeError, ValueError):
         fine = False

@@ -71,6 +71,43 @@ def test_select(cuda, dtype, R, K, V, n):
     check_select(x, scores, n, eos=1, last=last)
 
 
+@pytest.mark.parametrize("dtype,R,K,V,n", [
+    (torch.bfloat16, 16, 16, 40001, 8), (torch.float32, 16, 16, 40001, 8),
+    (torch.float32, 60, 16, 18433, 16), (torch.bfloat16, 75, 16, 20483, 32),
+    (torch.bfloat16, 230, 16, 14403, 4)])
+def test_select_many_rows(cuda, dtype, R, K, V, n):
+    """Rows enough for several steps of a wavefront, with rows of every kind among
+    them: ties, sorted ones, values masked, far from zero, infinite or NaN."""
+    print(f"select {dtype} R={R} K={K} V={V} n={n}", flush=True)
+    inf = float("inf")
+    g = torch.Generator(device=cuda).manual_seed(V + K)
+    x = torch.randn((R * K, V), generator=g, device=cuda) * 2.5
+    i = torch.arange(V, device=cuda).float()
+    x[1::29] = 0.25
+    x[2::29] = i / 512
+    x[3::29] = -i / 512
+    x[4::29] = i % 5
+    x[5::29, ::2] = -inf
+    x[6::29] = -inf
+    x[7::29, :-1] = -inf
+    x[8::29, V // 2] = float("nan")
+    x[9::29, -1] = inf
+    x[10::29] += 1e5
+    x[11::29] -= 3e4
+    x[12::29] = torch.where(i < 40, 0.0, torch.finfo(dtype).min)
+    x[13::29] *= 1e36
+    x[14::29] = torch.where(i >= V - 3, 5000.0 + i - V, 4990.0)
+    x[15::29, : V - 5] = torch.finfo(dtype).min
+    scores = -20 * torch.rand((R, K), generator=g, device=cuda)
+    x = x.to(dtype)
+    check_select(x, scores, n)
+    # From odd addresses, and with beams that have ended.
+    wide = torch.empty((R * K, V + 1), dtype=dtype, device=cuda)
+    wide[:, 1:] = x
+    last = torch.randint(0, 3, (R, K), generator=g, device=cuda, dtype=torch.int32)
+    check_select(wide[:, 1:], scores, n, eos=1, last=last)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_select_ties_and_order(cuda, dtype):
     """Equal logits everywhere, few distinct values, sorted rows, equal beams."""
