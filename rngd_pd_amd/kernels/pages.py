@@ -1,4 +1,6 @@
 """torch-facing wrapper of the copies of whole blocks inside the paged cache."""
+import array
+
 import numpy as np
 import torch
 
@@ -46,6 +48,13 @@ def _ids(ids, name, num_blocks):
         raise TypeError(f"{name} must be on the host (a list, a numpy array or a CPU tensor)")
     if type(ids) is np.ndarray and ids.dtype == np.int32 and ids.ndim == 1:
         return ids if ids.flags.c_contiguous else np.ascontiguousarray(ids)
+    if type(ids) is list and ids:
+        try:
+            return np.frombuffer(array.array("i", ids), np.int32)
+        except OverflowError:
+            raise ValueError(f"{name} holds ids outside [0, {num_blocks})") from None
+        except TypeError:
+            raise TypeError(f"{name} must be a list of block ids") from None
     a = np.asarray(ids)
     if a.ndim != 1 or (a.size and a.dtype.kind not in "iu"):
         raise TypeError(f"{name} must be a list of block ids")
