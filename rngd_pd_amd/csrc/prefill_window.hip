@@ -23,16 +23,16 @@
 // off) and for the reads of the tile whose buffer is filled next.
 //
 // A token that a query does not see has the weight 0 whatever its score; but 0
-// times a V of NaN or infinity is NaN. Where an output comes out not finite, the
-// unit is done over token by token with the hidden ones left out (exact_unit), so
-// what stands in a hidden place reaches no query.
+// times a V of NaN or infinity is NaN. Where an output comes out NaN and a tile that
+// hides tokens from the unit's queries holds such a V, it is done over token by
+// token (without_hidden), so what stands in a hidden place reaches no query.
 //
 // Bound by the wavefronts' issue: per tile and wavefront 16 MFMA (512 cycles) and
 // some 100 vector instructions, of which 16 exp2; counted over a prompt of 8000
 // with a window of 1024 the matrix cores are busy 40 % of the time and the vector
 // units 50 %, half of it together, at 2.0 GHz. Three workgroups per CU (164
 // registers, 48 KiB) hide the rest best. In us, 32 query and 8 KV heads, (tokens,
-// window): (8000, 1024) 169, (4000, whole) 146, (8000, 128) 46, (470, 128) 11.0.
+// window): (8000, 1024) 150, (4000, whole) 140, (8000, 128) 46, (470, 128) 10.6.
 // Tried and slower there: two workgroups per CU with the scores of the next tile
 // computed beside the weights of this one (176, 161, 51, 10.6), two tiles at a
 // time (178, 163, 52, 11.2), two units per wavefront (180, 213, 63, 22.6), tiles
@@ -108,15 +108,46 @@ struct Rows {
   int64_t ld;
 };
 
-// One unit done over, token by token: for outputs that are not finite.
-__device__ void exact_unit(const Rows& q, const Rows& k, const Rows& v, int T, int head, int kvh,
-                           int qt, int lane, float c, int window, int sinks, f32x16 (&o)[4],
-                           float& l) {
+// Whether some query of the unit does not see some token of tile t0.
+__device__ __forceinline__ bool hides(int t0, int p0, int window, int sinks) {
+  return t0 + kTile - 1 > p0 || (t0 + window < p0 + kTile && t0 + kTile > sinks);
+}
+
+// Whether tile t0's V (rows past T: row T - 1) holds a NaN or an infinity.
+__device__ bool not_finite(const Rows& v, int T, int kvh, int t0, int lane) {
+  const uint16_t* p = v.p + (int64_t)min(t0 + (lane >> 1), T - 1) * v.ld + kvh * kD + (lane & 1) * 64;
+  uint32_t found = 0;
+#pragma unroll 1
+  for (int x = 0; x < 8; ++x) {
+    const v8 a = pdk::ld16(p + 8 * x);
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+      found |= (a.w[w] & 0x7f80u) == 0x7f80u || (a.w[w] & 0x7f800000u) == 0x7f800000u;
+  }
+  return __any(found);
+}
+
+// The outputs that are NaN done over, token by token without the hidden ones; m is
+// the maximum that the others' weights have been taken with. It ends as soon as
+// each of them is NaN by a token that is seen.
+__device__ void without_hidden(const Rows& q, const Rows& k, const Rows& v, int T, int head, int kvh,
+                               int qt, int lane, float c, int window, int sinks, float m, float l,
+                               f32x16 (&o)[4]) {
   const int j = lane & 31, hh = lane >> 5, p = min(qt * kTile + j, T - 1);
   const int last = min(qt * kTile + kTile, T) - 1, first = max(qt * kTile - window + 1, 0);
   const uint16_t* qp = q.p + (int64_t)p * q.ld + head * kD + 8 * hh;
-  // The scaled score of token t and the lane's query, and whether it is seen.
-  auto score = [&](int t, bool& seen) __attribute__((always_inline)) {
+  const float mc = m == -INFINITY ? 0.f : m * c;
+  uint32_t open[2] = {0, 0};               // a bit for each of the lane's outputs to be done over
+#pragma unroll
+  for (int n = 0; n < 4; ++n)
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (l == l && o[n][i] != o[n][i]) {
+        open[n >> 1] |= 1u << (16 * (n & 1) + i);
+        o[n][i] = 0.f;
+      }
+#pragma unroll 1
+  for (int t = 0; t <= last; t = t + 1 < first && t + 1 >= sinks ? first : t + 1) {
     const uint16_t* kp = k.p + (int64_t)t * k.ld + kvh * kD + 8 * hh;
     float s = 0.f;
 #pragma unroll 1
@@ -129,29 +160,10 @@ __device__ void exact_unit(const Rows& q, const Rows& k, const Rows& v, int T, i
       }
     }
     const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(s), __float_as_uint(s), false, false);
-    seen = t <= p && (t > p - window || t < sinks);
-    return (__uint_as_float(x[0]) + __uint_as_float(x[1])) * c;
-  };
-  float m = -INFINITY;
-  bool seen;
-#pragma unroll 1
-  for (int t = 0; t <= last; t = t + 1 < first && t + 1 >= sinks ? first : t + 1) {
-    const float s = score(t, seen);
-    if (seen) m = vmax(m, s);
-  }
-  const float mc = m == -INFINITY ? 0.f : m;
-  l = 0.f;
-#pragma unroll
-  for (int n = 0; n < 4; ++n)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) o[n][i] = 0.f;
-#pragma unroll 1
-  for (int t = 0; t <= last; t = t + 1 < first && t + 1 >= sinks ? first : t + 1) {
-    const float s = score(t, seen);
-    const float w = __builtin_amdgcn_exp2f(s - mc);
-    // Each half holds the whole score: the halves' sums are added at the end.
-    if (seen && hh == 0) l += w;
+    const bool seen = t <= p && (t > p - window || t < sinks);
+    const float w = __builtin_amdgcn_exp2f((__uint_as_float(x[0]) + __uint_as_float(x[1])) * c - mc);
     const uint16_t* vp = v.p + (int64_t)t * v.ld + kvh * kD + 4 * hh;
+    bool left = false;
 #pragma unroll
     for (int n = 0; n < 4; ++n)
 #pragma unroll
@@ -159,9 +171,15 @@ __device__ void exact_unit(const Rows& q, const Rows& k, const Rows& v, int T, i
         const uint2 u = *reinterpret_cast<const uint2*>(vp + 32 * n + 8 * g);
         const uint32_t h[4] = {u.x & 0xffffu, u.x >> 16, u.y & 0xffffu, u.y >> 16};
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (seen) o[n][4 * g + e] += w * pdk::bf16_to_f32(h[e]);
+        for (int e = 0; e < 4; ++e) {
+          const int i = 4 * g + e;
+          if (open[n >> 1] >> (16 * (n & 1) + i) & 1) {
+            if (seen) o[n][i] += w * pdk::bf16_to_f32(h[e]);
+            left |= o[n][i] == o[n][i];
+          }
+        }
       }
+    if (!__any(left)) break;
   }
 }
 
@@ -273,7 +291,7 @@ __global__ __launch_bounds__(64 * kWaves, 3) void prefill_window_kernel(
     const int t0 = tile_at(i) * kTile, p0 = qt * kTile;
     // Tokens after some query (and so those past T), or that have left some
     // query's window.
-    if (t0 + kTile - 1 > p0 || (t0 + window < p0 + kTile && t0 + kTile > sinks)) {
+    if (hides(t0, p0, window, sinks)) {
       const int ago = p0 + j - t0 - 8 * hh;                      // of the lane's first token
       const int sink = sinks - t0 - 8 * hh;
 #pragma unroll
@@ -334,8 +352,17 @@ __global__ __launch_bounds__(64 * kWaves, 3) void prefill_window_kernel(
   for (int n = 0; n < 4; ++n)
 #pragma unroll
     for (int i = 0; i < 16; ++i) bad += o[n][i] * 0.f;
-  if (__builtin_expect(__any(bad != bad || l != l), 0))
-    exact_unit(q, k, v, T, head, kvh, qt, lane, c, window, sinks, o, l);
+  if (__builtin_expect(__any(bad != bad), 0)) {
+    bool hidden = false;
+#pragma unroll 1
+    for (int i = 0; i < n_walk && !hidden; ++i) {
+      const int t0 = tile_at(i) * kTile;
+      if (hides(t0, qt * kTile, window, sinks)) hidden = not_finite(v, T, kvh, t0, lane);
+    }
+    int ln = lane;                        // q's addresses anew: kept, they would be spilled
+    asm("" : "+v"(ln));
+    if (hidden) without_hidden(q, k, v, T, head, kvh, qt, ln, c, window, sinks, m, l, o);
+  }
 
   // Lane (hh, j) holds dims 32n + 8g + 4hh + 0..3 of query j (g = 0..3); a lane
   // swap of groups g, g + 1 gives each half 8 consecutive dims: 16-byte stores.

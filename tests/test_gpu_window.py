@@ -368,6 +368,40 @@ def test_prompt_hidden_values_reach_no_query(cuda, window, sinks, value):
     assert not torch.isfinite(got[at[1]]).any()
 
 
+@pytest.mark.parametrize("T,window,sinks", [(230, 40, 4), (1500, 1500, 0), (33, 33, 0)])
+def test_prompt_values_that_are_not_finite(cuda, T, window, sinks):
+    """A dim that is NaN in every token of one head, an infinity in one token's dim
+    and one of each sign in two tokens': as the sums over the seen tokens have them."""
+    from rngd_pd_amd import kernels as K
+    rng = np.random.default_rng(21)
+    q = to_dev(rand_bf16(rng, (T, 8, D)))
+    k, v = (to_dev(rand_bf16(rng, (T, 2, D))) for _ in range(2))
+    want, bound = _prompt_reference(q, k, v, window, sinks, SCALE)
+    want, bound = want.clone(), bound.clone()
+    inf, t = float("inf"), torch.arange(T, device=cuda)
+
+    def sees(a):
+        return ((t >= a) & ((t - a < window) | (a < sinks))).cpu().to(want.device)
+
+    v[:, 0, 5] = float("nan")
+    v[20, 1, 7] = inf
+    v[9, 0, 90] = inf
+    v[25, 0, 90] = -inf
+    got = K.prefill_attention(q, k, v, scale=SCALE, window=window, sinks=sinks)
+    assert torch.isnan(got[:, :4, 5]).all()
+    s20, s9, s25 = sees(20), sees(9), sees(25)
+    assert (got[s20.to(cuda), 4:, 7] == inf).all()
+    assert (got[(s9 & ~s25).to(cuda), :4, 90] == inf).all()
+    assert (got[(s25 & ~s9).to(cuda), :4, 90] == -inf).all()
+    assert torch.isnan(got[(s9 & s25).to(cuda), :4, 90]).all()
+    # All others.
+    plain = torch.ones_like(want, dtype=torch.bool)
+    plain[:, :4, 5] = False
+    plain[s20, 4:, 7] = False
+    plain[s9 | s25, :4, 90] = False
+    assert_within(got[plain.to(cuda)], want[plain], bound[plain])
+
+
 def test_refusals(cuda):
     from rngd_pd_amd import kernels as K
     from rngd_pd_amd._lib import PdkError
