@@ -433,31 +433,36 @@ __global__ __launch_bounds__(64 * kMaxBeams) void beam_join_kernel(
   const int r = blockIdx.x, lane = threadIdx.x & 63;
   const int k = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int row = r * K + k;
+  // Heads of the parts' lists; only lists whose head reaches the n-th largest of the
+  // lanes' own best heads hold any of the n best: those of at most n lanes. Where
+  // there are fewer than 64 lists, the other lanes' keys are the next of them. Of up
+  // to 128 parts all is asked for at once, an ended beam's (never written) too.
+  const Key* kp = keys + (int64_t)row * n_parts * n;
+  const Part* pp = parts + (int64_t)row * n_parts;
+  const int next = n_parts < 64 ? lane / n_parts : 0;
+  const bool in0 = next < n, in1 = lane + 64 < n_parts;
+  const Key key0 = kp[in0 ? (lane - next * n_parts) * n + next : 0];
+  const Key key1 = kp[in1 ? (lane + 64) * n : 0];
+  const Part part0 = pp[min(lane, n_parts - 1)], part1 = pp[in1 ? lane + 64 : 0];
   const bool ended = last_tokens && last_tokens[row] == eos;
   const float score = scores[row];
   const bool alive = score > -INFINITY && score < INFINITY;
   double total = lane == 0 && alive ? (double)score : -INFINITY;   // of an ended beam
   int32_t token = eos;
   if (!ended) {
-    // Heads of the parts' lists; only lists whose head reaches the n-th largest of
-    // the lanes' own best heads hold any of the n best: those of at most n lanes.
-    const Key* kp = keys + (int64_t)row * n_parts * n;
-    const Part* pp = parts + (int64_t)row * n_parts;
-    // Where there are fewer than 64, the lanes' keys are the next of them.
-    Key mine = 0;
-    double top = -INFINITY, sum = 0.0;
+    const Key head0 = in0 ? key0 : 0, head1 = in1 ? key1 : 0;
+    Key mine = head0 > head1 ? head0 : head1;
+    double top = fmax(part0.top, in1 ? part1.top : -INFINITY), sum = 0.0;
 #pragma unroll 1
-    for (int s = lane; s < n_parts; s += 64) {
+    for (int s = lane + 128; s < n_parts; s += 64) {
       const Key head = kp[s * n];
       mine = head > mine ? head : mine;
       top = fmax(top, pp[s].top);
     }
-    const int next = lane / n_parts;
-    if (next && next < n) mine = kp[(lane - next * n_parts) * n + next];
     top = wave_all(top, [](double a, double b) { return fmax(a, b); });
 #pragma unroll 1
-    for (int s = lane; s < n_parts; s += 64) {
-      const Part q = pp[s];
+    for (int s = lane, i = 0; s < n_parts; s += 64, ++i) {
+      const Part q = i == 0 ? part0 : i == 1 ? part1 : pp[s];
       // NaN in q.sum stays; a part without a finite value adds nothing.
       sum += q.sum != 0.0 ? q.sum * exp_of(fmax(q.top - top, -690.0)) : 0.0;
     }
@@ -472,8 +477,9 @@ __global__ __launch_bounds__(64 * kMaxBeams) void beam_join_kernel(
     }
     int m = 0;                                           // lists that reach it
 #pragma unroll 1
-    for (int s = lane; s - lane < n_parts; s += 64) {
-      const bool in = s < n_parts && kp[s * n] >= least;
+    for (int s = lane, i = 0; s - lane < n_parts; s += 64, ++i) {
+      const Key head = i == 0 ? head0 : i == 1 ? head1 : kp[min(s, n_parts - 1) * n];
+      const bool in = s < n_parts && head >= least;
       const uint64_t who = __ballot(in);
       if (in) lists[k][m + below(who)] = (uint16_t)s;
       m += __popcll(who);
