@@ -286,7 +286,8 @@ int pdk_decode_attn_rope_rms(const float* qkv_partials, int splits,
  * may be freed and their table entries set to -1, and contexts may be as long as
  * the table (max_blocks <= 65535); window, sinks and max_ctx together may leave
  * up to 16384 tokens to read (pdk_decode_attn_window_span; else PDK_ENOTSUP).
- * Other arguments as pdk_decode_attn (masked and invalid blocks included), any
+ * Other arguments as pdk_decode_attn (masked and invalid blocks included; out
+ * must not overlap q), any
  * Hq/Hkv from 1 to 16; the workspace is pdk_decode_attn_workspace_bytes() of
  * max_ctx, or of pdk_decode_attn_window_span(max_ctx, window, sinks), which is
  * smaller. No counterpart in the reference, whose lanes are attended to whole
@@ -837,7 +838,8 @@ int pdk_prefill_attn(const uint16_t* q, int64_t q_tok_stride, const uint16_t* kt
  * q [T] rows of [Hq][128], k and v [T] rows of [Hkv][128] after RoPE (token
  * strides in elements, multiples of 8), out [T][Hq][128]. The query at position p
  * sees the tokens t <= p with t > p - window or t < sinks; a window of T or more
- * is plain causal attention. A weight is rounded to bf16 once. */
+ * is plain causal attention. A weight is rounded to bf16 once. out overlaps none of
+ * q, k and v. */
 int pdk_prefill_attn_window(const uint16_t* q, int64_t q_tok_stride,
                             const uint16_t* k, int64_t k_tok_stride,
                             const uint16_t* v, int64_t v_tok_stride, int T,

@@ -1203,6 +1203,11 @@ int launch_attn(const uint16_t* q, const uint16_t* cache_k, const uint16_t* cach
   const int64_t n_wg = units << (p.qsplit + p.vsplit);
   const uint32_t hgw = (uint32_t)n_kv_heads | ((uint32_t)G << 16) | ((uint32_t)p.qsplit << 24);
   const uint32_t mb_b = (uint32_t)max_blocks | ((uint32_t)B << 16);
+  if (win && q) {   // two workgroups may read the same query rows and write parts of their output
+    const int64_t rows = (int64_t)B * n_q_heads * head_dim;
+    PDK_REQUIRE(!std::less<const uint16_t*>()(q, out + rows) ||
+                    !std::less<const uint16_t*>()(out, q + rows), "out must not overlap q");
+  }
   const uint32_t st_ns = (uint32_t)p.split_tokens | ((uint32_t)p.nsplit << 16);
   const dim3 grid((uint32_t)n_wg), block(64 * kMaxWaves);
   const void* src = rope.part ? static_cast<const void*>(rope.part) : static_cast<const void*>(a.q);

@@ -10,7 +10,7 @@ import torch
 
 from .. import _lib
 from .handoff import _current_device, _need, launch_scope, need_device, stream_handle
-from .prefill import check_window
+from .prefill import check_window, overlap
 
 BF16 = torch.bfloat16
 
@@ -128,6 +128,8 @@ def _check_window_operands(q, new, cache_k, cache_v, block_tables, ctx_lens, out
         need_device(q.device, out, "out")
         if out.shape != q.shape or not out.is_contiguous():
             raise ValueError(f"out must be contiguous {tuple(q.shape)}")
+        if overlap(out, q):
+            raise ValueError("out must not overlap q")
     if workspace is not None:
         need_device(q.device, workspace, "workspace")
         if not workspace.is_contiguous():

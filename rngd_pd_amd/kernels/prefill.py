@@ -31,7 +31,7 @@ def _rows(t, T):
     return t, ld
 
 
-def _overlap(a, b):
+def overlap(a, b):
     """Whether the memory that a and b span has bytes in common."""
     def span(t):
         size = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1 if t.numel() else 0
@@ -71,7 +71,7 @@ def prefill_attention(q, k, v, scale=1.0, window=None, sinks=0, out=None, stream
         need_device(dev, out, "out")
         if out.shape != q.shape or not out.is_contiguous() or out.data_ptr() % 16:
             raise ValueError(f"out must be contiguous and 16-byte aligned {tuple(q.shape)}")
-        if any(_overlap(out, t) for t in (q, k, v)):
+        if any(overlap(out, t) for t in (q, k, v)):
             raise ValueError("out must not overlap q, k or v")
     if T == 0:
         return out

@@ -420,6 +420,8 @@ def test_refusals(cuda):
         K.decode_attention(q, ck, cv, big, ctx, 80000, window=20000)
     with pytest.raises(ValueError):
         K.decode_attention(q, ck, cv, tab, ctx, 64, window=4, out=q[:, :8])
+    with pytest.raises(ValueError, match="overlap"):
+        K.decode_attention(q, ck, cv, tab, ctx, 64, window=4, out=q)
     with pytest.raises(ValueError):
         K.decode_attention(q, ck, cv, tab.cpu(), ctx, 64, window=4)
     wide = to_dev(rand_bf16(rng, (1, 17 * 8, D)))
