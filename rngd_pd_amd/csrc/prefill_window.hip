@@ -31,8 +31,10 @@
 // some 100 vector instructions, of which 16 exp2; counted over a prompt of 8000
 // with a window of 1024 the matrix cores are busy 40 % of the time and the vector
 // units 50 %, half of it together, at 2.0 GHz. Three workgroups per CU (164
-// registers, 48 KiB) hide the rest best. In us, 32 query and 8 KV heads, (tokens,
-// window): (8000, 1024) 150, (4000, whole) 140, (8000, 128) 46, (470, 128) 10.6.
+// registers, 48 KiB) hide the rest best; where there are no more workgroups than CUs
+// a second team of wavefronts shares the walk (the entry point has the rule). In us,
+// 32 query and 8 KV heads, (tokens, window): (8000, 1024) 150, (4000, whole) 140,
+// (8000, 128) 46, (470, 128) 10.6.
 // Tried and slower there: two workgroups per CU with the scores of the next tile
 // computed beside the weights of this one (176, 161, 51, 10.6), two tiles at a
 // time (178, 163, 52, 11.2), two units per wavefront (180, 213, 63, 22.6), tiles
@@ -58,6 +60,7 @@ constexpr int kTile = 32;                 // tokens per K/V tile and queries per
 constexpr int kTileElems = kTile * kD;    // 8 KiB of K, 8 KiB of V
 constexpr int kWaves = 4;
 constexpr int kRing = 3;                  // tiles in LDS: 48 KiB, three workgroups per CU
+constexpr int kCUs = 256;
 constexpr int kLoads = 4;                 // of a wavefront per tile, 1 KiB each
 
 __device__ __forceinline__ f32x16 mfma32(const v8& a, const v8& b, f32x16 c) {
@@ -188,11 +191,16 @@ __device__ void without_hidden(const Rows& q, const Rows& k, const Rows& v, int 
 // the same tiles; the KV head is the fastest index of the grid, so that 8 of them
 // spread over the 8 XCDs. The last query tiles go first: without a window they
 // have the most to walk.
-__global__ __launch_bounds__(64 * kWaves, 3) void prefill_window_kernel(
+// kTeams 2: a second team of kWaves walks every other tile with buffers of its own,
+// and hands its sums to the first at the end.
+template <int kTeams>
+__global__ __launch_bounds__(64 * kWaves * kTeams, kTeams == 1 ? 3 : 2) void prefill_window_kernel(
     Rows q, Rows k, Rows v, int T, int NH, int NKV, float c, int window, int sinks,
     uint16_t* out) {
-  __shared__ __align__(1024) uint16_t sm[2 * kRing * kTileElems];   // K tiles, V tiles
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  __shared__ __align__(1024) uint16_t smem[kTeams][2 * kRing * kTileElems];   // K tiles, V tiles
+  const int team = kTeams == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & (kWaves - 1), lane = threadIdx.x & 63;
+  uint16_t* const sm = smem[team];
   const int j = lane & 31, hh = lane >> 5;
   const int G = NH / NKV, units = (T + kTile - 1) / kTile * G;
   const int kvh = blockIdx.x % NKV;
@@ -202,10 +210,14 @@ __global__ __launch_bounds__(64 * kWaves, 3) void prefill_window_kernel(
   // i + skip from there on (those from its first query's window to its last query).
   const int w_tile = max(u_first / G * kTile - window + 1, 0) / kTile;
   const int lead = min((sinks + kTile - 1) / kTile, w_tile), skip = w_tile - lead;
-  const int n_walk = u_last / G + 1 - skip;
+  const int n_all = u_last / G + 1 - skip;
+  const int n_walk = kTeams == 1 ? n_all : (n_all + 1 - team) / 2;   // the team's, from its `team`th on
   const int u = min(u_first + wave, units - 1);                  // a spare one repeats the last
   const int qt = u / G, head = kvh * G + (u - qt * G);
-  auto tile_at = [&](int i) { return i >= lead ? i + skip : i; };
+  auto tile_at = [&](int i) {
+    const int x = kTeams * i + team;
+    return x >= lead ? x + skip : x;
+  };
 
   // Staging: load l of a wavefront covers tokens 8 wave + 4 l + lane / 16. A whole
   // tile's offsets from its first row are the same for every tile.
@@ -346,6 +358,38 @@ __global__ __launch_bounds__(64 * kWaves, 3) void prefill_window_kernel(
     step(i, sm + r * kTileElems, sm + r2 * kTileElems, r * kTileElems * 2);
     r = r + 1 == kRing ? 0 : r + 1;
   }
+  if constexpr (kTeams == 2) {
+    // The barriers match: the second team has as many tiles, or one less.
+    if (n_walk < (n_all + 1) / 2) tile_barrier<0>();
+    tile_barrier<0>();                                           // nobody reads tiles any more
+    float4* const mem = reinterpret_cast<float4*>(smem) + wave * (17 * 64) + lane;
+    if (team == 1) {
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+#pragma unroll
+        for (int x = 0; x < 16; x += 4)
+          mem[(4 * n + x / 4) * 64] = make_float4(o[n][x], o[n][x + 1], o[n][x + 2], o[n][x + 3]);
+      mem[16 * 64] = make_float4(m, l, 0.f, 0.f);
+    }
+    tile_barrier<0>();
+    if (team == 1) return;
+    const float4 ml = mem[16 * 64];
+    const float m_new = vmax(m, ml.x);
+    const float a0 = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - m_new) * c);
+    const float a1 = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ml.x - m_new) * c);
+    m = m_new;
+    l = l * a0 + ml.y * a1;
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int x = 0; x < 16; x += 4) {
+        const float4 y = mem[(4 * n + x / 4) * 64];
+        o[n][x] = o[n][x] * a0 + y.x * a1;
+        o[n][x + 1] = o[n][x + 1] * a0 + y.y * a1;
+        o[n][x + 2] = o[n][x + 2] * a0 + y.z * a1;
+        o[n][x + 3] = o[n][x + 3] * a0 + y.w * a1;
+      }
+  }
 
   float bad = 0.f;                        // NaN once an output is not finite
 #pragma unroll
@@ -355,8 +399,8 @@ __global__ __launch_bounds__(64 * kWaves, 3) void prefill_window_kernel(
   if (__builtin_expect(__any(bad != bad), 0)) {
     bool hidden = false;
 #pragma unroll 1
-    for (int i = 0; i < n_walk && !hidden; ++i) {
-      const int t0 = tile_at(i) * kTile;
+    for (int i = 0; i < n_all && !hidden; ++i) {
+      const int t0 = (i >= lead ? i + skip : i) * kTile;
       if (hides(t0, qt * kTile, window, sinks)) hidden = not_finite(v, T, kvh, t0, lane);
     }
     int ln = lane;                        // q's addresses anew: kept, they would be spilled
@@ -427,7 +471,16 @@ extern "C" int pdk_prefill_attn_window(const uint16_t* q, int64_t q_tok_stride, 
   const int64_t units = (int64_t)((T + kTile - 1) / kTile) * (n_q_heads / n_kv_heads);
   const int64_t blocks = (units + kWaves - 1) / kWaves * n_kv_heads;
   PDK_REQUIRE(units < (1ll << 30) && blocks < (1ll << 31), "launch too large");
-  hipLaunchKernelGGL(prefill_window_kernel, dim3((unsigned)blocks), dim3(64 * kWaves), 0,
+  // A second team where a workgroup has a CU to itself and more than 8 tiles to walk:
+  // it halves that chain (0.7 us a tile) for 1.5 us of handing over. us with one team
+  // and with two, 32 query and 8 KV heads, (tokens, window): (1000, whole) 29.9 and 25.2,
+  // (1000, 512) 20.4 and 18.2, (470, whole) 16.4 and 14.4, (256, whole) 11.0 and 11.0,
+  // (470, 128) 10.7 and 11.0, (100, 64) 7.5 and 8.6.
+  const int walk = std::min((T + kTile - 1) / kTile,
+                            (window + kTile - 2) / kTile + 1 + (sinks + kTile - 1) / kTile);
+  const bool two = blocks <= kCUs && walk > 8;
+  hipLaunchKernelGGL(two ? prefill_window_kernel<2> : prefill_window_kernel<1>,
+                     dim3((unsigned)blocks), dim3(64 * kWaves * (two ? 2 : 1)), 0,
                      pdk::as_stream(stream), Rows{q, q_tok_stride}, Rows{k, k_tok_stride},
                      Rows{v, v_tok_stride}, T, n_q_heads, n_kv_heads, scale * 1.4426950408889634f,
                      window, sinks, out);

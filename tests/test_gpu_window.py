@@ -255,6 +255,9 @@ PROMPT = [
     (64, 12, 4, 33, 33), (65, 32, 8, 31, 40), (129, 7, 1, 50, 3), (200, 32, 8, 1, 4),
     (200, 32, 8, 500, 4), (470, 32, 8, 128, 4), (513, 40, 8, 100, 64), (700, 24, 8, 255, 1),
     (1000, 16, 16, 97, 129), (1111, 64, 8, 512, 0), (300, 20, 1, 64, 16),
+    # Two teams: even and odd numbers of tiles, sinks in front, several query tiles in a workgroup.
+    (470, 32, 8, 470, 0), (289, 8, 8, 289, 0), (1000, 8, 2, 1000, 0), (777, 7, 1, 400, 40),
+    (600, 6, 6, 300, 70), (1024, 16, 2, 260, 0),
 ]
 
 
