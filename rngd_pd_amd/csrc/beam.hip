@@ -272,7 +272,9 @@ __global__ __launch_bounds__(64 * kWaves) void beam_part_kernel(const T* logits,
   const int first = part * (kMany ? steps : 1) * kStep;  // of the part's values
   if (kMany) steps = min(steps, (V - first + kStep - 1) / kStep);
   else steps = 1;
-  auto value_at = [&](int step, int unit, int of) { return first + step * kStep + (unit * 64 + of) * kEl; };
+  auto value_at = [&](int step, int unit, int of) {
+    return first + step * kStep + (unit * 64 + of) * kEl;
+  };
   auto load = [&](int e) __attribute__((always_inline)) {
     Unit u;
     if constexpr (kShort) u = short_row(p, V);
@@ -295,6 +297,7 @@ __global__ __launch_bounds__(64 * kWaves) void beam_part_kernel(const T* logits,
   };
   // sum is that of e^(x - ref), ref the first step's maximum: 64 bits hold what lies
   // up to 600 above it, and only beyond that it is taken anew.
+  auto larger = [](float a, float b) { return __builtin_elementwise_maximum(a, b); };
   float ref = -INFINITY, best = -INFINITY;               // of the part; of the lane
   double sum = 0.0;                                      // the lane's
   auto use = [&](const Unit* u, int step) __attribute__((always_inline)) {
@@ -307,7 +310,7 @@ __global__ __launch_bounds__(64 * kWaves) void beam_part_kernel(const T* logits,
     if (kMany) most[wave][step * 64 + lane] = m;
     best = __builtin_elementwise_maximum(best, m);
     if (__ballot(m > ref + 600.f)) {
-      const float top = wave_all(m, [](float a, float b) { return __builtin_elementwise_maximum(a, b); });
+      const float top = wave_all(m, larger);
       if (!(top < INFINITY)) {                           // the part counts for nothing (below)
         ref = 0.f;
       } else {
@@ -352,7 +355,7 @@ __global__ __launch_bounds__(64 * kWaves) void beam_part_kernel(const T* logits,
     }
   }
   sum = wave_sum(sum);
-  const float top = wave_all(best, [](float a, float b) { return __builtin_elementwise_maximum(a, b); });
+  const float top = wave_all(best, larger);
   if (kMany) sum *= exp_of(fmax((double)ref - (double)top, -690.0));
   if (!(top < INFINITY)) sum = NAN;
   const int64_t at = (int64_t)row * n_parts + part;
@@ -397,20 +400,20 @@ __global__ __launch_bounds__(64 * kWaves) void beam_part_kernel(const T* logits,
         k1 = k > k1 && k < last && (!kMany || start + i >= e) ? k : k1;
       });
     };
-    auto larger = [](Key a, Key b) { return a > b ? a : b; };
+    auto larger_key = [](Key a, Key b) { return a > b ? a : b; };
     Key mine = 0;                                        // the lane's best that is not taken yet
 #pragma unroll 1
     for (int i = 0; i < steps * kUnits; ++i) best_of(mine, i / kUnits, i % kUnits, lane, ~0ull);
 #pragma unroll 1
     for (c = 0; c < n; ++c) {
-      const Key taken = wave_all(mine, larger);
+      const Key taken = wave_all(mine, larger_key);
       if (!taken) break;
       list[c] = taken;
       // All lanes look for the next of the lane that had it.
       const int of = __builtin_ctzll(__ballot(mine == taken));
       Key next = 0;
       if (lane < steps * kUnits) best_of(next, lane / kUnits, lane % kUnits, of, taken);
-      next = wave_all(next, larger);
+      next = wave_all(next, larger_key);
       if (lane == of) mine = next;
     }
   }

@@ -25,7 +25,6 @@ namespace {
 constexpr int kPairs = 448;               // per launch: 3.5 KiB of the 4 KiB of arguments
 constexpr int kFew = 16;                  // and of a launch of few
 
-
 // The launch's arguments are copied by the host at every call: few pairs travel
 // in a small struct (3 pairs, an eager call 9.4 -> 7 us).
 template <int kN>
@@ -78,7 +77,8 @@ int launch(uint16_t* cache_k, uint16_t* cache_v, int64_t layer_stride, int n_lay
   std::copy(dst, dst + n, p.dst);
   constexpr int kChunk = 256 * kUnits;      // 16-byte units of one workgroup
   const auto kern = copy_blocks_kernel<kN, kUnits, kStream>;
-  hipLaunchKernelGGL(kern, dim3((units + kChunk - 1) / kChunk, n, 2 * n_layers), dim3(256), 0, st, cache_k, cache_v, layer_stride, units, p);
+  hipLaunchKernelGGL(kern, dim3((units + kChunk - 1) / kChunk, n, 2 * n_layers), dim3(256),
+                     0, st, cache_k, cache_v, layer_stride, units, p);
   return pdk::check_launch("copy_blocks_kernel");
 }
 
@@ -91,7 +91,8 @@ extern "C" int pdk_copy_blocks(uint16_t* cache_k, uint16_t* cache_v, int64_t cac
   PDK_REQUIRE(n >= 0, "n must be >= 0 (got %d)", n);
   PDK_REQUIRE(cache_k && cache_v && (n == 0 || (src && dst)), "null pointer argument");
   PDK_REQUIRE(pdk::aligned16(cache_k) && pdk::aligned16(cache_v), "caches must be 16-byte aligned");
-  PDK_REQUIRE(n_layers >= 1 && n_layers <= 32767 && num_blocks >= 1, "n_layers or num_blocks out of range");
+  PDK_REQUIRE(n_layers >= 1 && n_layers <= 32767 && num_blocks >= 1,
+              "n_layers or num_blocks out of range");
   PDK_REQUIRE(n_kv_heads >= 1 && n_kv_heads <= 65535 && head_dim >= 1 && head_dim <= 4096,
               "n_kv_heads or head_dim out of range");
   const int64_t block = (int64_t)n_kv_heads * PDK_BLOCK_SIZE * head_dim;

@@ -103,7 +103,8 @@ __device__ __forceinline__ void read_v(uint32_t at0, uint32_t at1, v8 (&va)[2][2
   for (int n = 0; n < 2; ++n)
 #pragma unroll
     for (int h = 0; h < 2; ++h)
-      va[n][h] = v8{{x[4 * n + 2 * h].x, x[4 * n + 2 * h].y, x[4 * n + 2 * h + 1].x, x[4 * n + 2 * h + 1].y}};
+      va[n][h] = v8{{x[4 * n + 2 * h].x, x[4 * n + 2 * h].y, x[4 * n + 2 * h + 1].x,
+                     x[4 * n + 2 * h + 1].y}};
 }
 
 struct Rows {
@@ -162,7 +163,8 @@ __device__ void without_hidden(const Rows& q, const Rows& k, const Rows& v, int 
         s += pdk::bf16_to_f32(a.w[w] >> 16) * pdk::bf16_to_f32(b.w[w] >> 16);
       }
     }
-    const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(s), __float_as_uint(s), false, false);
+    const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(s), __float_as_uint(s), false,
+                                                    false);
     const bool seen = t <= p && (t > p - window || t < sinks);
     const float w = __builtin_amdgcn_exp2f((__uint_as_float(x[0]) + __uint_as_float(x[1])) * c - mc);
     const uint16_t* vp = v.p + (int64_t)t * v.ld + kvh * kD + 4 * hh;
@@ -199,7 +201,8 @@ __global__ __launch_bounds__(64 * kWaves * kTeams, kTeams == 1 ? 3 : 2) void pre
     uint16_t* out) {
   __shared__ __align__(1024) uint16_t smem[kTeams][2 * kRing * kTileElems];   // K tiles, V tiles
   const int team = kTeams == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & (kWaves - 1), lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & (kWaves - 1);
+  const int lane = threadIdx.x & 63;
   uint16_t* const sm = smem[team];
   const int j = lane & 31, hh = lane >> 5;
   const int G = NH / NKV, units = (T + kTile - 1) / kTile * G;
@@ -245,7 +248,8 @@ __global__ __launch_bounds__(64 * kWaves * kTeams, kTeams == 1 ? 3 : 2) void pre
     uint16_t* at = to + 8 * wave * kD;
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      __builtin_amdgcn_global_load_lds((global_void*)(tk + ko[x]), (lds_void*)(at + 4 * x * kD), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((global_void*)(tk + ko[x]), (lds_void*)(at + 4 * x * kD), 16,
+                                       0, 0);
       __builtin_amdgcn_global_load_lds((global_void*)(tv + vo[x]),
                                        (lds_void*)(at + (kRing * kTileElems + 4 * x * kD)), 16, 0, 0);
     }
@@ -265,7 +269,8 @@ __global__ __launch_bounds__(64 * kWaves * kTeams, kTeams == 1 ? 3 : 2) void pre
   // + 16 (j / 16) + 4 (lane & 3).
   const int k_at = pi(j) * kD + ((hh ^ pi(j)) & 15) * 8;
   const int vr = (lane & 15) >> 2;
-  const int v_at = (8 * hh + vr) * kD + ((2 * (j >> 4) + ((lane & 3) >> 1)) ^ (vr << 2)) * 8 + (lane & 1) * 4;
+  const int v_at = (8 * hh + vr) * kD + ((2 * (j >> 4) + ((lane & 3) >> 1)) ^ (vr << 2)) * 8 +
+                   (lane & 1) * 4;
   uint32_t v_addr[4];
 #pragma unroll
   for (int n = 0; n < 4; ++n)
@@ -291,7 +296,8 @@ __global__ __launch_bounds__(64 * kWaves * kTeams, kTeams == 1 ? 3 : 2) void pre
     for (int x = 0; x < 8; ++x) r = mfma32(kr[x], qv[x], r);
     return r;
   };
-  auto step = [&](int i, const uint16_t* __restrict__ at_k, uint16_t* __restrict__ to, uint32_t at_v) __attribute__((always_inline)) {
+  auto step = [&](int i, const uint16_t* __restrict__ at_k, uint16_t* __restrict__ to,
+                  uint32_t at_v) __attribute__((always_inline)) {
     if (i + 1 < n_walk) tile_barrier<kLoads>();
     else tile_barrier<0>();
     if (i + 2 < n_walk) fetch(to, i + 2);
