@@ -72,7 +72,10 @@ class BatchDecodeAttention:
         each stream's blocks to hold its new token)."""
         for r in req_ids:
             self.cache.ensure(r, self.positions[r] + 1)
-        key = (tuple(req_ids), tuple(len(self.cache._tables[r]) for r in req_ids))
+        # Between two steps tables grow by whole blocks; anything else is a new
+        # generation of the cache (read before the tables are).
+        key = (self.cache.generation, tuple(req_ids),
+               tuple(len(self.cache._tables[r]) for r in req_ids))
         if key != self._batch_key:
             self._tables = self.cache.batch_tables(req_ids)
             self._batch_key = key

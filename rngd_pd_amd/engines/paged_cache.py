@@ -111,6 +111,9 @@ class PagedKVCache:
         self._tables = {}          # req_id -> [block ids]
         self._dev_tables = {}      # req_id -> device int32 tensor
         self._shared = {}          # block -> holders beyond the first
+        # Raised whenever an entry of a table is replaced or a table goes; tables that
+        # only grow keep it. What is kept from tables holds for one generation.
+        self.generation = 0
         self._lock = threading.Lock()
 
     # -- block tables ---------------------------------------------------------
@@ -135,6 +138,8 @@ class PagedKVCache:
 
     def free(self, req_id):
         with self._lock:
+            if req_id in self._tables:
+                self.generation += 1
             blocks = self._tables.pop(req_id, [])
             self._dev_tables.pop(req_id, None)
             self.alloc.release(self._let_go(blocks))
@@ -193,6 +198,7 @@ class PagedKVCache:
             gone = [j for j in range(-(-max(keep, 0) // BLOCK), min(num_tokens // BLOCK, len(have)))
                     if have[j] >= 0]
             if gone:
+                self.generation += 1
                 free = self._let_go([have[j] for j in gone])
                 for j in gone:
                     have[j] = -1
@@ -203,7 +209,8 @@ class PagedKVCache:
     def compact(self, stream=None):
         """Move held blocks onto the lowest free ids until no free id lies below a
         held one's; returns how many moved. Tables change: device tables and
-        graphs made before are stale, and no other stream may be using the cache."""
+        graphs made before are stale (BatchDecodeAttention.prepare makes its own
+        anew), and no other stream may be using the cache."""
         with self._lock:
             moved = {}
 
@@ -216,6 +223,9 @@ class PagedKVCache:
                                        stream=stream)
                 return list(moved)
             self.alloc.repack(plan)
+            if not moved:
+                return 0
+            self.generation += 1
             for t in self._tables.values():
                 t[:] = [moved.get(b, b) for b in t]
             self._shared = {moved.get(b, b): n for b, n in self._shared.items()}
