@@ -34,7 +34,7 @@ class BatchDecodeAttention:
         self.positions = {}                  # req_id -> next decode position
         self._batch_key = None
         self._tables = None
-        self._ws = None
+        self._ws = _attn.Workspace(cache.device)
 
     def admit(self, req_id, frame, num_tokens, S, stream=None):
         """Place a handed-off request: its S-wide frame, first decode position num_tokens."""
@@ -91,11 +91,9 @@ class BatchDecodeAttention:
         need = _attn.workspace_bytes(q.shape[0], self.Hq,
                                      _attn.window_span(max_ctx, self.window, self.sinks),
                                      self.cache.head_dim)
-        if need and (self._ws is None or self._ws.numel() * 4 < need):
-            self._ws = torch.zeros(need // 4 + 64, dtype=torch.float32, device=self.cache.device)
         return _attn.decode_attention_append(q, k_new, v_new, ck, cv, tables, ctx, max_ctx,
                                              scale=self.scale, out=out,
-                                             workspace=self._ws if need else None, stream=stream,
+                                             workspace=self._ws.take(need, stream), stream=stream,
                                              window=self.window, sinks=self.sinks)
 
     def advance(self, req_ids):

@@ -199,7 +199,7 @@ class LlamaDecoder:
         self.ssq_a = torch.zeros((B, H // 16), dtype=torch.float32, device=dev)
         self.inv = cfg.inv_freq().to(dev)
         self.scale = 1.0 / math.sqrt(cfg.head_dim)
-        self._ws = None
+        self._ws = _attn.Workspace(dev)
         # Per-layer operands resolved once: the step loop makes no views.
         w = weights
         if max_batch > 64:
@@ -245,23 +245,26 @@ class LlamaDecoder:
     def reserve(self, max_ctx):
         """Allocate the attention workspace for max_batch streams at ``max_ctx``
         now, so that no later step (or graph capture) allocates it."""
+        before = self._ws.buffer
         self._workspace(self.plan_batch, max_ctx)
+        if self._ws.buffer is not before and not torch.cuda.is_current_stream_capturing():
+            # Steps may run on another stream: nothing queued on this one uses the
+            # memory any more.
+            torch.cuda.current_stream(self.device).synchronize()
 
-    def _workspace(self, B, max_ctx):
-        """The attention workspace, grown when a step needs more. A captured
-        graph holds the address it was captured with, so once any graph exists
-        a step that would need a larger one raises instead (reserve() the
-        largest max_ctx before capturing)."""
+    def _workspace(self, B, max_ctx, stream=None):
+        """The attention workspace for a step on ``stream``, grown when it needs
+        more. A captured graph holds the address it was captured with, so once any
+        graph exists a step that would need a larger one raises instead (reserve()
+        the largest max_ctx before capturing)."""
         need = _attn.workspace_bytes(B, self.cfg.n_heads,
                                      _attn.window_span(max_ctx, self.cfg.window, self.cfg.sinks),
                                      self.cfg.head_dim)
-        if need and (self._ws is None or self._ws.numel() * 4 < need):
-            if self._captured:
-                raise RuntimeError(f"the attention workspace would have to grow to {need} bytes "
-                                   f"after a graph was captured with the old one; reserve() the "
-                                   f"largest max_ctx before capturing")
-            self._ws = torch.zeros(need // 4 + 64, dtype=torch.float32, device=self.device)
-        return self._ws if need else None
+        if self._captured and not self._ws.holds(need):
+            raise RuntimeError(f"the attention workspace would have to grow to {need} bytes "
+                               f"after a graph was captured with the old one; reserve() the "
+                               f"largest max_ctx before capturing")
+        return self._ws.take(need, stream)
 
     def step(self, tokens, ctx_lens, tables, max_ctx, stream=None):
         """tokens int64/int32 [B] on the device (this step's input token per
@@ -291,7 +294,7 @@ class LlamaDecoder:
         st = stream_handle(stream)
         H, NH, NKV, HD, M = cfg.hidden, cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, cfg.inter
         QKV, eps = cfg.qkv_dim, cfg.eps
-        ws = self._workspace(max(B, self.plan_batch), max_ctx)
+        ws = self._workspace(max(B, self.plan_batch), max_ctx, stream)
         ws_ptr = ws.data_ptr() if ws is not None else None
         ws_bytes = ws.numel() * 4 if ws is not None else 0
         mb, nb = tables.shape[1], cache.num_blocks

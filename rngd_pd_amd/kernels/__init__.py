@@ -4,7 +4,7 @@ from .handoff import (pack_kv, pack_kv_batch, scatter_paged, scatter_paged_batch
                       stream_probe, check_skipped)
 from .attention import (decode_attention, decode_attention_append, decode_attention_rope,
                         cache_append, greedy_argmax,
-                        workspace_bytes, get_workspace, attn_read_probe, window_span)
+                        workspace_bytes, get_workspace, Workspace, attn_read_probe, window_span)
 from .prefill import prefill_attention
 from .pages import copy_blocks
 from .beam import beam_select, beam_select_workspace_bytes, beam_reorder
@@ -19,7 +19,7 @@ __all__ = ["pack_kv", "pack_kv_batch", "scatter_paged", "scatter_paged_batch", "
            "check_skipped",
            "stream_probe",
            "decode_attention", "decode_attention_append", "decode_attention_rope",
-           "cache_append", "greedy_argmax", "workspace_bytes", "get_workspace",
+           "cache_append", "greedy_argmax", "workspace_bytes", "get_workspace", "Workspace",
            "attn_read_probe", "window_span", "prefill_attention", "copy_blocks",
            "beam_select", "beam_select_workspace_bytes", "beam_reorder",
            "rmsnorm", "rope_cache_append", "rope_cache_append_partials", "swiglu", "linear", "linear_swiglu", "linear_argmax",

@@ -19,22 +19,64 @@ def workspace_bytes(B, n_q_heads, max_ctx, head_dim=128):
     return int(_lib.lib().pdk_decode_attn_workspace_bytes(B, n_q_heads, max_ctx, head_dim))
 
 
+class Workspace:
+    """The attention workspace of a caller that makes many calls: one fp32 buffer,
+    replaced when a call needs more.
+
+    It holds the per-split partial maxima, sums and outputs of a split context;
+    every entry a call reads is written earlier in that call, so it is neither
+    cleared nor filled. It serves one stream at a time: a caller that goes from one
+    to another orders them. A buffer is allocated on the stream of the call that
+    needs it; one that was replaced is given out again only when what was queued
+    on the streams that used it is done, and not at all if a graph being captured
+    used it (the graph holds its address)."""
+
+    def __init__(self, device):
+        self.device = torch.device(device)
+        self.buffer = None
+        self._streams = set()                # handles of the streams that used it
+        self._in_graph = False
+        self._kept = []
+
+    def _new(self, nbytes):
+        return torch.empty(nbytes // 4 + 64, dtype=torch.float32, device=self.device)
+
+    def holds(self, nbytes):
+        return nbytes == 0 or (self.buffer is not None and self.buffer.numel() * 4 >= nbytes)
+
+    def take(self, nbytes, stream=None):
+        """The buffer, of at least ``nbytes``, for a call on ``stream`` (default: the
+        current one); None where it needs none."""
+        if not nbytes:
+            return None
+        with launch_scope(self.device, stream):
+            on = stream_handle()
+            if not self.holds(nbytes):
+                if self._in_graph:
+                    self._kept.append(self.buffer)
+                self.buffer = self._new(nbytes)
+                self._streams, self._in_graph = {on}, False
+            elif on not in self._streams:
+                self.buffer.record_stream(torch.cuda.current_stream(self.device))
+                self._streams.add(on)
+            self._in_graph = self._in_graph or torch.cuda.is_current_stream_capturing()
+            return self.buffer
+
+
 _WORKSPACES = {}
 
 
-def get_workspace(nbytes, device):
-    """An fp32 workspace of at least ``nbytes`` on ``device``, kept per device.
-
-    It holds the per-split partial maxima, sums and outputs of a split
-    context; every entry a call reads is written earlier in that call, so one
-    buffer is reused across calls without clearing. It serves one stream at a
-    time: concurrent calls on different streams need their own."""
-    key = torch.device(device).index or 0
+def get_workspace(nbytes, device, stream=None):
+    """The Workspace kept per device: at least ``nbytes`` of it for a call on
+    ``stream`` (default: the current one). Concurrent calls on different streams
+    need their own."""
+    key = torch.device(device).index
+    if key is None:
+        key = _current_device()
     ws = _WORKSPACES.get(key)
-    if ws is None or ws.numel() * 4 < nbytes:
-        ws = torch.zeros(max(nbytes, 1 << 20) // 4 + 64, dtype=torch.float32, device=device)
-        _WORKSPACES[key] = ws
-    return ws
+    if ws is None:
+        ws = _WORKSPACES[key] = Workspace(torch.device("cuda", key))
+    return ws.take(max(nbytes, 1 << 20), stream)
 
 
 def _check_layer_cache(cache_k, cache_v):
@@ -51,7 +93,7 @@ def _check_layer_cache(cache_k, cache_v):
 
 
 def _attention_call(q, cache_k, cache_v, block_tables, ctx_lens, max_ctx, out, workspace,
-                    span=None):
+                    stream=None, span=None):
     """Checked operands of one attention call: (geometry, workspace pointer and
     bytes, out). ``span``: the tokens read at most, under a window; such a call's
     workspace is its own where none is given."""
@@ -78,7 +120,7 @@ def _attention_call(q, cache_k, cache_v, block_tables, ctx_lens, max_ctx, out, w
         elif span is not None:
             ws = torch.empty(need, dtype=torch.uint8, device=q.device)
         else:
-            ws = get_workspace(need, q.device)
+            ws = get_workspace(need, q.device, stream)
     ws_ptr = ws.data_ptr() if ws is not None else None
     ws_bytes = ws.numel() * ws.element_size() if ws is not None else 0
     return (nb, B, Hq, H, D), ws_ptr, ws_bytes, out
@@ -215,7 +257,7 @@ def decode_attention(q, cache_k, cache_v, block_tables, ctx_lens, max_ctx, scale
         return _window_attention(q, None, cache_k, cache_v, block_tables, ctx_lens, max_ctx, scale,
                                  out, workspace, stream, window, sinks)
     (nb, B, Hq, H, D), ws_ptr, ws_bytes, out = _attention_call(
-        q, cache_k, cache_v, block_tables, ctx_lens, max_ctx, out, workspace)
+        q, cache_k, cache_v, block_tables, ctx_lens, max_ctx, out, workspace, stream)
     _lib.call("pdk_decode_attn", q.data_ptr(), cache_k.data_ptr(), cache_v.data_ptr(), nb,
               block_tables.data_ptr(), block_tables.shape[1], ctx_lens.data_ptr(), int(max_ctx),
               B, Hq, H, D, float(scale), ws_ptr, ws_bytes, out.data_ptr(), stream_handle(stream))
@@ -244,7 +286,7 @@ def decode_attention_append(q, k_new, v_new, cache_k, cache_v, block_tables, ctx
         return decode_attention(q, cache_k, cache_v, block_tables, ctx_lens, max_ctx, scale=scale,
                                 out=out, workspace=workspace, stream=stream)
     (nb, B, Hq, H, D), ws_ptr, ws_bytes, out = _attention_call(
-        q, cache_k, cache_v, block_tables, ctx_lens, max_ctx, out, workspace)
+        q, cache_k, cache_v, block_tables, ctx_lens, max_ctx, out, workspace, stream)
     _lib.call("pdk_decode_attn_append", q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(),
               cache_k.data_ptr(), cache_v.data_ptr(), nb, block_tables.data_ptr(),
               block_tables.shape[1], ctx_lens.data_ptr(), int(max_ctx), B, Hq, H, D, float(scale),
@@ -288,7 +330,7 @@ def decode_attention_rope(qkv_partials, inv_freq, cache_k, cache_v, block_tables
                 raise ValueError(f"workspace holds fewer than the {need} bytes needed")
             ws = workspace
         else:
-            ws = get_workspace(need, cache_k.device)
+            ws = get_workspace(need, cache_k.device, stream)
     if ssq is not None:
         _need(ssq, "ssq", torch.float32)
         if ssq.dim() != 2 or ssq.shape[0] != B or not ssq.is_contiguous():

@@ -69,7 +69,7 @@ def launch_scope(device, stream=None):
     """The context of a call that works on tensors of ``device``: what it launches
     and allocates belongs to that device and to ``stream`` (a torch stream or a
     handle; None: that device's current stream), whatever is current outside."""
-    if stream is None and device.index == _current_device():
+    if stream is None and device.index in (None, _current_device()):
         return _AS_IT_IS
     return _Scope(device, stream)
 
