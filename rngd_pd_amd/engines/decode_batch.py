@@ -88,13 +88,14 @@ class BatchDecodeAttention:
         (streams may share blocks: each sees the others' new tokens in them).
         q [B, Hq, D], k_new/v_new [B, Hkv, D] bf16 on the device."""
         ck, cv = self.cache.k[layer], self.cache.v[layer]
+        sinks = min(self.sinks, max_ctx)
         need = _attn.workspace_bytes(q.shape[0], self.Hq,
-                                     _attn.window_span(max_ctx, self.window, self.sinks),
+                                     _attn.window_span(max_ctx, self.window, sinks),
                                      self.cache.head_dim)
         return _attn.decode_attention_append(q, k_new, v_new, ck, cv, tables, ctx, max_ctx,
                                              scale=self.scale, out=out,
                                              workspace=self._ws.take(need, stream), stream=stream,
-                                             window=self.window, sinks=self.sinks)
+                                             window=self.window, sinks=sinks)
 
     def advance(self, req_ids):
         """After all layers of a step: every stream moves to its next position."""

@@ -258,7 +258,8 @@ class LlamaDecoder:
         graph exists a step that would need a larger one raises instead (reserve()
         the largest max_ctx before capturing)."""
         need = _attn.workspace_bytes(B, self.cfg.n_heads,
-                                     _attn.window_span(max_ctx, self.cfg.window, self.cfg.sinks),
+                                     _attn.window_span(max_ctx, self.cfg.window,
+                                                       min(self.cfg.sinks, max_ctx)),
                                      self.cfg.head_dim)
         if self._captured and not self._ws.holds(need):
             raise RuntimeError(f"the attention workspace would have to grow to {need} bytes "
@@ -310,6 +311,7 @@ class LlamaDecoder:
         down_ws = None if self.down_ws is None else (self.down_ws.data_ptr(),
                                                      self.down_ws.numel() * 4)
         window, sinks = self._window
+        sinks = min(sinks, int(max_ctx))     # a config may name more than any context has
         emb, attn = g["pdk_embed_ssq"], g["pdk_decode_attn_rope"]
         with torch.cuda.stream(stream) if stream is not None else contextlib.nullcontext():
             call(emb, w.embed.data_ptr(), cfg.vocab, tokens.data_ptr(),

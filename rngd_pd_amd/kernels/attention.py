@@ -250,7 +250,7 @@ def decode_attention(q, cache_k, cache_v, block_tables, ctx_lens, max_ctx, scale
     and ctx_lens int32 [B] on the device; ``max_ctx`` >= every ctx_lens[b].
 
     With ``window`` stream b sees only its last ``window`` tokens and the first
-    ``sinks``: no block between them is read (its table entry may be -1), contexts
+    ``sinks`` (up to 16384): no block between them is read (its table entry may be -1), contexts
     may be as long as the table, and any Hq/Hkv up to 16 is taken. Without
     ``workspace`` such a call allocates its own."""
     if window is not None or sinks:
