@@ -1102,6 +1102,7 @@ struct RopeIn {
   bool act = false;              // out in the tiled activation layout (pdk::act_at)
   int window = 0;                // > 0: a sliding window, with sinks
   int sinks = 0;
+  bool check_only = false;       // nothing is launched: whether the call would be refused
 };
 
 // The kernel for a plan: V in halves or whole, and on the plain path and the
@@ -1208,6 +1209,7 @@ int launch_attn(const uint16_t* q, const uint16_t* cache_k, const uint16_t* cach
     PDK_REQUIRE(!std::less<const uint16_t*>()(q, out + rows) ||
                     !std::less<const uint16_t*>()(out, q + rows), "out must not overlap q");
   }
+  if (rope.check_only) return PDK_OK;
   const uint32_t st_ns = (uint32_t)p.split_tokens | ((uint32_t)p.nsplit << 16);
   const dim3 grid((uint32_t)n_wg), block(64 * kMaxWaves);
   const void* src = rope.part ? static_cast<const void*>(rope.part) : static_cast<const void*>(a.q);
@@ -1289,15 +1291,20 @@ int attn_append(const uint16_t* q, const uint16_t* k_new, const uint16_t* v_new,
   const bool rounds = pairs > kTargetWorkgroups &&
                       (span <= 128 || (pairs > 352 && span > 640 && span <= 1536));
   if (B > kMaxShared || rounds || overwritten(k_new) || overwritten(v_new)) {
-    if (int rc = pdk_cache_append(k_new, v_new, cache_k, cache_v, num_blocks, block_tables,
-                                  max_blocks, ctx_lens, B, n_kv_heads, head_dim, stream))
-      return rc;
     RopeIn in{nullptr, 0, nullptr, nullptr, nullptr};
     in.window = window;
     in.sinks = sinks;
-    return launch_attn(q, cache_k, cache_v, num_blocks, block_tables, max_blocks, ctx_lens,
-                       max_ctx, B, n_q_heads, n_kv_heads, head_dim, scale, workspace,
-                       workspace_bytes, out, stream, in, B);
+    auto attend = [&](bool check_only) {
+      in.check_only = check_only;
+      return launch_attn(q, cache_k, cache_v, num_blocks, block_tables, max_blocks, ctx_lens,
+                         max_ctx, B, n_q_heads, n_kv_heads, head_dim, scale, workspace,
+                         workspace_bytes, out, stream, in, B);
+    };
+    if (int rc = attend(true)) return rc;        // a refused call leaves the cache as it is
+    if (int rc = pdk_cache_append(k_new, v_new, cache_k, cache_v, num_blocks, block_tables,
+                                  max_blocks, ctx_lens, B, n_kv_heads, head_dim, stream))
+      return rc;
+    return attend(false);
   }
   RopeIn in{nullptr, 0, nullptr, cache_k, cache_v};
   in.k_new = k_new;
