@@ -362,7 +362,9 @@ int pdk_copy_blocks(uint16_t* cache_k, uint16_t* cache_v,
  * its score), its logits are not read. No candidates come from -inf logits, from
  * a beam whose score is not finite, nor from one whose row holds NaN or +inf, or
  * only -inf. Where there are fewer than n, the rest is token -1, parent -1,
- * score -inf. With n = K, tokens may be last_tokens and out_scores scores.
+ * score -inf. With n = K, tokens may be last_tokens and out_scores scores; any
+ * other overlap of the outputs with each other, with those or with the workspace
+ * is refused with PDK_EINVAL.
  * 1 <= K <= 16, 1 <= n <= 32, V <= 2^20. The workspace (16-byte
  * aligned, one call at a time) needs no clearing. The reference samples greedily
  * only (greedy_tokens, engines/decode_batch.py:162-171). */

@@ -684,6 +684,30 @@ extern "C" int pdk_beam_select(const void* logits, int elem_bytes, int64_t ld, i
               "workspace of %lld bytes needed (got %lld)", (long long)need,
               (long long)workspace_bytes);
   const int rows = R * K;
+  // A request's workgroup reads its beams' scores and last tokens before it writes, and
+  // others' not at all: an output may lie place for place where they do.
+  struct Range {
+    const void* p;
+    int64_t bytes;
+  };
+  auto overlap = [](const Range& a, const Range& b) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
+    return a.p && b.p && x < y + b.bytes && y < x + a.bytes;
+  };
+  const int64_t outs = (int64_t)R * n * 4;
+  const Range in[2] = {{scores, (int64_t)rows * 4}, {last_tokens, (int64_t)rows * 4}};
+  const Range out[3] = {{tokens, outs}, {parents, outs}, {out_scores, outs}};
+  const Range ws{workspace, need};
+  PDK_REQUIRE(!overlap(ws, Range{logits, ((int64_t)(rows - 1) * ld + V) * elem_bytes}),
+              "the workspace must not overlap the logits");
+  for (const Range& i : in) PDK_REQUIRE(!overlap(ws, i), "the workspace must not overlap an input");
+  for (int o = 0; o < 3; ++o) {
+    PDK_REQUIRE(!overlap(ws, out[o]), "the workspace must not overlap an output");
+    for (int p = 0; p < o; ++p) PDK_REQUIRE(!overlap(out[o], out[p]), "outputs must not overlap");
+    for (const Range& i : in)
+      PDK_REQUIRE(!overlap(out[o], i) || (n == K && out[o].p == i.p),
+                  "an output may overlap scores or last_tokens only in their places, with n = K");
+  }
   const Cut cut = cut_of(rows, V);
   const int n_parts = cut.n_parts;
   Part* parts = static_cast<Part*>(workspace);

@@ -35,7 +35,8 @@ def beam_select(logits, scores, n_out=None, eos=None, last_tokens=None, out=None
     and score -inf.
 
     ``out``: the three tensors to write; with n_out = K they may be last_tokens and
-    scores themselves (each request's are read before they are written).
+    scores themselves (each request's are read before they are written). Other
+    overlaps of theirs, or of the workspace, are refused.
     ``workspace``: at least
     beam_select_workspace_bytes of device memory for one call at a time (default:
     allocated by the call on its stream)."""
