@@ -18,7 +18,8 @@ of a layer, the short prompt's on the right:
   qkv = h . Wqkv^T                     library              pdk_prefill_gemm
   RoPE; K/V rows; attention's operands pdk_prefill_rope_kv  pdk_prefill_rope_kv_partials
   ao = causal GQA attention            pdk_prefill_attn (fp32 weights), or
-                                       pdk_prefill_attn_window for a config with one
+                                       pdk_prefill_attn_window where a config's window
+                                       hides some of the prompt
   o = ao . Wo^T                        library              pdk_prefill_gemm
   h = rmsnorm(x + o)                   pdk_rmsnorm          pdk_prefill_rmsnorm_partials
   gu = h . Wgu^T                       library              pdk_prefill_gemm_swiglu, with
@@ -146,6 +147,9 @@ class LlamaPrefill:
         ao = torch.empty((T, NH * HD), dtype=BF16, device=dev)
         q_rows = None
         window, sinks = check_window(cfg.window, cfg.sinks)
+        # A window that hides nothing of this prompt leaves it to pdk_prefill_attn, whose
+        # weights keep 32 bits where the windowed kernel's are rounded to bf16.
+        hides = 0 < window < T - sinks
 
         def attention(qkv, k_l, v_l, before):
             nonlocal q_rows
@@ -171,7 +175,7 @@ class LlamaPrefill:
             if v is not v_l:
                 v_l.copy_(v)
             before()
-            if window:
+            if hides:
                 _lib.call("pdk_prefill_attn_window", qkv.data_ptr(), qkv.stride(0), k.data_ptr(),
                           rows[0][1], v.data_ptr(), rows[1][1], T, NH, NKV, HD, self.scale, window,
                           sinks, ao.data_ptr(), stream_handle())
