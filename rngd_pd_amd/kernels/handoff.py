@@ -68,9 +68,17 @@ class _Scope:
 def launch_scope(device, stream=None):
     """The context of a call that works on tensors of ``device``: what it launches
     and allocates belongs to that device and to ``stream`` (a torch stream or a
-    handle; None: that device's current stream), whatever is current outside."""
-    if stream is None and device.index in (None, _current_device()):
-        return _AS_IT_IS
+    handle; None: that device's current stream), whatever is current outside. A
+    stream of another device is refused: it would make that one current."""
+    if stream is None:
+        if device.index in (None, _current_device()):
+            return _AS_IT_IS
+    elif not isinstance(stream, int):
+        on = getattr(stream, "device", None)
+        if on is None or not hasattr(stream, "cuda_stream"):
+            raise TypeError(f"stream must be a torch.cuda.Stream or a handle, got {type(stream)}")
+        if device.index is not None and on.index != device.index:
+            raise ValueError(f"the tensors are on {device}, the stream on {on}")
     return _Scope(device, stream)
 
 
