@@ -357,7 +357,8 @@ int pdk_copy_blocks(uint16_t* cache_k, uint16_t* cache_v,
  * (elem_bytes 2) or fp32 (4). Results in order of total, the lower beam first
  * among equals, a beam's tokens in order of their logits, the lower token first
  * among equals: tokens, parents (the beam) and out_scores (the total) [R][n].
- * Sums and totals are 64-bit; out_scores is rounded once. last_tokens [R][K] (may
+ * Sums and totals are 64-bit, of exponentials good to 6e-11 (totals of two beams
+ * nearer than about 1e-10 may change places); out_scores is rounded once. last_tokens [R][K] (may
  * be NULL): a beam whose last token is eos has ended; its one candidate is (eos,
  * its score), its logits are not read. No candidates come from -inf logits, from
  * a beam whose score is not finite, nor from one whose row holds NaN or +inf, or
@@ -840,7 +841,8 @@ int pdk_prefill_attn(const uint16_t* q, int64_t q_tok_stride, const uint16_t* kt
  * q [T] rows of [Hq][128], k and v [T] rows of [Hkv][128] after RoPE (token
  * strides in elements, multiples of 8), out [T][Hq][128]. The query at position p
  * sees the tokens t <= p with t > p - window or t < sinks; a window of T or more
- * is plain causal attention. A weight is rounded to bf16 once. out overlaps none of
+ * is plain causal attention. A weight is rounded to bf16 once (pdk_prefill_attn keeps
+ * 32 bits of it). out overlaps none of
  * q, k and v. */
 int pdk_prefill_attn_window(const uint16_t* q, int64_t q_tok_stride,
                             const uint16_t* k, int64_t k_tok_stride,

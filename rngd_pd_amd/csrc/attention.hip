@@ -1052,8 +1052,10 @@ constexpr int kTargetWorkgroups = 256;
 // layer with the new token's write, 8 KV heads, one launch / splits of 512 / of
 // 128: B=1 window 512 8.4 / 9.6 / 8.9, 1024 10.9 / 10.1 / 9.9, 2048 14.8 / 10.4 /
 // 11.2, 4096 24.8 / 11.4 / 13.6; B=4 512 9.3 / 10.2 / 10.5, 1024 11.4 / 11.2 / 11.8;
-// B=8 512 10.1 / 11.3 / 11.8, 1024 12.4 / 13.8 / 13.3, 2048 17.4 / 17.6 / 17.5. (The
-// second launch also costs an eager caller's host some 3 us.)
+// B=8 512 10.1 / 11.3 / 11.8, 1024 12.4 / 13.8 / 13.3, 2048 17.4 / 17.6 / 17.5. (From 32
+// pairs on the two are within 2 % of each other at 1024 for B=4 and at 2048 for B=8, and
+// a second launch costs an eager caller's host some 3 us more; B=1 gains from splits from
+// 1024 on.)
 Plan plan_for(int B, int plan_B, int Hkv, int G, int max_ctx, bool win = false) {
   const int64_t pairs = (int64_t)plan_B * Hkv;
   int min_split = pairs >= 128 ? 2048 : pairs >= 32 ? 512 : 128;

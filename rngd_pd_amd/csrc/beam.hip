@@ -6,17 +6,21 @@
 // K beams of a request and the vocabulary; the n largest, the lower beam and then
 // the lower token first among equals. Inside a beam the order of the totals is
 // that of the logits, so the vocabulary is read once: a wavefront takes a part of
-// a row into registers and leaves its maximum, its sum of exponentials and its n
-// best tokens; one workgroup per request joins the parts.
+// a row and leaves its maximum, its sum of exponentials and its n best tokens; one
+// workgroup per request joins the parts. A part is one step of the wavefront, whose
+// values stay in LDS, or several, of which only each lane's maximum stays and the
+// few values that the selection needs are read again from memory.
 //
 // The sums and totals are 64-bit: which of two beams' tokens comes first hangs on
 // their difference, and 32 bits of a sum over a vocabulary of 1e5 leave 1e-6 of a
-// total undecided, which a search over a thousand candidates a step does meet.
+// total undecided, which a search over a thousand candidates a step does meet. (The
+// exponentials are good to 6e-11, so totals nearer than about 1e-10 may change places.)
 //
 // n best of a wavefront's values: the n-th largest of the 64 lanes' own maxima
-// bounds the n-th largest value from below, bit by bit with one ballot each until
-// exactly n lanes reach it (some 10 to 15 bits). Mostly a few more than n values
-// then reach the bound, all in those lanes; they are compacted into LDS and ranked
+// bounds the n-th largest value from below. nth_largest finds it two bits a round,
+// with three ballots, and ends as soon as exactly n lanes reach the bound; where no
+// more than n lanes hold anything, everything is taken. Mostly a few more than n
+// values then reach the bound, all in those lanes; they are listed in LDS and ranked
 // by counting. Where equal values let more than 64 reach it, the best is taken n
 // times: the largest of the lanes' best keys (the value in an order-preserving code
 // above the complement of the token, so that no two are equal), after which the lane

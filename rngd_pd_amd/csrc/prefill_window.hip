@@ -11,7 +11,8 @@
 // Scores, maxima, sums and O are fp32; a weight is rounded to bf16 once, for the
 // product with V (half a step, 2^-8 of each weight, adds a share of 2^-8 / sqrt(3)
 // rms to the output's own rounding of that size, and takes 8 MFMA per tile where
-// an exact split into three bf16 parts takes 24).
+// an exact split into three bf16 parts takes 24, as pdk_prefill_attn does: 4000 tokens
+// whole 137 us here and 246 there).
 //
 // K and V come as rows. A tile is 32 tokens, staged row by row into LDS by
 // global_load_lds (16 lanes a row of 256 bytes, no registers, two tiles ahead),
@@ -30,7 +31,7 @@
 // Bound by the wavefronts' issue: per tile and wavefront 16 MFMA (512 cycles) and
 // some 100 vector instructions, of which 16 exp2; counted over a prompt of 8000
 // with a window of 1024 the matrix cores are busy 40 % of the time and the vector
-// units 50 %, half of it together, at 2.0 GHz. Three workgroups per CU (164
+// units 45 to 50 %, half of it together, at 2.0 to 2.1 GHz. Three workgroups per CU (164
 // registers, 48 KiB) hide the rest best; where there are no more workgroups than CUs
 // a second team of wavefronts shares the walk (the entry point has the rule). In us,
 // 32 query and 8 KV heads, (tokens, window): (8000, 1024) 150, (4000, whole) 140,

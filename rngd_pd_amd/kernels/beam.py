@@ -25,7 +25,8 @@ def beam_select(logits, scores, n_out=None, eos=None, last_tokens=None, out=None
     logits bf16 or float32 [R*K, V] (unit column stride; row r*K + k is beam k of
     request r), scores float32 [R, K] contiguous: the beams' summed log
     probabilities. A continuation's total is the beam's score + logit - the row's
-    log-sum-exp, in 64 bits, rounded once in the returned scores; the lower beam,
+    log-sum-exp, in 64 bits (exponentials good to 6e-11: totals nearer than about
+    1e-10 may change places), rounded once in the returned scores; the lower beam,
     then the lower token, comes first among equals (inside a beam the logits
     decide). With ``eos`` and ``last_tokens`` (int32, R*K of them, contiguous) a
     beam whose last token is eos has ended: it stays in the race as the one

@@ -47,7 +47,9 @@ def prefill_attention(q, k, v, scale=1.0, window=None, sinks=0, out=None, stream
     head h // (Hq/Hkv)); columns of one projection's tensor are taken as they lie,
     other layouts than contiguous [heads, 128] rows are copied first. With
     ``window`` the query at position p sees the tokens t <= p with t > p - window
-    or t < ``sinks``."""
+    or t < ``sinks``. fp32 between the products; a weight is rounded to bf16 once,
+    as the product's operand (LlamaPrefill's own prompts without a window keep 32
+    bits of it, from K and V laid out for that)."""
     if not isinstance(q, torch.Tensor) or not q.is_cuda:
         raise TypeError("q must be a CUDA tensor")
     dev = q.device
