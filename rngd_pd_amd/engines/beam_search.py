@@ -48,7 +48,7 @@ class BeamSearch:
         R, K = len(requests), self.K
         rows = [[("beam", req, k) for k in range(K)] for req, _, _ in requests]
         ids = [r for row in rows for r in row]
-        captured = self.dec._captured
+        captured, graphs = self.dec._captured, self.dec._ws.graphs()
         forked = []
         try:
             for (req, n, _), row in zip(requests, rows):
@@ -61,6 +61,7 @@ class BeamSearch:
             # What was queued may still use the blocks: they go back when it is done.
             torch.cuda.synchronize(self.dec.device)
             self.dec._captured = captured                # this search's graph is gone
+            self.dec._ws.graphs_gone(graphs)
             for r in forked:
                 self.cache.free(r)
         return [self._beams(hist_tokens[:, r], hist_parents[:, r], scores[r], length_penalty)

@@ -62,6 +62,14 @@ class Workspace:
             self._in_graph = self._in_graph or torch.cuda.is_current_stream_capturing()
             return self.buffer
 
+    def graphs(self):
+        """What graphs hold of it now, for graphs_gone."""
+        return self.buffer, self._in_graph
+
+    def graphs_gone(self, before):
+        """The graphs that were captured since graphs() returned ``before`` are gone."""
+        self._in_graph = before[1] and self.buffer is before[0]
+
 
 _WORKSPACES = {}
 

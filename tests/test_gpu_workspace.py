@@ -127,3 +127,21 @@ def test_decoder_on_another_stream(cuda):
     assert sizes[0] < sizes[1] and all(bool((t == 7).all()) for t in own)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     del busy
+
+
+def test_searches_keep_no_old_workspaces(cuda):
+    """A search's graph goes with it, and so does the workspace it held when a longer
+    search needs more."""
+    from rngd_pd_amd.engines.beam_search import BeamSearch
+    from rngd_pd_amd.engines.llama_decode import LlamaConfig, LlamaDecoder, LlamaWeights
+    from rngd_pd_amd.engines.paged_cache import PagedKVCache
+    cfg = LlamaConfig(hidden=512, n_heads=8, n_kv_heads=2, head_dim=128, inter=1024, vocab=1000,
+                      n_layers=2)
+    cache = PagedKVCache(2, 160, 2, D, device=cuda)
+    dec = LlamaDecoder(LlamaWeights.random(cfg, seed=3, device=cuda), cache, max_batch=2)
+    cache.allocate("r", 900)
+    search, sizes = BeamSearch(dec, 2), []
+    for n in (200, 500, 900):
+        search.search([("r", n, 1)], 5)
+        sizes.append(dec._ws.buffer.numel())
+    assert sizes == sorted(set(sizes)) and dec._ws._kept == []

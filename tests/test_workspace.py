@@ -86,3 +86,22 @@ def test_get_workspace_per_device_and_stream(gpu, monkeypatch):
     assert a.allocated_on == 3 and at.get_workspace(1 << 20, torch.device("cuda", 0), 3) is a
     assert at.get_workspace(100, "cuda") is not a       # the current device's
     assert set(at._WORKSPACES) == {0, 1}
+
+
+def test_workspace_of_a_graph_that_is_gone_goes(gpu):
+    ws = at.Workspace("cuda:0")
+    ws.take(1000)
+    before = ws.graphs()
+    gpu["capturing"] = True
+    ws.take(1000)
+    gpu["capturing"] = False
+    ws.graphs_gone(before)
+    ws.take(4000)
+    assert ws._kept == []
+    # A graph from before still holds what it used then.
+    gpu["capturing"] = True
+    held = ws.take(4000)
+    gpu["capturing"] = False
+    ws.graphs_gone(ws.graphs())
+    ws.take(9000)
+    assert ws._kept == [held]
