@@ -15,6 +15,7 @@ from .prefill import check_window, overlap
 BF16 = torch.bfloat16
 
 
+@functools.lru_cache(maxsize=4096)
 def workspace_bytes(B, n_q_heads, max_ctx, head_dim=128):
     return int(_lib.lib().pdk_decode_attn_workspace_bytes(B, n_q_heads, max_ctx, head_dim))
 
@@ -34,6 +35,7 @@ class Workspace:
     def __init__(self, device):
         self.device = torch.device(device)
         self.buffer = None
+        self._bytes = 0                      # of the buffer
         self._streams = set()                # handles of the streams that used it
         self._in_graph = False
         self._kept = []
@@ -42,19 +44,25 @@ class Workspace:
         return torch.empty(nbytes // 4 + 64, dtype=torch.float32, device=self.device)
 
     def holds(self, nbytes):
-        return nbytes == 0 or (self.buffer is not None and self.buffer.numel() * 4 >= nbytes)
+        return self._bytes >= nbytes
 
     def take(self, nbytes, stream=None):
         """The buffer, of at least ``nbytes``, for a call on ``stream`` (default: the
         current one); None where it needs none."""
         if not nbytes:
             return None
+        # The usual call: large enough, and nothing new about the stream.
+        if self._bytes >= nbytes and stream is None and self.device.index == _current_device() \
+                and stream_handle() in self._streams \
+                and (self._in_graph or not torch.cuda.is_current_stream_capturing()):
+            return self.buffer
         with launch_scope(self.device, stream):
             on = stream_handle()
             if not self.holds(nbytes):
                 if self._in_graph:
                     self._kept.append(self.buffer)
                 self.buffer = self._new(nbytes)
+                self._bytes = self.buffer.numel() * 4
                 self._streams, self._in_graph = {on}, False
             elif on not in self._streams:
                 self.buffer.record_stream(torch.cuda.current_stream(self.device))

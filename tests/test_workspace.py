@@ -33,6 +33,7 @@ def gpu(monkeypatch):
         yield
         state["stream"] = before
     monkeypatch.setattr(at, "launch_scope", scope)
+    monkeypatch.setattr(at, "_current_device", lambda: 0)
     monkeypatch.setattr(at, "stream_handle", lambda s=None: state["stream"] if s is None else s)
     monkeypatch.setattr(torch.cuda, "current_stream", lambda d=None: state["stream"])
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: state["capturing"])
