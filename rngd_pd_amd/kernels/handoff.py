@@ -54,8 +54,8 @@ class _Scope:
         self.on = None
         if self.stream is not None:
             st = self.stream
-            if isinstance(st, int):
-                st = torch.cuda.ExternalStream(st)
+            if isinstance(st, int):          # (0, the default stream's, ExternalStream takes for none)
+                st = torch.cuda.ExternalStream(st) if st else torch.cuda.default_stream()
             self.on = torch.cuda.stream(st)
             self.on.__enter__()
 

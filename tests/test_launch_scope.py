@@ -22,3 +22,23 @@ def test_stream_of_another_device_is_refused():
 def test_what_is_no_stream_is_refused(bad):
     with pytest.raises(TypeError):
         h.launch_scope(torch.device("cuda", 0), bad)
+
+
+def test_handle_zero_is_the_default_stream(monkeypatch):
+    """torch.cuda.ExternalStream takes a handle of 0 for none and makes a new stream."""
+    import contextlib
+    entered = []
+
+    @contextlib.contextmanager
+    def stream(s):
+        entered.append(s)
+        yield
+    monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
+    monkeypatch.setattr(torch.cuda, "stream", stream)
+    monkeypatch.setattr(torch.cuda, "default_stream", lambda d=None: ("default", d))
+    monkeypatch.setattr(torch.cuda, "ExternalStream", lambda h, **kw: ("external", h))
+    dev = torch.device("cuda", 1)
+    for handle in (0, 77):
+        with h.launch_scope(dev, handle):
+            pass
+    assert entered == [("default", None), ("external", 77)]   # the default of the device made current
