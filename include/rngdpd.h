@@ -851,6 +851,81 @@ int pdk_prefill_attn_window(const uint16_t* q, int64_t q_tok_stride,
                             float scale, int window, int sinks, uint16_t* out,
                             uintptr_t stream);
 
+/* ---- several requests' next tokens at once -------------------------------------
+ * A step over R requests' new tokens (pieces of prompts, drafts to be verified, single
+ * tokens) on the paged cache; request r has past[r] tokens there and gets added[r].
+ *
+ * The map: with held = ceil(past / 16), need = ceil((past + added) / 16) - held and
+ * first = the sum of need over the requests before r, tables[r][held + i] = free_ids[first
+ * + i] (i < need; -1 past n_free). starts [R + 1]: sums of added; ctx_lens [R] = past +
+ * added; positions and slots [max_tokens] of token starts[r] + i: past + i and its block *
+ * 16 + its place (-1 without a block, and both -1 behind the last token); taken [1]: the
+ * sum of need. Lengths outside [0, 16 max_blocks] count as the nearest. R <= 4096, R *
+ * max_blocks < 2^27. */
+int pdk_chunk_map(const int32_t* past, const int32_t* added, int R,
+                  int32_t* tables, int max_blocks, const int32_t* free_ids,
+                  int n_free, int max_tokens, int32_t* starts,
+                  int32_t* ctx_lens, int32_t* positions, int32_t* slots,
+                  int32_t* taken, uintptr_t stream);
+
+/* RoPE at positions [N] (below 0: 0) and the keys and values into slots [N] (block * 16
+ * + place; outside the cache: not written) of one layer's cache. qkv [N] rows of [Hq + 2
+ * Hkv][128] bf16, ld elements apart (a multiple of 8); q_out [N][Hq][128]. head_dim 128.
+ * The angle is position * inv_freq, exact before its cosine and sine. */
+int pdk_rope_cache_write(const uint16_t* qkv, int64_t ld, const float* inv_freq,
+                         const int32_t* positions, const int32_t* slots, int N,
+                         int n_q_heads, int n_kv_heads, int head_dim,
+                         uint16_t* q_out, uint16_t* cache_k, uint16_t* cache_v,
+                         int num_blocks, uintptr_t stream);
+
+/* Causal GQA attention of the new tokens: rows starts[r] .. starts[r + 1] - 1 of q [N] (n of
+ * them, rows of [Hq][128], q_tok_stride elements apart) stand at positions ctx_lens[r] - n
+ * + i and see the cached tokens up to their own, with window > 0 those of the last window
+ * positions and the first sinks. Tokens of blocks that the table does not name are seen by
+ * nobody; a token that sees nothing gets zeros. out [N][Hq][128]; rows of no request are
+ * left as they are. max_new and max_ctx are at least any request's. head_dim 128, Hq / Hkv
+ * from 1 to 16, max_blocks <= 65535, N <= 2^20. The workspace (16-byte aligned) serves
+ * one call at a time; pdk_chunk_attn_workspace_bytes is -1 for sizes out of range. */
+int64_t pdk_chunk_attn_workspace_bytes(int N, int R, int max_new, int max_ctx,
+                                       int n_q_heads, int n_kv_heads, int window,
+                                       int sinks);
+int pdk_chunk_attn(const uint16_t* q, int64_t q_tok_stride,
+                   const uint16_t* cache_k, const uint16_t* cache_v,
+                   int num_blocks, const int32_t* block_tables, int max_blocks,
+                   const int32_t* starts, const int32_t* ctx_lens, int N, int R,
+                   int max_new, int max_ctx, int n_q_heads, int n_kv_heads,
+                   int head_dim, float scale, int window, int sinks,
+                   void* workspace, size_t workspace_bytes, uint16_t* out,
+                   uintptr_t stream);
+
+/* ---- 8-bit projections -----------------------------------------------------------
+ * e4m3 (OCP) values with fp32 scales: a scale for each 128 columns of a row, scales[g *
+ * scale_ld + t] (scale_ld >= T); for each block of 128 x 128 of a weight, w_scales
+ * [ceil(N / 128)][K / 128].
+ *
+ * pdk_rmsnorm_fp8: y = s * rsqrt(mean(s^2) + eps) * weight over rows of H (a multiple of
+ * 128 up to 8192), s = x, or bf16(x + add), written to sum_out (x itself is allowed); scale
+ * = max(|y|, 2^-100) / 448 per group, out = y / scale. pdk_quantize_fp8 and
+ * pdk_swiglu_fp8: the same of rows x [T][K] and of silu(g) * u, rows [g | u] of 2 M; ld
+ * elements apart (a multiple of 8). */
+int pdk_rmsnorm_fp8(const uint16_t* x, const uint16_t* add,
+                    const uint16_t* weight, int T, int H, float eps,
+                    uint16_t* sum_out, uint8_t* out, float* scales,
+                    int64_t scale_ld, uintptr_t stream);
+int pdk_quantize_fp8(const uint16_t* x, int64_t ld, int T, int K, uint8_t* out,
+                     float* scales, int64_t scale_ld, uintptr_t stream);
+int pdk_swiglu_fp8(const uint16_t* gate_up, int64_t ld, int T, int M,
+                   uint8_t* out, float* scales, int64_t scale_ld,
+                   uintptr_t stream);
+
+/* y [T][N] bf16 = x . w^T: x [T] rows of K, x_ld bytes apart (a multiple of 16 below
+ * 2^24), their scales at x_scales[t * xs_tok_stride + g * xs_group_stride], w [N][K]. K a
+ * multiple of 128, N of 8. fp32 sums, rounded once. */
+int pdk_linear_fp8(const uint8_t* x, int64_t x_ld, const float* x_scales,
+                   int64_t xs_tok_stride, int64_t xs_group_stride,
+                   const uint8_t* w, const float* w_scales, int T, int K, int N,
+                   uint16_t* y, uintptr_t stream);
+
 /* ---- streams and events ------------------------------------------------------
  * Fences for the side-stream staging and for wait_for_save()
  * (connector/rngd_kv.py:129-131), which becomes a real barrier once saves

@@ -1,0 +1,272 @@
+// What a step over several requests' next tokens (pieces of prompts, a draft's
+// tokens, single ones) does to the paged cache, gfx950: the map of the tokens
+// (chunk_map_kernel) and their keys and values (rope_write_kernel).
+//
+// Map. Request r holds past_r tokens and gets new_r: with held = ceil(past / 16)
+// blocks, need = ceil((past + new) / 16) - held and first_r = the sum of need over
+// the requests before it, entry held + i of its table becomes free[first_r + i].
+// Every workgroup adds up all requests' lengths itself (a few loads a thread), so
+// one launch does it all; a token finds its request by bisection in LDS and reads
+// its block from the free list where its entry is new, so no workgroup waits for
+// another's entries. Bound by one launch and a chain of two loads.
+//
+// Write. Token i's q and k heads turn by the angle positions[i] * inv_freq: the
+// product in 64 bits, in turns, so that far positions keep their angle (in 32 bits
+// position 10^6 is off by up to 0.03). A workgroup computes the 64 angles of 16
+// tokens once and takes some of the heads: a lane turns the dims d .. d + 7 and
+// d + 64 .. d + 71 of a head (two 16-byte loads and stores). V lies dim by dim in
+// the cache: where eight tokens fill one half of a block, a lane transposes their 8
+// dims and stores 16 bytes for each; any other token is stored value by value.
+// Bound by HBM: each byte is read and written once.
+#include <math.h>
+
+#include <algorithm>
+
+#include "pdk_common.h"
+
+namespace {
+
+using pdk::v8;
+
+constexpr int kMaxRequests = 4096;
+constexpr int kThreads = 256;
+constexpr int kD = 128;
+constexpr int kTok = 16;                  // tokens of a write workgroup
+
+__device__ __forceinline__ int clamp_to(int x, int lo, int hi) { return min(max(x, lo), hi); }
+
+__global__ __launch_bounds__(kThreads) void chunk_map_kernel(
+    const int32_t* past, const int32_t* added, int R, int32_t* tables, int W, const int32_t* free_ids,
+    int n_free, int N, int32_t* starts, int32_t* ctx, int32_t* positions, int32_t* slots,
+    int32_t* taken) {
+  // Per request the sums before it: tokens in the launch, blocks taken.
+  __shared__ int32_t s_tok[kMaxRequests + 1], s_blk[kMaxRequests + 1];
+  __shared__ int32_t w_tok[kThreads / 64], w_blk[kThreads / 64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, cap = W * 16;
+  const int per = (R + kThreads - 1) / kThreads, r0 = min(tid * per, R), r1 = min(r0 + per, R);
+  auto length = [&](int r, int& p, int& n) {
+    p = clamp_to(past[r], 0, cap);
+    n = clamp_to(added[r], 0, cap - p);
+  };
+  auto blocks = [](int t) { return (t + 15) >> 4; };
+  int tok = 0, blk = 0;
+  for (int r = r0; r < r1; ++r) {
+    int p, n;
+    length(r, p, n);
+    tok += n;
+    blk += blocks(p + n) - blocks(p);
+  }
+  int tok_to = tok, blk_to = blk;         // inclusive sums over the wavefront
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int a = __shfl_up(tok_to, o), b = __shfl_up(blk_to, o);
+    if (lane >= o) {
+      tok_to += a;
+      blk_to += b;
+    }
+  }
+  if (lane == 63) {
+    w_tok[wave] = tok_to;
+    w_blk[wave] = blk_to;
+  }
+  __syncthreads();
+  tok = tok_to - tok;
+  blk = blk_to - blk;
+  for (int w = 0; w < wave; ++w) {
+    tok += w_tok[w];
+    blk += w_blk[w];
+  }
+  for (int r = r0; r < r1; ++r) {
+    int p, n;
+    length(r, p, n);
+    s_tok[r] = tok;
+    s_blk[r] = blk;
+    tok += n;
+    blk += blocks(p + n) - blocks(p);
+    if (r == R - 1) {
+      s_tok[R] = tok;
+      s_blk[R] = blk;
+    }
+  }
+  __syncthreads();
+  if (blockIdx.x == 0) {
+    for (int r = tid; r <= R; r += kThreads) {
+      starts[r] = s_tok[r];
+      if (r < R) ctx[r] = clamp_to(past[r], 0, cap) + s_tok[r + 1] - s_tok[r];
+    }
+    if (tid == 0) *taken = s_blk[R];
+  }
+  auto fresh = [&](int at) { return at < n_free ? free_ids[at] : -1; };
+  for (int r = blockIdx.x; r < R; r += gridDim.x) {
+    const int held = blocks(clamp_to(past[r], 0, cap)), first = s_blk[r], need = s_blk[r + 1] - first;
+    for (int i = tid; i < need; i += kThreads) tables[(int64_t)r * W + held + i] = fresh(first + i);
+  }
+  const int j = blockIdx.x * kThreads + tid;
+  if (j >= N) return;
+  int pos = -1, slot = -1;
+  if (j < s_tok[R]) {
+    int lo = 0, hi = R;                   // s_tok[lo] <= j < s_tok[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (s_tok[mid] <= j) lo = mid;
+      else hi = mid;
+    }
+    const int p = clamp_to(past[lo], 0, cap), held = blocks(p);
+    pos = p + j - s_tok[lo];
+    const int e = pos >> 4;
+    const int id = e < held ? tables[(int64_t)lo * W + e] : fresh(s_blk[lo] + e - held);
+    if (id >= 0 && id < (1 << 27)) slot = id * 16 + (pos & 15);
+  }
+  positions[j] = pos;
+  slots[j] = slot;
+}
+
+struct Turn {
+  float c, s;
+};
+
+// grid: x = 16 tokens, y = a share of the heads' units. Unit u < rot turns two q or
+// k heads; the others move V of eight heads.
+__global__ __launch_bounds__(kThreads) void rope_write_kernel(
+    const uint16_t* qkv, int64_t ld, const float* inv_freq, const int32_t* positions,
+    const int32_t* slots, int N, int NH, int NKV, uint16_t* q_out, uint16_t* cache_k,
+    uint16_t* cache_v, int64_t n_slots) {
+  __shared__ Turn turn[kTok][kD / 2 + 1];
+  __shared__ int32_t slot_of[kTok + 14];  // of tokens j0 - 7 .. j0 + kTok + 6
+  const int tid = threadIdx.x, j0 = blockIdx.x * kTok;
+  if (tid < kTok + 14) {
+    const int j = j0 - 7 + tid;
+    const int s = j >= 0 && j < N ? slots[j] : -1;
+    slot_of[tid] = s < n_slots ? s : -1;
+  }
+  const int rot = (NH + NKV + 1) / 2, units = rot + (NKV + 7) / 8;
+  if ((int)blockIdx.y < rot) {
+#pragma unroll
+    for (int x = 0; x < kTok * (kD / 2) / kThreads; ++x) {
+      const int i = tid & 63, t = (tid >> 6) + x * (kThreads / 64);
+      const int pos = max(positions[min(j0 + t, N - 1)], 0);
+      const double turns = (double)pos * ((double)inv_freq[i] * 0.15915494309189535);
+      float s, c;
+      sincosf((float)((turns - rint(turns)) * 6.283185307179586), &s, &c);
+      turn[t][i] = Turn{c, s};
+    }
+  }
+  __syncthreads();
+  for (int u = blockIdx.y; u < units; u += gridDim.y) {
+    if (u < rot) {
+      const int head = 2 * u + (tid >> 7), t = (tid >> 3) & 15, d = (tid & 7) * 8, j = j0 + t;
+      if (head >= NH + NKV || j >= N) continue;
+      const uint16_t* from = qkv + (int64_t)j * ld + (int64_t)head * kD + d;
+      const v8 a = pdk::ld16(from), b = pdk::ld16(from + 64);
+      v8 x, y;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        float r[2][2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const Turn z = turn[t][d + 2 * w + e];
+          pdk::rope_pair(pdk::bf16_to_f32(e ? a.w[w] >> 16 : a.w[w] & 0xffffu),
+                         pdk::bf16_to_f32(e ? b.w[w] >> 16 : b.w[w] & 0xffffu), z.c, z.s, r[0][e],
+                         r[1][e]);
+        }
+        x.w[w] = pdk::pack_bf16x2_rne(r[0][0], r[0][1]);
+        y.w[w] = pdk::pack_bf16x2_rne(r[1][0], r[1][1]);
+      }
+      if (head < NH) {
+        uint16_t* to = q_out + ((int64_t)j * NH + head) * kD + d;
+        pdk::st16(to, x);
+        pdk::st16(to + 64, y);
+      } else {
+        const int s = slot_of[t + 7];
+        if (s < 0) continue;
+        uint16_t* to = cache_k + ((int64_t)(s >> 4) * NKV + head - NH) * (16 * kD);
+        pdk::st16(to + pdk::k_unit(s & 15, d, kD) * 8, x);
+        pdk::st16(to + pdk::k_unit(s & 15, d + 64, kD) * 8, y);
+      }
+      continue;
+    }
+    // V: a lane has 8 dims of a head, of its token or of the eight from it on.
+    const int d = (tid & 15) * 8;
+    for (int h = (u - rot) * 8 + (tid >> 7); h < min((u - rot) * 8 + 8, NKV); h += 2)
+      for (int x = 0; x < 2; ++x) {
+        const int t = ((tid >> 4) & 7) + 8 * x, j = j0 + t, s = slot_of[t + 7];
+        if (j >= N || s < 0) continue;
+        // The token of the same half's slot 0, and whether the eight from it on fill it.
+        const int lead = t + 7 - (s & 7);
+        bool whole = true;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) whole &= slot_of[lead + i] == (s & ~7) + i;
+        const uint16_t* from = qkv + (int64_t)j * ld + (int64_t)(NH + NKV + h) * kD + d;
+        uint16_t* to = cache_v + (((int64_t)(s >> 4) * NKV + h) * kD + d) * 16 + (s & 15);
+        if (!whole) {
+          const v8 a = pdk::ld16(from);
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            to[32 * w] = (uint16_t)a.w[w];
+            to[32 * w + 16] = (uint16_t)(a.w[w] >> 16);
+          }
+        } else if ((s & 7) == 0) {
+          v8 in[8], out[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) in[i] = pdk::ld16(from + i * ld);
+          pdk::transpose8x8(in, out);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) pdk::st16(to + 16 * i, out[i]);
+        }
+      }
+  }
+}
+
+}  // namespace
+
+extern "C" int pdk_chunk_map(const int32_t* past, const int32_t* added, int R, int32_t* tables,
+                             int max_blocks, const int32_t* free_ids, int n_free, int max_tokens,
+                             int32_t* starts, int32_t* ctx_lens, int32_t* positions, int32_t* slots,
+                             int32_t* taken, uintptr_t stream) {
+  pdk::clear_error();
+  PDK_REQUIRE(R >= 1 && R <= kMaxRequests, "R must be in [1, %d] (got %d)", kMaxRequests, R);
+  PDK_REQUIRE(max_blocks >= 1 && (int64_t)R * max_blocks < (1ll << 27),
+              "tables of %d x %d blocks hold none or 2^31 tokens or more", R, max_blocks);
+  PDK_REQUIRE(n_free >= 0 && max_tokens >= 0 && max_tokens < (1 << 30),
+              "n_free or max_tokens out of range");
+  PDK_REQUIRE(past && added && tables && starts && ctx_lens && taken && (n_free == 0 || free_ids) &&
+                  (max_tokens == 0 || (positions && slots)),
+              "null pointer argument");
+  const int grid = std::max((max_tokens + kThreads - 1) / kThreads, 1);
+  hipLaunchKernelGGL(chunk_map_kernel, dim3(grid), dim3(kThreads), 0, pdk::as_stream(stream), past,
+                     added, R, tables, max_blocks, free_ids, n_free, max_tokens, starts, ctx_lens,
+                     positions, slots, taken);
+  return pdk::check_launch("chunk_map_kernel");
+}
+
+extern "C" int pdk_rope_cache_write(const uint16_t* qkv, int64_t ld, const float* inv_freq,
+                                    const int32_t* positions, const int32_t* slots, int N,
+                                    int n_q_heads, int n_kv_heads, int head_dim, uint16_t* q_out,
+                                    uint16_t* cache_k, uint16_t* cache_v, int num_blocks,
+                                    uintptr_t stream) {
+  pdk::clear_error();
+  if (head_dim != kD) {
+    pdk::set_error("the chunk kernels implement head_dim %d only (got %d)", kD, head_dim);
+    return PDK_ENOTSUP;
+  }
+  PDK_REQUIRE(N >= 0 && N <= (1 << 20), "N must be in [0, 2^20] (got %d)", N);
+  PDK_REQUIRE(n_q_heads >= 1 && n_kv_heads >= 1 && n_q_heads <= 65535 && n_kv_heads <= 65535,
+              "head counts out of range");
+  PDK_REQUIRE(ld >= (int64_t)(n_q_heads + 2 * n_kv_heads) * kD && ld % 8 == 0 && ld < (1ll << 31),
+              "ld must be a multiple of 8 and hold the heads");
+  PDK_REQUIRE(num_blocks >= 1 && num_blocks <= (1 << 27), "num_blocks out of range");
+  if (N == 0) return PDK_OK;
+  PDK_REQUIRE(qkv && inv_freq && positions && slots && q_out && cache_k && cache_v,
+              "null pointer argument");
+  PDK_REQUIRE(pdk::aligned16(qkv) && pdk::aligned16(q_out) && pdk::aligned16(cache_k) &&
+                  pdk::aligned16(cache_v),
+              "tensors must be 16-byte aligned");
+  const int tiles = (N + kTok - 1) / kTok;
+  const int units = (n_q_heads + n_kv_heads + 1) / 2 + (n_kv_heads + 7) / 8;
+  // Heads apart until there are four workgroups for every CU.
+  const int shares = std::min(units, std::max(1, (1024 + tiles - 1) / tiles));
+  hipLaunchKernelGGL(rope_write_kernel, dim3(tiles, shares), dim3(kThreads), 0,
+                     pdk::as_stream(stream), qkv, ld, inv_freq, positions, slots, N, n_q_heads,
+                     n_kv_heads, q_out, cache_k, cache_v, (int64_t)num_blocks * 16);
+  return pdk::check_launch("rope_write_kernel");
+}

@@ -1,0 +1,208 @@
+"""torch-facing wrappers of the 8-bit projections: rows and weights in e4m3 with
+32-bit scales, and their product.
+
+A row x [K] is kept as e4m3 values and a scale for each 128 columns, a weight [N, K]
+as e4m3 values and a scale for each block of 128 x 128 (the last rows' block may be
+smaller): the value stands for itself times its scale. Scales of rows come as [T,
+K / 128] with a group's lying together (strides 1 and T). The reference's
+projections are 16-bit (kernels/decode_batch.py:73-91).
+"""
+import torch
+
+from .. import _lib
+from .handoff import BF16, _current_device, _need, launch_scope, need_device, stream_handle
+from .prefill import overlap
+
+FP8 = torch.float8_e4m3fn
+GROUP = 128
+TOP = 448.0                # the largest e4m3 value
+LEAST = 2.0 ** -100        # a group's largest value counts as at least this
+
+
+def _rows_of(t, name, dev, width=None):
+    """(t, T, columns, row stride) of bf16 rows, copied where they are strided or off
+    16 bytes in a way the kernels do not take."""
+    _need(t, name)
+    need_device(dev, t, name)
+    if t.dim() != 2:
+        raise ValueError(f"{name} must be [T, columns], got {tuple(t.shape)}")
+    T, K = t.shape
+    ld = t.stride(0) if T > 1 else K
+    if (K > 1 and t.stride(1) != 1) or ld < K or ld % 8 or t.data_ptr() % 16:
+        t, ld = t.clone(memory_format=torch.contiguous_format), K
+    return t, T, K, ld
+
+
+def _outputs(out, T, K, dev, others):
+    """(values [T, K] e4m3, scales [T, K / 128] float32), new or the caller's."""
+    if out is None:
+        return (torch.empty((T, K), dtype=FP8, device=dev),
+                torch.empty((K // GROUP, T), dtype=torch.float32, device=dev).t())
+    values, scales = out
+    _need(values, "out values", FP8)
+    _need(scales, "out scales", torch.float32)
+    for t, name in ((values, "out values"), (scales, "out scales")):
+        need_device(dev, t, name)
+        if any(overlap(t, o) for o in others) or overlap(values, scales):
+            raise ValueError(f"{name} must not overlap the other tensors")
+    if tuple(values.shape) != (T, K) or not values.is_contiguous() or values.data_ptr() % 16:
+        raise ValueError(f"out values must be contiguous and 16-byte aligned {(T, K)}")
+    if tuple(scales.shape) != (T, K // GROUP) or not scales.t().is_contiguous():
+        raise ValueError(f"out scales must be {(T, K // GROUP)} with a group's lying together")
+    return values, scales
+
+
+def rmsnorm_fp8(x, weight, eps, add=None, sum_out=None, out=None, stream=None):
+    """RMSNorm over the last dim of x [T, H] bf16 in 8 bits -> (values [T, H] e4m3,
+    scales [T, H / 128] float32).
+
+    With ``add`` [T, H] the norm is of bf16(x + add), which is written to ``sum_out``
+    (default: x itself, as rmsnorm does). y = x * rsqrt(mean(x^2) + eps) * weight is
+    32-bit until it is 8: a group's scale is max(|y|, 2^-100) / 448, its values
+    y / scale. H a multiple of 128 up to 8192."""
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        raise TypeError("x must be a CUDA tensor")
+    dev = x.device
+    if stream is not None or dev.index != _current_device():
+        with launch_scope(dev, stream):
+            return rmsnorm_fp8(x, weight, eps, add, sum_out, out)
+    _need(x, "x")
+    if x.dim() != 2 or not x.is_contiguous() or x.data_ptr() % 16:
+        raise ValueError(f"x must be contiguous and 16-byte aligned [T, H], got {tuple(x.shape)}")
+    T, H = x.shape
+    if H % GROUP or not GROUP <= H <= 8192:
+        raise ValueError(f"H={H} is no multiple of {GROUP} in [{GROUP}, 8192]")
+    _need(weight, "weight")
+    need_device(dev, weight, "weight")
+    if weight.numel() != H or not weight.is_contiguous() or weight.data_ptr() % 16:
+        raise ValueError(f"weight must hold H={H} contiguous values, 16-byte aligned")
+    if add is not None:
+        _need(add, "add")
+        need_device(dev, add, "add")
+        if add.shape != x.shape or not add.is_contiguous() or add.data_ptr() % 16:
+            raise ValueError("add must be contiguous, 16-byte aligned and shaped like x")
+        if sum_out is None:
+            sum_out = x
+        elif sum_out.data_ptr() != x.data_ptr():
+            if overlap(sum_out, x):
+                raise ValueError("sum_out must be x itself or not overlap it")
+        _need(sum_out, "sum_out")
+        need_device(dev, sum_out, "sum_out")
+        if sum_out.shape != x.shape or not sum_out.is_contiguous() or sum_out.data_ptr() % 16:
+            raise ValueError("sum_out must be contiguous, 16-byte aligned and shaped like x")
+        if overlap(sum_out, weight) or (overlap(sum_out, add)
+                                        and sum_out.data_ptr() != add.data_ptr()):
+            raise ValueError("sum_out must not overlap weight, nor add unless it is add itself")
+    elif sum_out is not None:
+        raise ValueError("sum_out needs add")
+    values, scales = _outputs(out, T, H, dev, [t for t in (x, weight, add, sum_out) if t is not None])
+    if T:
+        _lib.call("pdk_rmsnorm_fp8", x.data_ptr(), None if add is None else add.data_ptr(),
+                  weight.data_ptr(), T, H, float(eps),
+                  None if sum_out is None else sum_out.data_ptr(), values.data_ptr(),
+                  scales.data_ptr(), T, stream_handle())
+    return values, scales
+
+
+def _quantized(entry, x, gated, out, stream):
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        raise TypeError("x must be a CUDA tensor")
+    dev = x.device
+    if stream is not None or dev.index != _current_device():
+        with launch_scope(dev, stream):
+            return _quantized(entry, x, gated, out, None)
+    x, T, K, ld = _rows_of(x, "x", dev)
+    K, rest = divmod(K, 2) if gated else (K, 0)
+    if rest or K % GROUP or K < GROUP:
+        raise ValueError(f"the columns must be a multiple of {GROUP}{' for each half' * gated}")
+    values, scales = _outputs(out, T, K, dev, [x])
+    if T:
+        _lib.call(entry, x.data_ptr(), ld, T, K, values.data_ptr(), scales.data_ptr(), T,
+                  stream_handle())
+    return values, scales
+
+
+def quantize_fp8(x, out=None, stream=None):
+    """x [T, K] bf16 in 8 bits -> (values, scales) as rmsnorm_fp8's."""
+    return _quantized("pdk_quantize_fp8", x, False, out, stream)
+
+
+def swiglu_fp8(gate_up, out=None, stream=None):
+    """silu(g) * u of gate_up = [g | u] [T, 2M] bf16, 32-bit until it is 8 -> (values
+    [T, M], scales) as rmsnorm_fp8's."""
+    return _quantized("pdk_swiglu_fp8", gate_up, True, out, stream)
+
+
+@torch.no_grad()
+def quantize_weight_fp8(w):
+    """w [N, K] (K a multiple of 128) in 8 bits, a scale for each block of 128 x 128 ->
+    (values [N, K] e4m3, scales [ceil(N / 128), K / 128] float32). For the loading of a
+    model: torch operations, some rows at a time."""
+    if w.dim() != 2 or w.shape[1] % GROUP or 0 in w.shape:
+        raise ValueError(f"w must be [N, K] with K a multiple of {GROUP}, got {tuple(w.shape)}")
+    N, K = w.shape
+    values = torch.empty((N, K), dtype=FP8, device=w.device)
+    scales = torch.empty((-(-N // GROUP), K // GROUP), dtype=torch.float32, device=w.device)
+    step = GROUP * 32
+    for at in range(0, N, step):
+        part = w[at:at + step].float()
+        n = part.shape[0]
+        part = torch.nn.functional.pad(part, (0, 0, 0, -n % GROUP)).view(-1, GROUP, K // GROUP, GROUP)
+        s = part.abs().amax((1, 3)).clamp(min=LEAST) / TOP
+        scales[at // GROUP:at // GROUP + s.shape[0]] = s
+        values[at:at + n] = (part / s[:, None, :, None]).view(-1, K)[:n].to(FP8)
+    return values, scales
+
+
+def linear_fp8(x, x_scales, w, w_scales, out=None, stream=None):
+    """x . w^T of 8-bit rows and weights -> [T, N] bf16.
+
+    x [T, K] e4m3 (unit column stride) with x_scales float32 [T, K / 128] (any positive
+    strides), w [N, K] e4m3 contiguous with w_scales float32 [ceil(N / 128), K / 128]
+    contiguous, as rmsnorm_fp8, quantize_fp8, swiglu_fp8 and quantize_weight_fp8 give
+    them. Products and sums of a group of 128 columns are 32-bit, scaled and added in
+    32 bits, rounded to bf16 once. K a multiple of 128, N of 8."""
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        raise TypeError("x must be a CUDA tensor")
+    dev = x.device
+    if stream is not None or dev.index != _current_device():
+        with launch_scope(dev, stream):
+            return linear_fp8(x, x_scales, w, w_scales, out)
+    _need(x, "x", FP8)
+    _need(w, "w", FP8)
+    _need(x_scales, "x_scales", torch.float32)
+    _need(w_scales, "w_scales", torch.float32)
+    for t, name in ((w, "w"), (x_scales, "x_scales"), (w_scales, "w_scales")):
+        need_device(dev, t, name)
+    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
+        raise ValueError(f"x [T, K] and w [N, K] expected, got {tuple(x.shape)}, {tuple(w.shape)}")
+    (T, K), N = x.shape, w.shape[0]
+    if K % GROUP or K < GROUP or N % 8 or N < 8:
+        raise ValueError(f"K={K} must be a multiple of {GROUP}, N={N} of 8")
+    if not w.is_contiguous() or w.data_ptr() % 16:
+        raise ValueError("w must be contiguous and 16-byte aligned")
+    groups = K // GROUP
+    if tuple(x_scales.shape) != (T, groups):
+        raise ValueError(f"x_scales must be {(T, groups)}, got {tuple(x_scales.shape)}")
+    if tuple(w_scales.shape) != (-(-N // GROUP), groups) or not w_scales.is_contiguous():
+        raise ValueError(f"w_scales must be contiguous {(-(-N // GROUP), groups)}")
+    xs_t = x_scales.stride(0) if T > 1 else 1
+    xs_g = x_scales.stride(1) if groups > 1 else 1
+    if xs_t < 1 or xs_g < 1:
+        x_scales, xs_t, xs_g = x_scales.contiguous(), groups, 1
+    ld = x.stride(0) if T > 1 else K
+    if x.stride(1) != 1 or ld < K or ld % 16 or ld >= 1 << 24 or x.data_ptr() % 16:
+        x, ld = x.clone(memory_format=torch.contiguous_format), K
+    if out is None:
+        out = torch.empty((T, N), dtype=BF16, device=dev)
+    else:
+        _need(out, "out")
+        need_device(dev, out, "out")
+        if tuple(out.shape) != (T, N) or not out.is_contiguous() or out.data_ptr() % 16:
+            raise ValueError(f"out must be contiguous and 16-byte aligned {(T, N)}")
+        if any(overlap(out, t) for t in (x, x_scales, w, w_scales)):
+            raise ValueError("out must not overlap the operands")
+    if T:
+        _lib.call("pdk_linear_fp8", x.data_ptr(), ld, x_scales.data_ptr(), xs_t, xs_g, w.data_ptr(),
+                  w_scales.data_ptr(), T, K, N, out.data_ptr(), stream_handle())
+    return out

@@ -1,0 +1,187 @@
+"""Rows and weights in 8 bits and their product, against 64 bits."""
+import pytest
+import torch
+
+from tests import _chunk_ref as ref
+
+pytestmark = pytest.mark.gpu
+BF16, EPS = torch.bfloat16, 1e-5
+
+
+def _randn(seed, *shape, std=1.0):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(shape, generator=gen, device="cuda") * std).to(BF16)
+
+
+def _check_8_bits(values, scales, y, rel, what):
+    """values and scales against the 64-bit rows y, known to ``rel``."""
+    T, K = y.shape
+    top = y.view(T, -1, 128).abs().amax(-1).clamp(min=2.0 ** -100) / 448
+    assert values.dtype == torch.float8_e4m3fn and tuple(scales.shape) == (T, K // 128)
+    assert scales.t().is_contiguous()
+    ref.within(scales, top, (rel + 2.0 ** -22) * top, what + " scales")
+    s = scales.double().repeat_interleave(128, 1)
+    ref.within(values.double() * s, y, ref.e4m3_bound(y, s, 2 * rel), what + " values")
+
+
+@pytest.mark.parametrize("T,H", [(1, 128), (1, 4096), (3, 384), (16, 4096), (7, 8192), (130, 2176),
+                                 (33, 6144), (1000, 4096), (5000, 256)])
+@pytest.mark.parametrize("add", [False, True])
+def test_norm(cuda, T, H, add):
+    from rngd_pd_amd import kernels as K
+    print(f"norm T={T} H={H} add={add}", flush=True)
+    x, more, w = _randn(T, T, H, std=3.0), _randn(T + 1, T, H), _randn(2, H, std=0.3) + 1
+    kept = x.clone()
+    if add:
+        total = (x.float() + more.float()).to(BF16)
+        into = torch.empty_like(x)
+        values, scales = K.rmsnorm_fp8(x, w, EPS, add=more, sum_out=into)
+        assert torch.equal(into, total) and torch.equal(x, kept)
+        v2, s2 = K.rmsnorm_fp8(x, w, EPS, add=more)          # into x itself
+        assert torch.equal(x, total)
+        assert torch.equal(v2.view(torch.uint8), values.view(torch.uint8)) and torch.equal(s2, scales)
+    else:
+        total = x
+        values, scales = K.rmsnorm_fp8(x, w, EPS)
+        assert torch.equal(x, kept)
+    t = total.double()
+    y = t / torch.sqrt(t.square().mean(-1, keepdim=True) + EPS) * w.double()
+    # The sum of H squares is off by H 2^-24, its root by half of that; rsqrt and the
+    # three products by less than 2^-21.
+    _check_8_bits(values, scales, y, H * 2.0 ** -25 + 2.0 ** -21, "norm")
+
+
+def test_norm_of_zeros_and_of_values_that_are_not_finite(cuda):
+    from rngd_pd_amd import kernels as K
+    x = _randn(0, 4, 256)
+    x[0] = 0
+    x[1, 5] = float("nan")
+    x[2, 200] = float("inf")
+    values, scales = K.rmsnorm_fp8(x, torch.ones(256, dtype=BF16, device=cuda), EPS)
+    assert not values[0].float().any() and (scales[0] == 2.0 ** -100 / 448).all()
+    assert torch.isnan(scales[1]).all() and torch.isnan(values[1].float()).all()
+    # inf * rsqrt(inf) is NaN, a finite value times 0 is 0.
+    assert torch.isnan(scales[2, 1]) and scales[2, 0] == 2.0 ** -100 / 448
+    y = x[3:].double()
+    y = y / torch.sqrt(y.square().mean(-1, keepdim=True) + EPS)
+    _check_8_bits(values[3:], scales[3:].t().contiguous().t(), y, 2.0 ** -17, "the row beside them")
+
+
+@pytest.mark.parametrize("T,K", [(1, 128), (5, 640), (300, 4096), (17, 14336)])
+def test_quantize_and_swiglu(cuda, T, K):
+    from rngd_pd_amd import kernels as Kn
+    print(f"quantize T={T} K={K}", flush=True)
+    wide = _randn(T, T, K + 8, std=2.0)
+    x = wide[:, :K]
+    values, scales = Kn.quantize_fp8(x)
+    _check_8_bits(values, scales, x.double(), 2.0 ** -23, "rows")
+    out = (torch.empty_like(values), torch.empty((K // 128, T), device=cuda).t())
+    assert Kn.quantize_fp8(x.contiguous(), out=out)[0] is out[0]
+    assert torch.equal(out[0].view(torch.uint8), values.view(torch.uint8)) and torch.equal(out[1], scales)
+    gu = _randn(T + 1, T, 2 * K, std=4.0)
+    values, scales = Kn.swiglu_fp8(gu)
+    g, u = gu[:, :K].double(), gu[:, K:].double()
+    # exp of an argument up to 24 here: 24 2^-24 from its scaling, and a few roundings.
+    _check_8_bits(values, scales, torch.nn.functional.silu(g) * u, 2.0 ** -18, "swiglu")
+
+
+def _weight(seed, N, K):
+    from rngd_pd_amd import kernels as Kn
+    w = _randn(seed, N, K, std=0.02)
+    q, s = Kn.quantize_weight_fp8(w)
+    full = s.double().repeat_interleave(128, 0)[:N].repeat_interleave(128, 1)
+    top = torch.nn.functional.pad(w, (0, 0, 0, -N % 128)).view(-1, 128, K // 128, 128).abs().amax((1, 3))
+    assert torch.equal(s, top.float().clamp(min=2.0 ** -100) / 448)
+    ref.within(q.double() * full, w.double(), ref.e4m3_bound(w.double(), full, 2.0 ** -22))
+    return q, s, full
+
+
+def _product(x, xs, w, full):
+    """(y, bound): the products of e4m3 values are exact; each of a group's 128 additions, and
+    of a group's sum, may lose 2^-23 of what has been added up; the two scales' product,
+    their multiplication and y's rounding follow."""
+    xd = x.double() * xs.double().repeat_interleave(128, 1)
+    wd = w.double() * full
+    y = xd @ wd.t().contiguous()
+    A = xd.abs() @ wd.abs().t().contiguous()
+    K = x.shape[1]
+    return y, (1 + 2.0 ** -8) * (128 + K // 128 + 4) * 2.0 ** -23 * A + 2.0 ** -8 * y.abs() + 2.0 ** -134
+
+
+LINEAR = [
+    (1, 8, 128), (1, 4096, 4096), (2, 136, 256), (16, 6144, 4096), (17, 264, 384), (15, 24, 14336),
+    (32, 4096, 14336), (33, 520, 1280), (64, 1000, 512), (100, 4096, 4096), (129, 136, 128),
+    (257, 8, 256), (470, 4096, 14336), (300, 2056, 640), (1000, 6144, 4096), (2049, 4104, 512),
+    (4100, 8200, 256),
+]
+
+
+@pytest.mark.parametrize("T,N,K", LINEAR)
+def test_linear(cuda, T, N, K):
+    from rngd_pd_amd import kernels as Kn
+    print(f"linear T={T} N={N} K={K}", flush=True)
+    x, xs = Kn.quantize_fp8(_randn(T + K, T, K) * torch.rand((T, 1), device=cuda).to(BF16))
+    w, ws, full = _weight(N, N, K)
+    want, bound = _product(x, xs, w, full)
+    got = Kn.linear_fp8(x, xs, w, ws)
+    ref.within(got, want, bound, "plain")
+    out = torch.full((T, N), 9.0, dtype=BF16, device=cuda)
+    rows = torch.zeros((T, K + 32), dtype=torch.uint8, device=cuda)
+    rows[:, :K] = x.view(torch.uint8)
+    cols = rows.view(torch.float8_e4m3fn)[:, :K]
+    assert Kn.linear_fp8(cols, xs.contiguous(), w, ws, out=out) is out     # strided rows, scales by row
+    assert torch.equal(out, got)
+
+
+def test_linear_where_groups_cancel(cuda):
+    """Large groups of opposite sign: what is left of them is 32-bit."""
+    from rngd_pd_amd import kernels as Kn
+    T, N, K = 40, 256, 512
+    x = _randn(1, T, K)
+    x[:, 128:256] = -x[:, :128] * 1
+    w = _randn(2, N, K)
+    w[:, 128:256] = w[:, :128]
+    x[:, 256:] *= 2.0 ** -8
+    x8, xs = Kn.quantize_fp8(x)
+    w8, ws = Kn.quantize_weight_fp8(w)
+    full = ws.double().repeat_interleave(128, 0)[:N].repeat_interleave(128, 1)
+    want, bound = _product(x8, xs, w8, full)
+    for rows in (T, 5):
+        ref.within(Kn.linear_fp8(x8[:rows], xs[:rows], w8, ws), want[:rows], bound[:rows])
+
+
+def test_linear_of_values_that_are_not_finite(cuda):
+    from rngd_pd_amd import kernels as Kn
+    for T in (8, 200):
+        x, xs = Kn.quantize_fp8(_randn(3, T, 256))
+        w, ws = Kn.quantize_weight_fp8(_randn(4, 512, 256))
+        x.view(torch.uint8)[3, 7] = 0x7f                         # NaN
+        xs[5, 1] = float("inf")
+        got = Kn.linear_fp8(x, xs, w, ws)
+        assert torch.isnan(got[3]).all() and not torch.isfinite(got[5]).any()
+        keep = [i for i in range(T) if i not in (3, 5)]
+        assert torch.isfinite(got[keep]).all()
+
+
+def test_side_stream_and_graph(cuda):
+    from rngd_pd_amd import kernels as Kn
+    x, w = _randn(5, 33, 512), torch.ones(512, dtype=BF16, device=cuda)
+    w8, ws = Kn.quantize_weight_fp8(_randn(6, 256, 512))
+
+    def chain():
+        return Kn.linear_fp8(*Kn.rmsnorm_fp8(x, w, EPS), w8, ws)
+    want = chain()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    v, s = Kn.rmsnorm_fp8(x, w, EPS, stream=side)
+    got = Kn.linear_fp8(v, s, w8, ws, stream=side)
+    side.synchronize()
+    assert torch.equal(got, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        out = chain()
+    for seed in (7, 8, 9):
+        x.copy_(_randn(seed, 33, 512))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, chain())
