@@ -136,6 +136,46 @@ class PagedKVCache:
                 have.extend(self.alloc.allocate(need - len(have)))
                 self._dev_tables.pop(req_id, None)
 
+    def extend(self, chunks):
+        """Blocks for the next tokens of several requests, as chunk_map takes them:
+        ``chunks`` holds (req_id, tokens in the cache before, new ones) of different
+        requests, one without tokens and blocks being a new request. Returns (tables,
+        free): host int32 [R, max_blocks] with the entries of the tokens that are there
+        (the others -1), and the ids that the new tokens' entries take, request after
+        request. Nothing changes if the blocks do not suffice."""
+        chunks = [(r, int(past), int(n)) for r, past, n in chunks]
+        if len({r for r, _, _ in chunks}) != len(chunks):
+            raise ValueError("a request comes twice")
+        with self._lock:
+            grow = []
+            for r, past, n in chunks:
+                have = self._tables.get(r, [])
+                if past < 0 or n < 0 or len(have) * BLOCK < past:
+                    raise ValueError(f"{r!r} holds {len(have)} blocks, fewer than {past} tokens, "
+                                     f"or its {n} new ones are negative")
+                # The blocks that are written: the partly filled one and those behind it.
+                last = -(-(past + n) // BLOCK)
+                written = have[past // BLOCK:last] if n else []
+                if any(b < 0 for b in written):
+                    raise ValueError(f"{r!r} has dropped blocks of tokens {past} to {past + n - 1}")
+                if any(b in self._shared for b in written):
+                    raise ValueError(f"{r!r} shares blocks of tokens {past} to {past + n - 1}")
+                grow.append(max(0, last - len(have)))
+            ids = self.alloc.allocate(sum(grow))
+            tables = np.full((len(chunks), max([1] + [-(-(p + n) // BLOCK) for _, p, n in chunks])),
+                             -1, np.int32)
+            free, at = [], 0
+            for i, ((r, past, n), g) in enumerate(zip(chunks, grow)):
+                have = self._tables.setdefault(r, [])
+                have.extend(ids[at:at + g])
+                at += g
+                if g:
+                    self._dev_tables.pop(r, None)
+                held = -(-past // BLOCK)
+                tables[i, :held] = have[:held]
+                free += have[held:-(-(past + n) // BLOCK)]
+        return tables, np.asarray(free, np.int32)
+
     def free(self, req_id):
         with self._lock:
             if req_id in self._tables:
