@@ -97,20 +97,25 @@ __global__ __launch_bounds__(kThreads) void chunk_map_kernel(
     if (tid == 0) *taken = s_blk[R];
   }
   auto fresh = [&](int at) { return at < n_free ? free_ids[at] : -1; };
-  for (int r = blockIdx.x; r < R; r += gridDim.x) {
-    const int held = blocks(clamp_to(past[r], 0, cap)), first = s_blk[r], need = s_blk[r + 1] - first;
-    for (int i = tid; i < need; i += kThreads) tables[(int64_t)r * W + held + i] = fresh(first + i);
+  // The request of item j of those that sums [R + 1] counts.
+  auto request_of = [&](const int32_t* sums, int j) {
+    int lo = 0, hi = R;                   // sums[lo] <= j < sums[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (sums[mid] <= j) lo = mid;
+      else hi = mid;
+    }
+    return lo;
+  };
+  for (int k = blockIdx.x * kThreads + tid; k < s_blk[R]; k += gridDim.x * kThreads) {
+    const int r = request_of(s_blk, k), held = blocks(clamp_to(past[r], 0, cap));
+    tables[(int64_t)r * W + held + k - s_blk[r]] = fresh(k);
   }
   const int j = blockIdx.x * kThreads + tid;
   if (j >= N) return;
   int pos = -1, slot = -1;
   if (j < s_tok[R]) {
-    int lo = 0, hi = R;                   // s_tok[lo] <= j < s_tok[hi]
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (s_tok[mid] <= j) lo = mid;
-      else hi = mid;
-    }
+    const int lo = request_of(s_tok, j);
     const int p = clamp_to(past[lo], 0, cap), held = blocks(p);
     pos = p + j - s_tok[lo];
     const int e = pos >> 4;
@@ -140,6 +145,18 @@ __global__ __launch_bounds__(kThreads) void rope_write_kernel(
     slot_of[tid] = s < n_slots ? s : -1;
   }
   const int rot = (NH + NKV + 1) / 2, units = rot + (NKV + 7) / 8;
+  // A lane's place in a unit of two turned heads; the first unit's values are under way
+  // while the angles are computed.
+  const int t_of = (tid >> 3) & 15, d_of = (tid & 7) * 8;
+  const uint16_t* const row = qkv + (int64_t)min(j0 + t_of, N - 1) * ld + d_of;
+  auto head_of = [&](int u) { return 2 * u + (tid >> 7); };
+  v8 a, b;
+  auto load = [&](int u) __attribute__((always_inline)) {
+    const uint16_t* from = row + (int64_t)min(head_of(u), NH + NKV - 1) * kD;
+    a = pdk::ld16(from);
+    b = pdk::ld16(from + 64);
+  };
+  load(min((int)blockIdx.y, rot - 1));
   if ((int)blockIdx.y < rot) {
 #pragma unroll
     for (int x = 0; x < kTok * (kD / 2) / kThreads; ++x) {
@@ -154,10 +171,7 @@ __global__ __launch_bounds__(kThreads) void rope_write_kernel(
   __syncthreads();
   for (int u = blockIdx.y; u < units; u += gridDim.y) {
     if (u < rot) {
-      const int head = 2 * u + (tid >> 7), t = (tid >> 3) & 15, d = (tid & 7) * 8, j = j0 + t;
-      if (head >= NH + NKV || j >= N) continue;
-      const uint16_t* from = qkv + (int64_t)j * ld + (int64_t)head * kD + d;
-      const v8 a = pdk::ld16(from), b = pdk::ld16(from + 64);
+      const int head = head_of(u), t = t_of, d = d_of, j = j0 + t;
       v8 x, y;
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
@@ -172,11 +186,13 @@ __global__ __launch_bounds__(kThreads) void rope_write_kernel(
         x.w[w] = pdk::pack_bf16x2_rne(r[0][0], r[0][1]);
         y.w[w] = pdk::pack_bf16x2_rne(r[1][0], r[1][1]);
       }
+      if (u + (int)gridDim.y < rot) load(u + gridDim.y);
+      if (j >= N) continue;
       if (head < NH) {
         uint16_t* to = q_out + ((int64_t)j * NH + head) * kD + d;
         pdk::st16(to, x);
         pdk::st16(to + 64, y);
-      } else {
+      } else if (head < NH + NKV) {
         const int s = slot_of[t + 7];
         if (s < 0) continue;
         uint16_t* to = cache_k + ((int64_t)(s >> 4) * NKV + head - NH) * (16 * kD);

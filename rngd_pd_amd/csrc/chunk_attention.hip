@@ -40,6 +40,7 @@ using pdk::v8;
 
 typedef __bf16 bf16x8_t __attribute__((__vector_size__(16)));
 typedef float f32x16 __attribute__((__vector_size__(64)));
+typedef float f32x4 __attribute__((__vector_size__(16)));
 
 constexpr int kD = 128;
 constexpr int kBlockElems = 16 * kD;      // of K or V in a block, per head
@@ -51,6 +52,8 @@ constexpr int kRing = 3;                  // tiles in LDS
 constexpr int kLoads = 4;                 // of a wavefront per tile, 1 KiB each
 constexpr int kMaxRequests = 65535;
 constexpr int kMaxSplits = 64;
+constexpr int kLeastSplit = 8;            // tiles of a split at least
+constexpr int kCUs = 256;
 constexpr int kRecord = 64 * 66;          // floats of a unit's sums: O 64 lanes x 64, (m, l)
 
 struct Args {
@@ -66,14 +69,20 @@ struct Args {
   int window, sinks;
   float* ws;
   uint16_t* out;
-  // Rows up to which a request is one unit's (32, or 0 where all are taken as longer
-  // ones); tiles of a split and splits at most, of the former and the latter; workgroups of
-  // the longer ones' rows at most.
-  int few_rows, few_per, few_splits, big_per, big_splits, big_tiles;
+  // Rows up to which a request has few (16 or 32, or 0 where all are taken as longer
+  // ones), tiles of a split and splits at most of those; of the longer ones, workgroups
+  // that run at once and splits of what they leave over.
+  int few_rows, few_per, few_splits, big_slots, big_splits;
+  int64_t big_base;                       // floats of the workspace before the longer ones' records
 };
 
 __device__ __forceinline__ f32x16 mfma32(const v8& a, const v8& b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a),
+                                                 __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+}
+
+__device__ __forceinline__ f32x4 mfma16(const v8& a, const v8& b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a),
                                                  __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
 }
 
@@ -250,6 +259,18 @@ __device__ __forceinline__ bool clean(v8& a) {
   return odd;
 }
 
+__device__ __forceinline__ uint32_t mark_of(uint32_t u) {
+  return (u & 0x7f80u) != 0x7f80u ? 0u : u == 0x7f80u ? 0x3f80u : u == 0xff80u ? 0x4280u : 0x4580u;
+}
+
+// What a mark's count comes to: infinities and NaN to add.
+__device__ __forceinline__ float found_value(float found) {
+  const uint32_t u = (uint32_t)found;
+  float add = u & 63 ? INFINITY : 0.f;
+  add = u & 0xfc0 ? add - INFINITY : add;
+  return u >> 12 ? __builtin_nanf("") : add;
+}
+
 // What clean() took from the tiles `first` to `end` of a walk that hide something:
 // infinities and NaN of the tokens that a row sees, added to its O. Marks of them (1 for
 // infinity, 64 for -infinity, 4096 for NaN) times 1 for each token that is seen: the
@@ -278,14 +299,7 @@ __device__ __forceinline__ void add_cleaned(const Args& a, const Walk& w, int fi
         v8 mark, seen;
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          uint32_t m = 0;
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const uint32_t u = v.w[x] >> (16 * e) & 0xffffu;
-            const uint32_t code = u == 0x7f80u ? 0x3f80u : u == 0xff80u ? 0x4280u : 0x4580u;
-            m |= ((u & 0x7f80u) == 0x7f80u ? code : 0u) << (16 * e);
-          }
-          mark.w[x] = m;
+          mark.w[x] = mark_of(v.w[x] & 0xffffu) | mark_of(v.w[x] >> 16) << 16;
           seen.w[x] = (at.hidden(8 * b + 2 * x) ? 0u : 0x3f80u) |
                       (at.hidden(8 * b + 2 * x + 1) ? 0u : 0x3f800000u);
         }
@@ -335,15 +349,8 @@ __device__ __forceinline__ float inverse(float l) { return l == 0.f ? 0.f : 1.f 
 
 // A split's sums of a unit: float4s [16][64 lanes], then (m, l) per lane, both halves'
 // weights in l.
-__device__ __forceinline__ float* record(const Args& a, int64_t unit, int splits, int z) {
-  return a.ws + (unit * splits + z) * kRecord;
-}
-
-__device__ __forceinline__ int64_t big_base(const Args& a) {
-  return a.few_splits > 1 ? (int64_t)a.R * a.NKV * a.few_splits * kRecord : 0;
-}
-
-__device__ __forceinline__ void keep_dims(float* rec, int n, int lane, const float (&o)[16]) {
+__device__ __forceinline__ void keep_dims(float* rec, int n, int lane, bool mine, const float (&o)[16]) {
+  if (!mine) return;                      // few rows: little to store and to join
   float4* p = reinterpret_cast<float4*>(rec) + 4 * n * 64 + lane;
 #pragma unroll
   for (int x = 0; x < 16; x += 4) p[x / 4 * 64] = make_float4(o[x], o[x + 1], o[x + 2], o[x + 3]);
@@ -353,154 +360,400 @@ __device__ __forceinline__ void keep_sums(float* rec, int lane, float m, float l
   reinterpret_cast<float2*>(rec + 64 * 64)[lane] = make_float2(m, l);
 }
 
-// ---- requests of one unit -----------------------------------------------------
-struct FewShared {
-  float4 o[kWaves][16][64];
-  float2 ml[kWaves][64];
+// ---- requests of few rows -----------------------------------------------------
+// Up to kSets x 16 rows; a lane's row of a set is i = lane & 15, and of 32 tokens it holds
+// 8 kg .. 8 kg + 7, kg = lane >> 4: S^T's tile u (v_mfma_f32_16x16x32_bf16) has token 8
+// (r / 4) + 4 u + r % 4 in row r, so that its accumulators are 4 kg + 0..3 of both tiles,
+// which are the B operand of O^T.
+template <int kSets>
+struct FewSums {
+  float m[kSets], l[kSets];
+  f32x4 o[kSets][8];                      // dims 16 n + 4 kg + 0..3
 };
 
-__device__ __forceinline__ void few_unit(const Args& a, FewShared& sm, int r, int kvh, int z) {
-  const int lane = threadIdx.x & 63, j = lane & 31, hh = lane >> 5;
+template <int kSets>
+struct FewShared {
+  f32x4 o[kWaves][kSets * 8][64];
+  float2 ml[kWaves][kSets][64];
+};
+
+template <int kSets>
+constexpr int kFewRecord = kSets * (8 * 64 * 4 + 64 * 2);        // floats
+
+// The largest, or the sum, over the four lanes that have a row.
+__device__ __forceinline__ float row_max(float x) {
+  auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = vmax(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return vmax(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+__device__ __forceinline__ float row_sum(float x) {
+  x = swap_add(x);
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// add_cleaned for one tile and these rows.
+template <int kSets>
+__device__ __forceinline__ void few_cleaned(const Args& a, int t0, int r, int kvh, const int (&p)[kSets],
+                                            int p0, int p1, int lane, f32x4 (&o)[kSets][8]) {
+  const int i = lane & 15, kg = lane >> 4;
+  const int id[2] = {block_id(a, r, t0 / 16), block_id(a, r, t0 / 16 + 1)};
+  if (!hides(a, t0, p0, p1, id[0] >= 0 && id[1] >= 0)) return;
+  const int mine = kg >> 1 ? id[1] : id[0];
+  const uint16_t* v = a.v + ((int64_t)max(mine, 0) * a.NKV + kvh) * kBlockElems + i * 16 + (kg & 1) * 8;
+  v8 seen[kSets];
+#pragma unroll
+  for (int c = 0; c < kSets; ++c)
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      const int t = t0 + 8 * kg + x;
+      const bool hid = t > p[c] || (p[c] - t >= a.window && t >= a.sinks) || mine < 0;
+      const uint32_t one = hid ? 0u : 0x3f80u;
+      seen[c].w[x >> 1] = x & 1 ? seen[c].w[x >> 1] | one << 16 : one;
+    }
+#pragma unroll
+  for (int n = 0; n < 8; ++n) {
+    const v8 x = pdk::ld16(v + 256 * n);
+    v8 mark;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) mark.w[w] = mine < 0 ? 0u : mark_of(x.w[w] & 0xffffu) | mark_of(x.w[w] >> 16) << 16;
+#pragma unroll
+    for (int c = 0; c < kSets; ++c) {
+      const f32x4 found = mfma16(mark, seen[c], f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[c][n][e] += found_value(found[e]);
+    }
+  }
+}
+
+__device__ __forceinline__ void store_four(const Args& a, const Row& r, int dim, float inv, const f32x4& o) {
+  if (r.mine)
+    *reinterpret_cast<uint2*>(a.out + ((int64_t)r.token * a.NH + r.head) * kD + dim) =
+        make_uint2(pdk::pack_bf16x2_rne(o[0] * inv, o[1] * inv), pdk::pack_bf16x2_rne(o[2] * inv, o[3] * inv));
+}
+
+// The four wavefronts' sums of set c added up, dims 32 wave .. by each wavefront.
+template <int kSlots, int kSets, class F>
+__device__ __forceinline__ void few_out(const Args& a, const f32x4 (&so)[kWaves][kSlots][64],
+                                        const float2 (&sml)[kWaves][kSets][64], int c, int wave,
+                                        int lane, F use) {
+  float m = -INFINITY, l = 0.f;
+  f32x4 o[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+  for (int u = 0; u < kWaves; ++u) m = vmax(m, sml[u][c][lane].x);
+#pragma unroll
+  for (int u = 0; u < kWaves; ++u) {
+    const float2 ml = sml[u][c][lane];
+    const float f = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ml.x - m) * a.c);
+    l += ml.y * f;
+#pragma unroll
+    for (int n = 0; n < 2; ++n) o[n] += so[u][8 * c + 2 * wave + n][lane] * f;
+  }
+  use(m, l, o);
+}
+
+template <int kSets>
+__device__ __forceinline__ void few_unit(const Args& a, FewShared<kSets>& sm, int r, int kvh, int z) {
+  const int lane = threadIdx.x & 63, i = lane & 15, kg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int G = a.NH / a.NKV;
   const Request q = request(a, r);
-  if (q.n == 0 || q.n > 32 || q.n * G > a.few_rows) return;
+  if (q.n == 0 || q.n > a.few_rows || q.n * G > a.few_rows) return;
   const int p0 = q.past, p1 = q.past + q.n - 1;
   const Walk w = walk(a, p0, p1);
   const int splits = splits_of(w.n, a.few_per, a.few_splits);
   if (z >= splits) return;
   const int first = z * a.few_per, end = z + 1 == splits ? w.n : first + a.few_per;
-  const Row row = row_at(a, q, kvh, j);
-  Sums sum;
-  sum.clear();
+  int p[kSets];
+  FewSums<kSets> sum;
+#pragma unroll
+  for (int c = 0; c < kSets; ++c) {
+    sum.m[c] = -INFINITY;
+    sum.l[c] = 0.f;
+#pragma unroll
+    for (int n = 0; n < 8; ++n) sum.o[c][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
   const int n_own = (end - first - wave + kWaves - 1) / kWaves;
   bool odd = false;
   if (n_own > 0) {
-    v8 qv[8], kr[8], va[2][4];
-    load_q(a, row, hh, qv);
-    auto tile_of = [&](int i) { return w.tile(first + wave + kWaves * min(i, n_own - 1)); };
-    BlockIds ids[2];                      // of both blocks
-    auto next_ids = [&](int i) __attribute__((always_inline)) {
+    auto tile_of = [&](int x) { return w.tile(first + wave + kWaves * min(x, n_own - 1)); };
+    BlockIds ids[2]{};                    // of both blocks
+    uint64_t ok_was[2] = {0, 0};          // of the 64 tiles before
+    auto next_ids = [&](int x) __attribute__((always_inline)) {
+      ok_was[0] = ids[0].ok[0];
+      ok_was[1] = ids[0].ok[1];
 #pragma unroll
-      for (int b = 0; b < 2; ++b) ids[b] = load_ids(a, r, tile_of(i + lane), b);
+      for (int b = 0; b < 2; ++b) ids[b] = load_ids(a, r, tile_of(x + lane), b);
     };
     next_ids(0);
-    // Where a lane's operands lie in a tile (elements): K's token pi(j) at dims 16 x + 8 hh
-    // is 256 x bytes on; V's dims 32 n + j, tokens 8 hh .. of block ks.
-    const int k_at = ((j >> 3) & 1) * 1024 + hh * 64 + (j & 7) * 8;
-    const int v_at = j * 16 + hh * 8;
-    auto block = [&](int i, int b) {
-      const int id = __builtin_amdgcn_readlane(ids[b].id, i & 63);
+    int ids_from = 0;
+    auto ok_of = [&](int x, int b) { return (x < ids_from ? ok_was[b] : ids[0].ok[b]) >> (x & 63) & 1; };
+    struct Tile {
+      v8 k[2][4], v[8];
+    };
+    v8 qv[kSets][4];
+#pragma unroll
+    for (int c = 0; c < kSets; ++c) {
+      const Row row = row_at(a, q, kvh, 16 * c + i);
+      const uint16_t* from = a.q + (int64_t)row.token * a.q_ld + row.head * kD + 8 * kg;
+      p[c] = row.p;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) qv[c][x] = pdk::ld16(from + 32 * x);
+    }
+    // Where a lane's operands lie in a tile (elements): K's tokens of tile u at dims 32 x + 8 kg
+    // are 1024 u + 256 x on, in the block of token 8 (i / 4); V's dims 16 n + i 256 n on, in
+    // the block of token 8 kg.
+    const int k_at = kg * 64 + (i & 7) * 8, v_at = i * 16 + (kg & 1) * 8;
+    auto block = [&](int x, int b) {
+      const int id = __builtin_amdgcn_readlane(ids[b].id, x & 63);
       return ((int64_t)id * a.NKV + kvh) * kBlockElems;
     };
-    auto load_k = [&](int i) __attribute__((always_inline)) {
-      const int64_t b0 = block(i, 0), b1 = block(i, 1);
-      const uint16_t* p = a.k + (j & 16 ? b1 : b0) + k_at;
+    // Tile x's loads, or past the last as many of one 16-byte piece each: no load is under a
+    // branch that would make the compiler wait for all of them.
+    auto load = [&](Tile& t, int x) __attribute__((always_inline)) {
+      const int64_t b0 = block(x, 0), b1 = block(x, 1);
+      const bool dead = x >= n_own;
+      const uint16_t* k = a.k + (dead ? 0 : (i & 8 ? b1 : b0) + k_at);
+      const uint16_t* v = a.v + (dead ? 0 : (kg & 2 ? b1 : b0) + v_at);
 #pragma unroll
-      for (int x = 0; x < 8; ++x) kr[x] = pdk::ld16(p + 128 * x);
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int d = 0; d < 4; ++d) t.k[u][d] = pdk::ld16(k + 1024 * u + 256 * d);
+#pragma unroll
+      for (int n = 0; n < 8; ++n) t.v[n] = pdk::ld16_stream(v + 256 * n);
     };
-    auto load_v = [&](int i) __attribute__((always_inline)) {
+    auto use = [&](Tile& t, int x) __attribute__((always_inline)) {
+      const bool ok0 = ok_of(x, 0), ok1 = ok_of(x, 1);
+      const int t0 = tile_of(x) * kTile;
+      f32x4 s[kSets][2];
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const uint16_t* p = a.v + block(i, b) + v_at;
+      for (int c = 0; c < kSets; ++c)
 #pragma unroll
-        for (int n = 0; n < 4; ++n) va[b][n] = pdk::ld16(p + 512 * n);
-      }
-    };
-    load_k(0);
-    load_v(0);
-    auto step = [&](int i, bool more) __attribute__((always_inline)) {
-      const bool ok0 = ids[0].ok[0] >> (i & 63) & 1, ok1 = ids[0].ok[1] >> (i & 63) & 1;
-      const int t0 = tile_of(i) * kTile;
-      if (more && (i & 63) == 63) next_ids(i + 1);
-      f32x16 s = scores(kr, qv);
-      if (more) load_k(i + 1);
-      const Place at = place(a, t0, row.p, hh, ok0, ok1);
+        for (int u = 0; u < 2; ++u) {
+          s[c][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int d = 0; d < 4; ++d) s[c][u] = mfma16(t.k[u][d], qv[c][d], s[c][u]);
+        }
       const bool edge = hides(a, t0, p0, p1, ok0 && ok1);
       if (edge) {
+        const bool ok = kg & 2 ? ok1 : ok0;
 #pragma unroll
-        for (int x = 0; x < 16; ++x) s[x] = at.hidden(x) ? -INFINITY : s[x];
+        for (int c = 0; c < kSets; ++c) {
+          const int ago = p[c] - t0 - 8 * kg, sink = a.sinks - t0 - 8 * kg;
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int at = 4 * u + e;
+              const bool hid = (at > ago) | ((ago - at >= a.window) & (at >= sink)) | !ok;
+              s[c][u][e] = hid ? -INFINITY : s[c][u][e];
+            }
+        }
       }
-      v8 p[2];
-      weigh(s, a.c, sum, p);
+      v8 wt[kSets];
+#pragma unroll
+      for (int c = 0; c < kSets; ++c) {
+        float mx = s[c][0][0];
+#pragma unroll
+        for (int e = 1; e < 8; ++e) mx = vmax(mx, s[c][e >> 2][e & 3]);
+        mx = row_max(mx);
+        // The maximum in use follows only when it falls more than 2^8 behind, as in weigh.
+        if (__any((mx - sum.m[c]) * a.c > 8.f)) {
+          const float m_new = vmax(sum.m[c], mx);
+          const float f = sum.m[c] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((sum.m[c] - m_new) * a.c);
+          sum.m[c] = m_new;
+          sum.l[c] *= f;
+#pragma unroll
+          for (int n = 0; n < 8; ++n) sum.o[c][n] *= f;
+        }
+        const float mc = sum.m[c] == -INFINITY ? 0.f : sum.m[c] * a.c;
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          const float u = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c][e >> 2][e & 3], a.c, -mc));
+          const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c][e >> 2][(e & 3) + 1], a.c, -mc));
+          sum.l[c] += u + v;
+          wt[c].w[e >> 1] = pdk::pack_bf16x2_rne(u, v);
+        }
+      }
       if (edge) {
         bool found = false;
 #pragma unroll
-        for (int x = 0; x < 8; ++x) found |= clean(va[x >> 2][x & 3]);
+        for (int n = 0; n < 8; ++n) found |= clean(t.v[n]);
         odd |= __any(found);
       }
 #pragma unroll
-      for (int x = 0; x < 8; ++x) sum.o[x & 3] = mfma32(va[x >> 2][x & 3], p[x >> 2], sum.o[x & 3]);
-      if (more) load_v(i + 1);
+      for (int c = 0; c < kSets; ++c)
+#pragma unroll
+        for (int n = 0; n < 8; ++n) sum.o[c][n] = mfma16(t.v[n], wt[c], sum.o[c][n]);
     };
+    // Two tiles in registers: while one is used the other is under way.
+    Tile ta, tb;
+    load(ta, 0);
+    load(tb, 1);
+    int x = 0;
 #pragma unroll 1
-    for (int i = 0; i + 1 < n_own; ++i) step(i, true);
-    step(n_own - 1, false);
+    for (; x + 2 < n_own; x += 2) {
+      if ((x & 63) == 62) next_ids(ids_from = x + 2);
+      use(ta, x);
+      load(ta, x + 2);
+      use(tb, x + 1);
+      load(tb, x + 3);
+    }
+    use(ta, x);
+    if (x + 1 < n_own) use(tb, x + 1);
   }
   // The wavefront's own tiles alone are its sums', any of which may be added to.
   if (__builtin_expect(odd, 0))
-    for (int i = first + wave; i < end; i += kWaves)
-      add_cleaned(a, w, i, i + 1, r, kvh, row.p, p0, p1, lane, sum.o);
+    for (int x = first + wave; x < end; x += kWaves)
+      few_cleaned<kSets>(a, w.tile(x) * kTile, r, kvh, p, p0, p1, lane, sum.o);
   // Wavefront n adds up dims 32 n .. of the four.
 #pragma unroll
-  for (int n = 0; n < 4; ++n)
+  for (int c = 0; c < kSets; ++c) {
 #pragma unroll
-    for (int x = 0; x < 16; x += 4)
-      sm.o[wave][4 * n + x / 4][lane] = make_float4(sum.o[n][x], sum.o[n][x + 1], sum.o[n][x + 2],
-                                                    sum.o[n][x + 3]);
-  sm.ml[wave][lane] = make_float2(sum.m, swap_add(sum.l));
+    for (int n = 0; n < 8; ++n) sm.o[wave][8 * c + n][lane] = sum.o[c][n];
+    sm.ml[wave][c][lane] = make_float2(sum.m[c], row_sum(sum.l[c]));
+  }
   __syncthreads();
-  float m = -INFINITY, l = 0.f, o[16];
 #pragma unroll
-  for (int u = 0; u < kWaves; ++u) m = vmax(m, sm.ml[u][lane].x);
+  for (int c = 0; c < kSets; ++c) {
+    const Row row = row_at(a, q, kvh, 16 * c + i);
+    few_out(a, sm.o, sm.ml, c, wave, lane, [&](float m, float l, const f32x4 (&o)[2]) {
+      if (splits == 1) {
+        const float inv = inverse(l);
 #pragma unroll
-  for (int x = 0; x < 16; ++x) o[x] = 0.f;
+        for (int n = 0; n < 2; ++n) store_four(a, row, 16 * (2 * wave + n) + 4 * kg, inv, o[n]);
+      } else if (row.mine) {              // few rows: little to store and to join
+        float* rec = a.ws + (((int64_t)r * a.NKV + kvh) * a.few_splits + z) * kFewRecord<kSets>;
 #pragma unroll
-  for (int u = 0; u < kWaves; ++u) {
-    const float2 ml = sm.ml[u][lane];
-    const float f = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ml.x - m) * a.c);
-    l += ml.y * f;
-#pragma unroll
-    for (int x = 0; x < 16; x += 4) {
-      const float4 y = sm.o[u][4 * wave + x / 4][lane];
-      o[x] += y.x * f;
-      o[x + 1] += y.y * f;
-      o[x + 2] += y.z * f;
-      o[x + 3] += y.w * f;
-    }
+        for (int n = 0; n < 2; ++n) reinterpret_cast<f32x4*>(rec)[(8 * c + 2 * wave + n) * 64 + lane] = o[n];
+        if (wave == 0) reinterpret_cast<float2*>(rec + kSets * 2048)[c * 64 + lane] = make_float2(m, l);
+      }
+    });
   }
-  if (splits == 1) {
-    store_dims(a, row, wave, hh, inverse(l), o);
-    return;
+}
+
+// A split request's sums: wavefront w adds up splits w, w + 4, ..., four of them in one
+// round of loads, then the four's are added in LDS.
+template <int kSets>
+__device__ __forceinline__ void few_join(const Args& a, FewShared<1>& sm, int r, int kvh) {
+  const int lane = threadIdx.x & 63, i = lane & 15, kg = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int G = a.NH / a.NKV;
+  const Request q = request(a, r);
+  if (q.n == 0 || q.n > a.few_rows || q.n * G > a.few_rows) return;
+  const int splits = splits_of(walk(a, q.past, q.past + q.n - 1).n, a.few_per, a.few_splits);
+  if (splits == 1) return;
+  const float* rec = a.ws + ((int64_t)r * a.NKV + kvh) * a.few_splits * kFewRecord<kSets>;
+#pragma unroll
+  for (int c = 0; c < kSets; ++c) {
+    const Row row = row_at(a, q, kvh, 16 * c + i);
+    float m = -INFINITY, l = 0.f;
+    f32x4 o[8];
+#pragma unroll
+    for (int n = 0; n < 8; ++n) o[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (row.mine)
+      for (int z0 = wave; z0 < splits; z0 += 16) {
+        float2 ml[4];
+        f32x4 y[4][8];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float* at = rec + (int64_t)min(z0 + 4 * k, splits - 1) * kFewRecord<kSets>;
+          ml[k] = reinterpret_cast<const float2*>(at + kSets * 2048)[c * 64 + lane];
+          if (z0 + 4 * k >= splits) ml[k] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+          for (int n = 0; n < 8; ++n) y[k][n] = reinterpret_cast<const f32x4*>(at)[(8 * c + n) * 64 + lane];
+        }
+        const float m_new = vmax(m, vmax(vmax(ml[0].x, ml[1].x), vmax(ml[2].x, ml[3].x)));
+        const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - m_new) * a.c);
+        m = m_new;
+        l *= f;
+#pragma unroll
+        for (int n = 0; n < 8; ++n) o[n] *= f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (z0 + 4 * k >= splits) break;
+          const float g = ml[k].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ml[k].x - m) * a.c);
+          l += ml[k].y * g;
+#pragma unroll
+          for (int n = 0; n < 8; ++n) o[n] += y[k][n] * g;
+        }
+      }
+    if (c) __syncthreads();
+#pragma unroll
+    for (int n = 0; n < 8; ++n) sm.o[wave][n][lane] = o[n];
+    sm.ml[wave][0][lane] = make_float2(m, l);
+    __syncthreads();
+    few_out(a, sm.o, sm.ml, 0, wave, lane, [&](float, float l, const f32x4 (&o)[2]) {
+      const float inv = inverse(l);
+#pragma unroll
+      for (int n = 0; n < 2; ++n) store_four(a, row, 16 * (2 * wave + n) + 4 * kg, inv, o[n]);
+    });
   }
-  float* rec = record(a, (int64_t)r * a.NKV + kvh, a.few_splits, z);
-  keep_dims(rec, wave, lane, o);
-  if (wave == 0) keep_sums(rec, lane, m, l);
 }
 
 // ---- longer requests ----------------------------------------------------------
-// The request of the tile-th 128 rows of longer requests, and which of its own it is
-// (the last ones first: they walk the most). False past the last.
-__device__ __forceinline__ bool find_rows(const Args& a, int tile, int& r, int& row0) {
-  const int lane = threadIdx.x & 63, G = a.NH / a.NKV;
+// How many workgroups' rows (128 each) 64 requests from `base` on have, up to lane's.
+__device__ __forceinline__ int rows_up_to(const Args& a, int base, int lane) {
+  const int G = a.NH / a.NKV;
+  int n = 0;
+  if (base + lane < a.R) {
+    const Request q = request(a, base + lane);
+    if (q.n * G > a.few_rows) n = (q.n * G + kRows - 1) / kRows;
+  }
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int x = __shfl_up(n, o);
+    if (lane >= o) n += x;
+  }
+  return n;
+}
+
+// A longer request's workgroup: 128 rows from row0 on of request r, split z of them.
+// Whole rounds of big_slots workgroups walk their contexts whole; the workgroups' rows
+// that are left over, fewer than would fill the card, are split.
+struct Big {
+  int r, row0;
+  int left;                               // number among those left over, or -1
+  int z;
+};
+
+// Of the rest-th workgroup of a KV head, or (kLeft) the first split of the rest-th of its
+// rows that are left over; false past the last.
+template <bool kLeft>
+__device__ __forceinline__ bool find_big(const Args& a, int rest, Big& w) {
+  const int lane = threadIdx.x & 63;
+  int all = 0, to = 0;
+  for (int base = 0; base < a.R; base += 64) {
+    to = rows_up_to(a, base, lane);
+    all += __shfl(to, 63);
+  }
+  all = __builtin_amdgcn_readfirstlane(all);
+  const int whole = (int)((int64_t)all * a.NKV / a.big_slots * a.big_slots / a.NKV), left = all - whole;
+  if (kLeft) {
+    if (rest >= left) return false;
+    rest += whole;
+  }
+  int tile = rest;
+  w.left = -1;
+  w.z = 0;
+  if (rest >= whole) {
+    if (left == 0) return false;
+    w.z = (rest - whole) / left;
+    w.left = rest - whole - w.z * left;
+    tile = whole + w.left;
+    if (w.z >= a.big_splits) return false;
+  }
   int before = 0;
   for (int base = 0; base < a.R; base += 64) {
-    int mine = 0;
-    if (base + lane < a.R) {
-      const Request q = request(a, base + lane);
-      if (q.n * G > a.few_rows) mine = (q.n * G + kRows - 1) / kRows;
-    }
-    int to = mine;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int x = __shfl_up(to, o);
-      if (lane >= o) to += x;
-    }
+    if (a.R > 64) to = rows_up_to(a, base, lane);
     const uint64_t hit = __ballot(before + to > tile);
     if (hit) {
       const int l = __builtin_ctzll(hit);
-      r = __builtin_amdgcn_readfirstlane(base + l);
-      row0 = __builtin_amdgcn_readfirstlane((before + __shfl(to, l) - 1 - tile) * kRows);
+      w.r = __builtin_amdgcn_readfirstlane(base + l);
+      // The last rows first: they walk the most.
+      w.row0 = __builtin_amdgcn_readfirstlane((before + __shfl(to, l) - 1 - tile) * kRows);
       return true;
     }
     before += __shfl(to, 63);
@@ -508,18 +761,25 @@ __device__ __forceinline__ bool find_rows(const Args& a, int tile, int& r, int& 
   return false;
 }
 
-__device__ __forceinline__ void big_unit(const Args& a, uint16_t* sm, int tile, int kvh, int z) {
+// The tiles of a split of a walk of n, of a longer request left over.
+__device__ __forceinline__ int big_per(const Args& a, int n) {
+  return max((n + a.big_splits - 1) / a.big_splits, kLeastSplit);
+}
+
+__device__ __forceinline__ void big_unit(const Args& a, uint16_t* sm, int rest, int kvh) {
   const int lane = threadIdx.x & 63, j = lane & 31, hh = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int G = a.NH / a.NKV;
-  int r, row0;
-  if (!find_rows(a, tile, r, row0)) return;
+  Big wg;
+  if (!find_big<false>(a, rest, wg)) return;
+  const int r = wg.r, row0 = wg.row0;
   const Request q = request(a, r);
   const int row1 = min(row0 + kRows, q.n * G) - 1;
   const Walk w = walk(a, q.past + row0 / G, q.past + row1 / G);
-  const int splits = splits_of(w.n, a.big_per, a.big_splits);
-  if (z >= splits) return;
-  const int first = z * a.big_per, n_walk = (z + 1 == splits ? w.n : first + a.big_per) - first;
+  const int per = wg.left < 0 ? w.n : big_per(a, w.n);
+  const int splits = wg.left < 0 ? 1 : splits_of(w.n, per, a.big_splits);
+  if (wg.z >= splits) return;
+  const int first = wg.z * per, n_walk = (wg.z + 1 == splits ? w.n : first + per) - first;
   v8 qv[8];
   int p;                                  // the lane's position
   {
@@ -615,76 +875,104 @@ __device__ __forceinline__ void big_unit(const Args& a, uint16_t* sm, int tile, 
   if (__builtin_expect(odd, 0))
     add_cleaned(a, w, first, first + n_walk, r, kvh, row.p, p0, p1, ln, sum.o);
   const float l = swap_add(sum.l), inv = inverse(l);
-  float* rec = record(a, ((int64_t)tile * a.NKV + kvh) * kWaves + wave, a.big_splits, z) + big_base(a);
+  float* rec = a.ws + a.big_base + ((((int64_t)wg.left * a.NKV + kvh) * kWaves + wave) * a.big_splits + wg.z) * kRecord;
 #pragma unroll
   for (int n = 0; n < 4; ++n) {
     float o[16];
 #pragma unroll
     for (int x = 0; x < 16; ++x) o[x] = sum.o[n][x];
     if (splits == 1) store_dims(a, row, n, ln >> 5, inv, o);
-    else keep_dims(rec, n, ln, o);
+    else keep_dims(rec, n, ln, row.mine, o);
   }
   if (splits > 1) keep_sums(rec, ln, sum.m, l);
 }
 
-__global__ __launch_bounds__(256, 2) void chunk_few_kernel(Args a) {
-  __shared__ FewShared sm;
+template <int kSets>
+__global__ __launch_bounds__(256, kSets == 1 ? 2 : 1) void chunk_few_kernel(Args a) {
+  __shared__ FewShared<kSets> sm;
   const int rest = blockIdx.x / a.NKV;
-  few_unit(a, sm, rest % a.R, blockIdx.x % a.NKV, rest / a.R);
+  few_unit<kSets>(a, sm, rest % a.R, blockIdx.x % a.NKV, rest / a.R);
 }
 
 __global__ __launch_bounds__(256, 3) void chunk_big_kernel(Args a) {
   __shared__ __align__(1024) uint16_t sm[2 * kRing * kTileElems];
-  const int rest = blockIdx.x / a.NKV;
-  big_unit(a, sm, rest % a.big_tiles, blockIdx.x % a.NKV, rest / a.big_tiles);
+  big_unit(a, sm, blockIdx.x / a.NKV, blockIdx.x % a.NKV);
+}
+
+// Requests of both kinds: eight workgroups of the one kind and eight of the other in turn
+// as long as both last, so that the ones that wait for memory and the ones that
+// multiply share the CUs.
+__global__ __launch_bounds__(256, 2) void chunk_both_kernel(Args a, int few, int big) {
+  constexpr int kTiles = 2 * kRing * kTileElems * sizeof(uint16_t);
+  __shared__ __align__(1024) char sm[std::max(kTiles, (int)sizeof(FewShared<1>))];
+  const int g = blockIdx.x >> 3, turns = min((few + 7) >> 3, (big + 7) >> 3);
+  const bool is_big = g < 2 * turns ? (g & 1) == 0 : big > few;
+  const int u = (g < 2 * turns ? g >> 1 : g - turns) * 8 + (blockIdx.x & 7);
+  if (u >= (is_big ? big : few)) return;
+  const int rest = u / a.NKV, kvh = u - rest * a.NKV;
+  if (is_big) big_unit(a, reinterpret_cast<uint16_t*>(sm), rest, kvh);
+  else few_unit<1>(a, *reinterpret_cast<FewShared<1>*>(sm), rest % a.R, kvh, rest / a.R);
 }
 
 // One workgroup per unit whose context was split: wavefront n adds up dims 32 n .. of
 // the splits, in order.
+template <int kSets>
 __global__ __launch_bounds__(256) void chunk_join_kernel(Args a, int few_units) {
+  if ((int)blockIdx.x < few_units) {
+    __shared__ FewShared<1> sm;
+    const int r = blockIdx.x / a.NKV;
+    few_join<kSets>(a, sm, r, blockIdx.x - r * a.NKV);
+    return;
+  }
   const int lane = threadIdx.x & 63, j = lane & 31, hh = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int G = a.NH / a.NKV;
-  int r, row0 = 0, kvh, splits;
-  const float* rec;
-  Request q;
-  if ((int)blockIdx.x < few_units) {
-    r = blockIdx.x / a.NKV;
-    kvh = blockIdx.x - r * a.NKV;
-    q = request(a, r);
-    if (q.n == 0 || q.n > 32 || q.n * G > a.few_rows) return;
-    splits = splits_of(walk(a, q.past, q.past + q.n - 1).n, a.few_per, a.few_splits);
-    rec = record(a, blockIdx.x, a.few_splits, 0);
-  } else {
-    const int unit = blockIdx.x - few_units, rest = unit / kWaves;
-    kvh = rest % a.NKV;
-    if (!find_rows(a, rest / a.NKV, r, row0)) return;
-    q = request(a, r);
-    const int row1 = min(row0 + kRows, q.n * G) - 1;
-    splits = splits_of(walk(a, q.past + row0 / G, q.past + row1 / G).n, a.big_per, a.big_splits);
-    rec = record(a, unit, a.big_splits, 0) + big_base(a);
-    row0 += 32 * (unit - rest * kWaves);
-    if (row0 > row1) return;
-  }
+  const int unit = blockIdx.x - few_units, at = unit / kWaves, left = at / a.NKV, kvh = at - left * a.NKV;
+  Big wg;
+  if (!find_big<true>(a, left, wg)) return;
+  const Request q = request(a, wg.r);
+  const int row1 = min(wg.row0 + kRows, q.n * G) - 1, row0 = wg.row0 + 32 * (unit - at * kWaves);
+  const Walk w = walk(a, q.past + wg.row0 / G, q.past + row1 / G);
+  const int splits = splits_of(w.n, big_per(a, w.n), a.big_splits);
+  const float* rec = a.ws + a.big_base + (int64_t)unit * a.big_splits * kRecord;
+  if (row0 > row1) return;
   if (splits == 1) return;
   const Row row = row_at(a, q, kvh, row0 + j);
+  if (!row.mine) return;                  // both lanes of a row alike
   auto sums = [&](int z) { return reinterpret_cast<const float2*>(rec + (int64_t)z * kRecord + 64 * 64)[lane]; };
+  // Four splits' loads at a time; the last one again past the end, with the factor 0.
   float m = -INFINITY, l = 0.f, o[16];
-  for (int z = 0; z < splits; ++z) m = vmax(m, sums(z).x);
+  for (int z = 0; z < splits; z += 4) {
+    float x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = sums(min(z + i, splits - 1)).x;
+    m = vmax(m, vmax(vmax(x[0], x[1]), vmax(x[2], x[3])));
+  }
 #pragma unroll
   for (int x = 0; x < 16; ++x) o[x] = 0.f;
-  for (int z = 0; z < splits; ++z) {
-    const float2 ml = sums(z);
-    const float f = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ml.x - m) * a.c);
-    l += ml.y * f;
-    const float4* p = reinterpret_cast<const float4*>(rec + (int64_t)z * kRecord) + 4 * wave * 64 + lane;
+  for (int z = 0; z < splits; z += 4) {
+    float2 ml[4];
+    float4 y[4][4];
 #pragma unroll
-    for (int x = 0; x < 16; x += 4) {
-      const float4 y = p[x / 4 * 64];
-      o[x] += y.x * f;
-      o[x + 1] += y.y * f;
-      o[x + 2] += y.z * f;
-      o[x + 3] += y.w * f;
+    for (int i = 0; i < 4; ++i) {
+      const int at = min(z + i, splits - 1);
+      ml[i] = sums(at);
+      const float4* p = reinterpret_cast<const float4*>(rec + (int64_t)at * kRecord) + 4 * wave * 64 + lane;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) y[i][x] = p[x * 64];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (z + i >= splits) break;
+      const float f = ml[i].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ml[i].x - m) * a.c);
+      l += ml[i].y * f;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        o[4 * x] += y[i][x].x * f;
+        o[4 * x + 1] += y[i][x].y * f;
+        o[4 * x + 2] += y[i][x].z * f;
+        o[4 * x + 3] += y[i][x].w * f;
+      }
     }
   }
   store_dims(a, row, wave, hh, inverse(l), o);
@@ -692,37 +980,64 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(Args a, int few_units) 
 
 // How a call is split up.
 struct Plan {
-  bool few, big;
-  int few_per, few_splits, big_per, big_splits, big_tiles;
+  bool big;
+  int few_rows;                           // 0 where no request is taken as one of few rows
+  int few_per, few_splits, big_slots, big_splits;
+  int64_t few_blocks, big_blocks;         // workgroups
+  int64_t few_units, big_units;           // units that may be split
+  int64_t few_floats;                     // of the former's records
   int64_t bytes;
 };
+
+// How long n equal workgroups per CU take, three at once, in the time that one of three
+// takes: one alone has 0.78 of the three's rate (4096 tokens after 28000: 588 us of 256
+// beside 1374 of 768), two 0.93.
+double rounds(int64_t n) {
+  return (double)(n / 3 * 3) + (n % 3 == 0 ? 0. : n % 3 == 1 ? 1 / 0.78 : 2 / 0.93);
+}
 
 Plan plan_for(int N, int R, int max_new, int64_t max_ctx, int NH, int NKV, int window, int sinks) {
   Plan p{};
   const int G = NH / NKV;
-  p.few = max_new >= 1;
   p.big = (int64_t)max_new * G > 32;
-  if (p.big && R == 1) p.few = false;
+  p.few_rows = p.big ? (R == 1 ? 0 : 16) : max_new * G > 16 ? 32 : 16;
   auto tiles = [&](int64_t span) {        // walked at most by rows over `span` positions
     const int64_t all = (max_ctx + kTile - 1) / kTile;
     return (int)std::max<int64_t>(
         1, std::min<int64_t>(all, (window + span + kTile - 2) / kTile + 1 + (sinks + kTile - 1) / kTile));
   };
-  auto split = [](int n, int64_t groups, int64_t wanted, int least, int& per, int& splits) {
-    const int64_t want = std::min<int64_t>(kMaxSplits, std::max<int64_t>(1, wanted / std::max<int64_t>(groups, 1)));
-    per = std::max<int>(least, (int)((n + want - 1) / want));
-    splits = std::max(1, (n + per - 1) / per);
-  };
-  split(tiles(32 / G), (int64_t)R * NKV, 1024, 8, p.few_per, p.few_splits);
-  const int64_t rows = (int64_t)N * G;
-  p.big_tiles = (int)(rows / kRows + std::min<int64_t>(R, rows / 33 + 1));
-  split(tiles(kRows / G + 1), (int64_t)std::max<int64_t>(1, rows / kRows) * NKV, 768, 8, p.big_per,
-        p.big_splits);
-  if (!p.few) p.few_splits = 1;
-  if (!p.big) p.big_splits = 1;
-  const int64_t units = (p.few_splits > 1 ? (int64_t)R * NKV * p.few_splits : 0) +
-                        (p.big_splits > 1 ? (int64_t)p.big_tiles * NKV * kWaves * p.big_splits : 0);
-  p.bytes = units * kRecord * 4;
+  p.few_splits = p.big_splits = 1;
+  p.few_per = 1 << 30;
+  p.big_slots = 3 * kCUs;
+  if (p.few_rows) {
+    const int n = tiles(p.few_rows / G);
+    const int64_t groups = (int64_t)R * NKV;
+    const int64_t want = std::min<int64_t>(kMaxSplits, std::max<int64_t>(1, (p.few_rows == 32 ? 256 : 512) / groups));
+    p.few_per = std::max<int>(kLeastSplit, (int)((n + want - 1) / want));
+    p.few_splits = (n + p.few_per - 1) / p.few_per;
+    p.few_blocks = groups * p.few_splits;
+    if (p.few_splits > 1) p.few_units = groups;
+  }
+  if (p.big) {
+    const int64_t rows = (int64_t)N * G, n = tiles(kRows / G + 1);
+    const int64_t most = rows / kRows + std::min<int64_t>(R, rows / (p.few_rows + 1) + 1);
+    // The split that ends soonest of the workgroups left over; each costs as much again as
+    // ten tiles for its start, for handing over its sums (136 KB) and for the join.
+    const int64_t left = std::max<int64_t>(1, (rows + kRows - 1) / kRows * NKV % p.big_slots);
+    double best = 1e30;
+    for (int s = 1; s <= kMaxSplits && (s == 1 || n / s >= kLeastSplit); ++s) {
+      const double t = rounds((left * s + kCUs - 1) / kCUs) * ((double)n / s + (s > 1 ? 10 : 0));
+      if (t < best) {
+        best = t;
+        p.big_splits = s;
+      }
+    }
+    const int64_t over = std::min<int64_t>(most, p.big_slots / NKV + 1);     // left over at most
+    p.big_blocks = (most + (p.big_splits - 1) * over) * NKV;
+    if (p.big_splits > 1) p.big_units = over * NKV * kWaves;
+  }
+  p.few_floats = p.few_units * p.few_splits * (p.few_rows == 32 ? kFewRecord<2> : kFewRecord<1>);
+  p.bytes = (p.few_floats + p.big_units * p.big_splits * kRecord) * 4;
   return p;
 }
 
@@ -790,28 +1105,29 @@ extern "C" int pdk_chunk_attn(const uint16_t* q, int64_t q_tok_stride, const uin
     pdk::set_error("workspace of %zu bytes, %lld needed", workspace_bytes, (long long)p.bytes);
     return PDK_ENOMEM;
   }
-  const int64_t few_blocks = (int64_t)R * n_kv_heads * p.few_splits;
-  const int64_t big_blocks = (int64_t)p.big_tiles * n_kv_heads * p.big_splits;
-  const int64_t big_units = p.big && p.big_splits > 1 ? (int64_t)p.big_tiles * n_kv_heads * kWaves : 0;
-  const int64_t few_units = p.few && p.few_splits > 1 ? (int64_t)R * n_kv_heads : 0;
-  PDK_REQUIRE(few_blocks < (1ll << 31) && big_blocks < (1ll << 31) && big_units + few_units < (1ll << 31),
+  PDK_REQUIRE(p.few_blocks < (1ll << 30) && p.big_blocks < (1ll << 30) &&
+                  p.big_units + p.few_units < (1ll << 31),
               "launch too large");
   const Args a{q, q_tok_stride, cache_k, cache_v, num_blocks, block_tables, max_blocks, starts,
                ctx_lens, N, R, n_q_heads, n_kv_heads, scale * 1.4426950408889634f, window, sinks,
-               static_cast<float*>(workspace), out, p.few ? 32 : 0, p.few_per, p.few_splits, p.big_per,
-               p.big_splits, p.big_tiles};
+               static_cast<float*>(workspace), out, p.few_rows, p.few_per, p.few_splits, p.big_slots,
+               p.big_splits, p.few_floats};
   const hipStream_t st = pdk::as_stream(stream);
-  if (p.big) {
-    hipLaunchKernelGGL(chunk_big_kernel, dim3((unsigned)big_blocks), dim3(256), 0, st, a);
-    if (int rc = pdk::check_launch("chunk_big_kernel")) return rc;
+  const bool two = p.few_rows == 32;
+  if (p.big && p.few_rows) {
+    const unsigned turns = (unsigned)((p.few_blocks + 7) / 8 + (p.big_blocks + 7) / 8);
+    hipLaunchKernelGGL(chunk_both_kernel, dim3(8 * turns), dim3(256), 0, st, a, (int)p.few_blocks,
+                       (int)p.big_blocks);
+  } else if (p.big) {
+    hipLaunchKernelGGL(chunk_big_kernel, dim3((unsigned)p.big_blocks), dim3(256), 0, st, a);
+  } else {
+    hipLaunchKernelGGL(two ? chunk_few_kernel<2> : chunk_few_kernel<1>, dim3((unsigned)p.few_blocks),
+                       dim3(256), 0, st, a);
   }
-  if (p.few) {
-    hipLaunchKernelGGL(chunk_few_kernel, dim3((unsigned)few_blocks), dim3(256), 0, st, a);
-    if (int rc = pdk::check_launch("chunk_few_kernel")) return rc;
-  }
-  if (few_units + big_units) {
-    hipLaunchKernelGGL(chunk_join_kernel, dim3((unsigned)(few_units + big_units)), dim3(256), 0, st, a,
-                       (int)few_units);
+  if (int rc = pdk::check_launch("chunk attention")) return rc;
+  if (p.few_units + p.big_units) {
+    hipLaunchKernelGGL(two ? chunk_join_kernel<2> : chunk_join_kernel<1>,
+                       dim3((unsigned)(p.few_units + p.big_units)), dim3(256), 0, st, a, (int)p.few_units);
     if (int rc = pdk::check_launch("chunk_join_kernel")) return rc;
   }
   return PDK_OK;

@@ -28,10 +28,12 @@ class ChunkMap(NamedTuple):
 
 
 def _int32(t, name, dev, dims=1):
+    if isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.device == dev \
+            and t.dim() == dims and t.is_contiguous():
+        return
     _need(t, name, torch.int32)
     need_device(dev, t, name)
-    if t.dim() != dims or not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous with {dims} dimension{'s' * (dims > 1)}")
+    raise ValueError(f"{name} must be contiguous with {dims} dimension{'s' * (dims > 1)}")
 
 
 def chunk_map(past, new, tables, free, max_tokens, stream=None):
@@ -54,13 +56,12 @@ def chunk_map(past, new, tables, free, max_tokens, stream=None):
         with launch_scope(dev, stream):
             return chunk_map(past, new, tables, free, max_tokens)
     _int32(tables, "tables", dev, 2)
-    for t, name in ((past, "past"), (new, "new"), (free, "free")):
-        _int32(t, name, dev)
+    _int32(past, "past", dev)
+    _int32(new, "new", dev)
+    _int32(free, "free", dev)
     R, W = tables.shape
     if past.numel() != R or new.numel() != R:
         raise ValueError(f"past and new must hold {R} lengths")
-    if any(overlap(tables, t) for t in (past, new, free)):
-        raise ValueError("tables must not overlap past, new or free")
     N = int(max_tokens)
     if not 0 <= N < 1 << 30:
         raise ValueError(f"max_tokens={N} outside [0, 2^30)")
@@ -127,9 +128,6 @@ def rope_cache_write(qkv, inv_freq, positions, slots, cache_k, cache_v, n_q_head
             raise ValueError(f"q_out must be contiguous and 16-byte aligned {(N, n_q_heads, D)}")
         if any(overlap(q_out, t) for t in (qkv, inv_freq, positions, slots, cache_k, cache_v)):
             raise ValueError("q_out must not overlap the other tensors")
-    if any(overlap(c, t) for c in (cache_k, cache_v) for t in (qkv, inv_freq, positions, slots)) \
-            or overlap(cache_k, cache_v):
-        raise ValueError("the caches must not overlap the other tensors")
     if N:
         _lib.call("pdk_rope_cache_write", qkv.data_ptr(), ld, inv_freq.data_ptr(),
                   positions.data_ptr(), slots.data_ptr(), N, n_q_heads, H, D, q_out.data_ptr(),

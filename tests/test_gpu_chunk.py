@@ -264,6 +264,20 @@ def test_long_cache_offsets(cuda):
         ref.within(got, want, bound)
 
 
+@pytest.mark.parametrize("new", [1, 3, 20])
+def test_long_contexts_beside_many_short_ones(cuda, new):
+    """So many requests that none is split: a walk longer than the ids that a wavefront
+    reads at a time."""
+    lens = [(9000 - new, new), (16900, new)] + [(i % 23, 1) for i in range(140)] + [(8190, new)]
+    print(f"long beside short, {new} new", flush=True)
+    rng = np.random.default_rng(new)
+    q, ck, cv, tables, ctx = _operands(rng, 16, 8, lens)
+    tables[1, 510:530:3] = -1                                # missing about where ids are read anew
+    tables[1, 770] = -1
+    want, bound = ref.attention(q, ck, cv, tables, [n for _, n in lens], ctx, 0, 0, SCALE)
+    ref.within(_attend(q, ck, cv, tables, lens), want, bound)
+
+
 def test_side_stream_and_own_workspace(cuda):
     from rngd_pd_amd import kernels as K
     rng = np.random.default_rng(9)
