@@ -107,7 +107,8 @@ SIGNATURES = {
     "pdk_rmsnorm_fp8": (_I, [_P, _P, _P, _I, _I, _F, _P, _P, _P, _I64, _U]),
     "pdk_quantize_fp8": (_I, [_P, _I64, _I, _I, _P, _P, _I64, _U]),
     "pdk_swiglu_fp8": (_I, [_P, _I64, _I, _I, _P, _P, _I64, _U]),
-    "pdk_linear_fp8": (_I, [_P, _I64, _P, _I64, _I64, _P, _P, _I, _I, _I, _P, _U]),
+    "pdk_linear_fp8_workspace_bytes": (_I64, [_I, _I, _I]),
+    "pdk_linear_fp8": (_I, [_P, _I64, _P, _I64, _I64, _P, _P, _I, _I, _I, _P, _SZ, _P, _U]),
     "pdk_cache_append": (_I, [_P, _P, _P, _P, _I, _P, _I, _P, _I, _I, _I, _U]),
     "pdk_greedy_argmax": (_I, [_P, _I, _I, _I64, _P, _U]),
     "pdk_rmsnorm": (_I, [_P, _P, _P, _I, _I, ctypes.c_float, _P, _U]),

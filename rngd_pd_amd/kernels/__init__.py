@@ -10,7 +10,8 @@ from .pages import copy_blocks
 from .beam import beam_select, beam_select_workspace_bytes, beam_reorder
 from .chunk import (ChunkMap, chunk_map, rope_cache_write, chunk_attention,
                     chunk_workspace_bytes)
-from .fp8 import rmsnorm_fp8, quantize_fp8, swiglu_fp8, quantize_weight_fp8, linear_fp8
+from .fp8 import (rmsnorm_fp8, quantize_fp8, swiglu_fp8, quantize_weight_fp8, linear_fp8,
+                  linear_fp8_workspace_bytes)
 from .decode_step import (rmsnorm, rope_cache_append, rope_cache_append_partials, swiglu, linear,
                           linear_swiglu, linear_argmax, linear_splitk, rmsnorm_partials,
                           linear_ssq, linear_swiglu_rms, fold_norm, linear_splitk_final, linear_splitk_rms,
@@ -27,6 +28,7 @@ __all__ = ["pack_kv", "pack_kv_batch", "scatter_paged", "scatter_paged_batch", "
            "beam_select", "beam_select_workspace_bytes", "beam_reorder",
            "ChunkMap", "chunk_map", "rope_cache_write", "chunk_attention", "chunk_workspace_bytes",
            "rmsnorm_fp8", "quantize_fp8", "swiglu_fp8", "quantize_weight_fp8", "linear_fp8",
+           "linear_fp8_workspace_bytes",
            "rmsnorm", "rope_cache_append", "rope_cache_append_partials", "swiglu", "linear", "linear_swiglu", "linear_argmax",
            "linear_splitk", "rmsnorm_partials", "linear_ssq", "linear_swiglu_rms", "fold_norm",
            "linear_splitk_final", "linear_splitk_rms", "linear_argmax_rms", "row_ssq", "embed_ssq",

@@ -7,6 +7,8 @@ smaller): the value stands for itself times its scale. Scales of rows come as [T
 K / 128] with a group's lying together (strides 1 and T). The reference's
 projections are 16-bit (kernels/decode_batch.py:73-91).
 """
+import functools
+
 import torch
 
 from .. import _lib
@@ -154,20 +156,36 @@ def quantize_weight_fp8(w):
     return values, scales
 
 
-def linear_fp8(x, x_scales, w, w_scales, out=None, stream=None):
+@functools.lru_cache(maxsize=4096)
+def linear_fp8_workspace_bytes(T, K, N):
+    """Bytes of linear_fp8's workspace (0: it needs none); raises for sizes it does not
+    take."""
+    for v in (T, K, N):
+        if not 0 <= v < 1 << 31:
+            raise ValueError(f"size {v} outside [0, 2^31)")
+    need = int(_lib.lib().pdk_linear_fp8_workspace_bytes(T, K, N))
+    if need < 0:
+        raise ValueError(_lib.last_error())
+    return need
+
+
+def linear_fp8(x, x_scales, w, w_scales, out=None, workspace=None, stream=None):
     """x . w^T of 8-bit rows and weights -> [T, N] bf16.
 
     x [T, K] e4m3 (unit column stride) with x_scales float32 [T, K / 128] (any positive
     strides), w [N, K] e4m3 contiguous with w_scales float32 [ceil(N / 128), K / 128]
     contiguous, as rmsnorm_fp8, quantize_fp8, swiglu_fp8 and quantize_weight_fp8 give
-    them. Products and sums of a group of 128 columns are 32-bit, scaled and added in
-    32 bits, rounded to bf16 once. K a multiple of 128, N of 8."""
+    them. A group's sums are 32-bit but for the matrix instruction's own cut: of 8
+    columns' products what lies 2^-13 below the largest is lost (some 2e-4 of a result).
+    They are scaled and added in 32 bits and rounded to bf16 once. K a multiple of 128, N of 8. ``workspace``: device
+    memory of linear_fp8_workspace_bytes for one call at a time (default: allocated by
+    the call)."""
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
         raise TypeError("x must be a CUDA tensor")
     dev = x.device
     if stream is not None or dev.index != _current_device():
         with launch_scope(dev, stream):
-            return linear_fp8(x, x_scales, w, w_scales, out)
+            return linear_fp8(x, x_scales, w, w_scales, out, workspace)
     _need(x, "x", FP8)
     _need(w, "w", FP8)
     _need(x_scales, "x_scales", torch.float32)
@@ -188,7 +206,7 @@ def linear_fp8(x, x_scales, w, w_scales, out=None, stream=None):
         raise ValueError(f"w_scales must be contiguous {(-(-N // GROUP), groups)}")
     xs_t = x_scales.stride(0) if T > 1 else 1
     xs_g = x_scales.stride(1) if groups > 1 else 1
-    if xs_t < 1 or xs_g < 1:
+    if xs_t < 1 or xs_g < 1 or xs_t >= 1 << 21:
         x_scales, xs_t, xs_g = x_scales.contiguous(), groups, 1
     ld = x.stride(0) if T > 1 else K
     if x.stride(1) != 1 or ld < K or ld % 16 or ld >= 1 << 24 or x.data_ptr() % 16:
@@ -202,7 +220,19 @@ def linear_fp8(x, x_scales, w, w_scales, out=None, stream=None):
             raise ValueError(f"out must be contiguous and 16-byte aligned {(T, N)}")
         if any(overlap(out, t) for t in (x, x_scales, w, w_scales)):
             raise ValueError("out must not overlap the operands")
+    need = linear_fp8_workspace_bytes(T, K, N)
+    ws_ptr, ws_bytes = None, 0
+    if workspace is not None:
+        need_device(dev, workspace, "workspace")
+        ws_ptr, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        if not workspace.is_contiguous() or ws_bytes < need or ws_ptr % 16:
+            raise ValueError(f"workspace must be contiguous, 16-byte aligned and hold {need} bytes")
+        if any(overlap(workspace, t) for t in (x, x_scales, w, w_scales, out)):
+            raise ValueError("workspace must not overlap the other tensors")
+    elif need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        ws_ptr, ws_bytes = workspace.data_ptr(), need
     if T:
         _lib.call("pdk_linear_fp8", x.data_ptr(), ld, x_scales.data_ptr(), xs_t, xs_g, w.data_ptr(),
-                  w_scales.data_ptr(), T, K, N, out.data_ptr(), stream_handle())
+                  w_scales.data_ptr(), T, K, N, ws_ptr, ws_bytes, out.data_ptr(), stream_handle())
     return out

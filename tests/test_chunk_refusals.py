@@ -27,7 +27,8 @@ ATTN = dict(q=P, ld=4096, ck=P, cv=P, nb=64, tables=P, W=512, starts=P, ctx=P, N
             out=P, stream=0)
 NORM = dict(x=P, add=P, w=P, T=4, H=256, eps=1e-5, sum=P, out=P, scales=P, ld=4, stream=0)
 QUANT = dict(x=P, ld=512, T=4, K=256, out=P, scales=P, sld=4, stream=0)
-LINEAR = dict(x=P, ld=256, xs=P, st=1, sg=4, w=P, ws=P, T=4, K=256, N=64, y=P, stream=0)
+LINEAR = dict(x=P, ld=256, xs=P, st=1, sg=4, w=P, ws=P, T=4, K=256, N=64, work=P, work_bytes=1 << 40,
+              y=P, stream=0)
 
 
 @pytest.mark.parametrize("name,base,kw,code,text", [
@@ -89,6 +90,10 @@ LINEAR = dict(x=P, ld=256, xs=P, st=1, sg=4, w=P, ws=P, T=4, K=256, N=64, y=P, s
     ("pdk_linear_fp8", LINEAR, dict(ld=264), INVAL, "x_ld"),
     ("pdk_linear_fp8", LINEAR, dict(ld=1 << 24), INVAL, "x_ld"),
     ("pdk_linear_fp8", LINEAR, dict(st=0), INVAL, "strides"),
+    ("pdk_linear_fp8", LINEAR, dict(st=1 << 21), INVAL, "strides"),
+    ("pdk_linear_fp8", LINEAR, dict(T=64, K=14336, ld=14336, work=None), INVAL, "workspace"),
+    ("pdk_linear_fp8", LINEAR, dict(T=64, K=14336, ld=14336, work=P + 8), INVAL, "workspace"),
+    ("pdk_linear_fp8", LINEAR, dict(T=64, K=14336, ld=14336, work_bytes=640), NOMEM, "workspace"),
     ("pdk_linear_fp8", LINEAR, dict(ws=None), INVAL, "null"),
     ("pdk_linear_fp8", LINEAR, dict(w=P + 4), INVAL, "aligned"),
 ])
@@ -115,6 +120,18 @@ def test_workspace_bytes():
     for bad in ((1, 0, 1, 64, 32, 8), (1, 1, 1, 0, 32, 8), (16, 16, 1, 1 << 20, 32, 8),
                 (1, 1, 1, 64, 33, 8), (-1, 1, 1, 64, 32, 8),
                 (1, 1, 1, 64, 32, 8, 0, 0)):
+        with pytest.raises(ValueError):
+            size(*bad)
+
+
+def test_linear_workspace_bytes():
+    size = K.linear_fp8_workspace_bytes
+    assert size(16, 14336, 4096) == 0 and size(8192, 4096, 28672) == 0
+    assert size(64, 14336, 4096) > 0
+    for T in (17, 64, 65, 128, 300, 470, 1000, 2000, 8192, 1 << 20):       # no plan takes much
+        for k, n in ((128, 8), (4096, 4096), (14336, 4096), (4096, 28672), (1 << 20, 8)):
+            assert size(T, k, n) <= 1 << 29
+    for bad in ((-1, 128, 8), (4, 100, 8), (4, 128, 12), (4, 128, 0), (1 << 21, 128, 8)):
         with pytest.raises(ValueError):
             size(*bad)
 
