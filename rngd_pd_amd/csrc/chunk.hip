@@ -130,8 +130,25 @@ struct Turn {
   float c, s;
 };
 
-// grid: x = 16 tokens, y = a share of the heads' units. Unit u < rot turns two q or
-// k heads; the others move V of eight heads.
+// A head's dims d .. d + 7 and d + 64 .. d + 71 turned by the angles z[d ..].
+__device__ __forceinline__ void turn_head(const Turn* z, const v8& a, const v8& b, v8& x, v8& y) {
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    float r[2][2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      pdk::rope_pair(pdk::bf16_to_f32(e ? a.w[w] >> 16 : a.w[w] & 0xffffu),
+                     pdk::bf16_to_f32(e ? b.w[w] >> 16 : b.w[w] & 0xffffu), z[2 * w + e].c,
+                     z[2 * w + e].s, r[0][e], r[1][e]);
+    x.w[w] = pdk::pack_bf16x2_rne(r[0][0], r[0][1]);
+    y.w[w] = pdk::pack_bf16x2_rne(r[1][0], r[1][1]);
+  }
+}
+
+// grid: x = 16 tokens, y = a share of their units. First the units of q: 256 of the tokens'
+// (token, head, 8 dims) in order, so that a unit reads and writes whole rows; then those
+// of k: two heads of the 16 tokens, whose 16 bytes at a dim lie together in the cache; then
+// those of v: eight heads.
 __global__ __launch_bounds__(kThreads) void rope_write_kernel(
     const uint16_t* qkv, int64_t ld, const float* inv_freq, const int32_t* positions,
     const int32_t* slots, int N, int NH, int NKV, uint16_t* q_out, uint16_t* cache_k,
@@ -144,24 +161,37 @@ __global__ __launch_bounds__(kThreads) void rope_write_kernel(
     const int s = j >= 0 && j < N ? slots[j] : -1;
     slot_of[tid] = s < n_slots ? s : -1;
   }
-  const int rot = (NH + NKV + 1) / 2, units = rot + (NKV + 7) / 8;
-  // A lane's place in a unit of two turned heads; the first unit's values are under way
-  // while the angles are computed.
-  const int t_of = (tid >> 3) & 15, d_of = (tid & 7) * 8;
-  const uint16_t* const row = qkv + (int64_t)min(j0 + t_of, N - 1) * ld + d_of;
-  auto head_of = [&](int u) { return 2 * u + (tid >> 7); };
+  const int units_q = (kTok * NH * 8 + kThreads - 1) / kThreads, units_k = (NKV + 1) / 2;
+  const int units = units_q + units_k + (NKV + 7) / 8, u0 = blockIdx.y;
+  const int d = (tid & 7) * 8;            // q and k: the lane's dims
+  struct Place {
+    int t, head;                          // token of the 16, head of qkv's
+    bool real;
+  };
+  auto place = [&](int u) {
+    if (u < units_q) {
+      const int i = u * (kThreads / 8) + (tid >> 3), t = i / NH;
+      return Place{min(t, kTok - 1), i - t * NH, t < kTok && j0 + t < N};
+    }
+    const int t = (tid >> 3) & 15, h = 2 * (u - units_q) + (tid >> 7);
+    return Place{t, NH + min(h, NKV - 1), h < NKV && j0 + t < N};
+  };
   v8 a, b;
   auto load = [&](int u) __attribute__((always_inline)) {
-    const uint16_t* from = row + (int64_t)min(head_of(u), NH + NKV - 1) * kD;
+    const Place p = place(u);
+    const uint16_t* from = qkv + (int64_t)min(j0 + p.t, N - 1) * ld + (int64_t)p.head * kD + d;
     a = pdk::ld16(from);
     b = pdk::ld16(from + 64);
   };
-  load(min((int)blockIdx.y, rot - 1));
-  if ((int)blockIdx.y < rot) {
-#pragma unroll
-    for (int x = 0; x < kTok * (kD / 2) / kThreads; ++x) {
-      const int i = tid & 63, t = (tid >> 6) + x * (kThreads / 64);
-      const int pos = max(positions[min(j0 + t, N - 1)], 0);
+  // The first unit's values are under way while the angles are computed: those of its own
+  // tokens where the workgroup has one unit, else of all.
+  if (u0 < units_q + units_k) {
+    load(u0);
+    const bool one = u0 + (int)gridDim.y >= units_q + units_k && u0 < units_q;
+    const int t_lo = one ? u0 * (kThreads / 8) / NH : 0;
+    const int t_hi = one ? min((u0 * (kThreads / 8) + kThreads / 8 - 1) / NH, kTok - 1) : kTok - 1;
+    for (int t = t_lo + (tid >> 6); t <= t_hi; t += kThreads / 64) {
+      const int i = tid & 63, pos = max(positions[min(j0 + t, N - 1)], 0);
       const double turns = (double)pos * ((double)inv_freq[i] * 0.15915494309189535);
       float s, c;
       sincosf((float)((turns - rint(turns)) * 6.283185307179586), &s, &c);
@@ -169,67 +199,68 @@ __global__ __launch_bounds__(kThreads) void rope_write_kernel(
     }
   }
   __syncthreads();
-  for (int u = blockIdx.y; u < units; u += gridDim.y) {
-    if (u < rot) {
-      const int head = head_of(u), t = t_of, d = d_of, j = j0 + t;
-      v8 x, y;
+  int u = u0;
+  for (; u < units_q + units_k; u += gridDim.y) {
+    const Place p = place(u);
+    v8 x, y;
+    turn_head(&turn[p.t][d], a, b, x, y);
+    if (u + (int)gridDim.y < units_q + units_k) load(u + gridDim.y);
+    if (!p.real) continue;
+    if (u < units_q) {
+      uint16_t* to = q_out + ((int64_t)(j0 + p.t) * NH + p.head) * kD + d;
+      pdk::st16(to, x);
+      pdk::st16(to + 64, y);
+    } else {
+      const int s = slot_of[p.t + 7];
+      if (s < 0) continue;
+      uint16_t* to = cache_k + ((int64_t)(s >> 4) * NKV + p.head - NH) * (16 * kD);
+      pdk::st16(to + pdk::k_unit(s & 15, d, kD) * 8, x);
+      pdk::st16(to + pdk::k_unit(s & 15, d + 64, kD) * 8, y);
+    }
+  }
+  if (u >= units) return;
+  // V: which of the 16 tokens lead eight that fill a half of a block (at most two), and
+  // which are in no such eight; the others' lead does them, here or in the tile before.
+  uint64_t leads, lone;
+  {
+    const int t = tid & 15, s = slot_of[t + 7], lead = t + 7 - (s & 7);
+    bool whole = s >= 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) whole &= slot_of[lead + i] == (s & ~7) + i;
+    const bool mine = (tid & 63) < kTok;
+    leads = __ballot(mine && whole && (s & 7) == 0);
+    lone = __ballot(mine && s >= 0 && !whole);
+  }
+  const int n_leads = __popcll(leads);
+  const int lead_at[2] = {__builtin_ctzll(leads | 1ull << kTok), 63 - __builtin_clzll(leads | 1)};
+  for (; u < units; u += gridDim.y) {
+    const int dv = ((tid >> 1) & 15) * 8, h = (u - units_q - units_k) * 8 + (tid >> 5);
+    if (h >= NKV) continue;
+    const uint16_t* const column = qkv + (int64_t)j0 * ld + (int64_t)(NH + NKV + h) * kD + dv;
+    auto target = [&](int s) { return cache_v + (((int64_t)(s >> 4) * NKV + h) * kD + dv) * 16 + (s & 15); };
+    if ((tid & 1) < n_leads) {
+      const int t = lead_at[tid & 1];
+      v8 in[8], out[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) in[i] = pdk::ld16(column + (t + i) * ld);
+      pdk::transpose8x8(in, out);
+      uint16_t* to = target(slot_of[t + 7]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) pdk::st16(to + 16 * i, out[i]);
+    }
+    // The lone tokens in turn, even and odd ones by the two lanes of 8 dims.
+    int k = 0;
+    for (uint64_t left = lone; left; left &= left - 1, ++k) {
+      if ((k ^ tid) & 1) continue;
+      const int t = __builtin_ctzll(left);
+      const v8 x = pdk::ld16(column + t * ld);
+      uint16_t* to = target(slot_of[t + 7]);
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        float r[2][2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const Turn z = turn[t][d + 2 * w + e];
-          pdk::rope_pair(pdk::bf16_to_f32(e ? a.w[w] >> 16 : a.w[w] & 0xffffu),
-                         pdk::bf16_to_f32(e ? b.w[w] >> 16 : b.w[w] & 0xffffu), z.c, z.s, r[0][e],
-                         r[1][e]);
-        }
-        x.w[w] = pdk::pack_bf16x2_rne(r[0][0], r[0][1]);
-        y.w[w] = pdk::pack_bf16x2_rne(r[1][0], r[1][1]);
+        to[32 * w] = (uint16_t)x.w[w];
+        to[32 * w + 16] = (uint16_t)(x.w[w] >> 16);
       }
-      if (u + (int)gridDim.y < rot) load(u + gridDim.y);
-      if (j >= N) continue;
-      if (head < NH) {
-        uint16_t* to = q_out + ((int64_t)j * NH + head) * kD + d;
-        pdk::st16(to, x);
-        pdk::st16(to + 64, y);
-      } else if (head < NH + NKV) {
-        const int s = slot_of[t + 7];
-        if (s < 0) continue;
-        uint16_t* to = cache_k + ((int64_t)(s >> 4) * NKV + head - NH) * (16 * kD);
-        pdk::st16(to + pdk::k_unit(s & 15, d, kD) * 8, x);
-        pdk::st16(to + pdk::k_unit(s & 15, d + 64, kD) * 8, y);
-      }
-      continue;
     }
-    // V: a lane has 8 dims of a head, of its token or of the eight from it on.
-    const int d = (tid & 15) * 8;
-    for (int h = (u - rot) * 8 + (tid >> 7); h < min((u - rot) * 8 + 8, NKV); h += 2)
-      for (int x = 0; x < 2; ++x) {
-        const int t = ((tid >> 4) & 7) + 8 * x, j = j0 + t, s = slot_of[t + 7];
-        if (j >= N || s < 0) continue;
-        // The token of the same half's slot 0, and whether the eight from it on fill it.
-        const int lead = t + 7 - (s & 7);
-        bool whole = true;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) whole &= slot_of[lead + i] == (s & ~7) + i;
-        const uint16_t* from = qkv + (int64_t)j * ld + (int64_t)(NH + NKV + h) * kD + d;
-        uint16_t* to = cache_v + (((int64_t)(s >> 4) * NKV + h) * kD + d) * 16 + (s & 15);
-        if (!whole) {
-          const v8 a = pdk::ld16(from);
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            to[32 * w] = (uint16_t)a.w[w];
-            to[32 * w + 16] = (uint16_t)(a.w[w] >> 16);
-          }
-        } else if ((s & 7) == 0) {
-          v8 in[8], out[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) in[i] = pdk::ld16(from + i * ld);
-          pdk::transpose8x8(in, out);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) pdk::st16(to + 16 * i, out[i]);
-        }
-      }
   }
 }
 
@@ -278,7 +309,8 @@ extern "C" int pdk_rope_cache_write(const uint16_t* qkv, int64_t ld, const float
                   pdk::aligned16(cache_v),
               "tensors must be 16-byte aligned");
   const int tiles = (N + kTok - 1) / kTok;
-  const int units = (n_q_heads + n_kv_heads + 1) / 2 + (n_kv_heads + 7) / 8;
+  const int units = (kTok * n_q_heads * 8 + kThreads - 1) / kThreads + (n_kv_heads + 1) / 2 +
+                    (n_kv_heads + 7) / 8;
   // Heads apart until there are four workgroups for every CU.
   const int shares = std::min(units, std::max(1, (1024 + tiles - 1) / tiles));
   hipLaunchKernelGGL(rope_write_kernel, dim3(tiles, shares), dim3(kThreads), 0,

@@ -68,42 +68,60 @@ def rmsnorm_fp8(x, weight, eps, add=None, sum_out=None, out=None, stream=None):
     if stream is not None or dev.index != _current_device():
         with launch_scope(dev, stream):
             return rmsnorm_fp8(x, weight, eps, add, sum_out, out)
-    _need(x, "x")
-    if x.dim() != 2 or not x.is_contiguous() or x.data_ptr() % 16:
-        raise ValueError(f"x must be contiguous and 16-byte aligned [T, H], got {tuple(x.shape)}")
-    T, H = x.shape
-    if H % GROUP or not GROUP <= H <= 8192:
-        raise ValueError(f"H={H} is no multiple of {GROUP} in [{GROUP}, 8192]")
-    _need(weight, "weight")
-    need_device(dev, weight, "weight")
-    if weight.numel() != H or not weight.is_contiguous() or weight.data_ptr() % 16:
-        raise ValueError(f"weight must hold H={H} contiguous values, 16-byte aligned")
+    for t, name in ((weight, "weight"), (add, "add"), (sum_out, "sum_out")):
+        if t is not None and not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a CUDA tensor")
+    # The usual operands pass one test; what does not is told apart.
+    xp, wp, ap, sp = x.data_ptr(), weight.data_ptr(), None, None
+    fine = x.dtype is BF16 and weight.dtype is BF16 and x.dim() == 2 and x.is_contiguous() \
+        and weight.is_contiguous() and weight.device == dev and not (xp | wp) % 16
+    T, H = x.shape if x.dim() == 2 else (0, 0)
+    fine = fine and weight.numel() == H and H % GROUP == 0 and GROUP <= H <= 8192
     if add is not None:
-        _need(add, "add")
-        need_device(dev, add, "add")
-        if add.shape != x.shape or not add.is_contiguous() or add.data_ptr() % 16:
-            raise ValueError("add must be contiguous, 16-byte aligned and shaped like x")
         if sum_out is None:
             sum_out = x
-        elif sum_out.data_ptr() != x.data_ptr():
-            if overlap(sum_out, x):
-                raise ValueError("sum_out must be x itself or not overlap it")
-        _need(sum_out, "sum_out")
-        need_device(dev, sum_out, "sum_out")
-        if sum_out.shape != x.shape or not sum_out.is_contiguous() or sum_out.data_ptr() % 16:
-            raise ValueError("sum_out must be contiguous, 16-byte aligned and shaped like x")
-        if overlap(sum_out, weight) or (overlap(sum_out, add)
-                                        and sum_out.data_ptr() != add.data_ptr()):
-            raise ValueError("sum_out must not overlap weight, nor add unless it is add itself")
-    elif sum_out is not None:
-        raise ValueError("sum_out needs add")
-    values, scales = _outputs(out, T, H, dev, [t for t in (x, weight, add, sum_out) if t is not None])
+        ap, sp, size = add.data_ptr(), sum_out.data_ptr(), 2 * T * H
+        fine = fine and add.dtype is BF16 and sum_out.dtype is BF16 and add.shape == x.shape \
+            and sum_out.shape == x.shape and add.is_contiguous() and sum_out.is_contiguous() \
+            and add.device == dev and sum_out.device == dev and not (ap | sp) % 16 \
+            and (sp == xp or sp >= xp + size or xp >= sp + size) \
+            and (sp == ap or sp >= ap + size or ap >= sp + size) \
+            and (sp >= wp + 2 * H or wp >= sp + size)
+    if not fine or (add is None and sum_out is not None):
+        _refuse_norm(x, weight, add, sum_out)
+    if out is None:
+        values = torch.empty((T, H), dtype=FP8, device=dev)
+        scales = torch.empty((H // GROUP, T), dtype=torch.float32, device=dev).t()
+    else:
+        values, scales = _outputs(out, T, H, dev, [t for t in (x, weight, add, sum_out) if t is not None])
     if T:
-        _lib.call("pdk_rmsnorm_fp8", x.data_ptr(), None if add is None else add.data_ptr(),
-                  weight.data_ptr(), T, H, float(eps),
-                  None if sum_out is None else sum_out.data_ptr(), values.data_ptr(),
-                  scales.data_ptr(), T, stream_handle())
+        _lib.call("pdk_rmsnorm_fp8", xp, ap, wp, T, H, eps, sp, values.data_ptr(), scales.data_ptr(),
+                  T, stream_handle())
     return values, scales
+
+
+def _refuse_norm(x, weight, add, sum_out):
+    """Raises for operands that rmsnorm_fp8's own test did not pass."""
+    dev = x.device
+    for t, name in ((x, "x"), (weight, "weight"), (add, "add"), (sum_out, "sum_out")):
+        if t is None:
+            continue
+        _need(t, name)
+        need_device(dev, t, name)
+        if not t.is_contiguous() or t.data_ptr() % 16:
+            raise ValueError(f"{name} must be contiguous and 16-byte aligned")
+    if x.dim() != 2:
+        raise ValueError(f"x must be [T, H], got {tuple(x.shape)}")
+    H = x.shape[1]
+    if H % GROUP or not GROUP <= H <= 8192:
+        raise ValueError(f"H={H} is no multiple of {GROUP} in [{GROUP}, 8192]")
+    if weight.numel() != H:
+        raise ValueError(f"weight must hold H={H} values")
+    if add is None:
+        raise ValueError("sum_out needs add")
+    if add.shape != x.shape or sum_out.shape != x.shape:
+        raise ValueError("add and sum_out must be shaped like x")
+    raise ValueError("sum_out must be x or add itself, or overlap none of x, add and weight")
 
 
 def _quantized(entry, x, gated, out, stream):
@@ -177,21 +195,22 @@ def linear_fp8(x, x_scales, w, w_scales, out=None, workspace=None, stream=None):
     contiguous, as rmsnorm_fp8, quantize_fp8, swiglu_fp8 and quantize_weight_fp8 give
     them. A group's sums are 32-bit but for the matrix instruction's own cut: of 8
     columns' products what lies 2^-13 below the largest is lost (some 2e-4 of a result).
-    They are scaled and added in 32 bits and rounded to bf16 once. K a multiple of 128, N of 8. ``workspace``: device
-    memory of linear_fp8_workspace_bytes for one call at a time (default: allocated by
-    the call)."""
+    They are scaled and added in 32 bits and rounded to bf16 once. K a multiple of 128,
+    N of 8. ``workspace``: device memory of linear_fp8_workspace_bytes for one call at a
+    time (default: allocated by the call)."""
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
         raise TypeError("x must be a CUDA tensor")
     dev = x.device
     if stream is not None or dev.index != _current_device():
         with launch_scope(dev, stream):
             return linear_fp8(x, x_scales, w, w_scales, out, workspace)
-    _need(x, "x", FP8)
-    _need(w, "w", FP8)
-    _need(x_scales, "x_scales", torch.float32)
-    _need(w_scales, "w_scales", torch.float32)
-    for t, name in ((w, "w"), (x_scales, "x_scales"), (w_scales, "w_scales")):
-        need_device(dev, t, name)
+    if not (x.dtype is FP8 and w.dtype is FP8 and x_scales.dtype is torch.float32
+            and w_scales.dtype is torch.float32 and w.device == dev and x_scales.device == dev
+            and w_scales.device == dev):
+        for t, name, dt in ((x, "x", FP8), (w, "w", FP8), (x_scales, "x_scales", torch.float32),
+                            (w_scales, "w_scales", torch.float32)):
+            _need(t, name, dt)
+            need_device(dev, t, name)
     if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
         raise ValueError(f"x [T, K] and w [N, K] expected, got {tuple(x.shape)}, {tuple(w.shape)}")
     (T, K), N = x.shape, w.shape[0]
@@ -200,9 +219,9 @@ def linear_fp8(x, x_scales, w, w_scales, out=None, workspace=None, stream=None):
     if not w.is_contiguous() or w.data_ptr() % 16:
         raise ValueError("w must be contiguous and 16-byte aligned")
     groups = K // GROUP
-    if tuple(x_scales.shape) != (T, groups):
+    if x_scales.shape != (T, groups):
         raise ValueError(f"x_scales must be {(T, groups)}, got {tuple(x_scales.shape)}")
-    if tuple(w_scales.shape) != (-(-N // GROUP), groups) or not w_scales.is_contiguous():
+    if w_scales.shape != (-(-N // GROUP), groups) or not w_scales.is_contiguous():
         raise ValueError(f"w_scales must be contiguous {(-(-N // GROUP), groups)}")
     xs_t = x_scales.stride(0) if T > 1 else 1
     xs_g = x_scales.stride(1) if groups > 1 else 1

@@ -347,3 +347,60 @@ def test_a_step_in_a_graph(cuda):
         assert torch.equal(tables, eager_tables) and torch.equal(m.slots, em.slots)
         have = [h + n for h, n in zip(have, lens)]
         taken += int(em.taken)
+
+
+def test_refusals_of_the_wrappers(cuda):
+    from rngd_pd_amd import kernels as K
+    lens = [(20, 3), (5, 1)]
+    q, ck, cv, tables, ctx = _operands(np.random.default_rng(0), 8, 2, lens)
+    tab = torch.from_numpy(tables).to(cuda)
+    past, new, free = (_int32(v, cuda) for v in ([20, 5], [3, 1], [1, 2]))
+    starts, ctx_d = _int32(_starts(lens), cuda), _int32(ctx, cuda)
+    inv = torch.ones(64, device=cuda)
+    qkv = torch.zeros((4, 12 * D), dtype=torch.bfloat16, device=cuda)
+    pos = _int32([20, 21, 22, 5], cuda)
+
+    def attend(**kw):
+        a = dict(q=q, ck=ck, cv=cv, tab=tab, starts=starts, ctx=ctx_d, new=3, max_ctx=23)
+        more = {k: v for k, v in kw.items() if k not in a}
+        a.update(kw)
+        return K.chunk_attention(a["q"], a["ck"], a["cv"], a["tab"], a["starts"], a["ctx"], a["new"],
+                                 a["max_ctx"], **more)
+
+    for at, (exc, call) in enumerate((
+            (TypeError, lambda: K.chunk_map(past.long(), new, tab, free, 4)),
+            (TypeError, lambda: K.chunk_map(past, new, tab, free.cpu(), 4)),
+            (ValueError, lambda: K.chunk_map(past[:1], new, tab, free, 4)),
+            (ValueError, lambda: K.chunk_map(past, new, tab.t(), free, 4)),
+            (ValueError, lambda: K.chunk_map(past, new, tab[0], free, 4)),
+            (ValueError, lambda: K.chunk_map(past, new, tab, free, -1)),
+            (ValueError, lambda: K.rope_cache_write(qkv[:, :11 * D], inv, pos, pos, ck, cv, 8)),
+            (ValueError, lambda: K.rope_cache_write(qkv, inv[:32], pos, pos, ck, cv, 8)),
+            (ValueError, lambda: K.rope_cache_write(qkv, inv, pos[:3], pos, ck, cv, 8)),
+            (ValueError, lambda: K.rope_cache_write(qkv, inv, pos, pos, ck, cv, 0)),
+            (TypeError, lambda: K.rope_cache_write(qkv, inv, pos.long(), pos, ck, cv, 8)),
+            (ValueError, lambda: K.rope_cache_write(qkv, inv, pos, pos, ck, cv, 8, q_out=q[:3])),
+            (ValueError, lambda: K.rope_cache_write(qkv, inv, pos, pos, ck, cv, 8,
+                                                    q_out=qkv[:, :8 * D].contiguous().view(4, 8, D)[:, :, :64])),
+            (ValueError, lambda: attend(q=q[:, :7])),
+            (ValueError, lambda: attend(q=q[:, :, :64])),
+            (TypeError, lambda: attend(q=q.float())),
+            (ValueError, lambda: attend(starts=starts[:2])),
+            (ValueError, lambda: attend(ctx=ctx_d[:1])),
+            (ValueError, lambda: attend(tab=tab.t())),
+            (ValueError, lambda: attend(max_ctx=0)),
+            (ValueError, lambda: attend(max_ctx=tab.shape[1] * 16 + 1)),
+            (ValueError, lambda: attend(new=-1)),
+            (ValueError, lambda: attend(window=0)),
+            (ValueError, lambda: attend(sinks=3)),
+            (ValueError, lambda: attend(out=q[:3])),
+            (TypeError, lambda: attend(stream="x")),
+    )):
+        print(at, exc, flush=True)
+        with pytest.raises(exc):
+            call()
+    none = q[:0]
+    assert tuple(attend(q=none, starts=_int32([0, 0, 0], cuda)).shape) == (0, 8, D)
+    assert tuple(K.rope_cache_write(qkv[:0], inv, pos[:0], pos[:0], ck, cv, 8).shape) == (0, 8, D)
+    m = K.chunk_map(past, new, tab.clone(), free[:0], 0)
+    assert m.positions.numel() == 0 and m.starts.tolist() == [0, 3, 4]

@@ -225,3 +225,49 @@ def test_side_stream_and_graph(cuda):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, chain())
+
+
+def test_refusals_of_the_wrappers(cuda):
+    from rngd_pd_amd import kernels as Kn
+    x, w = _randn(1, 8, 256), torch.ones(256, dtype=BF16, device=cuda)
+    more, buf = _randn(2, 8, 256), torch.empty(4096, dtype=BF16, device=cuda)
+    cpu = torch.empty((8, 256), dtype=BF16)
+    for at, (exc, call) in enumerate((
+            (TypeError, lambda: Kn.rmsnorm_fp8(x.float(), w, EPS)),
+            (TypeError, lambda: Kn.rmsnorm_fp8(x, [1.0] * 256, EPS)),
+            (TypeError, lambda: Kn.rmsnorm_fp8(x, w.cpu(), EPS)),
+            (TypeError, lambda: Kn.rmsnorm_fp8(x, w, EPS, add=cpu)),
+            (ValueError, lambda: Kn.rmsnorm_fp8(x.t(), w[:8], EPS)),
+            (ValueError, lambda: Kn.rmsnorm_fp8(x[:, :200].contiguous(), w[:200], EPS)),
+            (ValueError, lambda: Kn.rmsnorm_fp8(x, w[:128], EPS)),
+            (ValueError, lambda: Kn.rmsnorm_fp8(x[0], w, EPS)),
+            (ValueError, lambda: Kn.rmsnorm_fp8(x, w, EPS, sum_out=more)),
+            (ValueError, lambda: Kn.rmsnorm_fp8(x, w, EPS, add=more[:4])),
+            (ValueError, lambda: Kn.rmsnorm_fp8(buf[:2048].view(8, 256), w, EPS, add=more,
+                                                sum_out=buf[256:2304].view(8, 256))),
+            (ValueError, lambda: Kn.quantize_fp8(x[:, :100])),
+            (ValueError, lambda: Kn.swiglu_fp8(x[:, :128])),
+            (ValueError, lambda: Kn.quantize_fp8(x, out=(torch.empty((8, 256), dtype=torch.float8_e4m3fn,
+                                                                     device=cuda), torch.empty((8, 2), device=cuda)))),
+    )):
+        print(at, exc, flush=True)
+        with pytest.raises(exc):
+            call()
+    q, s = Kn.quantize_fp8(x)
+    w8, ws = Kn.quantize_weight_fp8(_randn(3, 64, 256))
+    for at, (exc, call) in enumerate((
+            (TypeError, lambda: Kn.linear_fp8(q.view(torch.uint8), s, w8, ws)),
+            (TypeError, lambda: Kn.linear_fp8(q, s.double(), w8, ws)),
+            (TypeError, lambda: Kn.linear_fp8(q, s, w8.cpu(), ws)),
+            (ValueError, lambda: Kn.linear_fp8(q, s, w8[:60], ws)),
+            (ValueError, lambda: Kn.linear_fp8(q, s[:, :1], w8, ws)),
+            (ValueError, lambda: Kn.linear_fp8(q, s, w8, ws[:, :1])),
+            (ValueError, lambda: Kn.linear_fp8(q[:, :128], s[:, :1], w8, ws)),
+            (ValueError, lambda: Kn.linear_fp8(q, s, w8, ws, out=torch.empty((8, 32), dtype=BF16, device=cuda))),
+    )):
+        print(at, exc, flush=True)
+        with pytest.raises(exc):
+            call()
+    none, scales = Kn.rmsnorm_fp8(x[:0], w, EPS)
+    assert tuple(none.shape) == (0, 256) and tuple(scales.shape) == (0, 2)
+    assert tuple(Kn.linear_fp8(none, scales, w8, ws).shape) == (0, 64)
