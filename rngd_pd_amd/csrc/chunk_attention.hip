@@ -839,11 +839,11 @@ __device__ __forceinline__ void big_unit(const Args& a, uint16_t* sm, int rest, 
     else pdk::copies_done<0>();
     const bool ok0 = ok_next & 1, ok1 = ok_next & 2;
     ok_next >>= 2;
-    if (i + 2 < n_walk) ok_next |= fetch(next, i + 2) << 2;
     v8 kr[8], va[2][4];
     load_k(st, kr);
     f32x16 s = scores(kr, qv);
     __builtin_amdgcn_sched_barrier(0);                           // V into K's registers
+    if (i + 2 < n_walk) ok_next |= fetch(next, i + 2) << 2;
     load_v(st, 0, va[0]);
     const int t0 = tile_of(i) * kTile;
     const Place at = place(a, t0, p, hh, ok0, ok1);
