@@ -54,6 +54,7 @@ constexpr int kMaxRequests = 65535;
 constexpr int kMaxSplits = 64;
 constexpr int kLeastSplit = 8;            // tiles of a split at least
 constexpr int kCUs = 256;
+constexpr int kMostRecords = 4096;        // of four units each
 constexpr int kRecord = 64 * 66;          // floats of a unit's sums: O 64 lanes x 64, (m, l)
 
 struct Args {
@@ -73,6 +74,7 @@ struct Args {
   // ones), tiles of a split and splits at most of those; of the longer ones, workgroups
   // that run at once and splits of what they leave over.
   int few_rows, few_per, few_splits, big_slots, big_splits;
+  int big_over;                           // workgroups' rows left over that there are records for
   int64_t big_base;                       // floats of the workspace before the longer ones' records
 };
 
@@ -712,7 +714,8 @@ __device__ __forceinline__ int rows_up_to(const Args& a, int base, int lane) {
 
 // A longer request's workgroup: 128 rows from row0 on of request r, split z of them.
 // Whole rounds of big_slots workgroups walk their contexts whole; the workgroups' rows
-// that are left over, fewer than would fill the card, are split.
+// that are left over, fewer than would fill the card, are split (none are where they are
+// more than the host could count on: one request with far fewer tokens than q has rows).
 struct Big {
   int r, row0;
   int left;                               // number among those left over, or -1
@@ -730,7 +733,9 @@ __device__ __forceinline__ bool find_big(const Args& a, int rest, Big& w) {
     all += __shfl(to, 63);
   }
   all = __builtin_amdgcn_readfirstlane(all);
-  const int whole = (int)((int64_t)all * a.NKV / a.big_slots * a.big_slots / a.NKV), left = all - whole;
+  int whole = (int)((int64_t)all * a.NKV / a.big_slots * a.big_slots / a.NKV);
+  if (all - whole > a.big_over) whole = all;                     // more than there are records for
+  const int left = all - whole;
   if (kLeft) {
     if (rest >= left) return false;
     rest += whole;
@@ -982,7 +987,7 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(Args a, int few_units) 
 struct Plan {
   bool big;
   int few_rows;                           // 0 where no request is taken as one of few rows
-  int few_per, few_splits, big_slots, big_splits;
+  int few_per, few_splits, big_slots, big_splits, big_over;
   int64_t few_blocks, big_blocks;         // workgroups
   int64_t few_units, big_units;           // units that may be split
   int64_t few_floats;                     // of the former's records
@@ -1020,19 +1025,24 @@ Plan plan_for(int N, int R, int max_new, int64_t max_ctx, int NH, int NKV, int w
   }
   if (p.big) {
     const int64_t rows = (int64_t)N * G, n = tiles(kRows / G + 1);
-    const int64_t most = rows / kRows + std::min<int64_t>(R, rows / (p.few_rows + 1) + 1);
+    const int64_t all = (rows + kRows - 1) / kRows;              // if they were one request's
+    const int64_t most = R == 1 ? all : rows / kRows + std::min<int64_t>(R, rows / (p.few_rows + 1) + 1);
+    const int64_t left = std::max<int64_t>(1, all * NKV % p.big_slots);
+    // Left over at most: known of one request, of several up to a whole round.
+    const int64_t over = R == 1 ? all - all * NKV / p.big_slots * p.big_slots / NKV
+                                : std::min<int64_t>(most, p.big_slots / NKV + 1);
     // The split that ends soonest of the workgroups left over; each costs as much again as
-    // ten tiles for its start, for handing over its sums (136 KB) and for the join.
-    const int64_t left = std::max<int64_t>(1, (rows + kRows - 1) / kRows * NKV % p.big_slots);
+    // ten tiles for its start, for handing over its sums (136 KB) and for the join. At most
+    // kMostRecords of them: 277 MB.
     double best = 1e30;
-    for (int s = 1; s <= kMaxSplits && (s == 1 || n / s >= kLeastSplit); ++s) {
+    for (int s = 1; s <= kMaxSplits && (s == 1 || (n / s >= kLeastSplit && s * over * NKV <= kMostRecords)); ++s) {
       const double t = rounds((left * s + kCUs - 1) / kCUs) * ((double)n / s + (s > 1 ? 10 : 0));
       if (t < best) {
         best = t;
         p.big_splits = s;
       }
     }
-    const int64_t over = std::min<int64_t>(most, p.big_slots / NKV + 1);     // left over at most
+    p.big_over = (int)over;
     p.big_blocks = (most + (p.big_splits - 1) * over) * NKV;
     if (p.big_splits > 1) p.big_units = over * NKV * kWaves;
   }
@@ -1111,7 +1121,7 @@ extern "C" int pdk_chunk_attn(const uint16_t* q, int64_t q_tok_stride, const uin
   const Args a{q, q_tok_stride, cache_k, cache_v, num_blocks, block_tables, max_blocks, starts,
                ctx_lens, N, R, n_q_heads, n_kv_heads, scale * 1.4426950408889634f, window, sinks,
                static_cast<float*>(workspace), out, p.few_rows, p.few_per, p.few_splits, p.big_slots,
-               p.big_splits, p.few_floats};
+               p.big_splits, p.big_over, p.few_floats};
   const hipStream_t st = pdk::as_stream(stream);
   const bool two = p.few_rows == 32;
   if (p.big && p.few_rows) {

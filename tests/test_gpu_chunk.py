@@ -278,6 +278,36 @@ def test_long_contexts_beside_many_short_ones(cuda, new):
     ref.within(_attend(q, ck, cv, tables, lens), want, bound)
 
 
+@pytest.mark.parametrize("new", [1544, 1400, 20])
+def test_rows_left_over_of_a_round(cuda, new):
+    """q with rows for just over a round of the card's workgroups, which are split, and a
+    request that has them all or fewer; its workspace holds what is left over alone."""
+    from rngd_pd_amd import kernels as K
+    N, past, Hq, Hkv = 1544, 1000, 64, 4
+    print(f"rows left over, {new} of {N} new", flush=True)
+    rng = np.random.default_rng(new)
+    q, ck, cv, tables, ctx = _operands(rng, Hq, Hkv, [(past, new)])
+    want, bound = ref.attention(q, ck, cv, tables, [new], ctx, 0, 0, SCALE)
+    more = torch.cat([q, torch.full((N - new, Hq, D), float("nan"), dtype=q.dtype, device=cuda)])
+    out = torch.full_like(more, 7.0)
+    need = K.chunk_workspace_bytes(N, 1, N, tables.shape[1] * 16, Hq, Hkv)
+    assert need < 64 << 20
+    ws = torch.full((need + 4096,), 85, dtype=torch.uint8, device=cuda)
+    _attend(more, ck, cv, tables, [(past, new)], out=out, max_new=N, max_ctx=tables.shape[1] * 16,
+            workspace=ws[:need])
+    ref.within(out[:new], want, bound)
+    assert (out[new:] == 7).all() and (ws[need:] == 85).all()
+
+
+@pytest.mark.parametrize("R", [1, 2, 5, 64])
+def test_workspaces_stay_small(R):
+    """Whatever is left over, the splits' sums take at most some 277 MB."""
+    from rngd_pd_amd import kernels as K
+    for N in (40, 776, 3104, 6208, 6300, 8192, 70000):
+        for Hq, Hkv in ((32, 8), (64, 4), (8, 8)):
+            assert K.chunk_workspace_bytes(N, R, N, 1 << 19, Hq, Hkv) <= 300 << 20
+
+
 def test_side_stream_and_own_workspace(cuda):
     from rngd_pd_amd import kernels as K
     rng = np.random.default_rng(9)
