@@ -492,9 +492,6 @@ __device__ __forceinline__ void few_unit(const Args& a, FewShared<kSets>& sm, in
     next_ids(0);
     int ids_from = 0;
     auto ok_of = [&](int x, int b) { return (x < ids_from ? ok_was[b] : ids[0].ok[b]) >> (x & 63) & 1; };
-    struct Tile {
-      v8 k[2][4], v[8];
-    };
     v8 qv[kSets][4];
 #pragma unroll
     for (int c = 0; c < kSets; ++c) {
@@ -514,19 +511,27 @@ __device__ __forceinline__ void few_unit(const Args& a, FewShared<kSets>& sm, in
     };
     // Tile x's loads, or past the last as many of one 16-byte piece each: no load is under a
     // branch that would make the compiler wait for all of them.
-    auto load = [&](Tile& t, int x) __attribute__((always_inline)) {
+    v8 k[2][4], v[8];
+    auto load_k = [&](int x) __attribute__((always_inline)) {
       const int64_t b0 = block(x, 0), b1 = block(x, 1);
-      const bool dead = x >= n_own;
-      const uint16_t* k = a.k + (dead ? 0 : (i & 8 ? b1 : b0) + k_at);
-      const uint16_t* v = a.v + (dead ? 0 : (kg & 2 ? b1 : b0) + v_at);
+      const uint16_t* from = a.k + (x >= n_own ? 0 : (i & 8 ? b1 : b0) + k_at);
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int d = 0; d < 4; ++d) t.k[u][d] = pdk::ld16(k + 1024 * u + 256 * d);
-#pragma unroll
-      for (int n = 0; n < 8; ++n) t.v[n] = pdk::ld16_stream(v + 256 * n);
+        for (int d = 0; d < 4; ++d) k[u][d] = pdk::ld16(from + 1024 * u + 256 * d);
     };
-    auto use = [&](Tile& t, int x) __attribute__((always_inline)) {
+    auto load_v = [&](int x) __attribute__((always_inline)) {
+      const int64_t b0 = block(x, 0), b1 = block(x, 1);
+      const uint16_t* from = a.v + (x >= n_own ? 0 : (kg & 2 ? b1 : b0) + v_at);
+#pragma unroll
+      for (int n = 0; n < 8; ++n) v[n] = pdk::ld16_stream(from + 256 * n);
+    };
+    load_k(0);
+    load_v(0);
+    // A tile's registers take the next one's K after the scores, its V after the products.
+#pragma unroll 1
+    for (int x = 0; x < n_own; ++x) {
+      if ((x & 63) == 63) next_ids(ids_from = x + 1);
       const bool ok0 = ok_of(x, 0), ok1 = ok_of(x, 1);
       const int t0 = tile_of(x) * kTile;
       f32x4 s[kSets][2];
@@ -536,8 +541,9 @@ __device__ __forceinline__ void few_unit(const Args& a, FewShared<kSets>& sm, in
         for (int u = 0; u < 2; ++u) {
           s[c][u] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int d = 0; d < 4; ++d) s[c][u] = mfma16(t.k[u][d], qv[c][d], s[c][u]);
+          for (int d = 0; d < 4; ++d) s[c][u] = mfma16(k[u][d], qv[c][d], s[c][u]);
         }
+      load_k(x + 1);
       const bool edge = hides(a, t0, p0, p1, ok0 && ok1);
       if (edge) {
         const bool ok = kg & 2 ? ok1 : ok0;
@@ -574,37 +580,23 @@ __device__ __forceinline__ void few_unit(const Args& a, FewShared<kSets>& sm, in
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {
           const float u = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c][e >> 2][e & 3], a.c, -mc));
-          const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c][e >> 2][(e & 3) + 1], a.c, -mc));
-          sum.l[c] += u + v;
-          wt[c].w[e >> 1] = pdk::pack_bf16x2_rne(u, v);
+          const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c][e >> 2][(e & 3) + 1], a.c, -mc));
+          sum.l[c] += u + y;
+          wt[c].w[e >> 1] = pdk::pack_bf16x2_rne(u, y);
         }
       }
       if (edge) {
         bool found = false;
 #pragma unroll
-        for (int n = 0; n < 8; ++n) found |= clean(t.v[n]);
+        for (int n = 0; n < 8; ++n) found |= clean(v[n]);
         odd |= __any(found);
       }
 #pragma unroll
       for (int c = 0; c < kSets; ++c)
 #pragma unroll
-        for (int n = 0; n < 8; ++n) sum.o[c][n] = mfma16(t.v[n], wt[c], sum.o[c][n]);
-    };
-    // Two tiles in registers: while one is used the other is under way.
-    Tile ta, tb;
-    load(ta, 0);
-    load(tb, 1);
-    int x = 0;
-#pragma unroll 1
-    for (; x + 2 < n_own; x += 2) {
-      if ((x & 63) == 62) next_ids(ids_from = x + 2);
-      use(ta, x);
-      load(ta, x + 2);
-      use(tb, x + 1);
-      load(tb, x + 3);
+        for (int n = 0; n < 8; ++n) sum.o[c][n] = mfma16(v[n], wt[c], sum.o[c][n]);
+      load_v(x + 1);
     }
-    use(ta, x);
-    if (x + 1 < n_own) use(tb, x + 1);
   }
   // The wavefront's own tiles alone are its sums', any of which may be added to.
   if (__builtin_expect(odd, 0))
@@ -893,7 +885,7 @@ __device__ __forceinline__ void big_unit(const Args& a, uint16_t* sm, int rest, 
 }
 
 template <int kSets>
-__global__ __launch_bounds__(256, kSets == 1 ? 2 : 1) void chunk_few_kernel(Args a) {
+__global__ __launch_bounds__(256, kSets == 1 ? 3 : 2) void chunk_few_kernel(Args a) {
   __shared__ FewShared<kSets> sm;
   const int rest = blockIdx.x / a.NKV;
   few_unit<kSets>(a, sm, rest % a.R, blockIdx.x % a.NKV, rest / a.R);
@@ -904,15 +896,16 @@ __global__ __launch_bounds__(256, 3) void chunk_big_kernel(Args a) {
   big_unit(a, sm, blockIdx.x / a.NKV, blockIdx.x % a.NKV);
 }
 
-// Requests of both kinds: eight workgroups of the one kind and eight of the other in turn
-// as long as both last, so that the ones that wait for memory and the ones that
-// multiply share the CUs.
-__global__ __launch_bounds__(256, 2) void chunk_both_kernel(Args a, int few, int big) {
+// Requests of both kinds: a workgroup for each CU of the one kind, then of the other, as
+// long as both last, so that those that wait for memory and those that multiply share
+// the CUs (2000 new tokens beside 31 single ones: 213 us; with 128 in turn 7 % more). Few
+// rows first, their walks are the longest (224 us the other way round).
+__global__ __launch_bounds__(256, 3) void chunk_both_kernel(Args a, int few, int big) {
   constexpr int kTiles = 2 * kRing * kTileElems * sizeof(uint16_t);
   __shared__ __align__(1024) char sm[std::max(kTiles, (int)sizeof(FewShared<1>))];
-  const int g = blockIdx.x >> 3, turns = min((few + 7) >> 3, (big + 7) >> 3);
-  const bool is_big = g < 2 * turns ? (g & 1) == 0 : big > few;
-  const int u = (g < 2 * turns ? g >> 1 : g - turns) * 8 + (blockIdx.x & 7);
+  const int g = blockIdx.x / kCUs, turns = min((few + kCUs - 1) / kCUs, (big + kCUs - 1) / kCUs);
+  const bool is_big = g < 2 * turns ? g & 1 : big > few;
+  const int u = (g < 2 * turns ? g >> 1 : g - turns) * kCUs + blockIdx.x % kCUs;
   if (u >= (is_big ? big : few)) return;
   const int rest = u / a.NKV, kvh = u - rest * a.NKV;
   if (is_big) big_unit(a, reinterpret_cast<uint16_t*>(sm), rest, kvh);
@@ -933,39 +926,45 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(Args a, int few_units) 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int G = a.NH / a.NKV;
   const int unit = blockIdx.x - few_units, at = unit / kWaves, left = at / a.NKV, kvh = at - left * a.NKV;
+  const float* rec = a.ws + a.big_base + (int64_t)unit * a.big_splits * kRecord;
+  // Four splits' loads at a time, the last one again past the end; the first four before
+  // anything says how many there are.
+  float2 ml[4];
+  float4 y[4][4];
+  auto load = [&](int z) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float* from = rec + (int64_t)min(z + i, a.big_splits - 1) * kRecord;
+      ml[i] = reinterpret_cast<const float2*>(from + 64 * 64)[lane];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) y[i][x] = reinterpret_cast<const float4*>(from)[(4 * wave + x) * 64 + lane];
+    }
+  };
+  load(0);
   Big wg;
   if (!find_big<true>(a, left, wg)) return;
   const Request q = request(a, wg.r);
   const int row1 = min(wg.row0 + kRows, q.n * G) - 1, row0 = wg.row0 + 32 * (unit - at * kWaves);
   const Walk w = walk(a, q.past + wg.row0 / G, q.past + row1 / G);
   const int splits = splits_of(w.n, big_per(a, w.n), a.big_splits);
-  const float* rec = a.ws + a.big_base + (int64_t)unit * a.big_splits * kRecord;
   if (row0 > row1) return;
   if (splits == 1) return;
   const Row row = row_at(a, q, kvh, row0 + j);
   if (!row.mine) return;                  // both lanes of a row alike
-  auto sums = [&](int z) { return reinterpret_cast<const float2*>(rec + (int64_t)z * kRecord + 64 * 64)[lane]; };
-  // Four splits' loads at a time; the last one again past the end, with the factor 0.
   float m = -INFINITY, l = 0.f, o[16];
-  for (int z = 0; z < splits; z += 4) {
-    float x[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = sums(min(z + i, splits - 1)).x;
-    m = vmax(m, vmax(vmax(x[0], x[1]), vmax(x[2], x[3])));
-  }
 #pragma unroll
   for (int x = 0; x < 16; ++x) o[x] = 0.f;
   for (int z = 0; z < splits; z += 4) {
-    float2 ml[4];
-    float4 y[4][4];
+    if (z) load(z);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int at = min(z + i, splits - 1);
-      ml[i] = sums(at);
-      const float4* p = reinterpret_cast<const float4*>(rec + (int64_t)at * kRecord) + 4 * wave * 64 + lane;
+    for (int i = 0; i < 4; ++i)
+      if (z + i >= splits) ml[i].x = -INFINITY;
+    const float m_new = vmax(m, vmax(vmax(ml[0].x, ml[1].x), vmax(ml[2].x, ml[3].x)));
+    const float g = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - m_new) * a.c);
+    m = m_new;
+    l *= g;
 #pragma unroll
-      for (int x = 0; x < 4; ++x) y[i][x] = p[x * 64];
-    }
+    for (int x = 0; x < 16; ++x) o[x] *= g;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if (z + i >= splits) break;
@@ -1017,7 +1016,7 @@ Plan plan_for(int N, int R, int max_new, int64_t max_ctx, int NH, int NKV, int w
   if (p.few_rows) {
     const int n = tiles(p.few_rows / G);
     const int64_t groups = (int64_t)R * NKV;
-    const int64_t want = std::min<int64_t>(kMaxSplits, std::max<int64_t>(1, (p.few_rows == 32 ? 256 : 512) / groups));
+    const int64_t want = std::min<int64_t>(kMaxSplits, std::max<int64_t>(1, (p.few_rows == 32 ? 1 : 3) * kCUs / groups));
     p.few_per = std::max<int>(kLeastSplit, (int)((n + want - 1) / want));
     p.few_splits = (n + p.few_per - 1) / p.few_per;
     p.few_blocks = groups * p.few_splits;
@@ -1125,8 +1124,8 @@ extern "C" int pdk_chunk_attn(const uint16_t* q, int64_t q_tok_stride, const uin
   const hipStream_t st = pdk::as_stream(stream);
   const bool two = p.few_rows == 32;
   if (p.big && p.few_rows) {
-    const unsigned turns = (unsigned)((p.few_blocks + 7) / 8 + (p.big_blocks + 7) / 8);
-    hipLaunchKernelGGL(chunk_both_kernel, dim3(8 * turns), dim3(256), 0, st, a, (int)p.few_blocks,
+    const unsigned turns = (unsigned)((p.few_blocks + kCUs - 1) / kCUs + (p.big_blocks + kCUs - 1) / kCUs);
+    hipLaunchKernelGGL(chunk_both_kernel, dim3(kCUs * turns), dim3(256), 0, st, a, (int)p.few_blocks,
                        (int)p.big_blocks);
   } else if (p.big) {
     hipLaunchKernelGGL(chunk_big_kernel, dim3((unsigned)p.big_blocks), dim3(256), 0, st, a);
