@@ -55,10 +55,18 @@ def chunk_map(past, new, tables, free, max_tokens, stream=None):
     if stream is not None or dev.index != _current_device():
         with launch_scope(dev, stream):
             return chunk_map(past, new, tables, free, max_tokens)
-    _int32(tables, "tables", dev, 2)
-    _int32(past, "past", dev)
-    _int32(new, "new", dev)
-    _int32(free, "free", dev)
+    # The usual operands pass one test; what does not is told apart.
+    if not (isinstance(past, torch.Tensor) and isinstance(new, torch.Tensor)
+            and isinstance(free, torch.Tensor)
+            and tables.dtype is past.dtype is new.dtype is free.dtype is torch.int32
+            and past.device == new.device == free.device == dev
+            and tables.dim() == 2 and past.dim() == new.dim() == free.dim() == 1
+            and tables.is_contiguous() and past.is_contiguous() and new.is_contiguous()
+            and free.is_contiguous()):
+        _int32(tables, "tables", dev, 2)
+        _int32(past, "past", dev)
+        _int32(new, "new", dev)
+        _int32(free, "free", dev)
     R, W = tables.shape
     if past.numel() != R or new.numel() != R:
         raise ValueError(f"past and new must hold {R} lengths")
@@ -66,7 +74,7 @@ def chunk_map(past, new, tables, free, max_tokens, stream=None):
     if not 0 <= N < 1 << 30:
         raise ValueError(f"max_tokens={N} outside [0, 2^30)")
     buf = torch.empty(2 * R + 2 + 2 * N, dtype=torch.int32, device=dev)
-    out = ChunkMap(*buf.split([R + 1, R, N, N, 1]))
+    out = ChunkMap(*buf.split_with_sizes([R + 1, R, N, N, 1]))
     at = buf.data_ptr()
     _lib.call("pdk_chunk_map", past.data_ptr(), new.data_ptr(), R, tables.data_ptr(), W,
               free.data_ptr(), free.numel(), N, at, at + 4 * (R + 1), at + 4 * (2 * R + 1),
@@ -92,32 +100,19 @@ def rope_cache_write(qkv, inv_freq, positions, slots, cache_k, cache_v, n_q_head
         with launch_scope(dev, stream):
             return rope_cache_write(qkv, inv_freq, positions, slots, cache_k, cache_v, n_q_heads,
                                     q_out)
-    _need(qkv, "qkv")
-    nb, H, D = _check_layer_cache(cache_k, cache_v)
-    need_device(dev, cache_k, "cache_k")
-    need_device(dev, cache_v, "cache_v")
-    if D != HEAD_DIM:
-        raise ValueError(f"head_dim must be {HEAD_DIM}, got {D}")
     n_q_heads = int(n_q_heads)
-    if n_q_heads < 1:
-        raise ValueError(f"n_q_heads must be >= 1, got {n_q_heads}")
-    if qkv.dim() != 2 or (qkv.shape[1] > 1 and qkv.stride(1) != 1):
-        raise ValueError("qkv must be [N, columns] with unit column stride")
-    N, width = qkv.shape[0], (n_q_heads + 2 * H) * D
-    if qkv.shape[1] < width:
-        raise ValueError(f"qkv rows hold {qkv.shape[1]} values, need {width}")
+    # The usual operands pass one test; what does not is told apart, or copied.
+    others = (inv_freq, positions, slots, cache_k, cache_v)
+    if not all(isinstance(t, torch.Tensor) and t.device == dev and t.is_contiguous() for t in others) \
+            or not qkv.dtype is cache_k.dtype is cache_v.dtype is BF16 \
+            or not positions.dtype is slots.dtype is torch.int32 \
+            or inv_freq.dtype is not torch.float32:
+        _refuse_write(qkv, *others)
+    nb, H, D, N, width = _write_sizes(qkv, *others, n_q_heads)
     ld = qkv.stride(0) if N > 1 else max(qkv.shape[1], width) + 7 & ~7
     if ld < width or ld % 8 or qkv.data_ptr() % 16:
         qkv = qkv[:, :width].clone(memory_format=torch.contiguous_format)
         ld = width
-    _need(inv_freq, "inv_freq", torch.float32)
-    need_device(dev, inv_freq, "inv_freq")
-    if inv_freq.numel() != D // 2 or not inv_freq.is_contiguous():
-        raise ValueError(f"inv_freq must hold head_dim/2 = {D // 2} contiguous values")
-    for t, name in ((positions, "positions"), (slots, "slots")):
-        _int32(t, name, dev)
-        if t.numel() != N:
-            raise ValueError(f"{name} must hold {N} entries")
     if q_out is None:
         q_out = torch.empty((N, n_q_heads, D), dtype=BF16, device=dev)
     else:
@@ -133,6 +128,46 @@ def rope_cache_write(qkv, inv_freq, positions, slots, cache_k, cache_v, n_q_head
                   positions.data_ptr(), slots.data_ptr(), N, n_q_heads, H, D, q_out.data_ptr(),
                   cache_k.data_ptr(), cache_v.data_ptr(), nb, stream_handle())
     return q_out
+
+
+def _refuse_write(qkv, inv_freq, positions, slots, cache_k, cache_v):
+    """Raises for operands that rope_cache_write's own test did not pass."""
+    dev = qkv.device
+    _need(qkv, "qkv")
+    _check_layer_cache(cache_k, cache_v)
+    _need(inv_freq, "inv_freq", torch.float32)
+    for t, name in ((cache_k, "cache_k"), (cache_v, "cache_v"), (inv_freq, "inv_freq")):
+        need_device(dev, t, name)
+    if not inv_freq.is_contiguous():
+        raise ValueError(f"inv_freq must hold head_dim/2 = {HEAD_DIM // 2} contiguous values")
+    _int32(positions, "positions", dev)
+    _int32(slots, "slots", dev)
+
+
+def _write_sizes(qkv, inv_freq, positions, slots, cache_k, cache_v, n_q_heads):
+    """(blocks, KV heads, head_dim, tokens, columns) of rope_cache_write's operands."""
+    if cache_k.dim() != 4 or cache_k.shape[2] != 16 or cache_v.dim() != 4 \
+            or positions.dim() != 1 or slots.dim() != 1:
+        _refuse_write(qkv, inv_freq, positions, slots, cache_k, cache_v)
+    nb, H, _, D = cache_k.shape
+    if cache_v.shape != (nb, H, D, 16):
+        raise ValueError(f"cache_v must be [nb, Hkv, D, 16], got {tuple(cache_v.shape)}")
+    if D != HEAD_DIM:
+        raise ValueError(f"head_dim must be {HEAD_DIM}, got {D}")
+    if n_q_heads < 1:
+        raise ValueError(f"n_q_heads must be >= 1, got {n_q_heads}")
+    if qkv.dim() != 2 or (qkv.shape[1] > 1 and qkv.stride(1) != 1):
+        raise ValueError("qkv must be [N, columns] with unit column stride")
+    N, columns = qkv.shape
+    width = (n_q_heads + 2 * H) * D
+    if columns < width:
+        raise ValueError(f"qkv rows hold {columns} values, need {width}")
+    if inv_freq.numel() != D // 2:
+        raise ValueError(f"inv_freq must hold head_dim/2 = {D // 2} contiguous values")
+    for t, name in ((positions, "positions"), (slots, "slots")):
+        if t.numel() != N:
+            raise ValueError(f"{name} must hold {N} entries")
+    return nb, H, D, N, width
 
 
 @functools.lru_cache(maxsize=4096)

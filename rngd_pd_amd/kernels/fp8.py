@@ -91,7 +91,7 @@ def rmsnorm_fp8(x, weight, eps, add=None, sum_out=None, out=None, stream=None):
         _refuse_norm(x, weight, add, sum_out)
     if out is None:
         values = torch.empty((T, H), dtype=FP8, device=dev)
-        scales = torch.empty((H // GROUP, T), dtype=torch.float32, device=dev).t()
+        scales = torch.empty_strided((T, H // GROUP), (1, T), dtype=torch.float32, device=dev)
     else:
         values, scales = _outputs(out, T, H, dev, [t for t in (x, weight, add, sum_out) if t is not None])
     if T:
