@@ -148,7 +148,8 @@ __device__ __forceinline__ void turn_head(const Turn* z, const v8& a, const v8& 
 // grid: x = 16 tokens, y = a share of their units. First the units of q: 256 of the tokens'
 // (token, head, 8 dims) in order, so that a unit reads and writes whole rows; then those
 // of k: two heads of the 16 tokens, whose 16 bytes at a dim lie together in the cache; then
-// those of v: eight heads.
+// those of v: 16 / kLanes heads, kLanes lanes for 8 dims of one.
+template <int kLanes>
 __global__ __launch_bounds__(kThreads) void rope_write_kernel(
     const uint16_t* qkv, int64_t ld, const float* inv_freq, const int32_t* positions,
     const int32_t* slots, int N, int NH, int NKV, uint16_t* q_out, uint16_t* cache_k,
@@ -162,7 +163,7 @@ __global__ __launch_bounds__(kThreads) void rope_write_kernel(
     slot_of[tid] = s < n_slots ? s : -1;
   }
   const int units_q = (kTok * NH * 8 + kThreads - 1) / kThreads, units_k = (NKV + 1) / 2;
-  const int units = units_q + units_k + (NKV + 7) / 8, u0 = blockIdx.y;
+  const int units = units_q + units_k + (NKV * kLanes + 15) / 16, u0 = blockIdx.y;
   const int d = (tid & 7) * 8;            // q and k: the lane's dims
   struct Place {
     int t, head;                          // token of the 16, head of qkv's
@@ -234,12 +235,13 @@ __global__ __launch_bounds__(kThreads) void rope_write_kernel(
   const int n_leads = __popcll(leads);
   const int lead_at[2] = {__builtin_ctzll(leads | 1ull << kTok), 63 - __builtin_clzll(leads | 1)};
   for (; u < units; u += gridDim.y) {
-    const int dv = ((tid >> 1) & 15) * 8, h = (u - units_q - units_k) * 8 + (tid >> 5);
+    const int sub = tid % kLanes, dv = (tid / kLanes % 16) * 8;
+    const int h = (u - units_q - units_k) * (16 / kLanes) + tid / (16 * kLanes);
     if (h >= NKV) continue;
     const uint16_t* const column = qkv + (int64_t)j0 * ld + (int64_t)(NH + NKV + h) * kD + dv;
     auto target = [&](int s) { return cache_v + (((int64_t)(s >> 4) * NKV + h) * kD + dv) * 16 + (s & 15); };
-    if ((tid & 1) < n_leads) {
-      const int t = lead_at[tid & 1];
+    if (sub < n_leads) {
+      const int t = sub ? lead_at[1] : lead_at[0];
       v8 in[8], out[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) in[i] = pdk::ld16(column + (t + i) * ld);
@@ -248,17 +250,31 @@ __global__ __launch_bounds__(kThreads) void rope_write_kernel(
 #pragma unroll
       for (int i = 0; i < 8; ++i) pdk::st16(to + 16 * i, out[i]);
     }
-    // The lone tokens in turn, even and odd ones by the two lanes of 8 dims.
-    int k = 0;
-    for (uint64_t left = lone; left; left &= left - 1, ++k) {
-      if ((k ^ tid) & 1) continue;
-      const int t = __builtin_ctzll(left);
-      const v8 x = pdk::ld16(column + t * ld);
-      uint16_t* to = target(slot_of[t + 7]);
+    // The lone tokens, every kLanes-th by each of the lanes of 8 dims: all loads first.
+    if (lone) {
+      v8 x[kTok / kLanes];
+      int at[kTok / kLanes];
+      uint64_t left = lone;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        to[32 * w] = (uint16_t)x.w[w];
-        to[32 * w + 16] = (uint16_t)(x.w[w] >> 16);
+      for (int i = 0; i < kTok / kLanes; ++i) {
+        at[i] = -1;
+#pragma unroll
+        for (int e = 0; e < kLanes; ++e) {
+          const int t = left ? __builtin_ctzll(left) : -1;
+          left &= left - 1;
+          at[i] = sub == e ? t : at[i];
+        }
+        x[i] = pdk::ld16(column + max(at[i], 0) * ld);
+      }
+#pragma unroll
+      for (int i = 0; i < kTok / kLanes; ++i) {
+        if (at[i] < 0) break;
+        uint16_t* to = target(slot_of[at[i] + 7]);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          to[32 * w] = (uint16_t)x[i].w[w];
+          to[32 * w + 16] = (uint16_t)(x[i].w[w] >> 16);
+        }
       }
     }
   }
@@ -309,12 +325,16 @@ extern "C" int pdk_rope_cache_write(const uint16_t* qkv, int64_t ld, const float
                   pdk::aligned16(cache_v),
               "tensors must be 16-byte aligned");
   const int tiles = (N + kTok - 1) / kTok;
+  // Units apart until there are four workgroups for every CU. Where they would not come to
+  // one, V's tokens are apart too: one is then likely to lie alone, and a lane of few would
+  // store 8 of them value by value (48 heads, with 16 lanes and with 2: 3.5 and 6.7 us for 16
+  // tokens, 8.5 and 9.8 for 1024, 12.4 and 12.7 for 2048).
+  const bool few = tiles <= 64;
   const int units = (kTok * n_q_heads * 8 + kThreads - 1) / kThreads + (n_kv_heads + 1) / 2 +
-                    (n_kv_heads + 7) / 8;
-  // Heads apart until there are four workgroups for every CU.
+                    (n_kv_heads * (few ? 16 : 2) + 15) / 16;
   const int shares = std::min(units, std::max(1, (1024 + tiles - 1) / tiles));
-  hipLaunchKernelGGL(rope_write_kernel, dim3(tiles, shares), dim3(kThreads), 0,
-                     pdk::as_stream(stream), qkv, ld, inv_freq, positions, slots, N, n_q_heads,
-                     n_kv_heads, q_out, cache_k, cache_v, (int64_t)num_blocks * 16);
+  hipLaunchKernelGGL(few ? rope_write_kernel<16> : rope_write_kernel<2>, dim3(tiles, shares),
+                     dim3(kThreads), 0, pdk::as_stream(stream), qkv, ld, inv_freq, positions, slots, N,
+                     n_q_heads, n_kv_heads, q_out, cache_k, cache_v, (int64_t)num_blocks * 16);
   return pdk::check_launch("rope_write_kernel");
 }

@@ -65,6 +65,7 @@ def test_map(cuda, past, new, width, short, spare):
     (1, 32, 8, 0, "run"), (16, 32, 8, 5, "run"), (37, 28, 4, 100, "run"), (64, 8, 8, 16000, "any"),
     (100, 5, 1, 999_983, "any"), (250, 40, 8, 3, "run"), (33, 6, 3, 12, "some"), (9, 32, 8, -4, "some"),
     (2000, 32, 8, 131_000, "run"), (24, 128, 16, 0, "run"),
+    (1100, 6, 3, 7, "any"), (1500, 5, 5, 3, "some"), (300, 8, 2, 40, "pieces"), (1333, 12, 12, 0, "pieces"),
 ])
 def test_write(cuda, N, Hq, Hkv, first, kind):
     from rngd_pd_amd import kernels as K
@@ -72,7 +73,17 @@ def test_write(cuda, N, Hq, Hkv, first, kind):
     print(f"write N={N} Hq={Hq} Hkv={Hkv} first={first} {kind}", flush=True)
     rng = np.random.default_rng(N + Hq)
     nb = N // 16 + 4
-    slots = rng.permutation(nb * 16)[:N]
+    if kind == "pieces":                  # of any length, each from somewhere in a block on
+        lens = rng.integers(1, 30, N)
+        nb = int(sum(-(-(n + 15) // 16) for n in lens)) + 4
+        ids, at, slots = rng.permutation(nb), 0, []
+        for n in lens:
+            piece = (ids[at:at + -(-(n + 15) // 16), None] * 16 + np.arange(16)).reshape(-1)
+            slots.append(piece[(off := int(rng.integers(16))):off + n])
+            at += -(-(n + 15) // 16)
+        slots = np.concatenate(slots)[:N]
+    else:
+        slots = rng.permutation(nb * 16)[:N]
     if kind == "run":                     # blocks one after another, from the middle of one
         slots = (rng.permutation(nb)[:, None] * 16 + np.arange(16)).reshape(-1)[3:3 + N]
     if kind == "some":                    # some tokens have no place, or one outside the cache
