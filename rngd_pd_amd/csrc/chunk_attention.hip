@@ -138,8 +138,8 @@ struct BlockIds {
 };
 
 __device__ __forceinline__ int block_id(const Args& a, int r, int e) {
-  const int id = a.tables[(int64_t)r * a.W + min(e, a.W - 1)];
-  return e < a.W && id >= 0 && id < a.num_blocks ? id : -1;
+  const int id = a.tables[(int64_t)r * a.W + min(max(e, 0), a.W - 1)];
+  return e >= 0 && e < a.W && id >= 0 && id < a.num_blocks ? id : -1;
 }
 
 __device__ __forceinline__ BlockIds load_ids(const Args& a, int r, int tile, int b) {
@@ -720,11 +720,15 @@ template <bool kLeft>
 __device__ __forceinline__ bool find_big(const Args& a, int rest, Big& w) {
   const int lane = threadIdx.x & 63;
   int all = 0, to = 0;
-  for (int base = 0; base < a.R; base += 64) {
-    to = rows_up_to(a, base, lane);
-    all += __shfl(to, 63);
+  if (a.R == 1) {
+    all = (request(a, 0).n * (a.NH / a.NKV) + kRows - 1) / kRows;
+  } else {
+    for (int base = 0; base < a.R; base += 64) {
+      to = rows_up_to(a, base, lane);
+      all += __shfl(to, 63);
+    }
+    all = __builtin_amdgcn_readfirstlane(all);
   }
-  all = __builtin_amdgcn_readfirstlane(all);
   int whole = (int)((int64_t)all * a.NKV / a.big_slots * a.big_slots / a.NKV);
   if (all - whole > a.big_over) whole = all;                     // more than there are records for
   const int left = all - whole;
@@ -742,6 +746,11 @@ __device__ __forceinline__ bool find_big(const Args& a, int rest, Big& w) {
     tile = whole + w.left;
     if (w.z >= a.big_splits) return false;
   }
+  if (a.R == 1) {
+    w.r = 0;
+    w.row0 = (all - 1 - tile) * kRows;    // the last rows first: they walk the most
+    return tile < all;
+  }
   int before = 0;
   for (int base = 0; base < a.R; base += 64) {
     if (a.R > 64) to = rows_up_to(a, base, lane);
@@ -749,7 +758,6 @@ __device__ __forceinline__ bool find_big(const Args& a, int rest, Big& w) {
     if (hit) {
       const int l = __builtin_ctzll(hit);
       w.r = __builtin_amdgcn_readfirstlane(base + l);
-      // The last rows first: they walk the most.
       w.row0 = __builtin_amdgcn_readfirstlane((before + __shfl(to, l) - 1 - tile) * kRows);
       return true;
     }
@@ -763,9 +771,14 @@ __device__ __forceinline__ int big_per(const Args& a, int n) {
   return max((n + a.big_splits - 1) / a.big_splits, kLeastSplit);
 }
 
-__device__ __forceinline__ void big_unit(const Args& a, uint16_t* sm, int rest, int kvh) {
+// kTeams times four wavefronts share the tiles of a split, each four with a ring of
+// their own.
+template <int kTeams>
+__device__ __forceinline__ void big_unit(const Args& a, uint16_t* shared, int rest, int kvh) {
   const int lane = threadIdx.x & 63, j = lane & 31, hh = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int number = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = number % kWaves, team = number / kWaves;
+  uint16_t* const sm = shared + team * 2 * kRing * kTileElems;
   const int G = a.NH / a.NKV;
   Big wg;
   if (!find_big<false>(a, rest, wg)) return;
@@ -776,7 +789,10 @@ __device__ __forceinline__ void big_unit(const Args& a, uint16_t* sm, int rest, 
   const int per = wg.left < 0 ? w.n : big_per(a, w.n);
   const int splits = wg.left < 0 ? 1 : splits_of(w.n, per, a.big_splits);
   if (wg.z >= splits) return;
-  const int first = wg.z * per, n_walk = (wg.z + 1 == splits ? w.n : first + per) - first;
+  // The team's tiles of the split's, at most n_most.
+  const int n_split = (wg.z + 1 == splits ? w.n : (wg.z + 1) * per) - wg.z * per;
+  const int n_most = (n_split + kTeams - 1) / kTeams;
+  const int first = wg.z * per + team * n_most, n_walk = min(n_most, n_split - team * n_most);
   v8 qv[8];
   int p;                                  // the lane's position
   {
@@ -861,23 +877,71 @@ __device__ __forceinline__ void big_unit(const Args& a, uint16_t* sm, int rest, 
 #pragma unroll
     for (int x = 0; x < 8; ++x) sum.o[x & 3] = mfma32(va[x >> 2][x & 3], wt[x >> 2], sum.o[x & 3]);
   };
-  for (int i = 0, at = 0; i < n_walk; ++i) {
+  for (int i = 0, at = 0; i < n_most; ++i) {
     const int next = at == 0 ? kRing - 1 : at - 1;               // of tile i + 2: that of tile i - 1
-    step(i, sm + at * kTileElems, next);
+    if (kTeams == 1 || i < n_walk) step(i, sm + at * kTileElems, next);
+    else pdk::copies_done<0>();                                  // the others' barrier
     at = at + 1 == kRing ? 0 : at + 1;
   }
   int ln = lane;                          // the row anew: kept, it would be spilled
   asm("" : "+v"(ln));
-  const Row row = row_at(a, q, kvh, row0 + 32 * wave + (ln & 31));
-  if (__builtin_expect(odd, 0))
+  if (__builtin_expect(odd, 0)) {
+    const Row row = row_at(a, q, kvh, row0 + 32 * wave + (ln & 31));
     add_cleaned(a, w, first, first + n_walk, r, kvh, row.p, p0, p1, ln, sum.o);
+  }
+  float4* const so = reinterpret_cast<float4*>(shared);
+  float share[kTeams];
+  if constexpr (kTeams > 1) {
+    // The other teams' sums by LDS, where the tiles were, the m and l of a lane last.
+    float2* const sml = reinterpret_cast<float2*>(shared) + (kTeams - 1) * kWaves * 64 * 32;
+    __syncthreads();
+    if (team > 0) {
+      const int to = (team - 1) * kWaves + wave;
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+#pragma unroll
+        for (int x = 0; x < 16; x += 4)
+          so[(to * 16 + 4 * n + x / 4) * 64 + ln] =
+              make_float4(sum.o[n][x], sum.o[n][x + 1], sum.o[n][x + 2], sum.o[n][x + 3]);
+      sml[to * 64 + ln] = make_float2(sum.m, sum.l);
+    }
+    __syncthreads();
+    if (team > 0) return;
+    float m = sum.m;
+    float2 ml[kTeams - 1];
+#pragma unroll
+    for (int t = 0; t < kTeams - 1; ++t) {
+      ml[t] = sml[(t * kWaves + wave) * 64 + ln];
+      m = vmax(m, ml[t].x);
+    }
+    share[0] = sum.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((sum.m - m) * a.c);
+    sum.m = m;
+    sum.l *= share[0];
+#pragma unroll
+    for (int t = 0; t < kTeams - 1; ++t) {
+      share[t + 1] = ml[t].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ml[t].x - m) * a.c);
+      sum.l += ml[t].y * share[t + 1];
+    }
+  }
+  asm("" : "+v"(ln));
+  const Row row = row_at(a, q, kvh, row0 + 32 * wave + (ln & 31));
   const float l = swap_add(sum.l), inv = inverse(l);
   float* rec = a.ws + a.big_base + ((((int64_t)wg.left * a.NKV + kvh) * kWaves + wave) * a.big_splits + wg.z) * kRecord;
 #pragma unroll
   for (int n = 0; n < 4; ++n) {
     float o[16];
 #pragma unroll
-    for (int x = 0; x < 16; ++x) o[x] = sum.o[n][x];
+    for (int x = 0; x < 16; ++x) o[x] = kTeams == 1 ? sum.o[n][x] : sum.o[n][x] * share[0];
+#pragma unroll
+    for (int t = 1; t < kTeams; ++t)
+#pragma unroll
+      for (int x = 0; x < 16; x += 4) {
+        const float4 y = so[(((t - 1) * kWaves + wave) * 16 + 4 * n + x / 4) * 64 + ln];
+        o[x] += y.x * share[t];
+        o[x + 1] += y.y * share[t];
+        o[x + 2] += y.z * share[t];
+        o[x + 3] += y.w * share[t];
+      }
     if (splits == 1) store_dims(a, row, n, ln >> 5, inv, o);
     else keep_dims(rec, n, ln, row.mine, o);
   }
@@ -891,9 +955,10 @@ __global__ __launch_bounds__(256, kSets == 1 ? 3 : 2) void chunk_few_kernel(Args
   few_unit<kSets>(a, sm, rest % a.R, blockIdx.x % a.NKV, rest / a.R);
 }
 
-__global__ __launch_bounds__(256, 3) void chunk_big_kernel(Args a) {
-  __shared__ __align__(1024) uint16_t sm[2 * kRing * kTileElems];
-  big_unit(a, sm, blockIdx.x / a.NKV, blockIdx.x % a.NKV);
+template <int kTeams>
+__global__ __launch_bounds__(256 * kTeams, 3) void chunk_big_kernel(Args a) {
+  __shared__ __align__(1024) uint16_t sm[kTeams * 2 * kRing * kTileElems];
+  big_unit<kTeams>(a, sm, blockIdx.x / a.NKV, blockIdx.x % a.NKV);
 }
 
 // Requests of both kinds: a workgroup for each CU of the one kind, then of the other, as
@@ -908,7 +973,7 @@ __global__ __launch_bounds__(256, 3) void chunk_both_kernel(Args a, int few, int
   const int u = (g < 2 * turns ? g >> 1 : g - turns) * kCUs + blockIdx.x % kCUs;
   if (u >= (is_big ? big : few)) return;
   const int rest = u / a.NKV, kvh = u - rest * a.NKV;
-  if (is_big) big_unit(a, reinterpret_cast<uint16_t*>(sm), rest, kvh);
+  if (is_big) big_unit<1>(a, reinterpret_cast<uint16_t*>(sm), rest, kvh);
   else few_unit<1>(a, *reinterpret_cast<FewShared<1>*>(sm), rest % a.R, kvh, rest / a.R);
 }
 
@@ -984,7 +1049,7 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(Args a, int few_units) 
 
 // How a call is split up.
 struct Plan {
-  bool big;
+  bool big, teams;
   int few_rows;                           // 0 where no request is taken as one of few rows
   int few_per, few_splits, big_slots, big_splits, big_over;
   int64_t few_blocks, big_blocks;         // workgroups
@@ -1036,11 +1101,21 @@ Plan plan_for(int N, int R, int max_new, int64_t max_ctx, int NH, int NKV, int w
     double best = 1e30;
     for (int s = 1; s <= kMaxSplits && (s == 1 || (n / s >= kLeastSplit && s * over * NKV <= kMostRecords)); ++s) {
       const double t = rounds((left * s + kCUs - 1) / kCUs) * ((double)n / s + (s > 1 ? 10 : 0));
+      // One request with less than a round of them: three teams a workgroup, one on a CU.
+      // Their common barrier costs some 5 %, a start and the teams' sums as much as 6 tiles.
+      const double teams = (left * s + kCUs - 1) / kCUs * ((double)n / s + (s > 1 ? 16 : 6)) * 1.05;
       if (t < best) {
         best = t;
         p.big_splits = s;
+        p.teams = false;
+      }
+      if (R == 1 && all * NKV < p.big_slots && teams < best) {
+        best = teams;
+        p.big_splits = s;
+        p.teams = true;
       }
     }
+    if (p.teams) p.big_slots = 1 << 30;
     p.big_over = (int)over;
     p.big_blocks = (most + (p.big_splits - 1) * over) * NKV;
     if (p.big_splits > 1) p.big_units = over * NKV * kWaves;
@@ -1128,7 +1203,8 @@ extern "C" int pdk_chunk_attn(const uint16_t* q, int64_t q_tok_stride, const uin
     hipLaunchKernelGGL(chunk_both_kernel, dim3(kCUs * turns), dim3(256), 0, st, a, (int)p.few_blocks,
                        (int)p.big_blocks);
   } else if (p.big) {
-    hipLaunchKernelGGL(chunk_big_kernel, dim3((unsigned)p.big_blocks), dim3(256), 0, st, a);
+    hipLaunchKernelGGL(p.teams ? chunk_big_kernel<3> : chunk_big_kernel<1>, dim3((unsigned)p.big_blocks),
+                       dim3(p.teams ? 768 : 256), 0, st, a);
   } else {
     hipLaunchKernelGGL(two ? chunk_few_kernel<2> : chunk_few_kernel<1>, dim3((unsigned)p.few_blocks),
                        dim3(256), 0, st, a);

@@ -54,13 +54,14 @@ def attention(q, ck, cv, tables, new, ctx, window, sinks, scale):
     out = torch.zeros(q.shape, dtype=torch.float64, device=dev)
     bound, at = torch.zeros_like(out), 0
     for r, (n, c) in enumerate(zip(new, ctx)):
-        if n == 0:
+        if n == 0 or c == 0:              # nothing asks, or nothing is there to be seen: zeros
+            at += n
             continue
         held = min(-(-c // 16), tables.shape[1])
         ids = [int(i) if 0 <= i < nb else -1 for i in tables[r, :held]]
         t = torch.arange(16 * held, device=dev)
-        there = torch.tensor(ids, device=dev).repeat_interleave(16) >= 0
-        idx = torch.tensor([max(i, 0) for i in ids], device=dev)
+        there = torch.tensor(ids, dtype=torch.int64, device=dev).repeat_interleave(16) >= 0
+        idx = torch.tensor([max(i, 0) for i in ids], dtype=torch.int64, device=dev)
         k = k_block_rows(ck[idx]).permute(1, 0, 2, 3).reshape(H, -1, D).double()
         v = cv[idx].permute(1, 0, 3, 2).reshape(H, -1, D).double()
         p = torch.arange(c - n, c, device=dev)[:, None]

@@ -241,6 +241,17 @@ def test_rows_behind_the_last_request_stay(cuda):
         assert torch.equal(out[:N], _attend(q, ck, cv, tables, lens))
 
 
+@pytest.mark.parametrize("lens", [[(-60, 100)], [(-60, 100), (5, 1)], [(-3, 4), (9, 2)], [(-9, 9)]])
+def test_contexts_shorter_than_the_new_tokens(cuda, lens):
+    """Tokens at positions below 0 see nothing."""
+    rng = np.random.default_rng(13)
+    q, ck, cv, tables, ctx = _operands(rng, 32, 8, lens, width=4)
+    want, bound = ref.attention(q, ck, cv, tables, [n for _, n in lens], ctx, 0, 0, SCALE)
+    got = _attend(q, ck, cv, tables, lens, max_ctx=64)
+    assert not got[:min(-lens[0][0], lens[0][1])].any()
+    ref.within(got, want, bound)
+
+
 def test_scores_far_apart(cuda):
     """Weights that underflow and maxima that grow along the context."""
     rng = np.random.default_rng(5)
