@@ -59,11 +59,15 @@ __global__ __launch_bounds__(256) void norm_fp8_kernel(const uint16_t* x, const 
   __shared__ float part[4];
   const int64_t row = blockIdx.x;
   const int n8 = H >> 3, tid = threadIdx.x;
-  v8 keep[kChunks], gain[kChunks];
+  // What the sum takes the place of is not read again: a stream leaves the caches to what is
+  // written (8192 x 4096: 39.6 us, without and with add behind the loop 46.9).
+  constexpr bool kSum = kNorm == 2;
+  v8 keep[kChunks], more[kChunks], gain[kChunks];
 #pragma unroll
   for (int j = 0; j < kChunks; ++j) {
     const int c = tid + 256 * j;
-    keep[j] = c < n8 ? pdk::ld16(x + row * ld + 8 * c) : pdk::zero8();
+    keep[j] = c < n8 ? pdk::ld16_as<kSum>(x + row * ld + 8 * c) : pdk::zero8();
+    if (kSum) more[j] = c < n8 ? pdk::ld16_stream(add + row * H + 8 * c) : pdk::zero8();
     if (kNorm) gain[j] = c < n8 ? pdk::ld16(w + 8 * c) : pdk::zero8();
   }
   float r = 1.f;
@@ -74,9 +78,9 @@ __global__ __launch_bounds__(256) void norm_fp8_kernel(const uint16_t* x, const 
       const int c = tid + 256 * j;
       float f[8];
       unpack(keep[j], f);
-      if (kNorm == 2 && c < n8) {
+      if (kSum && c < n8) {
         float g[8];
-        unpack(pdk::ld16(add + row * H + 8 * c), g);
+        unpack(more[j], g);
 #pragma unroll
         for (int k = 0; k < 4; ++k) keep[j].w[k] = pdk::pack_bf16x2_rne(f[2 * k] + g[2 * k], f[2 * k + 1] + g[2 * k + 1]);
         pdk::st16(sum + row * H + 8 * c, keep[j]);

@@ -66,6 +66,7 @@ def test_map(cuda, past, new, width, short, spare):
     (100, 5, 1, 999_983, "any"), (250, 40, 8, 3, "run"), (33, 6, 3, 12, "some"), (9, 32, 8, -4, "some"),
     (2000, 32, 8, 131_000, "run"), (24, 128, 16, 0, "run"),
     (1100, 6, 3, 7, "any"), (1500, 5, 5, 3, "some"), (300, 8, 2, 40, "pieces"), (1333, 12, 12, 0, "pieces"),
+    (5000, 32, 2, 9, "pieces"),           # a q past 32 MB
 ])
 def test_write(cuda, N, Hq, Hkv, first, kind):
     from rngd_pd_amd import kernels as K
