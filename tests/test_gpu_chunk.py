@@ -230,6 +230,28 @@ def test_hidden_values_that_are_not_finite(cuda, lens, odd):
     ref.within(_attend(q, ck, cv, tables, lens, window=n // 2 + 1), want, bound, "window")
 
 
+@pytest.mark.parametrize("past,new,window,sinks", [
+    (3500, 256, 0, 0), (4000, 1000, 0, 0), (3500, 256, 1500, 100), (3490, 251, 1, 0), (0, 1000, 0, 0),
+    (16001, 127, 0, 0)])
+def test_one_request_shared_by_teams(cuda, past, new, window, sinks):
+    """A request alone, its splits shared by teams of a workgroup: plain, with blocks missing
+    and with values that are not finite hidden and seen."""
+    print(f"one request {past} + {new} window={window}", flush=True)
+    rng = np.random.default_rng(past + new)
+    q, ck, cv, tables, ctx = _operands(rng, 32, 8, [(past, new)])
+    check = lambda what: ref.within(                                         # noqa: E731
+        _attend(q, ck, cv, tables, [(past, new)], window, sinks),
+        *ref.attention(q, ck, cv, tables, [new], ctx, window, sinks, SCALE), what)
+    check("plain")
+    tables[0, 3:40:6] = -1
+    tables[0, -1] = ck.shape[0]
+    check("missing blocks")
+    for t in range(past + 5, past + new, 61):
+        if (b := int(tables[0, t // 16])) >= 0 and b < ck.shape[0]:
+            cv[b, :, t % 7::9, t % 16] = (float("inf"), -float("inf"), float("nan"))[t % 3]
+    check("not finite")
+
+
 def test_rows_behind_the_last_request_stay(cuda):
     rng = np.random.default_rng(3)
     for lens in ([(100, 3), (20, 1)], [(100, 60), (20, 1)]):

@@ -175,6 +175,10 @@ def test_refusals(cuda):
     with pytest.raises(MemoryError):
         eng.step([("a", 0, [1] * 65)])
     assert cache.alloc.free_blocks() == 4
+    many = ChunkPrefill(w, cache, max_tokens=5000)
+    with pytest.raises(ValueError, match="4096 requests"):
+        many.step([(i, 0, [1]) for i in range(4097)])
+    assert cache.alloc.free_blocks() == 4
     with pytest.raises(ValueError, match="cache"):
         ChunkPrefill(w, PagedKVCache(1, 4, 2, 128, device=cuda))
     with pytest.raises(ValueError, match="max_tokens"):
