@@ -19,7 +19,7 @@
 // 16 tokens' places in a block are stored together. V lies dim by dim in the cache: where
 // eight tokens fill one half of a block, a lane transposes their 8 dims and stores 16
 // bytes for each; any other token is stored value by value. Bound by HBM where there are
-// many tokens (8192 with 32 + 16 heads: 41.8 us, 4.8 TB/s; V's are
+// many tokens (8192 with 32 + 16 heads: 39.8 us, 5.1 TB/s; V's are
 // pieces of 32 bytes), by one launch and a chain of three loads where there are few (16: 3.5 us).
 #include <math.h>
 
@@ -328,14 +328,15 @@ extern "C" int pdk_rope_cache_write(const uint16_t* qkv, int64_t ld, const float
                   pdk::aligned16(cache_v),
               "tensors must be 16-byte aligned");
   const int tiles = (N + kTok - 1) / kTok;
-  // Units apart until there are four workgroups for every CU. Where they would not come to
-  // one, V's tokens are apart too: one is then likely to lie alone, and a lane of few would
-  // store 8 of them value by value (48 heads, with 16 lanes and with 2: 3.5 and 6.7 us for 16
-  // tokens, 8.5 and 9.8 for 1024, 12.4 and 12.7 for 2048).
+  // Units apart until there are four workgroups for every CU, and in four parts at least (8192
+  // tokens: 39.8 us, in two 41.8). Up to 1024 tokens a token that lies alone in V's block, as
+  // single tokens do, has a lane of its own for 8 dims, stored value by value; beyond, a
+  // lane has 8 of them (48 heads, a lane each and a lane for 8: 3.5 and 6.7 us for 16 tokens,
+  // 8.5 and 9.8 for 1024, 12.4 and 12.7 for 2048).
   const bool few = tiles <= 64;
   const int units = (kTok * n_q_heads * 8 + kThreads - 1) / kThreads + (n_kv_heads + 1) / 2 +
                     (n_kv_heads * (few ? 16 : 2) + 15) / 16;
-  const int shares = std::min(units, std::max(1, (1024 + tiles - 1) / tiles));
+  const int shares = std::min(units, std::max(4, (1024 + tiles - 1) / tiles));
   // A q larger than the eight L2s passes them by (8192 tokens of 32 heads, 67 MB: 41.8 us, 50.4
   // through them; with the attention that reads it 109 and 108. 2048 tokens of 16 MB 13.3 both ways,
   // with the attention 36 and 35).
