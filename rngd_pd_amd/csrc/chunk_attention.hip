@@ -1005,8 +1005,9 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(Args a, int few_units) 
   const int G = a.NH / a.NKV;
   const int unit = blockIdx.x - few_units, at = unit / kWaves, left = at / a.NKV, kvh = at - left * a.NKV;
   const float* rec = a.ws + a.big_base + (int64_t)unit * a.big_splits * kRecord;
-  // Four splits' loads at a time, the last one again past the end; the first four before
-  // anything says how many there are.
+  // Four splits' loads at a time, the last one again past the end. One request's first four
+  // wait for nothing that says how many there are; of several requests fewer rows may be
+  // left over than there are records for.
   float2 ml[4];
   float4 y[4][4];
   auto load = [&](int z) __attribute__((always_inline)) {
@@ -1018,7 +1019,7 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(Args a, int few_units) 
       for (int x = 0; x < 4; ++x) y[i][x] = reinterpret_cast<const float4*>(from)[(4 * wave + x) * 64 + lane];
     }
   };
-  load(0);
+  if (a.R == 1) load(0);
   Big wg;
   if (!find_big<true>(a, left, wg)) return;
   const Request q = request(a, wg.r);
@@ -1033,7 +1034,7 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(Args a, int few_units) 
 #pragma unroll
   for (int x = 0; x < 16; ++x) o[x] = 0.f;
   for (int z = 0; z < splits; z += 4) {
-    if (z) load(z);
+    if (z || a.R > 1) load(z);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (z + i >= splits) ml[i].x = -INFINITY;
