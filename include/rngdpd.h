@@ -921,7 +921,8 @@ int pdk_swiglu_fp8(const uint16_t* gate_up, int64_t ld, int T, int M,
 /* y [T][N] bf16 = x . w^T: x [T] rows of K, x_ld bytes apart (a multiple of 16 below
  * 2^24), their scales at x_scales[t * xs_tok_stride + g * xs_group_stride] (token stride
  * below 2^21), w [N][K]. K a multiple of 128, N of 8. fp32 sums, rounded once (of the
- * products of 8 columns, what lies 2^-13 below the largest is cut). The workspace (16-byte aligned, 0 bytes for some sizes) serves one call at a time;
+ * products of 8 columns, what lies 2^-13 below the largest is cut). The workspace
+ * (16-byte aligned, 0 bytes for some sizes) serves one call at a time;
  * pdk_linear_fp8_workspace_bytes is -1 for sizes out of range. */
 int64_t pdk_linear_fp8_workspace_bytes(int T, int K, int N);
 int pdk_linear_fp8(const uint8_t* x, int64_t x_ld, const float* x_scales,

@@ -25,8 +25,8 @@
 // without the exponentials is 6 % faster, one without copies 11, one without the product with
 // V 21): a workgroup takes 128 rows, its four wavefronts (v_mfma_f32_32x32x16_bf16, 32
 // rows each) share tiles of 32 tokens staged into LDS two ahead by copies that pass no
-// register, one barrier per tile, three workgroups on a CU. 4096 tokens on 28000: 1820 to
-// 1890 us, 1070 to 1110 TFLOP/s, where library products of 8192^3 have 1290 to 1555.
+// register, one barrier per tile, three workgroups on a CU. 4096 tokens on 28000: 1740 to
+// 1800 us, 1120 to 1160 TFLOP/s, where library products of 8192^3 have 1290 to 1555.
 // With two wavefronts per SIMD and the next scores under the weights it was 2026 to 2107.
 //
 // Contexts are split over workgroups where those are few; a second launch joins the splits
@@ -867,7 +867,12 @@ __device__ __forceinline__ void big_unit(const Args& a, uint16_t* shared, int re
     ok_next >>= 2;
     v8 kr[8], va[2][4];
     load_k(st, kr);
+    // Scores before weights before the products with V, of the wavefronts that share a SIMD
+    // (4096 tokens on 28000 1891 us without, 1800 so; 6000 from the first on 305 and 282, 4000
+    // 147 and 153).
+    __builtin_amdgcn_s_setprio(2);
     f32x16 s = scores(kr, qv);
+    __builtin_amdgcn_s_setprio(1);
     __builtin_amdgcn_sched_barrier(0);                           // V into K's registers
     if (i + 2 < n_walk) ok_next |= fetch(next, i + 2) << 2;
     load_v(st, 0, va[0]);
@@ -881,6 +886,7 @@ __device__ __forceinline__ void big_unit(const Args& a, uint16_t* shared, int re
     v8 wt[2];
     weigh(s, a.c, sum, wt);
     load_v(st, 1, va[1]);
+    __builtin_amdgcn_s_setprio(0);
     if (edge) {
       bool found = false;
 #pragma unroll

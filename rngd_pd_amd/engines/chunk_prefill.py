@@ -126,8 +126,10 @@ class ChunkPrefill:
         if all_ids.min() < 0 or all_ids.max() >= cfg.vocab:
             raise ValueError(f"a token outside [0, {cfg.vocab})")
         # What the kernels would refuse is refused before the requests' blocks have grown.
-        if len(lens) > MAX_REQUESTS or max(p + n for _, p, n in lens) > MAX_CONTEXT:
-            raise ValueError(f"a step takes {MAX_REQUESTS} requests of {MAX_CONTEXT} tokens at most")
+        max_ctx = max(p + n for _, p, n in lens)
+        if len(lens) > MAX_REQUESTS or max_ctx > MAX_CONTEXT or len(lens) * -(-max_ctx // 16) >= 1 << 27:
+            raise ValueError(f"a step takes {MAX_REQUESTS} requests of {MAX_CONTEXT} tokens at most, "
+                             f"and tables of fewer than 2^27 entries")
         with torch.cuda.device(self.device):
             tables, free = cache.extend(lens)
             past, new, tables, free, tokens = self._upload(
@@ -135,7 +137,7 @@ class ChunkPrefill:
                  np.asarray([n for _, _, n in lens], np.int32), tables, free,
                  all_ids.astype(np.int32)])
             m = chunk_map(past, new, tables, free, N)
-            max_new, max_ctx = max(n for _, _, n in lens), max(p + n for _, p, n in lens)
+            max_new = max(n for _, _, n in lens)
             span = {"window": cfg.window, "sinks": min(cfg.sinks, max_ctx)} if cfg.window else {}
             x = w.embed.index_select(0, tokens)
             down = None
