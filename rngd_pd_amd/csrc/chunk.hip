@@ -19,7 +19,7 @@
 // 16 tokens' places in a block are stored together. V lies dim by dim in the cache: where
 // eight tokens fill one half of a block, a lane transposes their 8 dims and stores 16
 // bytes for each; any other token is stored value by value. Bound by HBM where there are
-// many tokens (8192 with 32 + 16 heads: 39.8 us, 5.1 TB/s; V's are
+// many tokens (8192 with 32 + 16 heads: 42.3 us, 4.8 TB/s; V's are
 // pieces of 32 bytes), by one launch and a chain of three loads where there are few (16: 3.5 us).
 #include <math.h>
 
@@ -184,8 +184,8 @@ __global__ __launch_bounds__(kThreads) void rope_write_kernel(
   auto load = [&](int u) __attribute__((always_inline)) {
     const Place p = place(u);
     const uint16_t* from = qkv + (int64_t)min(j0 + p.t, N - 1) * ld + (int64_t)p.head * kD + d;
-    a = pdk::ld16(from);
-    b = pdk::ld16(from + 64);
+    a = pdk::ld16_as<kStream>(from);
+    b = pdk::ld16_as<kStream>(from + 64);
   };
   // The first unit's values are under way while the angles are computed: those of its own
   // tokens where the workgroup has one unit, else of all.
@@ -337,9 +337,9 @@ extern "C" int pdk_rope_cache_write(const uint16_t* qkv, int64_t ld, const float
   const int units = (kTok * n_q_heads * 8 + kThreads - 1) / kThreads + (n_kv_heads + 1) / 2 +
                     (n_kv_heads * (few ? 16 : 2) + 15) / 16;
   const int shares = std::min(units, std::max(4, (1024 + tiles - 1) / tiles));
-  // A q larger than the eight L2s passes them by (8192 tokens of 32 heads, 67 MB: 41.8 us, 50.4
-  // through them; with the attention that reads it 109 and 108. 2048 tokens of 16 MB 13.3 both ways,
-  // with the attention 36 and 35).
+  // q and k of more than the eight L2s pass them by, read and written (8192 tokens with 48 heads
+  // over three sets of tensors in turn: 42.3 us, q's stores alone 46.7, none 50.3; with the product
+  // before and the attention behind 283, 285, 289; 5000 tokens 187, 188, 185).
   const auto kern = few ? rope_write_kernel<16, false>
                     : (int64_t)N * n_q_heads * kD * 2 > (32 << 20) ? rope_write_kernel<2, true>
                                                                    : rope_write_kernel<2, false>;
