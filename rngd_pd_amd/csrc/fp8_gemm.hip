@@ -320,8 +320,14 @@ __global__ __launch_bounds__(64 * kNW) void fp8_few_kernel(Args a) {
     uint4 w[kRT][2], x[2];
     float xs, ws;
   };
+  // Every workgroup begins at another group: rows lie a power of two apart, and at the same
+  // columns they all ask the same channels of the memory (28672 x 4096 26.0 us, so 23.2; 4096
+  // x 14336 14.6 and 14.9).
+  const int first = (int)(blockIdx.x * (kNW + 1) % groups);
   auto load = [&](int g) __attribute__((always_inline)) {
     Operands o;
+    g += first;
+    if (g >= groups) g -= groups;
     const int64_t at = (int64_t)g * kGroup;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
