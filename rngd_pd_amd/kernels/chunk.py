@@ -185,6 +185,19 @@ def chunk_workspace_bytes(N, R, max_new, max_ctx, n_q_heads, n_kv_heads, window=
     return need
 
 
+def _refuse_attention(q, cache_k, cache_v, block_tables, starts, ctx_lens):
+    """Raises for operands that chunk_attention's own test did not pass."""
+    dev = q.device
+    _need(q, "q")
+    D = _check_layer_cache(cache_k, cache_v)[2]
+    need_device(dev, cache_k, "cache_k")
+    need_device(dev, cache_v, "cache_v")
+    _int32(block_tables, "block_tables", dev, 2)
+    _int32(starts, "starts", dev)
+    _int32(ctx_lens, "ctx_lens", dev)
+    raise ValueError(f"q must be [N, Hq, {D}], got {tuple(q.shape)}")
+
+
 def chunk_attention(q, cache_k, cache_v, block_tables, starts, ctx_lens, max_new, max_ctx,
                     scale=1.0, window=None, sinks=0, out=None, workspace=None, stream=None):
     """Causal GQA attention of every request's new tokens over all it has in one
@@ -209,11 +222,23 @@ def chunk_attention(q, cache_k, cache_v, block_tables, starts, ctx_lens, max_new
         with launch_scope(dev, stream):
             return chunk_attention(q, cache_k, cache_v, block_tables, starts, ctx_lens, max_new,
                                    max_ctx, scale, window, sinks, out, workspace)
-    _need(q, "q")
-    nb, H, D = _check_layer_cache(cache_k, cache_v)
-    need_device(dev, cache_k, "cache_k")
-    need_device(dev, cache_v, "cache_v")
-    if q.dim() != 3 or q.shape[2] != D:
+    # The usual operands pass one test; what does not is told apart.
+    if not (isinstance(cache_k, torch.Tensor) and isinstance(cache_v, torch.Tensor)
+            and isinstance(block_tables, torch.Tensor) and isinstance(starts, torch.Tensor)
+            and isinstance(ctx_lens, torch.Tensor)
+            and q.dtype is cache_k.dtype is cache_v.dtype is BF16
+            and block_tables.dtype is starts.dtype is ctx_lens.dtype is torch.int32
+            and cache_k.device == cache_v.device == block_tables.device == starts.device
+            == ctx_lens.device == dev
+            and q.dim() == 3 and cache_k.dim() == cache_v.dim() == 4 and block_tables.dim() == 2
+            and starts.dim() == ctx_lens.dim() == 1
+            and cache_k.is_contiguous() and cache_v.is_contiguous() and block_tables.is_contiguous()
+            and starts.is_contiguous() and ctx_lens.is_contiguous()):
+        _refuse_attention(q, cache_k, cache_v, block_tables, starts, ctx_lens)
+    nb, H, size, D = cache_k.shape
+    if size != 16 or cache_v.shape != (nb, H, D, 16):
+        _check_layer_cache(cache_k, cache_v)
+    if q.shape[2] != D:
         raise ValueError(f"q must be [N, Hq, {D}], got {tuple(q.shape)}")
     if D != HEAD_DIM:
         raise ValueError(f"head_dim must be {HEAD_DIM}, got {D}")
@@ -225,9 +250,6 @@ def chunk_attention(q, cache_k, cache_v, block_tables, starts, ctx_lens, max_new
             or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)
         ld = Hq * D
-    _int32(block_tables, "block_tables", dev, 2)
-    _int32(starts, "starts", dev)
-    _int32(ctx_lens, "ctx_lens", dev)
     R, W = block_tables.shape
     if starts.numel() != R + 1 or ctx_lens.numel() != R:
         raise ValueError(f"starts and ctx_lens must hold {R + 1} and {R} entries")

@@ -36,10 +36,7 @@ def _rows_of(t, name, dev, width=None):
 
 
 def _outputs(out, T, K, dev, others):
-    """(values [T, K] e4m3, scales [T, K / 128] float32), new or the caller's."""
-    if out is None:
-        return (torch.empty((T, K), dtype=FP8, device=dev),
-                torch.empty((K // GROUP, T), dtype=torch.float32, device=dev).t())
+    """(values [T, K] e4m3, scales [T, K / 128] float32) of the caller's."""
     values, scales = out
     _need(values, "out values", FP8)
     _need(scales, "out scales", torch.float32)
@@ -131,11 +128,19 @@ def _quantized(entry, x, gated, out, stream):
     if stream is not None or dev.index != _current_device():
         with launch_scope(dev, stream):
             return _quantized(entry, x, gated, out, None)
-    x, T, K, ld = _rows_of(x, "x", dev)
+    if x.dtype is BF16 and x.dim() == 2 and x.is_contiguous() and x.data_ptr() % 16 == 0 \
+            and x.shape[1] % 8 == 0:
+        (T, K), ld = x.shape, x.shape[1]
+    else:
+        x, T, K, ld = _rows_of(x, "x", dev)
     K, rest = divmod(K, 2) if gated else (K, 0)
     if rest or K % GROUP or K < GROUP:
         raise ValueError(f"the columns must be a multiple of {GROUP}{' for each half' * gated}")
-    values, scales = _outputs(out, T, K, dev, [x])
+    if out is None:
+        values = torch.empty((T, K), dtype=FP8, device=dev)
+        scales = torch.empty_strided((T, K // GROUP), (1, T), dtype=torch.float32, device=dev)
+    else:
+        values, scales = _outputs(out, T, K, dev, [x])
     if T:
         _lib.call(entry, x.data_ptr(), ld, T, K, values.data_ptr(), scales.data_ptr(), T,
                   stream_handle())
