@@ -881,7 +881,8 @@ int pdk_rope_cache_write(const uint16_t* qkv, int64_t ld, const float* inv_freq,
 /* Causal GQA attention of the new tokens: rows starts[r] .. starts[r + 1] - 1 of q [N] (n of
  * them, rows of [Hq][128], q_tok_stride elements apart) stand at positions ctx_lens[r] - n
  * + i and see the cached tokens up to their own, with window > 0 those of the last window
- * positions and the first sinks. Tokens of blocks that the table does not name are seen by
+ * positions and the first sinks. Tokens beyond row N - 1 are left out, the others stand
+ * where they are. Tokens of blocks that the table does not name are seen by
  * nobody; a token that sees nothing gets zeros. out [N][Hq][128]; rows of no request are
  * left as they are. max_new and max_ctx are at least any request's. head_dim 128, Hq / Hkv
  * from 1 to 16, max_blocks <= 65535, N <= 2^20. The workspace (16-byte aligned) serves

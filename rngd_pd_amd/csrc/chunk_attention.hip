@@ -105,17 +105,19 @@ __device__ __forceinline__ float swap_add(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// A request's new tokens as far as the tensors hold them.
+// A request's new tokens as far as q has rows for them: n of them from row `start` on, the
+// first at position `past`. The others count for the positions all the same: token i of the
+// whole request stands at ctx - (e - s) + i, cut off or not.
 struct Request {
   int start, n, past;
 };
 
 __device__ __forceinline__ Request request(const Args& a, int r) {
-  const int s = a.starts[r], e = a.starts[r + 1];
   Request q;
-  q.start = min(max(s, 0), a.N);
-  q.n = max(min(e, a.N) - q.start, 0);
-  q.past = min(max(a.ctx[r], 0), 1 << 30) - q.n;
+  q.start = min(max(a.starts[r], 0), a.N);
+  const int e = min(max(a.starts[r + 1], q.start), 1 << 30);
+  q.n = min(e, a.N) - q.start;
+  q.past = min(max(a.ctx[r], 0), 1 << 30) - (e - q.start);
   return q;
 }
 

@@ -209,7 +209,8 @@ def chunk_attention(q, cache_k, cache_v, block_tables, starts, ctx_lens, max_new
     the new tokens (chunk_map's). ``max_new`` and ``max_ctx`` (<= max_blocks * 16) are
     at least any request's new tokens and context. Token i of n stands at position p =
     ctx - n + i and sees the tokens t <= p; with ``window`` those with t > p - window
-    or t < ``sinks``. Tokens in blocks that the table does not name (-1, or past it)
+    or t < ``sinks``. Tokens beyond q's last row are left out, as chunk_map leaves out
+    those beyond ``max_tokens``; the others stand where they are. Tokens in blocks that the table does not name (-1, or past it)
     are seen by nobody, and a token that sees nothing gets zeros. Rows behind the last
     request are left as they are. Any Hq/Hkv up to 16. fp32 between the products; a
     weight is rounded to bf16 once, as the product's operand. ``workspace``: device
