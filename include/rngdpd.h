@@ -871,7 +871,8 @@ int pdk_chunk_map(const int32_t* past, const int32_t* added, int R,
 /* RoPE at positions [N] (below 0: 0) and the keys and values into slots [N] (block * 16
  * + place; outside the cache: not written) of one layer's cache. qkv [N] rows of [Hq + 2
  * Hkv][128] bf16, ld elements apart (a multiple of 8); q_out [N][Hq][128]. head_dim 128.
- * The angle is position * inv_freq, exact before its cosine and sine. */
+ * The angle is position * inv_freq, exact before its cosine and sine. q_out and the caches
+ * overlap neither each other nor what the call reads. */
 int pdk_rope_cache_write(const uint16_t* qkv, int64_t ld, const float* inv_freq,
                          const int32_t* positions, const int32_t* slots, int N,
                          int n_q_heads, int n_kv_heads, int head_dim,

@@ -690,14 +690,8 @@ extern "C" int pdk_beam_select(const void* logits, int elem_bytes, int64_t ld, i
   const int rows = R * K;
   // A request's workgroup reads its beams' scores and last tokens before it writes, and
   // others' not at all: an output may lie place for place where they do.
-  struct Range {
-    const void* p;
-    int64_t bytes;
-  };
-  auto overlap = [](const Range& a, const Range& b) {
-    const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
-    return a.p && b.p && x < y + b.bytes && y < x + a.bytes;
-  };
+  using pdk::Range;
+  using pdk::overlap;
   const int64_t outs = (int64_t)R * n * 4;
   const Range in[2] = {{scores, (int64_t)rows * 4}, {last_tokens, (int64_t)rows * 4}};
   const Range out[3] = {{tokens, outs}, {parents, outs}, {out_scores, outs}};

@@ -327,6 +327,14 @@ extern "C" int pdk_rope_cache_write(const uint16_t* qkv, int64_t ld, const float
   PDK_REQUIRE(pdk::aligned16(qkv) && pdk::aligned16(q_out) && pdk::aligned16(cache_k) &&
                   pdk::aligned16(cache_v),
               "tensors must be 16-byte aligned");
+  const int64_t width = (int64_t)(n_q_heads + 2 * n_kv_heads) * kD, cache = (int64_t)num_blocks * n_kv_heads * 16 * kD;
+  const pdk::Range out[3] = {{q_out, (int64_t)N * n_q_heads * kD * 2}, {cache_k, cache * 2}, {cache_v, cache * 2}};
+  const pdk::Range in[4] = {{qkv, ((N - 1) * ld + width) * 2}, {inv_freq, kD / 2 * 4}, {positions, N * 4ll}, {slots, N * 4ll}};
+  for (int o = 0; o < 3; ++o) {
+    for (int p = 0; p < o; ++p) PDK_REQUIRE(!pdk::overlap(out[o], out[p]), "q_out and the caches must not overlap");
+    for (const pdk::Range& i : in)
+      PDK_REQUIRE(!pdk::overlap(out[o], i), "q_out and the caches must not overlap what the call reads");
+  }
   const int tiles = (N + kTok - 1) / kTok;
   // Units apart until there are four workgroups for every CU, and in four parts at least (8192
   // tokens: 39.8 us, in two 41.8). Up to 1024 tokens a token that lies alone in V's block, as

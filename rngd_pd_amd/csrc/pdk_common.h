@@ -23,6 +23,17 @@ inline hipStream_t as_stream(uintptr_t s) { return reinterpret_cast<hipStream_t>
 inline hipEvent_t as_event(uintptr_t e) { return reinterpret_cast<hipEvent_t>(e); }
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// Memory of an operand, and whether two have bytes in common (one that is absent has none).
+struct Range {
+  const void* p;
+  int64_t bytes;
+};
+
+inline bool overlap(const Range& a, const Range& b) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
+  return a.p && b.p && x < y + b.bytes && y < x + a.bytes;
+}
+
 // 8 bf16 values in one 16-byte register group: word w holds elements 2w (low
 // half) and 2w+1 (high half).
 struct v8 {

@@ -92,7 +92,7 @@ def rope_cache_write(qkv, inv_freq, positions, slots, cache_k, cache_v, n_q_head
     slot lies outside the cache is not written; a position below 0 counts as 0. The
     angle is position * inv_freq exactly (rope_cache_append rounds it to 32 bits).
     Slots are different: of two tokens for one slot either may be left, or parts of
-    both."""
+    both. Neither q_out nor the caches overlap another tensor of the call."""
     if not isinstance(qkv, torch.Tensor) or not qkv.is_cuda:
         raise TypeError("qkv must be a CUDA tensor")
     dev = qkv.device
