@@ -861,7 +861,8 @@ int pdk_prefill_attn_window(const uint16_t* q, int64_t q_tok_stride,
  * added; positions and slots [max_tokens] of token starts[r] + i: past + i and its block *
  * 16 + its place (-1 without a block, and both -1 behind the last token); taken [1]: the
  * sum of need. Lengths outside [0, 16 max_blocks] count as the nearest. R <= 4096, R *
- * max_blocks < 2^27. */
+ * max_blocks < 2^27. The tables and the outputs overlap neither each other nor the
+ * lengths and the list. */
 int pdk_chunk_map(const int32_t* past, const int32_t* added, int R,
                   int32_t* tables, int max_blocks, const int32_t* free_ids,
                   int n_free, int max_tokens, int32_t* starts,

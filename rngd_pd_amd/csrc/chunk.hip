@@ -298,6 +298,17 @@ extern "C" int pdk_chunk_map(const int32_t* past, const int32_t* added, int R, i
   PDK_REQUIRE(past && added && tables && starts && ctx_lens && taken && (n_free == 0 || free_ids) &&
                   (max_tokens == 0 || (positions && slots)),
               "null pointer argument");
+  const int64_t tokens = max_tokens * 4ll;
+  const pdk::Range out[6] = {{tables, (int64_t)R * max_blocks * 4}, {starts, (R + 1) * 4ll},
+                             {ctx_lens, R * 4ll}, {positions, tokens}, {slots, tokens}, {taken, 4}};
+  const pdk::Range in[3] = {{past, R * 4ll}, {added, R * 4ll}, {free_ids, n_free * 4ll}};
+  for (int o = 0; o < 6; ++o) {
+    for (int p = 0; p < o; ++p)
+      PDK_REQUIRE(!pdk::overlap(out[o], out[p]), "the tables and the outputs must not overlap");
+    for (const pdk::Range& i : in)
+      PDK_REQUIRE(!pdk::overlap(out[o], i),
+                  "the tables and the outputs must not overlap what the call reads");
+  }
   const int grid = std::max((max_tokens + kThreads - 1) / kThreads, 1);
   hipLaunchKernelGGL(chunk_map_kernel, dim3(grid), dim3(kThreads), 0, pdk::as_stream(stream), past,
                      added, R, tables, max_blocks, free_ids, n_free, max_tokens, starts, ctx_lens,
@@ -327,9 +338,14 @@ extern "C" int pdk_rope_cache_write(const uint16_t* qkv, int64_t ld, const float
   PDK_REQUIRE(pdk::aligned16(qkv) && pdk::aligned16(q_out) && pdk::aligned16(cache_k) &&
                   pdk::aligned16(cache_v),
               "tensors must be 16-byte aligned");
-  const int64_t width = (int64_t)(n_q_heads + 2 * n_kv_heads) * kD, cache = (int64_t)num_blocks * n_kv_heads * 16 * kD;
-  const pdk::Range out[3] = {{q_out, (int64_t)N * n_q_heads * kD * 2}, {cache_k, cache * 2}, {cache_v, cache * 2}};
-  const pdk::Range in[4] = {{qkv, ((N - 1) * ld + width) * 2}, {inv_freq, kD / 2 * 4}, {positions, N * 4ll}, {slots, N * 4ll}};
+  const int64_t width = (int64_t)(n_q_heads + 2 * n_kv_heads) * kD;
+  const int64_t cache = (int64_t)num_blocks * n_kv_heads * 16 * kD;
+  const pdk::Range out[3] = {
+      {q_out, (int64_t)N * n_q_heads * kD * 2}, {cache_k, cache * 2}, {cache_v, cache * 2}};
+  const pdk::Range in[4] = {{qkv, ((N - 1) * ld + width) * 2},
+                            {inv_freq, kD / 2 * 4},
+                            {positions, N * 4ll},
+                            {slots, N * 4ll}};
   for (int o = 0; o < 3; ++o) {
     for (int p = 0; p < o; ++p) PDK_REQUIRE(!pdk::overlap(out[o], out[p]), "q_out and the caches must not overlap");
     for (const pdk::Range& i : in)

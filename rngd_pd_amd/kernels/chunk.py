@@ -48,7 +48,7 @@ def chunk_map(past, new, tables, free, max_tokens, stream=None):
     more than F the entries and slots left over are -1 (rope_cache_write skips those
     tokens, chunk_attention hides them), so a caller that cannot know compares.
     ``max_tokens``: the length of positions and slots, at least the sum of ``new``;
-    tokens beyond it are left out."""
+    tokens beyond it are left out. ``tables`` overlaps none of the others."""
     if not isinstance(tables, torch.Tensor) or not tables.is_cuda:
         raise TypeError("tables must be a CUDA tensor")
     dev = tables.device

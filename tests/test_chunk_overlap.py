@@ -33,3 +33,29 @@ def test_write_takes(kw):
 def test_write_refuses(kw):
     assert _write(**kw) == _lib.PDK_EINVAL
     assert "overlap" in _lib.last_error()
+
+
+R, W, FREE = 3, 8, 20
+TABLES = R * W * 4
+
+
+def _map(n_free=FREE, **kw):
+    a = {**AT, **kw}
+    return _lib.lib().pdk_chunk_map(a["past"], a["added"], R, a["tables"], W, a["free"], n_free, N, a["starts"],
+                                    a["ctx"], a["pos"], a["slots"], a["taken"], 0)
+
+
+@pytest.mark.parametrize("kw", [
+    {}, dict(added=AT["past"]), dict(past=AT["tables"] + TABLES), dict(free=AT["tables"] - FREE * 4),
+    dict(n_free=0, free=AT["tables"] + 4), dict(ctx=AT["starts"] + 4 * (R + 1)), dict(free=AT["past"])])
+def test_map_takes(kw):
+    assert _map(**kw) == _lib.PDK_EHIP
+
+
+@pytest.mark.parametrize("kw", [
+    dict(past=AT["tables"]), dict(added=AT["tables"] + TABLES - 4), dict(free=AT["tables"] - FREE * 4 + 4),
+    dict(starts=AT["past"]), dict(ctx=AT["starts"] + 4 * R), dict(slots=AT["pos"]), dict(taken=AT["tables"]),
+    dict(pos=AT["free"])])
+def test_map_refuses(kw):
+    assert _map(**kw) == _lib.PDK_EINVAL
+    assert "overlap" in _lib.last_error()
