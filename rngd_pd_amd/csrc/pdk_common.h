@@ -23,7 +23,8 @@ inline hipStream_t as_stream(uintptr_t s) { return reinterpret_cast<hipStream_t>
 inline hipEvent_t as_event(uintptr_t e) { return reinterpret_cast<hipEvent_t>(e); }
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-// Memory of an operand, and whether two have bytes in common (one that is absent has none).
+// Memory of an operand, and whether two have bytes in common (one that is absent or empty
+// has none).
 struct Range {
   const void* p;
   int64_t bytes;
@@ -31,7 +32,7 @@ struct Range {
 
 inline bool overlap(const Range& a, const Range& b) {
   const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
-  return a.p && b.p && x < y + b.bytes && y < x + a.bytes;
+  return a.p && b.p && a.bytes > 0 && b.bytes > 0 && x < y + b.bytes && y < x + a.bytes;
 }
 
 // 8 bf16 values in one 16-byte register group: word w holds elements 2w (low
