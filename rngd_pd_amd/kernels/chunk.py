@@ -270,6 +270,8 @@ def chunk_attention(q, cache_k, cache_v, block_tables, starts, ctx_lens, max_new
     window, sinks = check_window(window, sinks)
     ws_ptr, ws_bytes = None, 0
     if workspace is not None:
+        if not isinstance(workspace, torch.Tensor):
+            raise TypeError("workspace must be a CUDA tensor")
         need_device(dev, workspace, "workspace")
         ws_ptr, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
         if not workspace.is_contiguous() or ws_bytes < need or ws_ptr % 16:

@@ -66,7 +66,7 @@ def rmsnorm_fp8(x, weight, eps, add=None, sum_out=None, out=None, stream=None):
         with launch_scope(dev, stream):
             return rmsnorm_fp8(x, weight, eps, add, sum_out, out)
     for t, name in ((weight, "weight"), (add, "add"), (sum_out, "sum_out")):
-        if t is not None and not isinstance(t, torch.Tensor):
+        if not isinstance(t, torch.Tensor) and (t is not None or name == "weight"):
             raise TypeError(f"{name} must be a CUDA tensor")
     # The usual operands pass one test; what does not is told apart.
     xp, wp, ap, sp = x.data_ptr(), weight.data_ptr(), None, None
@@ -163,6 +163,8 @@ def quantize_weight_fp8(w):
     """w [N, K] (K a multiple of 128) in 8 bits, a scale for each block of 128 x 128 ->
     (values [N, K] e4m3, scales [ceil(N / 128), K / 128] float32). For the loading of a
     model: torch operations, some rows at a time."""
+    if not isinstance(w, torch.Tensor):
+        raise TypeError("w must be a tensor")
     if w.dim() != 2 or w.shape[1] % GROUP or 0 in w.shape:
         raise ValueError(f"w must be [N, K] with K a multiple of {GROUP}, got {tuple(w.shape)}")
     N, K = w.shape
@@ -209,9 +211,10 @@ def linear_fp8(x, x_scales, w, w_scales, out=None, workspace=None, stream=None):
     if stream is not None or dev.index != _current_device():
         with launch_scope(dev, stream):
             return linear_fp8(x, x_scales, w, w_scales, out, workspace)
-    if not (x.dtype is FP8 and w.dtype is FP8 and x_scales.dtype is torch.float32
-            and w_scales.dtype is torch.float32 and w.device == dev and x_scales.device == dev
-            and w_scales.device == dev):
+    if not (isinstance(w, torch.Tensor) and isinstance(x_scales, torch.Tensor)
+            and isinstance(w_scales, torch.Tensor) and x.dtype is FP8 and w.dtype is FP8
+            and x_scales.dtype is torch.float32 and w_scales.dtype is torch.float32
+            and w.device == dev and x_scales.device == dev and w_scales.device == dev):
         for t, name, dt in ((x, "x", FP8), (w, "w", FP8), (x_scales, "x_scales", torch.float32),
                             (w_scales, "w_scales", torch.float32)):
             _need(t, name, dt)
@@ -247,6 +250,8 @@ def linear_fp8(x, x_scales, w, w_scales, out=None, workspace=None, stream=None):
     need = linear_fp8_workspace_bytes(T, K, N)
     ws_ptr, ws_bytes = None, 0
     if workspace is not None:
+        if not isinstance(workspace, torch.Tensor):
+            raise TypeError("workspace must be a CUDA tensor")
         need_device(dev, workspace, "workspace")
         ws_ptr, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
         if not workspace.is_contiguous() or ws_bytes < need or ws_ptr % 16:

@@ -479,3 +479,25 @@ def test_refusals_of_the_wrappers(cuda):
     assert tuple(K.rope_cache_write(qkv[:0], inv, pos[:0], pos[:0], ck, cv, 8).shape) == (0, 8, D)
     m = K.chunk_map(past, new, tab.clone(), free[:0], 0)
     assert m.positions.numel() == 0 and m.starts.tolist() == [0, 3, 4]
+
+
+def test_operands_that_are_no_tensors(cuda):
+    """TypeError for each, whichever it is."""
+    from rngd_pd_amd import kernels as K
+    lens = [(3000, 100)]
+    q, ck, cv, tables, ctx = _operands(np.random.default_rng(0), 8, 2, lens)
+    tab, starts, ctx_d = torch.from_numpy(tables).to(cuda), _int32(_starts(lens), cuda), _int32(ctx, cuda)
+    inv, pos = torch.ones(64, device=cuda), _int32([0] * 100, cuda)
+    qkv = torch.zeros((100, 12 * D), dtype=torch.bfloat16, device=cuda)
+    attention = [q, ck, cv, tab, starts, ctx_d, 100, 3100]
+    calls = [lambda i=i: K.chunk_attention(*attention[:i], [1], *attention[i + 1:]) for i in range(6)]
+    calls += [lambda: K.chunk_attention(*attention, workspace=1 << 28), lambda: K.chunk_attention(*attention, out=[])]
+    write = [qkv, inv, pos, pos, ck, cv, 8]
+    calls += [lambda i=i: K.rope_cache_write(*write[:i], [1], *write[i + 1:]) for i in range(6)]
+    calls += [lambda: K.rope_cache_write(*write, q_out=[])]
+    lengths = [ctx_d, ctx_d, tab, pos, 100]
+    calls += [lambda i=i: K.chunk_map(*lengths[:i], [1], *lengths[i + 1:]) for i in range(4)]
+    for at, call in enumerate(calls):
+        print(at, flush=True)
+        with pytest.raises(TypeError):
+            call()

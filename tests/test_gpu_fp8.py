@@ -271,3 +271,20 @@ def test_refusals_of_the_wrappers(cuda):
     none, scales = Kn.rmsnorm_fp8(x[:0], w, EPS)
     assert tuple(none.shape) == (0, 256) and tuple(scales.shape) == (0, 2)
     assert tuple(Kn.linear_fp8(none, scales, w8, ws).shape) == (0, 64)
+
+
+def test_operands_that_are_no_tensors(cuda):
+    """TypeError for each, whichever it is."""
+    from rngd_pd_amd import kernels as Kn
+    q, s = Kn.quantize_fp8(_randn(1, 64, 8192))
+    w, ws = Kn.quantize_weight_fp8(_randn(3, 512, 8192))
+    for at, call in enumerate((
+            lambda: Kn.linear_fp8(q, [1.0], w, ws), lambda: Kn.linear_fp8(q, s, None, ws),
+            lambda: Kn.linear_fp8(q, s, w, 1.0), lambda: Kn.linear_fp8(q, s, w, ws, out=[]),
+            lambda: Kn.linear_fp8(q, s, w, ws, workspace=1 << 20),
+            lambda: Kn.linear_fp8(q, s, w, ws, workspace=bytearray(1 << 20)),
+            lambda: Kn.quantize_fp8([1.0]), lambda: Kn.quantize_fp8(_randn(1, 4, 128), out=(None, None)),
+            lambda: Kn.rmsnorm_fp8(_randn(1, 4, 128), None, EPS), lambda: Kn.quantize_weight_fp8([[1.0] * 128]))):
+        print(at, flush=True)
+        with pytest.raises(TypeError):
+            call()
