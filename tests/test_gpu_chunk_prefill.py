@@ -183,3 +183,49 @@ def test_refusals(cuda):
         ChunkPrefill(w, PagedKVCache(1, 4, 2, 128, device=cuda))
     with pytest.raises(ValueError, match="max_tokens"):
         ChunkPrefill(w, cache, max_tokens=0)
+
+
+def _near_best(tokens, rows, w, eps):
+    """Each token's logit among those of its hidden row in 64 bits: h, rounded to bf16
+    from 32 bits (norm and weight), is off by at most 2^-8 of itself and 2^-17 before
+    that; a logit's sum of H products by H 2^-24 of their magnitudes and its rounding by
+    2^-8; the largest and the token's may be off in opposite ways. How many rows have no
+    other token as near."""
+    x = rows.double()
+    h = x / torch.sqrt(x.square().mean(-1, keepdim=True) + eps) * w.norm_f.double()
+    head = w.lm_head.double().t().contiguous()
+    logits, size = h @ head, h.abs() @ head.abs()
+    off = (2.0 ** -8 + 2.0 ** -16 + x.shape[1] * 2.0 ** -24) * size + 2.0 ** -8 * logits.abs()
+    best = (logits - off).amax(1, keepdim=True)
+    near = logits + off >= best
+    assert near.gather(1, torch.tensor(tokens, device=x.device)[:, None]).all()
+    return int((near.sum(1) == 1).sum())
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_tokens_of_every_request(cuda, fp8):
+    """The tokens that a step returns, request by request: with ``every`` those after each
+    new token, without the last of them, and of its hidden rows the greedy ones."""
+    cfg, w = _model(cuda)
+    rng = np.random.default_rng(8)
+    cache = _cache(cfg, cuda)
+    eng = ChunkPrefill(w, cache, fp8=fp8)
+    eng.step([(r, 0, rng.integers(0, cfg.vocab, n).tolist()) for r, n in (("a", 40), ("c", 3))])
+    chunks = [(r, p, rng.integers(0, cfg.vocab, n).tolist())
+              for r, p, n in (("a", 40, 7), ("b", 0, 33), ("c", 3, 1), ("d", 0, 18))]
+    ends = np.cumsum([len(t) for *_, t in chunks])
+    every, rows = eng.step(chunks, every=True), eng.x.clone()
+    last, same = eng.step(chunks), eng.x.clone()
+    assert [len(t) for t in every] == [7, 33, 1, 18] and rows.shape == same.shape == (59, cfg.hidden)
+    # The same kernels and products on the same rows.
+    h = K.rmsnorm(rows, w.norm_f, cfg.eps)
+    want = K.greedy_argmax(torch.nn.functional.linear(h, w.lm_head)).tolist()
+    assert every == [want[e - len(t):e] for e, (*_, t) in zip(ends, chunks)]
+    h = K.rmsnorm(same[torch.tensor(ends - 1, device=cuda)].contiguous(), w.norm_f, cfg.eps)
+    assert last == K.greedy_argmax(torch.nn.functional.linear(h, w.lm_head)).tolist()
+    # In 64 bits.
+    assert _near_best(sum(every, []), rows, w, cfg.eps) > 0
+    alone = [_near_best([t], same[e - 1:e], w, cfg.eps) for t, e in zip(last, ends)]
+    if torch.equal(rows, same):
+        assert all(t[-1] == one for t, one, sure in zip(every, last, alone) if sure)
+    _near(same, rows, SHARE)
