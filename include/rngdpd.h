@@ -925,7 +925,7 @@ int pdk_swiglu_fp8(const uint16_t* gate_up, int64_t ld, int T, int M,
  * 2^24), their scales at x_scales[t * xs_tok_stride + g * xs_group_stride] (token stride
  * below 2^21), w [N][K]. K a multiple of 128, N of 8. fp32 sums, rounded once (of the
  * products of 8 columns, what lies 2^-13 below the largest is cut). The workspace
- * (16-byte aligned, 0 bytes for some sizes) serves one call at a time;
+ * (16-byte aligned, 0 bytes for some sizes, 512 MiB at most) serves one call at a time;
  * pdk_linear_fp8_workspace_bytes is -1 for sizes out of range. */
 int64_t pdk_linear_fp8_workspace_bytes(int T, int K, int N);
 int pdk_linear_fp8(const uint8_t* x, int64_t x_ld, const float* x_scales,

@@ -385,6 +385,9 @@ constexpr Shape kShapes[] = {
     {64, 128, 512, 0.54, 0.84},
 };
 
+// Items of a product whose K is split: the splits' sums take at most 2048 tiles of 256 KB, 512 MiB.
+constexpr int kMostItems = 2048;
+
 struct Plan {
   int shape, splits, per;                 // groups of a split
   int64_t bytes;                          // of the splits' sums
@@ -407,7 +410,7 @@ Plan plan_for(int T, int K, int N) {
       const int per = (groups + splits - 1) / splits;
       if (per * (splits - 1) >= groups) continue;              // the last one would be empty
       const int64_t items = tiles * splits, bytes = splits > 1 ? items * s.t * s.w * 4 : 0;
-      if (splits > 1 && items > 2048) break;
+      if (splits > 1 && items > kMostItems) break;
       const double rounds = (double)((items + s.at_once - 1) / s.at_once);
       const double us = rounds * (per * (items <= 256 ? s.alone : s.full) + 2.0) +
                         (splits > 1 ? 3.0 + 2.0 * bytes / 4.5e6 : 0.0);

@@ -183,8 +183,8 @@ def quantize_weight_fp8(w):
 
 @functools.lru_cache(maxsize=4096)
 def linear_fp8_workspace_bytes(T, K, N):
-    """Bytes of linear_fp8's workspace (0: it needs none); raises for sizes it does not
-    take."""
+    """Bytes of linear_fp8's workspace (0: it needs none; 512 MiB at most); raises for sizes
+    it does not take."""
     for v in (T, K, N):
         if not 0 <= v < 1 << 31:
             raise ValueError(f"size {v} outside [0, 2^31)")

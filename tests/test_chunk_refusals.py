@@ -165,3 +165,14 @@ def test_weights_in_8_bits():
     for bad in (w[:, :100], w[0], w[:0]):
         with pytest.raises(ValueError):
             K.quantize_weight_fp8(bad)
+
+
+def test_linear_workspaces_up_to_their_bound():
+    """512 MiB at most, as the header states, and sizes that come near it."""
+    size, most = K.linear_fp8_workspace_bytes, 0
+    for T in (17, 100, 300, 470, 700, 1000, 1500, 2000, 3000, 4096, 5000, 16384):
+        for N in (8, 4096, 6144, 8192, 14336, 28672, 57344):
+            for k in (4096, 14336, 28672, 57344, 1 << 17, 1 << 20):
+                most = max(most, size(T, k, N))
+    assert 500 << 20 <= most <= 512 << 20
+    assert size(5000, 28672, 8192) <= 320 << 20
