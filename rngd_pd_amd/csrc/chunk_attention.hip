@@ -64,7 +64,7 @@ constexpr int kMaxRequests = 65535;
 constexpr int kMaxSplits = 64;
 constexpr int kLeastSplit = 8;            // tiles of a split at least
 constexpr int kCUs = 256;
-constexpr int kMostRecords = 4096;        // of four units each
+constexpr int kMostRecords = 4096;        // of four units each, of longer requests: 277 MB
 constexpr int kRecord = 64 * 66;          // floats of a unit's sums: O 64 lanes x 64, (m, l)
 
 struct Args {
@@ -1119,7 +1119,7 @@ Plan plan_for(int N, int R, int max_new, int64_t max_ctx, int NH, int NKV, int w
                                 : std::min<int64_t>(most, p.big_slots / NKV + 1);
     // The split that ends soonest of the workgroups left over; each costs as much again as
     // ten tiles for its start, for handing over its sums (136 KB) and for the join. At most
-    // kMostRecords of them: 277 MB.
+    // kMostRecords of them; beside those of few rows, 768 of 9 KB, the workspace is 284 MB at most.
     double best = 1e30;
     for (int s = 1; s <= kMaxSplits && (s == 1 || (n / s >= kLeastSplit && s * over * NKV <= kMostRecords)); ++s) {
       const double t = rounds((left * s + kCUs - 1) / kCUs) * ((double)n / s + (s > 1 ? 10 : 0));

@@ -176,3 +176,16 @@ def test_linear_workspaces_up_to_their_bound():
                 most = max(most, size(T, k, N))
     assert 500 << 20 <= most <= 512 << 20
     assert size(5000, 28672, 8192) <= 320 << 20
+
+
+def test_attention_workspaces_up_to_their_bound():
+    """The records of longer requests (4096 of four units of 64 x 66 floats) and of those
+    of few rows beside them (768 of 2176 floats), 284 MB, and sizes that come near it."""
+    most = 0
+    for R in (1, 2, 16, 32, 64, 768, 4000):
+        for N in (40, 776, 3104, 6208, 8192, 1 << 20):
+            for hq, hkv in ((32, 8), (64, 4), (8, 8), (16, 1), (8, 1), (128, 8)):
+                for ctx in (4096, 1 << 17, 65535 * 16):
+                    most = max(most, K.chunk_workspace_bytes(N, R, N, ctx, hq, hkv))
+    bound = 4096 * 4 * 64 * 66 * 4 + 768 * 2176 * 4
+    assert 0.99 * bound <= most <= bound <= 284e6
