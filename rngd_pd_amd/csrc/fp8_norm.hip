@@ -41,11 +41,21 @@ __device__ __forceinline__ void store_group(const float (&y)[8], uint8_t* to, fl
 #pragma unroll
   for (int o = 1; o < 16; o <<= 1) top = vmax(top, __shfl_xor(top, o));
   const float s = vmax(top, kLeast) / kTop, r = 1.f / s;
+  // y / s rounded once: the product with 1 / s and what it leaves of y. Quotients of bf16
+  // values often lie right between two of 8 bits, where the product alone (rounded twice)
+  // goes to the wrong one. An infinite scale leaves nothing: 0 for what is finite.
+  const float left = s == INFINITY ? 0.f : s;
+  float z[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float q = y[e] * r;
+    z[e] = __builtin_fmaf(__builtin_fmaf(-q, left, y[e]), r, q);
+  }
   int lo = 0, hi = 0;
-  lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[0] * r, y[1] * r, lo, false);
-  lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[2] * r, y[3] * r, lo, true);
-  hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[4] * r, y[5] * r, hi, false);
-  hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[6] * r, y[7] * r, hi, true);
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32(z[0], z[1], lo, false);
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32(z[2], z[3], lo, true);
+  hi = __builtin_amdgcn_cvt_pk_fp8_f32(z[4], z[5], hi, false);
+  hi = __builtin_amdgcn_cvt_pk_fp8_f32(z[6], z[7], hi, true);
   *reinterpret_cast<int2*>(to) = make_int2(lo, hi);
   if ((threadIdx.x & 15) == 0) *scale = s;
 }

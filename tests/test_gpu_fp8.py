@@ -288,3 +288,18 @@ def test_operands_that_are_no_tensors(cuda):
         print(at, flush=True)
         with pytest.raises(TypeError):
             call()
+
+
+@pytest.mark.parametrize("T,K,std", [(1, 128, 1.0), (300, 4096, 2.0), (64, 1024, 1e-30), (64, 1024, 1e30)])
+def test_rows_are_divided_by_their_scales(cuda, T, K, std):
+    """The values are those of x / scale in 32 bits, rounded once more to 8, ties to the even
+    one: many quotients of two bf16 values lie right between two of 8 bits."""
+    from rngd_pd_amd import kernels as Kn
+    x = _randn(T + K, T, K, std=std)
+    x[0, 3], x[-1, 100] = 0, float("inf")                # the finite ones of that group: 0
+    values, scales = Kn.quantize_fp8(x)
+    quotients = x.float() / scales.repeat_interleave(128, 1)
+    got, want = values.float(), quotients.to(torch.float8_e4m3fn).float()
+    assert torch.equal(torch.isnan(got), torch.isnan(want)) and int(torch.isnan(want).sum()) == 1
+    off = (got != want) & ~torch.isnan(want)
+    assert not off.any(), (int(off.sum()), x[off][:4], quotients[off][:4], got[off][:4])
