@@ -117,6 +117,7 @@ class ChunkPrefill:
         The requests' blocks are grown in the cache; what stands behind the tokens given as
         there (a rejected draft's) is written over."""
         cfg, w, cache = self.cfg, self.w, self.cache
+        chunks = list(chunks)
         ids = [np.asarray(t, np.int64).reshape(-1) for _, _, t in chunks]
         lens = [(r, int(past), t.size) for (r, past, _), t in zip(chunks, ids)]
         N = sum(n for _, _, n in lens)

@@ -229,3 +229,13 @@ def test_tokens_of_every_request(cuda, fp8):
     if torch.equal(rows, same):
         assert all(t[-1] == one for t, one, sure in zip(every, last, alone) if sure)
     _near(same, rows, SHARE)
+
+
+def test_chunks_may_come_from_an_iterator(cuda):
+    """As PagedKVCache.extend takes them, and tokens as an array."""
+    cfg, w = _model(cuda)
+    tokens = np.random.default_rng(9).integers(0, cfg.vocab, 30)
+    one, two = (ChunkPrefill(w, _cache(cfg, cuda)) for _ in range(2))
+    want = one.step([("a", 0, tokens.tolist()), ("b", 0, [7])])
+    assert two.step((r, 0, t) for r, t in (("a", tokens), ("b", [7]))) == want
+    assert torch.equal(one.x, two.x)
