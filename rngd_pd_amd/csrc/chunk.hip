@@ -18,9 +18,10 @@
 // a head (two 16-byte loads and stores); lanes go through q in whole rows, through k so that
 // 16 tokens' places in a block are stored together. V lies dim by dim in the cache: where
 // eight tokens fill one half of a block, a lane transposes their 8 dims and stores 16
-// bytes for each; any other token is stored value by value. Bound by HBM where there are
-// many tokens (8192 with 32 + 16 heads: 42.3 us, 4.8 TB/s; V's are
-// pieces of 32 bytes), by one launch and a chain of three loads where there are few (16: 3.5 us).
+// bytes for each; any other token is stored value by value. Bound by memory where there
+// are many tokens (8192 with 32 + 16 heads, eager over several sets of tensors: 41.8 us, 4.8 TB/s
+// of the bytes that must move; HBM sees 2 % more), by one launch and a chain of three loads
+// where there are few (16: 3.5 us).
 #include <math.h>
 
 #include <algorithm>
@@ -353,7 +354,7 @@ extern "C" int pdk_rope_cache_write(const uint16_t* qkv, int64_t ld, const float
   }
   const int tiles = (N + kTok - 1) / kTok;
   // Units apart until there are four workgroups for every CU, and in four parts at least (8192
-  // tokens: 39.8 us, in two 41.8). Up to 1024 tokens a token that lies alone in V's block, as
+  // tokens, one set of tensors again and again: 39.8 us, in two 41.8). Up to 1024 tokens a token that lies alone in V's block, as
   // single tokens do, has a lane of its own for 8 dims, stored value by value; beyond, a
   // lane has 8 of them (48 heads, a lane each and a lane for 8: 3.5 and 6.7 us for 16 tokens,
   // 8.5 and 9.8 for 1024, 12.4 and 12.7 for 2048).

@@ -25,8 +25,8 @@
 // without the exponentials is 6 % faster, one without copies 11, one without the product with
 // V 21): a workgroup takes 128 rows, its four wavefronts (v_mfma_f32_32x32x16_bf16, 32
 // rows each) share tiles of 32 tokens staged into LDS two ahead by copies that pass no
-// register, one barrier per tile, three workgroups on a CU. 4096 tokens on 28000: 1740 to
-// 1800 us, 1120 to 1160 TFLOP/s, where library products of 8192^3 have 1290 to 1555.
+// register, one barrier per tile, three workgroups on a CU. 4096 tokens on 28000: 1750 to
+// 1850 us, 1090 to 1150 TFLOP/s, where library products of 8192^3 have 1290 to 1555.
 // With two wavefronts per SIMD and the next scores under the weights it was 2026 to 2107.
 //
 // Contexts are split over workgroups where those are few; a second launch joins the splits

@@ -22,7 +22,7 @@
 // come the same way (as vector loads of each wavefront 899, so 861). A tile's scaled addition
 // runs under the next tile's products (one after the other 1003, so 961).
 //
-// Bound by the matrix cores' power at the largest sizes: 861 to 890 us, 2160 to 2230
+// Bound by the matrix cores' power at the largest sizes: 870 to 900 us, 2140 to 2210
 // TFLOP/s, where the loop without any copy takes 737 and the library's product with one
 // scale for all 769. Smaller ones are bound by a group's chain (barrier, LDS read, two
 // products, addition), 0.54 to 1.5 us by tile, so that the tile and the split of K are chosen
@@ -341,7 +341,8 @@ __global__ __launch_bounds__(64 * kNW) void fp8_few_kernel(Args a) {
   };
   if (wave < groups) {
     // The next group's operands are under way as soon as this one's have been taken; more
-    // of them gained nothing (28672 x 4096, 16 rows: 26.9 us, two 29.1, three 31.9).
+    // of them gained nothing (28672 x 4096, 16 rows, before the starts at other groups: 26.9 us,
+    // two 29.1, three 31.9).
     Operands o = load(wave);
     for (int g = wave; g < groups; g += kNW) {
       const i32x8 x = join(o.x[0], o.x[1]);
@@ -395,10 +396,10 @@ struct Plan {
 
 // The shape and split that end soonest: rounds of workgroups, each its groups and 2 us for
 // its start and its store; where K is split another launch (3 us) and the splits' sums
-// written and read, 4.5 TB/s. Chosen and best measured, us: 64 x 4096 x 14336 (rows, weights,
-// columns) 64 x 128 split in 8 19.1, unsplit 57; 470 x 4096 x 14336 128 x 256 in 4 43.9, 64 x 64
-// unsplit 72; 470 x 28672 x 4096 256 x 256 70, 128 x 256 84; 1000 x 4096 x 4096 128 x 128 25.8, 256 x
-// 256 49; 2000 x 4096 x 14336 256 x 256 in 2 126, 128 x 256 127.
+// written and read, 4.5 TB/s. Chosen and another, us, operands from memory: 64 x 4096 x 14336
+// (rows, weights, columns) 64 x 128 split in 8 20.0, unsplit 63.5; 470 x 4096 x 14336 128 x 256 in 4
+// 46 to 51, 64 x 128 unsplit 68; 470 x 28672 x 4096 256 x 256 69, 128 x 256 83; 1000 x 4096 x 4096
+// 128 x 128 25.7, 256 x 256 49; 2000 x 4096 x 14336 256 x 256 in 2 126, 128 x 256 132.
 Plan plan_for(int T, int K, int N) {
   const int groups = K / kGroup;
   Plan best{};
@@ -477,9 +478,10 @@ extern "C" int pdk_linear_fp8(const uint8_t* x, int64_t x_ld, const float* x_sca
   Args a{x, x_ld, x_scales, xs_tok_stride, xs_group_stride, w, w_scales, T, N, K, y, 1, K / kGroup, nullptr};
   const hipStream_t st = pdk::as_stream(stream);
   if (T <= kFewRows) {
-    // Weights of a workgroup: as many as leave every CU one. us with 16, 32 and 64, 16 rows: 28672 x
-    // 4096 36.6, 32.4, 26.9; 6144 x 4096 11.2, 9.2, 12.5; 4096 x 4096 7.1, 9.0, 12.4; 4096 x 14336 19.0,
-    // 23.2, 35.5.
+    // Weights of a workgroup: as many as leave every CU one. us with 16, 32 and 64, 16 rows, operands
+    // from memory: 28672 x 4096 32.7, 26.5, 23.3; 16384 x 4096 19.7, 14.8, 16.4; 6144 x 4096 10.5, 7.7,
+    // 12.7; 4096 x 4096 6.0, 7.6, 12.6; 4096 x 14336 18.2, 21.6, 45.9. Not always the best: 18432 x 4096
+    // 23.8, 19.8, 21.9; 57344 x 8192 116, 87, 90.
     if (N > 64 * 256) launch_few<4, 4>(a, st);
     else if (N > 16 * 256) launch_few<2, 8>(a, st);
     else launch_few<1, 8>(a, st);

@@ -9,8 +9,8 @@
 // A row is held in registers between its sum of squares and its output, one
 // 16-byte load per 8 columns; 16 lanes hold a group and find its largest value by
 // four exchanges. A NaN makes its group's scale NaN, an infinity makes it
-// infinite. Bound by HBM: 7 bytes a column with the addition (8192 x 4096: 39.6 us,
-// 6.0 TB/s; 16 rows 3.2 us), 3 without.
+// infinite. Bound by HBM: 7 bytes a column with the addition (8192 x 4096: 40.7 us,
+// 5.8 TB/s; 16 rows 3.2 us), 3 without (23.4 us, 4.3 TB/s).
 #include <math.h>
 
 #include "pdk_common.h"
@@ -154,7 +154,9 @@ extern "C" int pdk_rmsnorm_fp8(const uint16_t* x, const uint16_t* add, const uin
 namespace {
 
 // Rows of K columns in 8 bits, 8 columns a thread. kGated: of silu(g) * u, a row of x
-// being g's K columns and then u's.
+// being g's K columns and then u's. 8192 x 4096 plain 21.8 us, 8192 x 14336 gated 121.5 (4.7 and 4.8
+// TB/s; 16 rows 2.0 and 2.4): beside the bytes the row's division in 64 bits and, gated, a division
+// for each value.
 template <bool kGated>
 __global__ __launch_bounds__(256) void quantize_fp8_kernel(const uint16_t* x, int64_t ld, int T, int K,
                                                            uint8_t* out, float* scales,
