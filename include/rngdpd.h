@@ -888,7 +888,8 @@ int pdk_rope_cache_write(const uint16_t* qkv, int64_t ld, const float* inv_freq,
  * nobody; a token that sees nothing gets zeros. out [N][Hq][128]; rows of no request are
  * left as they are. max_new and max_ctx are at least any request's. head_dim 128, Hq / Hkv
  * from 1 to 16, max_blocks <= 65535, N <= 2^20. The workspace (16-byte aligned, 284
- * MB at most) serves one call at a time; pdk_chunk_attn_workspace_bytes is -1 for sizes out of range. */
+ * MB at most) serves one call at a time; pdk_chunk_attn_workspace_bytes is -1 for sizes
+ * out of range. */
 int64_t pdk_chunk_attn_workspace_bytes(int N, int R, int max_new, int max_ctx,
                                        int n_q_heads, int n_kv_heads, int window,
                                        int sinks);
